@@ -20,6 +20,8 @@ from .runtime import (INDEX_BLOCK_META_SIZE, TiledPackedWeight, TileConfig, _bui
                       resolve_plan)
 from .select import (_energy_expanded_active_blocks, _select_active_blocks, _select_active_blocks_l1,
                      _topk_energy_ratio, select_sparse_gemm, select_topk, select_topk_l1)
+from .serving import (KVCache, TokenLogprobs, kv_append, kv_attention, pages_compact, pages_copy, pages_extend, pages_fork,
+                      pages_free, read_pages, token_logprobs)
 from .sparse2d import (INDEX_BLOCK_OUT_META_SIZE, _get_cached_active_n_blocks_delta,
                        _prepacked_block_sparse_gemm_2d_bitmap_from_active_blocks,
                        _prepacked_block_sparse_gemm_2d_compact_from_active_blocks,
@@ -43,4 +45,6 @@ __all__ = [
     "_prepacked_block_sparse_gemm_2d_bitmap_from_active_blocks",
     "_prepacked_block_sparse_gemm_2d_compact_from_active_blocks", "_scatter_compact_to_dense_output",
     "_get_cached_active_n_blocks_delta", "gemm_2d_packed", "scatter_nblocks", "nmask_blocks",
+    "KVCache", "TokenLogprobs", "kv_append", "kv_attention", "pages_copy", "pages_fork", "pages_extend", "pages_free",
+    "pages_compact", "read_pages", "token_logprobs",
 ]

@@ -27,6 +27,7 @@ BSG_ERR_HIP = -100
 
 BSG_F16 = 0
 BSG_BF16 = 1
+BSG_F32 = 2  # logits only
 BLOCK_K = 64
 MAX_NBLK = 2048
 NOALLOC_SCRATCH_BYTES = 16 * 1024 * 1024  # BSG_NOALLOC_SCRATCH_BYTES
@@ -98,13 +99,54 @@ class SelectOpts(ctypes.Structure):
     ]
 
 
+class KvCache(ctypes.Structure):
+    """Mirror of `bsg_kv_cache`."""
+
+    _fields_ = [
+        ("pages", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("num_pages", ctypes.c_int64),
+        ("n_heads", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("num_slots", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("table_stride", ctypes.c_int64),
+        ("page_table", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+    ]
+
+
+class PagePool(ctypes.Structure):
+    """Mirror of `bsg_page_pool`."""
+
+    _fields_ = [
+        ("pages", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("layers", ctypes.c_int64),
+        ("num_pages", ctypes.c_int64),
+        ("page_bytes", ctypes.c_int64),
+        ("page_scales", ctypes.c_int64),
+        ("page_size", ctypes.c_int32),
+        ("num_slots", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("table_stride", ctypes.c_int64),
+        ("page_table", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("refcounts", ctypes.c_void_p),
+    ]
+
+
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
 _int = ctypes.c_int
+_f32 = ctypes.c_float
 _pplan = ctypes.POINTER(Plan)
+_pkv = ctypes.POINTER(KvCache)
+_ppool = ctypes.POINTER(PagePool)
 
-# name -> (restype, argtypes); every function declared in include/bsgemm.h
+# name -> (restype, argtypes); every function declared in include/bsgemm.h and include/bsgserve.h
 SIGNATURES = {
     "bsg_version": (ctypes.c_char_p, []),
     "bsg_last_error": (ctypes.c_char_p, []),
@@ -135,6 +177,19 @@ SIGNATURES = {
     "bsg_select_gemm_noalloc": (_int, [_vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _vp, _vp, _i64, _int,
                                        _pplan, _vp]),
     "bsg_read_calibrate": (_int, [_vp, _i64, _vp, _vp]),
+    # include/bsgserve.h
+    "bsg_kv_append": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i64, _pkv, _vp, _i32, _vp, _i32, _int, _vp]),
+    "bsg_kv_attention_workspace_bytes": (_i64, [_pkv, _i32, _i32, _i32, _i64, _i32]),
+    "bsg_kv_attention": (_int, [_vp, _i64, _i64, _i64, _i32, _pkv, _vp, _i32, _vp, _i32, _i64, _f32, _vp, _i64, _i64,
+                                _vp, _int, _vp, _i64, _i32, _vp]),
+    "bsg_pages_workspace_bytes": (_i64, [_i64]),
+    "bsg_pages_copy": (_int, [_ppool, _vp, _vp, _i32, _vp]),
+    "bsg_pages_fork": (_int, [_ppool, _vp, _vp, _i32, _vp]),
+    "bsg_pages_extend": (_int, [_ppool, _vp, _vp, _i32, _vp, _vp, _i64, _vp]),
+    "bsg_pages_free": (_int, [_ppool, _vp, _i32, _vp]),
+    "bsg_pages_compact": (_int, [_ppool, _vp, _vp, _i64, _vp]),
+    "bsg_token_logprobs_workspace_bytes": (_i64, [_i64, _i64, _i32, _int, _i32]),
+    "bsg_token_logprobs": (_int, [_vp, _i64, _i64, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _int, _vp, _i64, _i32, _vp]),
     # include/bsgemm_timeline.h
     "bsg_timeline_attach": (_int, [_vp, _i64, _i64]),
     "bsg_timeline_clock_khz": (_i64, []),

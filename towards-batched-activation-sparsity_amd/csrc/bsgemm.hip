@@ -58,9 +58,12 @@
 #define BSG_VERSION_STR "bsgemm 0.1 (gfx950, mfma_f32_16x16x32)"
 
 namespace {
-
 thread_local char g_err[512] = "";
+}  // namespace
 
+namespace bsgk {
+
+// The message behind bsg_last_error(), for every unit of the library.
 int fail(int code, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
@@ -68,6 +71,12 @@ int fail(int code, const char* fmt, ...) {
   va_end(ap);
   return code;
 }
+
+}  // namespace bsgk
+
+namespace {
+
+using bsgk::fail;
 
 int hip_fail(hipError_t e, const char* what) {
   return fail(BSG_ERR_HIP, "%s: %s", what, hipGetErrorString(e));

@@ -1,0 +1,500 @@
+// kv_attention.hip — attention over the 8-bit paged cache (include/bsgserve.h).
+//
+// Per cached head, the rows of a call are its new tokens x the query heads that share it.  With
+// every product transposed, S^T = K Q^T and O^T = V^T P^T, a cache tile of 16 tokens is the A
+// operand of v_mfma_f32_16x16x32 as it lies in memory, 16 query rows are its columns, and the
+// accumulator layout of S^T (column = row of the call, four consecutive tokens per lane) is the B
+// operand that O^T needs: nothing is shuffled between the two products.
+//
+// Scales and softmax in one exponent: with s2 = log2(e) sm_scale ks (q . k8) and lv = log2(vs), the weight of a
+// token is w = 2^(s2 + lv - M + 14) against the running maximum M of s2 + lv, so that O = sum w v8 /
+// sum w / vs whatever M is.  w is at most 2^14 and goes to the matrix unit as fp16: every weight
+// down to 2^-28 of the largest keeps 11 bits.
+
+#include "serve.hpp"
+
+using namespace bsgk;
+
+namespace bsgk {
+int check_kv_cache(const bsg_kv_cache* c);
+int check_kv_batch(int64_t tokens, int32_t rows, const int32_t* slots, const int32_t* cu, int32_t max_new,
+                   const bsg_kv_cache* c, int dtype);
+}  // namespace bsgk
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kShift = 14.f;  // weights go up to 2^14
+
+struct AttnParams {
+  const uint16_t* q;
+  uint16_t* out;
+  float* lse;
+  const uint8_t* pages;
+  const float* scales;
+  const int32_t* table;
+  const int32_t* lengths;
+  const int32_t* slots;
+  const int32_t* cu;
+  float* part;         // [tile of rows][split][rows][D + 2]
+  uint32_t* counters;  // [tile of rows]
+  int64_t q_st, q_sh, o_st, o_sh, table_stride, tokens;
+  float scale2;        // sm_scale * log2(e)
+  int32_t num_pages, kv_heads, group, num_slots, max_pages, page_shift, max_new, row_tiles, splits, chunk;
+};
+
+template <typename T>
+struct Elem;
+template <>
+struct Elem<_Float16> {
+  typedef f16x8 x8;
+  static __device__ __forceinline__ uint32_t word(uint32_t w, bool high) {
+    return __builtin_bit_cast(uint32_t, high ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true)
+                                             : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false));
+  }
+  static __device__ __forceinline__ f32x4 mfma(x8 a, x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
+  }
+};
+template <>
+struct Elem<__bf16> {
+  typedef bf16x8 x8;
+  static __device__ __forceinline__ uint32_t word(uint32_t w, bool high) {
+    return __builtin_bit_cast(uint32_t, high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true)
+                                             : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false));
+  }
+  static __device__ __forceinline__ f32x4 mfma(x8 a, x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+  }
+};
+
+// Eight e4m3 numbers as 16-bit ones (exact in either type).
+template <typename T>
+__device__ __forceinline__ typename Elem<T>::x8 widen(uint32_t lo, uint32_t hi) {
+  return __builtin_bit_cast(typename Elem<T>::x8, u32x4{Elem<T>::word(lo, false), Elem<T>::word(lo, true),
+                                                        Elem<T>::word(hi, false), Elem<T>::word(hi, true)});
+}
+
+// Over the four lanes that hold one column: lanes l, l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ float column_max(float v) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, v);
+  const auto x = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  v = fmaxf(as_float(x[0]), as_float(x[1]));
+  const uint32_t c = __builtin_bit_cast(uint32_t, v);
+  const auto y = __builtin_amdgcn_permlane16_swap(c, c, false, false);
+  return fmaxf(as_float(y[0]), as_float(y[1]));
+}
+__device__ __forceinline__ float column_sum(float v) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, v);
+  const auto x = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  v = as_float(x[0]) + as_float(x[1]);
+  const uint32_t c = __builtin_bit_cast(uint32_t, v);
+  const auto y = __builtin_amdgcn_permlane16_swap(c, c, false, false);
+  return as_float(y[0]) + as_float(y[1]);
+}
+
+// The bytes of four consecutive tokens of which the first n exist.
+__device__ __forceinline__ uint32_t byte_mask(int n) {
+  return n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
+}
+// 0x38 (1.0 in e4m3) in each byte that is NaN (0x7f or 0xff).
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
+  const uint32_t x = (w & 0x7f7f7f7fu) + 0x01010101u;  // bit 7 of a byte: all seven bits were set
+  return ((x & 0x80808080u) >> 7) * 0x38u;
+}
+
+// A work-group of four waves computes RT x 16 rows of one cached head of one sequence over one chunk
+// of its tokens; wave w takes the 32-token steps w, w + 4, ..., each with its own running maximum, and the
+// waves meet in LDS at the end.  Chunks meet in the workspace: the last one to arrive sums them in order.
+template <typename T, int D, int RT>
+__global__ __launch_bounds__(256) void bsg_kv_attention_kernel(AttnParams p) {
+  constexpr int C = D / 64, DT = D / 16, ROWS = 16 * RT, LD = D + 4;
+  typedef typename Elem<T>::x8 x8;
+  __shared__ float s_acc[ROWS * LD];
+  __shared__ float s_m[4][ROWS], s_l[4][ROWS];
+  __shared__ uint32_t s_last;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int col = lane & 15, g = lane >> 4;
+  const int head = blockIdx.x / p.row_tiles, rt = blockIdx.x - head * p.row_tiles;
+  const int split = blockIdx.y, row = blockIdx.z;
+
+  const int slot = p.slots ? p.slots[row] : row;
+  int64_t from = (int64_t)row * p.max_new, to = from + p.max_new;
+  if (p.cu) from = p.cu[row], to = p.cu[row + 1];
+  if (from < 0 || to > p.tokens || from >= to) return;
+  const int count = (int)(to - from < p.max_new ? to - from : p.max_new);
+  const int rows = count * p.group - rt * ROWS;  // rows of this tile that exist (at most ROWS count)
+  if (rows <= 0) return;
+  int len = slot >= 0 && slot < p.num_slots ? p.lengths[slot] : 0;
+  const int most = p.max_pages << p.page_shift;
+  len = len < 0 ? 0 : len > most ? most : len;
+  const int first = len - (int)(to - from);  // position of the first new token (below 0: it sees nothing)
+
+  // tokens that the tile's rows see: row r is new token r / group
+  const int r_last = rt * ROWS + (rows < ROWS ? rows : ROWS) - 1;
+  int end = first + r_last / p.group + 1;
+  end = end < 0 ? 0 : end;
+  const int all_see = first + rt * ROWS / p.group + 1;  // tokens that every row sees
+  const int chunks = end <= p.chunk ? 1 : (end + p.chunk - 1) / p.chunk < p.splits ? (end + p.chunk - 1) / p.chunk : p.splits;
+  if (split >= chunks) return;
+  const int t_begin = split * p.chunk;
+  const int t_end = split == chunks - 1 ? end : t_begin + p.chunk;
+
+  // Q^T as the B operand: column = row of the tile, channels in the order the keys' tiles have them
+  x8 qf[RT][2 * C];
+  int sees[RT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    const int r = rt * ROWS + 16 * i + col;
+    const int tok = r / p.group, h = r - tok * p.group;
+    const bool on = 16 * i + col < rows;
+    sees[i] = on ? first + tok + 1 : 0;
+#pragma unroll
+    for (int c = 0; c < 2 * C; ++c) {
+      u32x4 v = {0u, 0u, 0u, 0u};
+      if (on)
+        v = *(const u32x4*)(p.q + (from + tok) * p.q_st + (int64_t)(head * p.group + h) * p.q_sh + 64 * (c >> 1) +
+                            16 * g + 8 * (c & 1));
+      qf[i][c] = __builtin_bit_cast(x8, v);
+    }
+  }
+
+  f32x4 acc[RT][DT];
+  float m[RT], l[RT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    m[i] = -__builtin_inff(), l[i] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  const int32_t* const table = p.table + (int64_t)(slot < 0 || slot >= p.num_slots ? 0 : slot) * p.table_stride;
+  const int64_t head_bytes = (int64_t)2 * D << p.page_shift;
+  for (int t0 = t_begin + 32 * wave; t0 < t_end; t0 += 128) {
+    u32x4 kr[2][C], vr[2][C];
+    float ks[2], vs[2];
+    bool there[2];
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const int t = t0 + 16 * a;
+      int page = t < t_end ? table[t >> p.page_shift] : -1;
+      there[a] = page >= 0 && page < p.num_pages;
+      page = there[a] ? page : 0;
+      const int64_t ph = (int64_t)page * p.kv_heads + head;
+      const uint8_t* const at = p.pages + ph * head_bytes + (int64_t)((t & ((1 << p.page_shift) - 1)) * D) + lane * 16;
+      const f32x2 s = *(const f32x2*)(p.scales + 2 * ph);
+      ks[a] = s.x * p.scale2, vs[a] = fmaxf(s.y, 0x1p-100f);
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        kr[a][c] = *(const u32x4*)(at + c * 1024);
+        vr[a][c] = *(const u32x4*)(at + (head_bytes >> 1) + c * 1024);
+      }
+    }
+    const bool partial = t0 + 32 > all_see || !there[0] || !there[1];
+    uint32_t nan = 0;
+    if (partial) {
+      // tokens past the tile's end may be anything
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const uint32_t mask = there[a] ? byte_mask(t_end - (t0 + 16 * a + 4 * g)) : 0u;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          vr[a][c] &= mask;
+          nan |= nan_bytes(vr[a][c].x) | nan_bytes(vr[a][c].y) | nan_bytes(vr[a][c].z) | nan_bytes(vr[a][c].w);
+        }
+      }
+    }
+    const bool some_nan = partial && __any(nan != 0);
+    const float lv[2] = {__builtin_amdgcn_logf(vs[0]), __builtin_amdgcn_logf(vs[1])};
+    const float iv[2] = {1.f / vs[0], 1.f / vs[1]};
+
+    f16x8 pf[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      f32x4 s[2];
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        s[a] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          s[a] = Elem<T>::mfma(widen<T>(kr[a][c].x, kr[a][c].y), qf[i][2 * c], s[a]);
+          s[a] = Elem<T>::mfma(widen<T>(kr[a][c].z, kr[a][c].w), qf[i][2 * c + 1], s[a]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s[a][j] = s[a][j] * ks[a] + lv[a];
+          if (partial && (!there[a] || t0 + 16 * a + 4 * g + j >= sees[i])) s[a][j] = -__builtin_inff();
+        }
+      }
+      float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                       fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+      mx = fmaxf(m[i], column_max(mx));
+      if (__any(mx > m[i])) {
+        const float alpha = mx == m[i] ? 1.f : __builtin_amdgcn_exp2f(m[i] - mx);
+        l[i] *= alpha;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[i][d] *= alpha;
+        m[i] = mx;
+      }
+      const float base = (m[i] == -__builtin_inff() ? 0.f : m[i]) - kShift;
+      float w[2][4];
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[a][j] = __builtin_amdgcn_exp2f(s[a][j] - base);
+        l[i] += ((w[a][0] + w[a][1]) + (w[a][2] + w[a][3])) * iv[a];
+      }
+      pf[i] = __builtin_bit_cast(
+          f16x8, u32x4{Elem<_Float16>::pack(w[0][0], w[0][1]), Elem<_Float16>::pack(w[0][2], w[0][3]),
+                       Elem<_Float16>::pack(w[1][0], w[1][1]), Elem<_Float16>::pack(w[1][2], w[1][3])});
+    }
+    if (some_nan) {
+      // A NaN among values that some rows do not see: the matrix unit would spread it to all rows
+      // (0 x NaN), so it goes to those that see it by a product of flags and leaves the values.
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        uint32_t f[4];
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int t = t0 + 16 * a + 4 * g + 2 * j;
+            f[2 * a + j] = Elem<_Float16>::pack(t < sees[i] ? 1.f : 0.f, t + 1 < sees[i] ? 1.f : 0.f);
+          }
+        const f16x8 flags = __builtin_bit_cast(f16x8, u32x4{f[0], f[1], f[2], f[3]});
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          f32x4 n = {0.f, 0.f, 0.f, 0.f};
+          n = Elem<_Float16>::mfma(
+              widen<_Float16>(nan_bytes(vr[0][d >> 2][d & 3]), nan_bytes(vr[1][d >> 2][d & 3])), flags, n);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n[j] > 0.f) acc[i][d][j] = __builtin_nanf("");
+        }
+      }
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            const uint32_t n = nan_bytes(vr[a][c][d]);
+            vr[a][c][d] &= ~(n | (n << 1) | (n << 2) | (n >> 1) | (n >> 2) | (n >> 3));
+          }
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      const f16x8 v = widen<_Float16>(vr[0][d >> 2][d & 3], vr[1][d >> 2][d & 3]);
+#pragma unroll
+      for (int i = 0; i < RT; ++i) acc[i][d] = Elem<_Float16>::mfma(v, pf[i], acc[i][d]);
+    }
+  }
+
+  // the waves' parts under a common maximum
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    l[i] = column_sum(l[i]);
+    if (g == 0) s_m[wave][16 * i + col] = m[i], s_l[wave][16 * i + col] = l[i];
+  }
+  __syncthreads();
+  float f[RT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    const int r = 16 * i + col;
+    const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+    f[i] = m[i] == top ? 1.f : __builtin_amdgcn_exp2f(m[i] - top);
+  }
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (wave == w) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          f32x4* const at = (f32x4*)(s_acc + (16 * i + col) * LD + 16 * d + 4 * g);
+          f32x4 v = acc[i][d] * f[i];
+          if (w > 0) v += *at;
+          *at = v;
+        }
+    }
+    __syncthreads();
+  }
+
+  const int used = rows < ROWS ? rows : ROWS;
+  const int64_t tile = ((int64_t)row * p.kv_heads + head) * p.row_tiles + rt;
+  float* const part = p.part + (tile * p.splits + split) * (ROWS * (D + 2));
+  if (chunks > 1) {
+    for (int e = threadIdx.x; e < used * D; e += 256) hand_store(part + e, s_acc[(e / D) * LD + e % D]);
+    if ((int)threadIdx.x < used) {
+      const int r = threadIdx.x;
+      const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) sum += s_l[w][r] * (s_m[w][r] == top ? 1.f : __builtin_amdgcn_exp2f(s_m[w][r] - top));
+      hand_store(part + ROWS * D + r, top);
+      hand_store(part + ROWS * (D + 1) + r, sum);
+    }
+    hand_publish();
+    __syncthreads();
+    if (threadIdx.x == 0) s_last = hand_arrive(p.counters + tile) == (uint32_t)(chunks - 1);
+    __syncthreads();
+    if (!s_last) return;
+    if (threadIdx.x == 0) hand_reset(p.counters + tile);
+  }
+  const float* const parts = p.part + tile * p.splits * (ROWS * (D + 2));
+  constexpr int E = 4, PER = D / E;  // a thread's numbers of one row
+  for (int e = threadIdx.x; e < used * PER; e += 256) {
+    const int r = e / PER, d = (e - r * PER) * E;
+    float top, sum = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    if (chunks > 1) {
+      top = -__builtin_inff();
+      for (int s = 0; s < chunks; ++s) top = fmaxf(top, hand_load(parts + s * (ROWS * (D + 2)) + ROWS * D + r));
+      for (int s = 0; s < chunks; ++s) {
+        const float* const q = parts + s * (ROWS * (D + 2));
+        const float ms = hand_load(q + ROWS * D + r);
+        const float fs = ms == top ? 1.f : __builtin_amdgcn_exp2f(ms - top);
+        sum += fs * hand_load(q + ROWS * (D + 1) + r);
+#pragma unroll
+        for (int j = 0; j < E; ++j) o[j] += fs * hand_load(q + r * D + d + j);
+      }
+    } else {
+      top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+#pragma unroll
+      for (int w = 0; w < 4; ++w) sum += s_l[w][r] * (s_m[w][r] == top ? 1.f : __builtin_amdgcn_exp2f(s_m[w][r] - top));
+      o = *(const f32x4*)(s_acc + r * LD + d);
+    }
+    const int rr = rt * ROWS + r, tok = rr / p.group, h = head * p.group + rr - tok * p.group;
+    const bool nothing = sum == 0.f;
+    const float inv = nothing ? 0.f : 1.f / sum;
+    u32x2* const at = (u32x2*)(p.out + (from + tok) * p.o_st + (int64_t)h * p.o_sh + d);
+    *at = u32x2{Elem<T>::pack(o[0] * inv, o[1] * inv), Elem<T>::pack(o[2] * inv, o[3] * inv)};
+    if (p.lse && d == 0)
+      p.lse[(from + tok) * ((int64_t)p.kv_heads * p.group) + h] =
+          nothing ? -__builtin_inff() : (top - kShift + __builtin_amdgcn_logf(sum)) * (1.f / kLog2e);
+  }
+}
+
+struct Shape {
+  int rt;               // 16-row tiles of a work-group
+  int32_t row_tiles;    // work-groups over the rows of a cached head
+  int32_t splits;
+  int32_t chunk;
+};
+
+// How a call is cut: few rows leave most compute units idle unless the long axis is split.
+Shape shape_of(int32_t rows, int32_t kv_heads, int32_t group, int32_t max_new, int64_t max_len, int32_t cus) {
+  Shape s;
+  const int64_t per_head = (int64_t)max_new * group;
+  s.rt = per_head <= 16 ? 1 : per_head <= 32 ? 2 : 4;
+  s.row_tiles = (int32_t)ceil_div(per_head, 16 * s.rt);
+  const int64_t tiles = (int64_t)rows * kv_heads * s.row_tiles;
+  int64_t want = ceil_div((int64_t)4 * cus, tiles > 0 ? tiles : 1);
+  const int64_t most = ceil_div(max_len > 0 ? max_len : 1, 256);
+  if (want > most) want = most;
+  if (tiles * 4 > BSG_KV_COUNTER_BYTES) want = 1;
+  s.chunk = (int32_t)(ceil_div(ceil_div(max_len > 0 ? max_len : 1, want), 128) * 128);
+  s.splits = (int32_t)ceil_div(max_len > 0 ? max_len : 1, s.chunk);
+  return s;
+}
+
+int64_t workspace_bytes(const Shape& s, int32_t rows, int32_t kv_heads, int32_t d) {
+  if (s.splits <= 1) return 0;
+  return BSG_KV_COUNTER_BYTES + (int64_t)rows * kv_heads * s.row_tiles * s.splits * (16 * s.rt) * (d + 2) * 4;
+}
+
+template <typename T, int D>
+void launch(const AttnParams& p, const Shape& s, dim3 grid, hipStream_t st) {
+  switch (s.rt) {
+    case 1: hipLaunchKernelGGL((bsg_kv_attention_kernel<T, D, 1>), grid, dim3(256), 0, st, p); break;
+    case 2: hipLaunchKernelGGL((bsg_kv_attention_kernel<T, D, 2>), grid, dim3(256), 0, st, p); break;
+    default: hipLaunchKernelGGL((bsg_kv_attention_kernel<T, D, 4>), grid, dim3(256), 0, st, p); break;
+  }
+}
+
+int check_heads(const bsg_kv_cache* c, int32_t q_heads) {
+  if (q_heads < 1 || q_heads % c->n_heads != 0)
+    return fail(BSG_ERR_ARG, "q_heads=%d is no multiple of the cache's %d heads", q_heads, c->n_heads);
+  return BSG_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t bsg_kv_attention_workspace_bytes(const bsg_kv_cache* cache, int32_t rows, int32_t q_heads,
+                                                    int32_t max_new, int64_t max_len, int32_t cu_count) {
+  if (check_kv_cache(cache) || check_heads(cache, q_heads) || rows < 0 || max_new < 0 || cu_count < 1) return -1;
+  const int64_t most = (int64_t)cache->max_pages * cache->page_size;
+  if (max_len <= 0 || max_len > most) max_len = most;
+  return workspace_bytes(shape_of(rows, cache->n_heads, q_heads / cache->n_heads, max_new, max_len, cu_count), rows,
+                         cache->n_heads, cache->head_dim);
+}
+
+extern "C" int bsg_kv_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, int64_t tokens,
+                                int32_t q_heads, const bsg_kv_cache* cache, const int32_t* slots, int32_t rows,
+                                const int32_t* cu, int32_t max_new, int64_t max_len, float sm_scale, void* out,
+                                int64_t o_stride_t, int64_t o_stride_h, float* lse, int dtype, void* ws,
+                                int64_t ws_bytes, int32_t cu_count, void* stream) {
+  if (const int rc = check_kv_cache(cache)) return rc;
+  if (const int rc = check_heads(cache, q_heads)) return rc;
+  if (const int rc = check_kv_batch(tokens, rows, slots, cu, max_new, cache, dtype)) return rc;
+  if (cu_count < 1) return fail(BSG_ERR_ARG, "cu_count=%d", cu_count);
+  if (tokens == 0 || rows == 0 || max_new == 0) return BSG_OK;
+  if (!q || !out) return fail(BSG_ERR_ARG, "null pointer (q=%p out=%p)", q, out);
+  if (!is_aligned(q, 16) || ((q_stride_t | q_stride_h) & 7) != 0)
+    return fail(BSG_ERR_ALIGN, "q rows must be 16-byte aligned (strides %lld, %lld)", (long long)q_stride_t,
+                (long long)q_stride_h);
+  if (!is_aligned(out, 8) || ((o_stride_t | o_stride_h) & 3) != 0)
+    return fail(BSG_ERR_ALIGN, "out rows must be 8-byte aligned (strides %lld, %lld)", (long long)o_stride_t,
+                (long long)o_stride_h);
+  const int64_t most = (int64_t)cache->max_pages * cache->page_size;
+  if (max_len <= 0 || max_len > most) max_len = most;
+  const int32_t group = q_heads / cache->n_heads;
+  if ((int64_t)max_new * group > 0x7fffffff / 2) return fail(BSG_ERR_UNSUPPORTED, "%d tokens x %d heads", max_new, group);
+  const Shape s = shape_of(rows, cache->n_heads, group, max_new, max_len, cu_count);
+  const int64_t need = workspace_bytes(s, rows, cache->n_heads, cache->head_dim);
+  if (need > 0 && (!ws || ws_bytes < need))
+    return fail(BSG_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)need);
+  if (need > 0 && !is_aligned(ws, 16)) return fail(BSG_ERR_ALIGN, "workspace must be 16-byte aligned");
+  const int64_t gx = (int64_t)cache->n_heads * s.row_tiles;
+  if (gx > 0x7fffffff || rows > 65535 || s.splits > 65535)
+    return fail(BSG_ERR_UNSUPPORTED, "grid of %lld x %d x %d", (long long)gx, s.splits, rows);
+  AttnParams p;
+  p.q = (const uint16_t*)q;
+  p.out = (uint16_t*)out;
+  p.lse = lse;
+  p.pages = (const uint8_t*)cache->pages;
+  p.scales = cache->scales;
+  p.table = cache->page_table;
+  p.lengths = cache->lengths;
+  p.slots = slots;
+  p.cu = cu;
+  p.counters = (uint32_t*)ws;
+  p.part = need > 0 ? (float*)((uint8_t*)ws + BSG_KV_COUNTER_BYTES) : nullptr;
+  p.q_st = q_stride_t, p.q_sh = q_stride_h, p.o_st = o_stride_t, p.o_sh = o_stride_h;
+  p.table_stride = cache->table_stride;
+  p.tokens = tokens;
+  p.scale2 = sm_scale * kLog2e;
+  p.num_pages = (int32_t)cache->num_pages;
+  p.kv_heads = cache->n_heads;
+  p.group = group;
+  p.num_slots = cache->num_slots;
+  p.max_pages = cache->max_pages;
+  p.page_shift = __builtin_ctz((unsigned)cache->page_size);
+  p.max_new = max_new;
+  p.row_tiles = s.row_tiles;
+  p.splits = s.splits;
+  p.chunk = s.chunk;
+  const dim3 grid((unsigned)gx, (unsigned)s.splits, (unsigned)rows);
+  const hipStream_t st = (hipStream_t)stream;
+  if (dtype == BSG_F16)
+    cache->head_dim == 64 ? launch<_Float16, 64>(p, s, grid, st) : launch<_Float16, 128>(p, s, grid, st);
+  else
+    cache->head_dim == 64 ? launch<__bf16, 64>(p, s, grid, st) : launch<__bf16, 128>(p, s, grid, st);
+  return launch_status("bsg_kv_attention");
+}

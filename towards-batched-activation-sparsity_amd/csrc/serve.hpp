@@ -1,0 +1,82 @@
+// serve.hpp — what the serving operators' units share: the C ABI's error message, argument helpers,
+// and small device primitives (16-bit element types, cross-lane sums, the hand-off of partials).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "bsgserve.h"
+
+namespace bsgk {
+
+// Sets the calling thread's bsg_last_error() message and returns `code` (bsgemm.hip).
+int fail(int code, const char* fmt, ...);
+
+inline int launch_status(const char* what) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? BSG_OK : fail(BSG_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
+}
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline bool is_aligned(const void* p, unsigned n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// By value: a bit cast of a vector's element in place reads its first one.
+__device__ __forceinline__ float as_float(uint32_t w) { return __builtin_bit_cast(float, w); }
+
+// Both halves of a 32-bit word of two 16-bit numbers, as fp32 (exact).
+template <typename T>
+__device__ __forceinline__ float low_half(uint32_t w);
+template <typename T>
+__device__ __forceinline__ float high_half(uint32_t w);
+template <>
+__device__ __forceinline__ float low_half<_Float16>(uint32_t w) {
+  return (float)__builtin_bit_cast(f16x2, w).x;
+}
+template <>
+__device__ __forceinline__ float high_half<_Float16>(uint32_t w) {
+  return (float)__builtin_bit_cast(f16x2, w).y;
+}
+template <>
+__device__ __forceinline__ float low_half<__bf16>(uint32_t w) {
+  return __builtin_bit_cast(float, w << 16);
+}
+template <>
+__device__ __forceinline__ float high_half<__bf16>(uint32_t w) {
+  return __builtin_bit_cast(float, w & 0xffff0000u);
+}
+
+// Partials cross work-groups with agent-scope relaxed atomics (device-coherent, with no fence that
+// would write back and invalidate a whole L2): every wave waits for its stores, the work-group
+// meets in a barrier, and one thread counts the arrival.
+__device__ __forceinline__ void hand_store(float* p, float v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void hand_store(uint64_t* p, uint64_t v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float hand_load(const float* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t hand_load(const uint64_t* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void hand_publish() {
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+}
+__device__ __forceinline__ uint32_t hand_arrive(uint32_t* c) {
+  return __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void hand_reset(uint32_t* c) {
+  __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+}  // namespace bsgk
