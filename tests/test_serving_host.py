@@ -144,7 +144,7 @@ def test_bad_pools_are_refused():
 def test_bad_logprobs_are_refused():
     lib = bsa.load()
 
-    def call(x=FAKE, rows=4, vocab=50000, k=3, ids=FAKE, dtype=0, ws=FAKE, ws_bytes=1 << 30, cus=256):
+    def call(x=FAKE, rows=4, vocab=1 << 20, k=3, ids=FAKE, dtype=0, ws=FAKE, ws_bytes=1 << 30, cus=256):
         return lib.bsg_token_logprobs(x, vocab, rows, vocab, FAKE, k, FAKE, FAKE, ids, FAKE, dtype, ws, ws_bytes, cus, None)
 
     assert call(x=None) == _lib.BSG_ERR_ARG
@@ -157,9 +157,10 @@ def test_bad_logprobs_are_refused():
     assert call(x=FAKE + 1) == _lib.BSG_ERR_ALIGN
     assert call(x=FAKE + 2, dtype=2) == _lib.BSG_ERR_ALIGN
     assert call(ws=None) == _lib.BSG_ERR_WORKSPACE
-    need = lib.bsg_token_logprobs_workspace_bytes(4, 50000, 3, 0, 256)
+    need = lib.bsg_token_logprobs_workspace_bytes(4, 1 << 20, 3, 0, 256)
     assert need > 0 and call(ws_bytes=need - 1) == _lib.BSG_ERR_WORKSPACE
     assert call(rows=0) == 0
+    assert lib.bsg_token_logprobs_workspace_bytes(0, 1 << 20, 3, 0, 256) == 0
 
 
 def test_python_layer_refuses_host_tensors():

@@ -23,14 +23,13 @@ int32 [pages] how many table entries name a page.
 """
 from __future__ import annotations
 
-import ctypes
 from typing import Dict, NamedTuple, Optional, Tuple
 
 import torch
 
 from . import _lib
 from ._lib import check, load
-from .runtime import _cu_count, _dtype_code, _require_cuda, _stream_handle
+from .runtime import _cu_count, _dtype_code, _require_cuda
 
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128)
@@ -42,24 +41,60 @@ _F8 = torch.float8_e4m3fn
 _WORKSPACES: Dict[tuple, list] = {}
 
 
-def _workspace(dev: torch.device, nbytes: int, prefix: Optional[str], stream: int) -> torch.Tensor:
+# What a call's shapes, strides, types and devices decide (the checks, the sizes, the library's
+# fixed arguments) is worked out once for each such signature; addresses and values come with each call.
+_CALLS: Dict[tuple, tuple] = {}
+_CALLS_MAX = 4096
+
+
+def _sig(t: Optional[torch.Tensor]):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
+def _remember(key: tuple, call: tuple) -> tuple:
+    if len(_CALLS) >= _CALLS_MAX:
+        _CALLS.clear()
+    _CALLS[key] = call
+    return call
+
+
+def _ptr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _launch(index: int, fn, *args) -> None:
+    """fn(*args, the current stream of device `index`), with that device current."""
+    if torch.cuda.current_device() == index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status != _lib.BSG_OK:
+        check(status)
+
+
+def _workspace(index: int, nbytes: int, prefix: Optional[str], cleared: bool = True) -> torch.Tensor:
     """At least `nbytes`, the first COUNTER_BYTES of them zero (the kernels leave them zero).
 
     Without a prefix an eager call takes the buffer of its stream, which calls on that stream use in
     turn, and a captured one a buffer of its own in the graph's memory, its counters cleared by the
-    graph: graphs may then replay beside each other.  With a prefix both take the prefix's buffer,
-    and calls that may overlap must not share one.  A buffer is never given back while a graph may
-    hold it: a larger one is made beside it."""
-    if prefix is None and torch.cuda.is_current_stream_capturing():
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        ws[:COUNTER_BYTES].zero_()
-        return ws
-    key = (dev.index, stream) if prefix is None else (dev.index, prefix)
+    graph (where `cleared`): graphs may then replay beside each other.  With a prefix both take the
+    prefix's buffer, and calls that may overlap must not share one.  A buffer is never given back while
+    a graph may hold it: a larger one is made beside it."""
+    key = (index, torch._C._cuda_getCurrentRawStream(index)) if prefix is None else (index, prefix)
+    if torch.cuda.is_current_stream_capturing():
+        if prefix is None:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+            if cleared:
+                ws[:COUNTER_BYTES].zero_()
+            return ws
+        held = _WORKSPACES.get(key)
+        if not held or held[-1].numel() < nbytes:
+            raise RuntimeError(f"workspace {prefix!r} is too small for this call: run it once before capturing it")
+        return held[-1]
     held = _WORKSPACES.setdefault(key, [])
     if not held or held[-1].numel() < nbytes:
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError(f"workspace {prefix!r} is too small for this call: run it once before capturing it")
-        held.append(torch.zeros(1 << max(20, (nbytes - 1).bit_length()), dtype=torch.uint8, device=dev))
+        held.append(torch.zeros(1 << max(20, (nbytes - 1).bit_length()), dtype=torch.uint8, device=torch.device("cuda", index)))
     return held[-1]
 
 
@@ -103,15 +138,13 @@ def _storage(pages: torch.Tensor, scales: torch.Tensor, dims: int) -> torch.devi
 
 
 def _layer(pages: torch.Tensor, scales: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor):
-    """The device and bsg_kv_cache of one layer's tensors."""
+    """The device of one layer's tensors, and the sizes of its bsg_kv_cache."""
     dev = _storage(pages, scales, 5)
     _table(page_table, dev)
     n, h, _, p, d = pages.shape
     slots, each = page_table.shape
-    cache = _lib.KvCache(pages.data_ptr(), scales.data_ptr(), n, h, p, d, slots, each,
-                         page_table.stride(0) if slots > 1 else each, page_table.data_ptr(),
-                         _i32(lengths, dev, "lengths", slots))
-    return dev, cache
+    _i32(lengths, dev, "lengths", slots)
+    return dev, (n, h, p, d, slots, each, page_table.stride(0) if slots > 1 else each)
 
 
 def _batch(x: torch.Tensor, what: str, heads: int, d: int, dev: torch.device, rows: int, cu, max_new) -> int:
@@ -149,18 +182,23 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, scales: tor
     magnitude to 448 or below, and no less than the scale of tokens that the page held before (which
     are rounded again where it grows).  Infinities become +-448 x scale, NaN stays NaN.  max_new bounds
     the tokens of one sequence (default: all of them; a tight one makes a smaller launch)."""
-    dev, cache = _layer(pages, scales, page_table, lengths)
-    rows = _rows(slots, cu_seqlens, lengths)
-    h, d = cache.n_heads, cache.head_dim
-    max_new = _batch(k, "k", h, d, dev, rows, cu_seqlens, max_new)
-    _batch(v, "v", h, d, dev, rows, cu_seqlens, None if cu_seqlens is None else max_new)
-    if v.dtype is not k.dtype or v.shape[0] != k.shape[0]:
-        raise ValueError(f"k and v must match, got {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
-    cu = _i32(cu_seqlens, dev, "cu_seqlens", rows + 1)
-    with torch.cuda.device(dev):
-        check(load().bsg_kv_append(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                                   k.shape[0], ctypes.byref(cache), _i32(slots, dev, "slots"), rows, cu, max_new,
-                                   _dtype_code(k), _stream_handle(dev)))
+    key = ("append", _sig(k), _sig(v), _sig(pages), _sig(scales), _sig(page_table), _sig(lengths), _sig(cu_seqlens), _sig(slots),
+           max_new)
+    call = _CALLS.get(key)
+    if call is None:
+        dev, sizes = _layer(pages, scales, page_table, lengths)
+        rows = _rows(slots, cu_seqlens, lengths)
+        most = _batch(k, "k", sizes[1], sizes[3], dev, rows, cu_seqlens, max_new)
+        _batch(v, "v", sizes[1], sizes[3], dev, rows, cu_seqlens, None if cu_seqlens is None else most)
+        if v.dtype is not k.dtype or v.shape[0] != k.shape[0]:
+            raise ValueError(f"k and v must match, got {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
+        _i32(cu_seqlens, dev, "cu_seqlens", rows + 1)
+        _i32(slots, dev, "slots")
+        call = _remember(key, (dev.index, load().bsg_kv_append, sizes, rows, most, _dtype_code(k), k.stride(0), k.stride(1),
+                               v.stride(0), v.stride(1), k.shape[0]))
+    index, fn, sizes, rows, most, code, kt, kh, vt, vh, tokens = call
+    cache = _lib.KvCache(pages.data_ptr(), scales.data_ptr(), *sizes, page_table.data_ptr(), lengths.data_ptr())
+    _launch(index, fn, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, tokens, cache, _ptr(slots), rows, _ptr(cu_seqlens), most, code)
 
 
 def kv_attention(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, page_table: torch.Tensor,
@@ -177,70 +215,93 @@ def kv_attention(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, pag
     1 / sqrt(head_dim) by default.  max_len, the longest sequence (default: what a table row holds),
     decides how the long axis is split and bounds nothing.  q rows must be 16-byte aligned, out rows
     8-byte aligned."""
-    dev, cache = _layer(pages, scales, page_table, lengths)
-    rows = _rows(slots, cu_seqlens, lengths)
-    max_new = _batch(q, "q", 0, cache.head_dim, dev, rows, cu_seqlens, max_new)
-    code = _dtype_code(q)
-    tokens, heads, d = q.shape
+    key = ("attend", _sig(q), _sig(pages), _sig(scales), _sig(page_table), _sig(lengths), _sig(cu_seqlens), _sig(slots), _sig(out),
+           _sig(lse), max_new, max_len)
+    call = _CALLS.get(key)
+    if call is None:
+        call = _remember(key, _attention_call(q, pages, scales, page_table, lengths, cu_seqlens, max_new, slots, max_len, out, lse))
+    index, fn, sizes, rows, most, code, qt, qh, shape, longest, need, cus, scale = call
     if out is None:
-        out = torch.empty((tokens, heads, d), dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype is not q.dtype or out.device != dev or out.stride(2) != 1:
-        raise ValueError(f"out must match q {tuple(q.shape)} {q.dtype} with contiguous channels, got {tuple(out.shape)} {out.dtype}")
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
     if lse is None:
-        lse = torch.empty((tokens, heads), dtype=torch.float32, device=dev)
-    elif lse.shape != q.shape[:2] or lse.dtype is not torch.float32 or lse.device != dev or not lse.is_contiguous():
-        raise ValueError(f"lse must be contiguous float32 [{tokens}, {heads}] on {dev}")
-    cu = _i32(cu_seqlens, dev, "cu_seqlens", rows + 1)
-    lib = load()
-    cus = _cu_count(dev)
-    most = 0 if max_len is None else max(1, int(max_len))
-    with torch.cuda.device(dev):
-        stream = _stream_handle(dev)
-        need = lib.bsg_kv_attention_workspace_bytes(ctypes.byref(cache), rows, heads, max_new, most, cus)
-        ws = _workspace(dev, need, workspace_prefix, stream) if need > 0 else None
-        check(lib.bsg_kv_attention(q.data_ptr(), q.stride(0), q.stride(1), tokens, heads, ctypes.byref(cache),
-                                   _i32(slots, dev, "slots"), rows, cu, max_new, most,
-                                   d ** -0.5 if sm_scale is None else float(sm_scale), out.data_ptr(), out.stride(0),
-                                   out.stride(1), lse.data_ptr(), code, ws.data_ptr() if ws is not None else 0,
-                                   ws.numel() if ws is not None else 0, cus, stream))
+        lse = torch.empty(shape[:2], dtype=torch.float32, device=q.device)
+    cache = _lib.KvCache(pages.data_ptr(), scales.data_ptr(), *sizes, page_table.data_ptr(), lengths.data_ptr())
+    ws, room = 0, 0
+    if need > 0:
+        held = _workspace(index, need, workspace_prefix)
+        ws, room = held.data_ptr(), held.numel()
+    _launch(index, fn, q.data_ptr(), qt, qh, shape[0], shape[1], cache, _ptr(slots), rows, _ptr(cu_seqlens), most, longest,
+            scale if sm_scale is None else sm_scale, out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), code, ws, room, cus)
     return out, lse
 
 
-def _pool(page_table=None, lengths=None, refcounts=None, pages=None, scales=None, page_size: int = 1):
-    """The device and bsg_page_pool of what a page call is given."""
-    dev = (page_table if page_table is not None else pages).device
-    if dev.type != "cuda":
-        raise ValueError("a cache's tensors must live on a ROCm (cuda) device")
-    pool = _lib.PagePool()
-    if pages is not None:
-        _storage(pages, scales, 6)
-        if pages.device != dev:
-            raise ValueError(f"pages must be on {dev}, got {pages.device}")
-        layers, n, h, _, p, d = pages.shape
-        pool.pages, pool.scales, pool.layers, pool.num_pages = pages.data_ptr(), scales.data_ptr(), layers, n
-        pool.page_bytes, pool.page_scales, pool.page_size = h * 2 * p * d, h * 2, p
-    else:
-        pool.page_size = page_size
-    if page_table is not None:
-        _table(page_table, dev)
-        slots, each = page_table.shape
-        pool.page_table, pool.num_slots, pool.max_pages = page_table.data_ptr(), slots, each
-        pool.table_stride = page_table.stride(0) if slots > 1 else each
-        if lengths is not None:
-            pool.lengths = _i32(lengths, dev, "lengths", slots)
-        pool.refcounts = _i32(refcounts, dev, "refcounts", None if pages is None else pages.shape[1])
-        pool.num_pages = refcounts.numel()
-    return dev, pool
+def _attention_call(q, pages, scales, page_table, lengths, cu_seqlens, max_new, slots, max_len, out, lse) -> tuple:
+    """The checks of kv_attention and what follows from its arguments' shapes."""
+    dev, sizes = _layer(pages, scales, page_table, lengths)
+    rows = _rows(slots, cu_seqlens, lengths)
+    most = _batch(q, "q", 0, sizes[3], dev, rows, cu_seqlens, max_new)
+    code = _dtype_code(q)
+    tokens, heads, d = q.shape
+    if out is not None and (out.shape != q.shape or out.dtype is not q.dtype or out.device != dev or out.stride(2) != 1):
+        raise ValueError(f"out must match q {tuple(q.shape)} {q.dtype} with contiguous channels, got {tuple(out.shape)} {out.dtype}")
+    if lse is not None and (lse.shape != q.shape[:2] or lse.dtype is not torch.float32 or lse.device != dev
+                            or not lse.is_contiguous()):
+        raise ValueError(f"lse must be contiguous float32 [{tokens}, {heads}] on {dev}")
+    _i32(cu_seqlens, dev, "cu_seqlens", rows + 1)
+    _i32(slots, dev, "slots")
+    lib, cus = load(), _cu_count(dev)
+    longest = 0 if max_len is None else max(1, int(max_len))
+    cache = _lib.KvCache(pages.data_ptr(), scales.data_ptr(), *sizes, page_table.data_ptr(), lengths.data_ptr())
+    need = int(lib.bsg_kv_attention_workspace_bytes(cache, rows, heads, most, longest, cus))
+    return (dev.index, lib.bsg_kv_attention, sizes, rows, most, code, q.stride(0), q.stride(1), tuple(q.shape), longest, need, cus,
+            d ** -0.5)
+
+
+def _pool(kind: str, page_table=None, lengths=None, refcounts=None, pages=None, scales=None, *others):
+    """The device index of what a page call is given, and its bsg_page_pool; `others` are int32 tensors
+    of the call."""
+    key = (kind, _sig(page_table), _sig(lengths), _sig(refcounts), _sig(pages), _sig(scales), *[_sig(t) for t in others])
+    call = _CALLS.get(key)
+    if call is None:
+        dev = (page_table if page_table is not None else pages).device
+        if dev.type != "cuda":
+            raise ValueError("a cache's tensors must live on a ROCm (cuda) device")
+        layers = page_bytes = page_scales = slots = each = stride = 0
+        page_size = 1
+        if pages is not None:
+            _storage(pages, scales, 6)
+            if pages.device != dev:
+                raise ValueError(f"pages must be on {dev}, got {pages.device}")
+            layers, count, h, _, page_size, d = pages.shape
+            page_bytes, page_scales = h * 2 * page_size * d, h * 2
+        if page_table is not None:
+            _table(page_table, dev)
+            slots, each = page_table.shape
+            stride = page_table.stride(0) if slots > 1 else each
+            _i32(lengths, dev, "lengths", slots)
+            _i32(refcounts, dev, "refcounts", None if pages is None else pages.shape[1])
+            count = refcounts.numel()
+        for i, t in enumerate(others):
+            _i32(t, dev, f"argument {i}")
+        call = _remember(key, (dev.index, (layers, count, page_bytes, page_scales, page_size, slots, each, stride)))
+    index, sizes = call
+    pool = _lib.PagePool(_ptr(pages), _ptr(scales), *sizes, _ptr(page_table), _ptr(lengths), _ptr(refcounts))
+    return index, pool
+
+
+def _same(n: int, **others) -> None:
+    for what, t in others.items():
+        if t is not None and t.numel() != n:
+            raise ValueError(f"{what} has {t.numel()} entries, needs {n}")
 
 
 def pages_copy(pages: torch.Tensor, scales: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
     """Copy pages src[i] -> dst[i] (int32) with their scales in every layer of pages [layers, pages,
     heads, 2, page_size, head_dim].  Pairs with an id out of range are skipped.  No page may be
     written twice, or both read and written, in one call."""
-    dev, pool = _pool(pages=pages, scales=scales)
-    s = _i32(src, dev, "src")
-    with torch.cuda.device(dev):
-        check(load().bsg_pages_copy(ctypes.byref(pool), s, _i32(dst, dev, "dst", src.numel()), src.numel(), _stream_handle(dev)))
+    index, pool = _pool("copy", None, None, None, pages, scales, src, dst)
+    _same(src.numel(), dst=dst)
+    _launch(index, load().bsg_pages_copy, pool, src.data_ptr(), dst.data_ptr(), src.numel())
 
 
 def pages_fork(page_table: torch.Tensor, lengths: torch.Tensor, refcounts: torch.Tensor, parents: torch.Tensor,
@@ -249,11 +310,9 @@ def pages_fork(page_table: torch.Tensor, lengths: torch.Tensor, refcounts: torch
     share, and its length, and releases what it held.  All pairs at once, so that a reordering of
     beams is one call.  Pairs with a slot out of range are skipped; of pairs with the same child the
     last one counts.  At most 1024 pairs."""
-    dev, pool = _pool(page_table, lengths, refcounts)
-    a = _i32(parents, dev, "parents")
-    with torch.cuda.device(dev):
-        check(load().bsg_pages_fork(ctypes.byref(pool), a, _i32(children, dev, "children", parents.numel()),
-                                    parents.numel(), _stream_handle(dev)))
+    index, pool = _pool("fork", page_table, lengths, refcounts, None, None, parents, children)
+    _same(parents.numel(), children=children)
+    _launch(index, load().bsg_pages_fork, pool, parents.data_ptr(), children.data_ptr(), parents.numel())
 
 
 def pages_extend(pages: torch.Tensor, scales: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
@@ -267,50 +326,39 @@ def pages_extend(pages: torch.Tensor, scales: torch.Tensor, page_table: torch.Te
     table row is too short, or the free pages do not reach.  Rows are served in order until the first
     that they do not reach; of the later ones only those that need no page and write to no shared
     one.  Slots must be distinct; at most 1024 rows."""
-    dev, pool = _pool(page_table, lengths, refcounts, pages, scales)
     n = new_tokens.numel()
-    add = _i32(new_tokens, dev, "new_tokens")
-    at = _i32(slots, dev, "slots", n)
     if served is None:
-        served = torch.empty(n, dtype=torch.int32, device=dev)
-    lib = load()
-    with torch.cuda.device(dev):
-        stream = _stream_handle(dev)
-        ws = _plan_workspace(lib, dev, pool.num_pages, workspace_prefix, stream)
-        check(lib.bsg_pages_extend(ctypes.byref(pool), at, add, n, _i32(served, dev, "served", n), ws.data_ptr(),
-                                   ws.numel(), stream))
+        served = torch.empty(n, dtype=torch.int32, device=new_tokens.device)
+    index, pool = _pool("extend", page_table, lengths, refcounts, pages, scales, new_tokens, slots, served)
+    _same(n, slots=slots, served=served)
+    ws = _plan_workspace(index, pool.num_pages, workspace_prefix)
+    _launch(index, load().bsg_pages_extend, pool, _ptr(slots), new_tokens.data_ptr(), n, served.data_ptr(), ws.data_ptr(), ws.numel())
     return served
 
 
-def _plan_workspace(lib, dev, num_pages: int, prefix: Optional[str], stream: int) -> torch.Tensor:
-    need = int(lib.bsg_pages_workspace_bytes(num_pages))
-    if prefix is None and torch.cuda.is_current_stream_capturing():
-        return torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-    # its lists lie past the counters that other calls need zero
-    return _workspace(dev, COUNTER_BYTES + need, prefix, stream)[COUNTER_BYTES:]
+def _plan_workspace(index: int, num_pages: int, prefix: Optional[str]) -> torch.Tensor:
+    """Room for a plan's lists, past the counters that other calls need zero."""
+    need = int(load().bsg_pages_workspace_bytes(num_pages))
+    return _workspace(index, COUNTER_BYTES + need, prefix, cleared=False)[COUNTER_BYTES:]
 
 
 def pages_free(page_table: torch.Tensor, lengths: torch.Tensor, refcounts: torch.Tensor, slots: torch.Tensor) -> None:
     """Release every page of the given slots (int32): their table rows become -1, their lengths 0.
     Slots out of range are skipped, one named twice is released once.  At most 1024 slots."""
-    dev, pool = _pool(page_table, lengths, refcounts)
-    at = _i32(slots, dev, "slots")
-    with torch.cuda.device(dev):
-        check(load().bsg_pages_free(ctypes.byref(pool), at, slots.numel(), _stream_handle(dev)))
+    index, pool = _pool("free", page_table, lengths, refcounts, None, None, slots)
+    _launch(index, load().bsg_pages_free, pool, slots.data_ptr(), slots.numel())
 
 
 def pages_compact(pages: torch.Tensor, scales: torch.Tensor, page_table: torch.Tensor, refcounts: torch.Tensor,
                   counts: Optional[torch.Tensor] = None, workspace_prefix: Optional[str] = None) -> torch.Tensor:
     """Make the pool dense: the live pages past the first `live` ids move, in order, to the free
     ids before, and every entry of page_table (all slots) follows.  Returns counts, int32 [live, moved]."""
-    dev, pool = _pool(page_table, None, refcounts, pages, scales)
     if counts is None:
-        counts = torch.empty(2, dtype=torch.int32, device=dev)
-    lib = load()
-    with torch.cuda.device(dev):
-        stream = _stream_handle(dev)
-        ws = _plan_workspace(lib, dev, pool.num_pages, workspace_prefix, stream)
-        check(lib.bsg_pages_compact(ctypes.byref(pool), _i32(counts, dev, "counts", 2), ws.data_ptr(), ws.numel(), stream))
+        counts = torch.empty(2, dtype=torch.int32, device=page_table.device)
+    index, pool = _pool("compact", page_table, None, refcounts, pages, scales, counts)
+    _same(2, counts=counts)
+    ws = _plan_workspace(index, pool.num_pages, workspace_prefix)
+    _launch(index, load().bsg_pages_compact, pool, counts.data_ptr(), ws.data_ptr(), ws.numel())
     return counts
 
 
@@ -332,6 +380,26 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0,
     A token outside the vocabulary gives NaN.  A row of nothing but -inf gives -inf, entropy 0 and the
     lowest ids; a NaN or +inf in a row makes its numbers NaN (NaN ranks first among the ids, -0 equals
     +0)."""
+    key = ("logprobs", _sig(logits), _sig(tokens), k)
+    call = _CALLS.get(key)
+    if call is None:
+        call = _remember(key, _logprobs_call(logits, tokens, k))
+    index, fn, rows, vocab, stride, k, code, need, cus = call
+    dev = logits.device
+    out = TokenLogprobs(torch.empty(rows, dtype=torch.float32, device=dev), torch.empty(rows, dtype=torch.float32, device=dev),
+                        torch.empty((rows, k), dtype=torch.int32, device=dev),
+                        torch.empty((rows, k), dtype=torch.float32, device=dev))
+    ws, room = 0, 0
+    if need > 0:
+        held = _workspace(index, need, workspace_prefix)
+        ws, room = held.data_ptr(), held.numel()
+    _launch(index, fn, logits.data_ptr(), stride, rows, vocab, tokens.data_ptr(), k, out[0].data_ptr(), out[1].data_ptr(),
+            out[2].data_ptr(), out[3].data_ptr(), code, ws, room, cus)
+    return out
+
+
+def _logprobs_call(logits: torch.Tensor, tokens: torch.Tensor, k: int) -> tuple:
+    """The checks of token_logprobs and what follows from its arguments' shapes."""
     dev = _require_cuda(logits)
     if logits.dtype not in _LOGIT_DTYPES:
         raise TypeError(f"logits must be float16, bfloat16 or float32, got {logits.dtype}")
@@ -343,22 +411,11 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0,
     k = int(k)
     if not 0 <= k <= min(MAX_ALTERNATIVES, vocab):
         raise ValueError(f"k={k} (0 to {min(MAX_ALTERNATIVES, vocab)})")
-    out = TokenLogprobs(torch.empty(rows, dtype=torch.float32, device=dev), torch.empty(rows, dtype=torch.float32, device=dev),
-                        torch.empty((rows, k), dtype=torch.int32, device=dev),
-                        torch.empty((rows, k), dtype=torch.float32, device=dev))
-    at = _i32(tokens, dev, "tokens", rows)
+    _i32(tokens, dev, "tokens", rows)
     code = _LOGIT_DTYPES[logits.dtype]
-    lib = load()
-    cus = _cu_count(dev)
-    with torch.cuda.device(dev):
-        stream = _stream_handle(dev)
-        need = lib.bsg_token_logprobs_workspace_bytes(rows, vocab, k, code, cus)
-        ws = _workspace(dev, need, workspace_prefix, stream) if need > 0 else None
-        check(lib.bsg_token_logprobs(logits.data_ptr(), logits.stride(0), rows, vocab, at, k, out.logprob.data_ptr(),
-                                     out.entropy.data_ptr(), out.top_ids.data_ptr(), out.top_logprobs.data_ptr(), code,
-                                     ws.data_ptr() if ws is not None else 0, ws.numel() if ws is not None else 0, cus,
-                                     stream))
-    return out
+    lib, cus = load(), _cu_count(dev)
+    need = int(lib.bsg_token_logprobs_workspace_bytes(rows, vocab, k, code, cus))
+    return dev.index, lib.bsg_token_logprobs, rows, vocab, logits.stride(0), k, code, need, cus
 
 
 def read_pages(pages: torch.Tensor, scales: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -1,13 +1,16 @@
 // logprobs.hip — log probabilities of given tokens, entropies and the likeliest alternatives of rows of
 // logits, in one pass over them (include/bsgserve.h).
 //
-// With M the running maximum of a row, l = sum 2^d and t = sum 2^d d over d = (x - M) log2(e):
-//   lse = M + ln l,  logprob = (x_token - M) - ln l,  entropy = ln 2 (log2 l - t / l).
+// With M the running maximum of a row, d = (x - M) log2(e), l = sum 2^d and t = sum 2^d d:
+//   logprob = (x_token - M) - ln l,  entropy = ln 2 (log2 l - t / l).
+//
 // The alternatives are found beside it.  A logit's key is its order among fp32 numbers (upper half) and
-// its id's complement (lower half), so that keys are distinct and (logit desc, id asc) is key desc.  The k
-// best keys so far wait in LDS; a tile of logits in registers adds to them what passes a threshold
-// that at least k keys reach: the worst of the k, or on the first tile the k-th largest of some
-// wave's 64 lane maxima.
+// its id's complement (lower half), so that keys are distinct and (logit desc, id asc) is key desc.
+// The unit of work is a wave: it keeps the 64 best keys of its slice sorted, one per lane, and
+// compares what it reads with the k-th of them; what passes waits in LDS and is merged 64 at a time by
+// bitonic networks over DPP moves.  Before the first tile there is nothing to compare with: the k-th
+// largest of the lanes' own maxima is a bound that at least k logits reach.  Waves of a row meet in
+// LDS, two lists at a time; no barrier before that.
 
 #include "serve.hpp"
 
@@ -15,9 +18,11 @@ using namespace bsgk;
 
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kVectors = 4;     // 16-byte vectors of a thread and tile
-constexpr int kList = 1024;     // candidates of one round; more of them take the search by bits
+constexpr int kVectors = 2;     // 16-byte vectors of a lane and tile
+constexpr int kAhead = 2;       // tiles in flight beside the one at work
+constexpr int kWaves = 4;       // of a work-group
+constexpr int kInsert = 8;      // keys up to which inserting one by one is quicker than a sort
+constexpr int kSplitTiles = 2;  // tiles of a wave that a split of a long row leaves
 constexpr int kMaxK = BSG_LOGPROBS_MAX_K;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kFloor = -1e4f;  // exponents below it weigh nothing; keeps 0 x -inf out of t
@@ -33,7 +38,7 @@ struct ScoreParams {
   uint64_t* keys;      // [rows][splits][k]
   float* sums;         // [rows][splits][4]
   int64_t stride, vocab, split_vectors;
-  int32_t k, splits;
+  int32_t rows, k, splits, log_waves;  // waves of a row and split: 1 << log_waves
 };
 
 template <typename T>
@@ -71,6 +76,64 @@ __device__ __forceinline__ float from_order(uint32_t o) {
 }
 __device__ __forceinline__ uint64_t key_of(uint32_t order, uint32_t id) { return (uint64_t)order << 32 | (uint32_t)~id; }
 
+// The value of lane ^ X.
+template <int X>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+  if constexpr (X == 1) return __builtin_amdgcn_mov_dpp(v, 0xb1, 0xf, 0xf, true);   // quad_perm 1 0 3 2
+  if constexpr (X == 2) return __builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, true);   // quad_perm 2 3 0 1
+  if constexpr (X == 4) {                                                           // 7 - i, then 3 - i in quads
+    v = __builtin_amdgcn_mov_dpp(v, 0x141, 0xf, 0xf, true);
+    return __builtin_amdgcn_mov_dpp(v, 0x1b, 0xf, 0xf, true);
+  }
+  if constexpr (X == 8) return __builtin_amdgcn_mov_dpp(v, 0x128, 0xf, 0xf, true);  // row_ror:8
+  if constexpr (X == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return threadIdx.x & 16 ? r[0] : r[1];
+  }
+  if constexpr (X == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return threadIdx.x & 32 ? r[0] : r[1];
+  }
+}
+template <int X>
+__device__ __forceinline__ float lane_xor(float v) {
+  return as_float(lane_xor<X>(__builtin_bit_cast(uint32_t, v)));
+}
+template <int X>
+__device__ __forceinline__ uint64_t lane_xor(uint64_t v) {
+  return (uint64_t)lane_xor<X>((uint32_t)(v >> 32)) << 32 | lane_xor<X>((uint32_t)v);
+}
+
+// One step of a bitonic network of one value per lane: blocks of N sorted, every second the other
+// way round, the last (N = 64) largest first.
+template <int N, int X, typename V>
+__device__ __forceinline__ V exchange(V v) {
+  const V o = lane_xor<X>(v);
+  const bool larger = ((threadIdx.x & X) == 0) == (N == 64 || (threadIdx.x & N) == 0);
+  return (v > o) == larger ? v : o;
+}
+template <int N, int X, typename V>
+__device__ __forceinline__ V merge_steps(V v) {
+  v = exchange<N, X>(v);
+  if constexpr (X > 1) v = merge_steps<N, X / 2>(v);
+  return v;
+}
+template <int N, typename V>
+__device__ __forceinline__ V sort_steps(V v) {
+  if constexpr (N > 2) v = sort_steps<N / 2>(v);
+  return merge_steps<N, N / 2>(v);
+}
+template <typename V>
+__device__ __forceinline__ V sorted(V v) {
+  return sort_steps<64>(v);
+}
+// The 64 largest of two lists, both largest first.
+__device__ __forceinline__ uint64_t merged(uint64_t a, uint64_t b) {
+  // b the other way round: lane 63 - i
+  b = lane_xor<32>(lane_xor<16>(lane_xor<8>(lane_xor<4>(lane_xor<2>(lane_xor<1>(b))))));
+  return merge_steps<64, 32>(a > b ? a : b);
+}
+
 struct Sums {
   float m, l, t;
 };
@@ -81,237 +144,256 @@ __device__ __forceinline__ Sums join(Sums a, Sums b) {
   const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
   return Sums{m, a.l * fa + b.l * fb, fa * (a.t + a.l * da) + fb * (b.t + b.l * db)};
 }
+template <int X>
+__device__ __forceinline__ Sums join_lanes(Sums s) {
+  s = join(s, Sums{lane_xor<X>(s.m), lane_xor<X>(s.l), lane_xor<X>(s.t)});
+  if constexpr (X < 32) s = join_lanes<2 * X>(s);
+  return s;
+}
 
-// The k-th largest (from 1) of the wave's 64 values: a bitonic sort of one value per lane, largest first.
-__device__ __forceinline__ uint32_t wave_kth(uint32_t v, int k) {
+// What a wave keeps of its slice.
+struct Best {
+  uint64_t list;    // lane i: the i-th best key so far (0: none)
+  uint64_t* wait;   // 128 keys of LDS, and a tile behind them
+  int waiting;      // of them in use, below 64 between calls
+  uint32_t bar;     // order that at least k logits of the slice so far reach; 0: fewer than k so far
+
+  // What waits goes into the list: a few keys one after the other, many by a sort.
+  __device__ __forceinline__ void settle(int k) {
+    const int lane = threadIdx.x & 63;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const uint64_t v = lane < waiting ? wait[lane] : 0;
+    const uint64_t rest = wait[64 + lane];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (waiting <= kInsert) {
+      for (int i = 0; i < waiting; ++i) {
+        const uint64_t key = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), i) << 32 |
+                             (uint32_t)__builtin_amdgcn_readlane((int)v, i);
+        const int at = __popcll(__ballot(list > key));
+        const uint64_t above = (uint64_t)(uint32_t)__builtin_amdgcn_mov_dpp((int)(list >> 32), 0x138, 0xf, 0xf, true) << 32 |
+                               (uint32_t)__builtin_amdgcn_mov_dpp((int)list, 0x138, 0xf, 0xf, true);  // wave_shr:1
+        list = lane < at ? list : lane == at ? key : above;
+      }
+      waiting = 0;
+    } else {
+      if (waiting > 64 && lane < waiting - 64) wait[lane] = rest;
+      waiting = waiting > 64 ? waiting - 64 : 0;
+      list = merged(list, sorted(v));
+    }
+    const uint32_t kth = (uint32_t)__builtin_amdgcn_readlane((int)(list >> 32), k - 1);
+    bar = bar > kth ? bar : kth;
+  }
+  __device__ __forceinline__ void add(bool take, uint64_t key) {
+    const uint64_t who = __ballot(take);
+    const int at = waiting + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u));
+    if (take) wait[at] = key;
+    waiting += __popcll(who);
+  }
+};
+
+template <typename T>
+struct Tile {
+  u32x4 raw[kVectors];
+  uint32_t valid[kVectors];  // one bit per element
+};
+
+template <typename T>
+__device__ __forceinline__ void load_tile(Tile<T>& tile, const T* x, int64_t v0, int64_t v_end, int skip, int64_t vocab) {
+  constexpr int N = Logit<T>::N;
   const int lane = threadIdx.x & 63;
 #pragma unroll
-  for (int n = 2; n <= 64; n <<= 1)
+  for (int i = 0; i < kVectors; ++i) {
+    const int64_t v = v0 + 64 * i + lane;
+    const int64_t e = v * N - skip;
+    tile.valid[i] = 0;
+    tile.raw[i] = u32x4{0u, 0u, 0u, 0u};
+    if (v < v_end) {
+      if (e >= 0 && e + N <= vocab) {
+        tile.raw[i] = __builtin_nontemporal_load((const u32x4*)(x + e));
+        tile.valid[i] = (1u << N) - 1u;
+      } else {
 #pragma unroll
-    for (int j = n >> 1; j > 0; j >>= 1) {
-      const uint32_t o = __shfl_xor(v, j);
-      const bool larger = ((lane & j) == 0) == ((lane & n) == 0 || n == 64);
-      v = larger ? (v > o ? v : o) : (v < o ? v : o);
+        for (int j = 0; j < N; ++j)
+          if (e + j >= 0 && e + j < vocab) {
+            tile.valid[i] |= 1u << j;
+            if constexpr (sizeof(T) == 4)
+              tile.raw[i][j] = ((const uint32_t*)x)[e + j];
+            else
+              tile.raw[i][j >> 1] |= (uint32_t)((const uint16_t*)x)[e + j] << (16 * (j & 1));
+          }
+      }
     }
-  return __builtin_amdgcn_readlane(v, k - 1);
+  }
+}
+
+// A tile into the sums and the alternatives.  FULL: every element is there.
+template <typename T, bool FULL>
+__device__ __forceinline__ void take_tile(const Tile<T>& tile, int64_t id0, int k, bool first, Sums& sum, Best& best) {
+  typedef Logit<T> L;
+  constexpr int N = L::N;
+  const int lane = threadIdx.x & 63;
+  const auto there = [&](int i, int j) { return FULL || (tile.valid[i] >> j & 1u) != 0; };
+  const auto logit = [&](int i, int j) { return there(i, j) ? L::at(tile.raw[i], j) : -__builtin_inff(); };
+
+  float top = -__builtin_inff();
+#pragma unroll
+  for (int i = 0; i < kVectors; ++i)
+#pragma unroll
+    for (int j = 0; j < N; ++j) top = fmaxf(top, logit(i, j));
+  const float base = top == -__builtin_inff() ? 0.f : top;
+  float l = 0.f, t = 0.f;
+#pragma unroll
+  for (int i = 0; i < kVectors; ++i)
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float d = (logit(i, j) - base) * kLog2e;
+      const float e = __builtin_amdgcn_exp2f(d);
+      l += e;
+      t = __builtin_fmaf(e, fmaxf(d, kFloor), t);
+    }
+  sum = join(sum, Sums{top, l, t});
+  if (k == 0) return;
+
+  if (first) {
+    uint32_t mine = order_of(top);
+    if (!FULL) {
+      uint32_t any = 0;
+#pragma unroll
+      for (int i = 0; i < kVectors; ++i) any |= tile.valid[i];
+      if (any == 0) mine = 0;
+    }
+    if (l != l) {  // a NaN or +inf among them
+#pragma unroll
+      for (int i = 0; i < kVectors; ++i)
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (there(i, j) && L::at(tile.raw[i], j) != L::at(tile.raw[i], j)) mine = 0xffffffffu;
+    }
+    // what equals the bar enters too: of the k at or above it the ids are not known
+    const uint32_t kth = (uint32_t)__builtin_amdgcn_readlane((int)sorted(mine), k - 1);
+    best.bar = kth < 2 ? 0 : kth - (kth == 0x80000000u ? 2 : 1);  // below +0 comes -0, its equal
+  }
+  // The bar as a number; what is above it enters, and a NaN.  No number is above a bar of +inf, every
+  // one above a bar of NaN, which stands for fewer than k keys so far.
+  const float bar = best.bar == 0 ? __builtin_nanf("") : best.bar >= 0xff800000u ? __builtin_inff() : from_order(best.bar);
+  if (!__any(!(top <= bar) || l != l)) return;
+
+  // Few enter; each lane takes its own one at a time, by position, from a copy of the tile in LDS.
+  uint32_t mask = 0;
+#pragma unroll
+  for (int i = 0; i < kVectors; ++i)
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (there(i, j) && !(L::at(tile.raw[i], j) <= bar)) mask |= 1u << (i * N + j);
+  u32x4* const copy = (u32x4*)(best.wait + 128);
+#pragma unroll
+  for (int i = 0; i < kVectors; ++i) copy[64 * i + lane] = tile.raw[i];
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  while (__any(mask != 0)) {
+    const int bit = mask != 0 ? __builtin_ctz(mask) : 0;
+    const int e = (64 * (bit / N) + lane) * N + bit % N;
+    best.add(mask != 0, key_of(order_of((float)((const T*)copy)[e]), (uint32_t)(id0 + e)));
+    mask &= mask - 1;
+    if (best.waiting >= 64) best.settle(k);
+  }
+  if (best.waiting > 0) best.settle(k);
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void bsg_token_logprobs_kernel(ScoreParams p) {
+__global__ __launch_bounds__(64 * kWaves) void bsg_token_logprobs_kernel(ScoreParams p) {
   typedef Logit<T> L;
   constexpr int N = L::N;
-  __shared__ uint64_t s_list[kList + kMaxK];
-  __shared__ uint64_t s_top[kMaxK];
-  __shared__ uint32_t s_tau[kWaves];
+  __shared__ alignas(16) uint64_t s_wait[kWaves][128 + 2 * 64 * kVectors];
   __shared__ Sums s_sum[kWaves];
-  __shared__ uint32_t s_counts[2], s_last;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t row = blockIdx.y;
-  const T* const x = (const T*)p.x + row * p.stride;
+  __shared__ uint32_t s_last;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int W = 1 << p.log_waves, part = wave & (W - 1);
+  const int64_t row = (int64_t)blockIdx.y * (blockDim.x >> (6 + p.log_waves)) + (wave >> p.log_waves);
+  const bool real = row < p.rows;
+  const T* const x = (const T*)p.x + (real ? row : 0) * p.stride;
+  const int k = p.k;
+  const int32_t token = real ? p.tokens[row] : -1;
+
   // 16-byte vectors from the granule in which the row begins: its element i is at i + skip
   const int skip = (int)(((uintptr_t)x & 15u) / sizeof(T));
-  const int64_t vectors = (p.vocab + skip + N - 1) / N;
-  const int64_t v_begin = (int64_t)blockIdx.x * p.split_vectors;
-  const int64_t v_end = v_begin + p.split_vectors < vectors ? v_begin + p.split_vectors : vectors;
-  const int k = p.k;
+  const int64_t vectors = real ? (p.vocab + skip + N - 1) / N : 0;
+  const int64_t s_begin = (int64_t)blockIdx.x * p.split_vectors;
+  const int64_t s_end = s_begin + p.split_vectors < vectors ? s_begin + p.split_vectors : vectors;
+  const int64_t per = (p.split_vectors + W - 1) >> p.log_waves;
+  const int64_t v_begin = s_begin + part * per;
+  const int64_t v_end = v_begin + per < s_end ? v_begin + per : s_end;
 
   Sums sum = {-__builtin_inff(), 0.f, 0.f};
-  int have = 0;  // keys in s_top, sorted
-  if (tid < 2) s_counts[tid] = 0;
-  __syncthreads();
-  int turn = 0;
-  for (int64_t v0 = v_begin; v0 < v_end; v0 += kThreads * kVectors) {
-    // counters by turns: threads that go on with nothing found may count again while others still read
-    uint32_t& s_count = s_counts[turn];
-    turn ^= 1;
-    u32x4 raw[kVectors];
-    uint32_t valid[kVectors];  // one bit per element
+  Best best = {0, s_wait[wave], 0, 0};
+  constexpr int STEP = 64 * kVectors;
+  Tile<T> next[kAhead];
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-      const int64_t v = v0 + i * kThreads + tid;
-      const int64_t e = v * N - skip;
-      valid[i] = 0;
-      raw[i] = u32x4{0u, 0u, 0u, 0u};
-      if (v < v_end) {
-        if (e >= 0 && e + N <= p.vocab) {
-          raw[i] = __builtin_nontemporal_load((const u32x4*)(x + e));
-          valid[i] = (1u << N) - 1u;
-        } else {
+  for (int a = 0; a < kAhead; ++a) load_tile(next[a], x, v_begin + a * STEP, v_end, skip, p.vocab);
+  const bool token_there = token >= 0 && token < p.vocab;
+  const float token_logit = token_there ? (float)x[token] : __builtin_nanf("");
+  for (int64_t v0 = v_begin; v0 < v_end; v0 += STEP) {
+    const Tile<T> tile = next[0];
 #pragma unroll
-          for (int j = 0; j < N; ++j)
-            if (e + j >= 0 && e + j < p.vocab) {
-              valid[i] |= 1u << j;
-              if constexpr (sizeof(T) == 4)
-                raw[i][j] = ((const uint32_t*)x)[e + j];
-              else
-                raw[i][j >> 1] |= (uint32_t)((const uint16_t*)x)[e + j] << (16 * (j & 1));
-            }
-        }
-      }
-    }
-    const auto logit = [&](int i, int j) { return valid[i] >> j & 1u ? L::at(raw[i], j) : -__builtin_inff(); };
-    const auto order = [&](int i, int j) { return valid[i] >> j & 1u ? order_of(L::at(raw[i], j)) : 0u; };
-
-    float m = sum.m;
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i)
-#pragma unroll
-      for (int j = 0; j < N; ++j) m = fmaxf(m, logit(i, j));
-    const float base = m == -__builtin_inff() ? 0.f : m;
-    float l = 0.f, t = 0.f;
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i)
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float d = (logit(i, j) - base) * kLog2e;
-        const float e = __builtin_amdgcn_exp2f(d);
-        l += e;
-        t += e * fmaxf(d, kFloor);
-      }
-    sum = join(sum, Sums{m, l, t});
-
-    if (k == 0) continue;
-    uint32_t tau;
-    if (have == k) {
-      tau = (uint32_t)(s_top[k - 1] >> 32);
-    } else {
-      uint32_t best = 0;
-#pragma unroll
-      for (int i = 0; i < kVectors; ++i)
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const uint32_t o = order(i, j);
-          best = best > o ? best : o;
-        }
-      tau = wave_kth(best, k);
-      if (lane == 0) s_tau[wave] = tau;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) tau = tau > s_tau[w] ? tau : s_tau[w];
-    }
-    const uint64_t worst = have == k ? s_top[k - 1] : 0;
-    // positions are taken by an atomic; the ranks below make their order irrelevant
-    int mine = 0;
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i)
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const uint32_t o = order(i, j);
-        mine += o != 0 && o >= tau;
-      }
-    if (mine > 0) {
-      uint32_t at = atomicAdd(&s_count, (uint32_t)mine);
-#pragma unroll
-      for (int i = 0; i < kVectors; ++i)
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const uint32_t o = order(i, j);
-          if (o != 0 && o >= tau) {
-            if (at < kList) s_list[at] = key_of(o, (uint32_t)((v0 + i * kThreads + tid) * N - skip + j));
-            ++at;
-          }
-        }
-    }
-    __syncthreads();
-    int n = (int)s_count;
-    if (n == 0) continue;
-    if (n > kList) {
-      // Too many equal or ascending logits for the list: the k-th largest key, one bit at a time.
-      uint64_t kth = 0;
-      for (int bit = 63; bit >= 0; --bit) {
-        const uint64_t probe = kth | (uint64_t)1 << bit;
-        int c = 0;
-#pragma unroll
-        for (int i = 0; i < kVectors; ++i)
-#pragma unroll
-          for (int j = 0; j < N; ++j) {
-            const uint32_t o = order(i, j);
-            c += o != 0 && key_of(o, (uint32_t)((v0 + i * kThreads + tid) * N - skip + j)) >= probe;
-          }
-        __syncthreads();
-        if (tid == 0) s_count = 0;
-        __syncthreads();
-        if (c > 0) atomicAdd(&s_count, (uint32_t)c);
-        __syncthreads();
-        if ((int)s_count >= k) kth = probe;
-      }
-      __syncthreads();
-      if (tid == 0) s_count = 0;
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < kVectors; ++i)
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const uint32_t o = order(i, j);
-          const uint64_t key = key_of(o, (uint32_t)((v0 + i * kThreads + tid) * N - skip + j));
-          if (o != 0 && key >= kth) s_list[atomicAdd(&s_count, 1u)] = key;
-        }
-      __syncthreads();
-      n = (int)s_count;
-    }
-    if (tid < have) s_list[n + tid] = s_top[tid];
-    __syncthreads();
-    const int all = n + have;
-    for (int e = tid; e < all; e += kThreads) {
-      const uint64_t key = s_list[e];
-      if (key < worst) continue;
-      int rank = 0;
-      for (int i = 0; i < all; ++i) rank += s_list[i] > key;
-      if (rank < k) s_top[rank] = key;
-    }
-    have = all < k ? all : k;
-    if (tid == 0) s_count = 0;
-    __syncthreads();
+    for (int a = 1; a < kAhead; ++a) next[a - 1] = next[a];
+    load_tile(next[kAhead - 1], x, v0 + kAhead * STEP, v_end, skip, p.vocab);
+    const int64_t id0 = v0 * N - skip;
+    const bool first = v0 == v_begin;
+    if (id0 >= 0 && v0 + STEP <= v_end && id0 + STEP * N <= p.vocab)
+      take_tile<T, true>(tile, id0, k, first, sum, best);
+    else
+      take_tile<T, false>(tile, id0, k, first, sum, best);
   }
+  sum = join_lanes<1>(sum);
 
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1)
-    sum = join(sum, Sums{__shfl_xor(sum.m, d), __shfl_xor(sum.l, d), __shfl_xor(sum.t, d)});
-  if (lane == 0) s_sum[wave] = sum;
-  __syncthreads();
-  sum = s_sum[0];
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) sum = join(sum, s_sum[w]);
+  // the waves of a row, two at a time; the lists go through the waves' own LDS
+  const auto meet = [&]() {
+    for (int step = 1; step < W; step <<= 1) {
+      if (part & step) {
+        s_wait[wave][lane] = best.list;
+        if (lane == 0) s_sum[wave] = sum;
+      }
+      __syncthreads();
+      if ((part & (2 * step - 1)) == 0) {
+        if (k > 0) best.list = merged(best.list, s_wait[wave + step][lane]);
+        sum = join(sum, s_sum[wave + step]);
+      }
+    }
+  };
+  meet();
 
   if (p.splits > 1) {
     const int64_t at = row * p.splits + blockIdx.x;
-    if (tid < k) hand_store(p.keys + at * k + tid, tid < have ? s_top[tid] : (uint64_t)0);
-    if (tid == 0) hand_store(p.sums + at * 4, sum.m), hand_store(p.sums + at * 4 + 1, sum.l), hand_store(p.sums + at * 4 + 2, sum.t);
-    hand_publish();
-    __syncthreads();
-    if (tid == 0) s_last = hand_arrive(p.counters + row) == (uint32_t)(p.splits - 1);
-    __syncthreads();
-    if (!s_last) return;
-    if (tid == 0) hand_reset(p.counters + row);
-    const int64_t first = row * p.splits;
-    sum = Sums{-__builtin_inff(), 0.f, 0.f};
-    for (int s = 0; s < p.splits; ++s)
-      sum = join(sum, Sums{hand_load(p.sums + (first + s) * 4), hand_load(p.sums + (first + s) * 4 + 1),
-                           hand_load(p.sums + (first + s) * 4 + 2)});
-    const int all = p.splits * k;  // at most kList
-    if (tid < all) s_list[tid] = hand_load(p.keys + first * k + tid);
-    __syncthreads();
-    if (tid < all && s_list[tid] != 0) {
-      const uint64_t key = s_list[tid];
-      int rank = 0;
-      for (int i = 0; i < all; ++i) rank += s_list[i] > key;
-      if (rank < k) s_top[rank] = key;
+    if (part == 0 && real) {
+      if (lane < k) hand_store(p.keys + at * k + lane, best.list);
+      if (lane == 0) hand_store(p.sums + at * 4, sum.m), hand_store(p.sums + at * 4 + 1, sum.l), hand_store(p.sums + at * 4 + 2, sum.t);
+      hand_publish();
     }
     __syncthreads();
+    if (threadIdx.x == 0) s_last = hand_arrive(p.counters + row) == (uint32_t)(p.splits - 1);
+    __syncthreads();
+    if (!s_last) return;
+    if (threadIdx.x == 0) hand_reset(p.counters + row);
+    sum = Sums{-__builtin_inff(), 0.f, 0.f};
+    best.list = 0;
+    for (int s = part; s < p.splits; s += W) {
+      const int64_t from = row * p.splits + s;
+      if (k > 0) best.list = merged(best.list, lane < k ? hand_load(p.keys + from * k + lane) : (uint64_t)0);
+      sum = join(sum, Sums{hand_load(p.sums + from * 4), hand_load(p.sums + from * 4 + 1), hand_load(p.sums + from * 4 + 2)});
+    }
+    meet();
   }
+  if (part != 0 || !real) return;
 
   // a NaN is in l even where it was never the maximum; nothing but -inf has l = 0
   const float log_l = __builtin_amdgcn_logf(sum.l);
   const float top = sum.m == -__builtin_inff() ? 0.f : sum.m;
   const auto logprob = [&](float v) { return sum.l == 0.f ? v : (v - top) - log_l * kLn2; };
-  if (tid < k) {
-    const uint64_t key = s_top[tid];
-    p.top_ids[row * k + tid] = (int32_t)~(uint32_t)key;
-    p.top_logprobs[row * k + tid] = logprob(from_order((uint32_t)(key >> 32)));
+  if (lane < k) {
+    p.top_ids[row * k + lane] = (int32_t)~(uint32_t)best.list;
+    p.top_logprobs[row * k + lane] = logprob(from_order((uint32_t)(best.list >> 32)));
   }
-  if (tid == 0) {
-    const int32_t token = p.tokens[row];
-    p.logprob[row] = token >= 0 && token < p.vocab ? logprob((float)x[token]) : __builtin_nanf("");
+  if (lane == 0) {
+    p.logprob[row] = token_there ? logprob(token_logit) : token_logit;
     p.entropy[row] = sum.l == 0.f ? 0.f : kLn2 * (log_l - sum.t / sum.l);
   }
 }
@@ -319,18 +401,21 @@ __global__ __launch_bounds__(kThreads) void bsg_token_logprobs_kernel(ScoreParam
 struct Shape {
   int32_t splits;
   int64_t split_vectors;
+  int32_t log_waves;  // waves of a row and split
 };
 
-// Rows alone fill the machine from two work-groups per compute unit on; fewer rows are split, down to one
-// vector per thread, and to what one list of alternatives holds.
-Shape shape_of(int64_t rows, int64_t vocab, int32_t k, int per_vector, int32_t cus) {
+// Waves of a row: enough rows fill the machine with one wave each (16 per compute unit); fewer take up
+// to the four of a work-group, and long ones several work-groups, of at least kSplitTiles tiles a
+// wave: a wave's sorts and merges cost as much as about four tiles, the meeting of work-groups another.
+Shape shape_of(int64_t rows, int64_t vocab, int per_vector, int32_t cus) {
   const int64_t vectors = ceil_div(vocab, per_vector) + 1;  // a row may begin inside a vector
-  int64_t want = ceil_div(2 * (int64_t)cus, rows > 0 ? rows : 1);
-  const int64_t most = ceil_div(vectors, kThreads);
-  if (want > most) want = most;
-  if (k > 0 && want > kList / k) want = kList / k;
-  if (rows * 4 > BSG_KV_COUNTER_BYTES) want = 1;
   Shape s;
+  s.log_waves = 0;
+  while ((1 << s.log_waves) < kWaves && (rows << s.log_waves) < 16 * (int64_t)cus && (64 << s.log_waves) < vectors)
+    ++s.log_waves;
+  int64_t want = vectors / (64 * kWaves * kVectors * kSplitTiles);
+  if (rows > 0 && want > 2 * cus / rows) want = 2 * cus / rows;
+  if (want < 1 || rows * 4 > BSG_KV_COUNTER_BYTES) want = 1;
   s.split_vectors = ceil_div(vectors, want);
   s.splits = (int32_t)ceil_div(vectors, s.split_vectors);
   return s;
@@ -339,7 +424,7 @@ Shape shape_of(int64_t rows, int64_t vocab, int32_t k, int per_vector, int32_t c
 int per_vector(int dtype) { return dtype == BSG_F32 ? 4 : 8; }
 
 int64_t workspace_bytes(const Shape& s, int64_t rows, int32_t k) {
-  return s.splits <= 1 ? 0 : BSG_KV_COUNTER_BYTES + rows * s.splits * (16 + 8 * (int64_t)k);
+  return s.splits <= 1 || rows == 0 ? 0 : BSG_KV_COUNTER_BYTES + rows * s.splits * (16 + 8 * (int64_t)k);
 }
 
 int check_sizes(int64_t rows, int64_t vocab, int32_t k, int dtype, int32_t cus) {
@@ -358,7 +443,7 @@ int check_sizes(int64_t rows, int64_t vocab, int32_t k, int dtype, int32_t cus) 
 extern "C" int64_t bsg_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int32_t k, int dtype,
                                                       int32_t cu_count) {
   if (check_sizes(rows, vocab, k, dtype, cu_count)) return -1;
-  return workspace_bytes(shape_of(rows, vocab, k, per_vector(dtype), cu_count), rows, k);
+  return workspace_bytes(shape_of(rows, vocab, per_vector(dtype), cu_count), rows, k);
 }
 
 extern "C" int bsg_token_logprobs(const void* logits, int64_t row_stride, int64_t rows, int64_t vocab,
@@ -371,7 +456,7 @@ extern "C" int bsg_token_logprobs(const void* logits, int64_t row_stride, int64_
     return fail(BSG_ERR_ARG, "null pointer (logits=%p tokens=%p logprob=%p entropy=%p top_ids=%p top_logprobs=%p)", logits,
                 (const void*)tokens, (void*)logprob, (void*)entropy, (void*)top_ids, (void*)top_logprobs);
   if (!is_aligned(logits, dtype == BSG_F32 ? 4 : 2)) return fail(BSG_ERR_ALIGN, "logits must be aligned to their type");
-  const Shape s = shape_of(rows, vocab, k, per_vector(dtype), cu_count);
+  const Shape s = shape_of(rows, vocab, per_vector(dtype), cu_count);
   const int64_t need = workspace_bytes(s, rows, k);
   if (need > 0 && (!ws || ws_bytes < need))
     return fail(BSG_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)need);
@@ -388,22 +473,25 @@ extern "C" int bsg_token_logprobs(const void* logits, int64_t row_stride, int64_
   p.sums = need > 0 ? (float*)(p.keys + rows * s.splits * k) : nullptr;
   const hipStream_t st = (hipStream_t)stream;
   const size_t es = dtype == BSG_F32 ? 4 : 2;
-  // one launch takes 65535 rows
-  for (int64_t r = 0; r < rows; r += 65535) {
-    const int64_t n = rows - r < 65535 ? rows - r : 65535;
+  // one launch takes 65535 work-groups of rows
+  const int64_t group = kWaves >> s.log_waves, most = 65535 * group;
+  p.log_waves = s.log_waves;
+  for (int64_t r = 0; r < rows; r += most) {
+    const int64_t n = rows - r < most ? rows - r : most;
+    p.rows = (int32_t)n;
     p.x = (const uint8_t*)logits + r * row_stride * (int64_t)es;
     p.tokens = tokens + r;
     p.logprob = logprob + r;
     p.entropy = entropy + r;
     p.top_ids = k > 0 ? top_ids + r * k : nullptr;
     p.top_logprobs = k > 0 ? top_logprobs + r * k : nullptr;
-    const dim3 grid((unsigned)s.splits, (unsigned)n);
+    const dim3 grid((unsigned)s.splits, (unsigned)ceil_div(n, group)), block(64 * kWaves);
     if (dtype == BSG_F16)
-      hipLaunchKernelGGL(bsg_token_logprobs_kernel<_Float16>, grid, dim3(kThreads), 0, st, p);
+      hipLaunchKernelGGL(bsg_token_logprobs_kernel<_Float16>, grid, block, 0, st, p);
     else if (dtype == BSG_BF16)
-      hipLaunchKernelGGL(bsg_token_logprobs_kernel<__bf16>, grid, dim3(kThreads), 0, st, p);
+      hipLaunchKernelGGL(bsg_token_logprobs_kernel<__bf16>, grid, block, 0, st, p);
     else
-      hipLaunchKernelGGL(bsg_token_logprobs_kernel<float>, grid, dim3(kThreads), 0, st, p);
+      hipLaunchKernelGGL(bsg_token_logprobs_kernel<float>, grid, block, 0, st, p);
   }
   return launch_status("bsg_token_logprobs");
 }
