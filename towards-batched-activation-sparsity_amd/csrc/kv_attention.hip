@@ -24,6 +24,7 @@ int check_kv_batch(int64_t tokens, int32_t rows, const int32_t* slots, const int
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMaxSplits = 32;    // parts of one row, which meet in LDS
 constexpr float kShift = 14.f;  // weights go up to 2^14
 
 struct AttnParams {
@@ -176,25 +177,55 @@ __global__ __launch_bounds__(256) void bsg_kv_attention_kernel(AttnParams p) {
 
   const int32_t* const table = p.table + (int64_t)(slot < 0 || slot >= p.num_slots ? 0 : slot) * p.table_stride;
   const int64_t head_bytes = (int64_t)2 * D << p.page_shift;
-  for (int t0 = t_begin + 32 * wave; t0 < t_end; t0 += 128) {
-    u32x4 kr[2][C], vr[2][C];
-    float ks[2], vs[2];
+  const int in_page = (1 << p.page_shift) - 1;
+  const uint8_t* const mine = p.pages + lane * 16;
+  struct Step {
+    u32x4 k[2][C], v[2][C];
+  };
+  // Up to 32 steps (64 tiles) of the wave at a time: lane j keeps the page and scales of its tile j,
+  // from where they come as scalars; the step after the one at work is on its way.
+  for (int b0 = t_begin + 32 * wave; b0 < t_end; b0 += 32 * 128) {
+    const int steps = (t_end - b0 + 127) / 128 < 32 ? (t_end - b0 + 127) / 128 : 32;
+    int lane_page = -1;
+    f32x2 lane_scale = {0.f, 0.f};
+    {
+      const int t = b0 + 128 * (lane >> 1) + 16 * (lane & 1);
+      if (t < t_end) {
+        const int page = table[t >> p.page_shift];
+        if (page >= 0 && page < p.num_pages) {
+          lane_page = page;
+          lane_scale = *(const f32x2*)(p.scales + 2 * ((int64_t)page * p.kv_heads + head));
+        }
+      }
+    }
+    const float lane_ks = lane_scale.x * p.scale2, lane_vs = fmaxf(lane_scale.y, 0x1p-100f);
+    const float lane_lv = __builtin_amdgcn_logf(lane_vs), lane_iv = 1.f / lane_vs;
+    const auto fetch = [&](int n, Step& s) {
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const int t = b0 + 128 * n + 16 * a;
+        const int page = __builtin_amdgcn_readlane(lane_page, 2 * n + a);
+        const uint8_t* const at =
+            mine + ((int64_t)(page < 0 ? 0 : page) * p.kv_heads + head) * head_bytes + (int64_t)((t & in_page) * D);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          s.k[a][c] = __builtin_nontemporal_load((const u32x4*)(at + c * 1024));
+          s.v[a][c] = __builtin_nontemporal_load((const u32x4*)(at + (head_bytes >> 1) + c * 1024));
+        }
+      }
+    };
+    const auto take = [&](int n, Step& s) {
+    const int t0 = b0 + 128 * n;
+    auto& kr = s.k;
+    auto& vr = s.v;
+    float ks[2], lv[2], iv[2];
     bool there[2];
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
-      const int t = t0 + 16 * a;
-      int page = t < t_end ? table[t >> p.page_shift] : -1;
-      there[a] = page >= 0 && page < p.num_pages;
-      page = there[a] ? page : 0;
-      const int64_t ph = (int64_t)page * p.kv_heads + head;
-      const uint8_t* const at = p.pages + ph * head_bytes + (int64_t)((t & ((1 << p.page_shift) - 1)) * D) + lane * 16;
-      const f32x2 s = *(const f32x2*)(p.scales + 2 * ph);
-      ks[a] = s.x * p.scale2, vs[a] = fmaxf(s.y, 0x1p-100f);
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        kr[a][c] = *(const u32x4*)(at + c * 1024);
-        vr[a][c] = *(const u32x4*)(at + (head_bytes >> 1) + c * 1024);
-      }
+      there[a] = __builtin_amdgcn_readlane(lane_page, 2 * n + a) >= 0;
+      ks[a] = as_float(__builtin_amdgcn_readlane(__builtin_bit_cast(int, lane_ks), 2 * n + a));
+      lv[a] = as_float(__builtin_amdgcn_readlane(__builtin_bit_cast(int, lane_lv), 2 * n + a));
+      iv[a] = as_float(__builtin_amdgcn_readlane(__builtin_bit_cast(int, lane_iv), 2 * n + a));
     }
     const bool partial = t0 + 32 > all_see || !there[0] || !there[1];
     uint32_t nan = 0;
@@ -211,8 +242,6 @@ __global__ __launch_bounds__(256) void bsg_kv_attention_kernel(AttnParams p) {
       }
     }
     const bool some_nan = partial && __any(nan != 0);
-    const float lv[2] = {__builtin_amdgcn_logf(vs[0]), __builtin_amdgcn_logf(vs[1])};
-    const float iv[2] = {1.f / vs[0], 1.f / vs[1]};
 
     f16x8 pf[RT];
 #pragma unroll
@@ -294,6 +323,16 @@ __global__ __launch_bounds__(256) void bsg_kv_attention_kernel(AttnParams p) {
 #pragma unroll
       for (int i = 0; i < RT; ++i) acc[i][d] = Elem<_Float16>::mfma(v, pf[i], acc[i][d]);
     }
+    };
+    Step even, odd;
+    fetch(0, even);
+    for (int n = 0; n < steps; n += 2) {
+      if (n + 1 < steps) fetch(n + 1, odd);
+      take(n, even);
+      if (n + 1 >= steps) break;
+      if (n + 2 < steps) fetch(n + 2, even);
+      take(n + 1, odd);
+    }
   }
 
   // the waves' parts under a common maximum
@@ -327,18 +366,24 @@ __global__ __launch_bounds__(256) void bsg_kv_attention_kernel(AttnParams p) {
   }
 
   const int used = rows < ROWS ? rows : ROWS;
-  const int64_t tile = ((int64_t)row * p.kv_heads + head) * p.row_tiles + rt;
-  float* const part = p.part + (tile * p.splits + split) * (ROWS * (D + 2));
+  // per row: the factor of each part (s_m), and one over the sum of weights (s_l)
+  const float* parts = nullptr;
   if (chunks > 1) {
-    for (int e = threadIdx.x; e < used * D; e += 256) hand_store(part + e, s_acc[(e / D) * LD + e % D]);
+    const int64_t tile = ((int64_t)row * p.kv_heads + head) * p.row_tiles + rt;
+    constexpr int PART = ROWS * (D + 2);
+    float* const part = p.part + (tile * p.splits + split) * PART;
+    parts = p.part + tile * p.splits * PART;
+    for (int e = threadIdx.x; e < used * (D / 2); e += 256) {
+      const int r = e / (D / 2), d = (e - r * (D / 2)) * 2;
+      hand_store((uint64_t*)(part + r * D + d), __builtin_bit_cast(uint64_t, *(const f32x2*)(s_acc + r * LD + d)));
+    }
     if ((int)threadIdx.x < used) {
       const int r = threadIdx.x;
       const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
       float sum = 0.f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) sum += s_l[w][r] * (s_m[w][r] == top ? 1.f : __builtin_amdgcn_exp2f(s_m[w][r] - top));
-      hand_store(part + ROWS * D + r, top);
-      hand_store(part + ROWS * (D + 1) + r, sum);
+      hand_store((uint64_t*)(part + ROWS * D) + r, __builtin_bit_cast(uint64_t, f32x2{top, sum}));
     }
     hand_publish();
     __syncthreads();
@@ -346,28 +391,55 @@ __global__ __launch_bounds__(256) void bsg_kv_attention_kernel(AttnParams p) {
     __syncthreads();
     if (!s_last) return;
     if (threadIdx.x == 0) hand_reset(p.counters + tile);
+    // every part's maximum and sum at once, then their factors, in s_acc ([row][part], two numbers each)
+    for (int e = threadIdx.x; e < used * chunks; e += 256) {
+      const int r = e / chunks, s = e - r * chunks;
+      const f32x2 v = __builtin_bit_cast(f32x2, hand_load((const uint64_t*)(parts + s * PART + ROWS * D) + r));
+      s_acc[r * LD + 2 * s] = v.x, s_acc[r * LD + 2 * s + 1] = v.y;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < used) {
+      float* const f = s_acc + threadIdx.x * LD;
+      float top = -__builtin_inff(), sum = 0.f;
+      for (int s = 0; s < chunks; ++s) top = fmaxf(top, f[2 * s]);
+      for (int s = 0; s < chunks; ++s) {
+        f[2 * s] = f[2 * s] == top ? 1.f : __builtin_amdgcn_exp2f(f[2 * s] - top);
+        sum += f[2 * s] * f[2 * s + 1];
+      }
+      s_m[0][threadIdx.x] = top, s_l[0][threadIdx.x] = sum;
+    }
+  } else if ((int)threadIdx.x < used) {
+    const int r = threadIdx.x;
+    const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) sum += s_l[w][r] * (s_m[w][r] == top ? 1.f : __builtin_amdgcn_exp2f(s_m[w][r] - top));
+    s_m[0][r] = top, s_l[0][r] = sum;
   }
-  const float* const parts = p.part + tile * p.splits * (ROWS * (D + 2));
-  constexpr int E = 4, PER = D / E;  // a thread's numbers of one row
+  __syncthreads();
+
+  constexpr int PER = D / 4;  // a thread writes four channels of a row
   for (int e = threadIdx.x; e < used * PER; e += 256) {
-    const int r = e / PER, d = (e - r * PER) * E;
-    float top, sum = 0.f;
+    const int r = e / PER, d = (e - r * PER) * 4;
+    const float top = s_m[0][r], sum = s_l[0][r];
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     if (chunks > 1) {
-      top = -__builtin_inff();
-      for (int s = 0; s < chunks; ++s) top = fmaxf(top, hand_load(parts + s * (ROWS * (D + 2)) + ROWS * D + r));
-      for (int s = 0; s < chunks; ++s) {
-        const float* const q = parts + s * (ROWS * (D + 2));
-        const float ms = hand_load(q + ROWS * D + r);
-        const float fs = ms == top ? 1.f : __builtin_amdgcn_exp2f(ms - top);
-        sum += fs * hand_load(q + ROWS * (D + 1) + r);
+      constexpr int PART = ROWS * (D + 2), BATCH = 8;  // parts in flight
+      for (int s0 = 0; s0 < chunks; s0 += BATCH) {
+        uint64_t v[BATCH][2];
 #pragma unroll
-        for (int j = 0; j < E; ++j) o[j] += fs * hand_load(q + r * D + d + j);
+        for (int j = 0; j < BATCH; ++j) {
+          const float* const q = parts + (s0 + j < chunks ? s0 + j : s0) * PART + r * D + d;
+          v[j][0] = hand_load((const uint64_t*)q), v[j][1] = hand_load((const uint64_t*)q + 1);
+        }
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+          const float f = s0 + j < chunks ? s_acc[r * LD + 2 * (s0 + j)] : 0.f;
+          const f32x2 a = __builtin_bit_cast(f32x2, v[j][0]), b = __builtin_bit_cast(f32x2, v[j][1]);
+          if (s0 + j < chunks) o += f32x4{a.x, a.y, b.x, b.y} * f;
+        }
       }
     } else {
-      top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
-#pragma unroll
-      for (int w = 0; w < 4; ++w) sum += s_l[w][r] * (s_m[w][r] == top ? 1.f : __builtin_amdgcn_exp2f(s_m[w][r] - top));
       o = *(const f32x4*)(s_acc + r * LD + d);
     }
     const int rr = rt * ROWS + r, tok = rr / p.group, h = head * p.group + rr - tok * p.group;
@@ -395,7 +467,8 @@ Shape shape_of(int32_t rows, int32_t kv_heads, int32_t group, int32_t max_new, i
   s.rt = per_head <= 16 ? 1 : per_head <= 32 ? 2 : 4;
   s.row_tiles = (int32_t)ceil_div(per_head, 16 * s.rt);
   const int64_t tiles = (int64_t)rows * kv_heads * s.row_tiles;
-  int64_t want = ceil_div((int64_t)4 * cus, tiles > 0 ? tiles : 1);
+  int64_t want = ceil_div((int64_t)2 * cus, tiles > 0 ? tiles : 1);
+  if (want > kMaxSplits) want = kMaxSplits;
   const int64_t most = ceil_div(max_len > 0 ? max_len : 1, 256);
   if (want > most) want = most;
   if (tiles * 4 > BSG_KV_COUNTER_BYTES) want = 1;
