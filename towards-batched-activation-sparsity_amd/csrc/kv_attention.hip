@@ -25,7 +25,9 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxSplits = 32;    // parts of one row, which meet in LDS
-constexpr float kShift = 14.f;  // weights go up to 2^14
+constexpr float kShift = 14.f;  // weights go up to 2^(kShift + kSlack), within fp16
+constexpr float kSlack = 1.5f;  // what a score may exceed the running maximum by before that moves
+constexpr float kMostWeight = 46340.f;  // 2^(kShift + kSlack)
 
 struct AttnParams {
   const uint16_t* q;
@@ -108,6 +110,38 @@ __device__ __forceinline__ uint32_t byte_mask(int n) {
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
   const uint32_t x = (w & 0x7f7f7f7fu) + 0x01010101u;  // bit 7 of a byte: all seven bits were set
   return ((x & 0x80808080u) >> 7) * 0x38u;
+}
+
+// A NaN among values that some rows do not see: the matrix unit would spread it to all rows (0 x
+// NaN), so it goes to those that see it by a product of flags, and leaves the values.  v: four tiles of 16 channels
+// of two 16-token tiles, t: the lane's first token, acc: their four accumulators of each 16 rows.
+template <int RT>
+__device__ __forceinline__ void nan_values(u32x4 v[2], int t, const int* sees, f32x4* acc, int stride) {
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    uint32_t f[4];
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        f[2 * a + j] = Elem<_Float16>::pack(t + 16 * a + 2 * j < sees[i] ? 1.f : 0.f, t + 16 * a + 2 * j + 1 < sees[i] ? 1.f : 0.f);
+    const f16x8 flags = __builtin_bit_cast(f16x8, u32x4{f[0], f[1], f[2], f[3]});
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      f32x4 n = {0.f, 0.f, 0.f, 0.f};
+      n = Elem<_Float16>::mfma(widen<_Float16>(nan_bytes(v[0][d]), nan_bytes(v[1][d])), flags, n);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n[j] > 0.f) acc[i * stride + d][j] = __builtin_nanf("");
+    }
+  }
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      const uint32_t n = nan_bytes(v[a][d]);  // 0x38 to 0xff
+      v[a][d] &= ~(n | (n << 1) | (n << 2) | (n >> 1) | (n >> 2) | (n >> 3));
+    }
 }
 
 // A work-group of four waves computes RT x 16 rows of one cached head of one sequence over one chunk
@@ -264,7 +298,7 @@ __global__ __launch_bounds__(256) void bsg_kv_attention_kernel(AttnParams p) {
       float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                        fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
       mx = fmaxf(m[i], column_max(mx));
-      if (__any(mx > m[i])) {
+      if (__any(mx > m[i] + kSlack)) {
         const float alpha = mx == m[i] ? 1.f : __builtin_amdgcn_exp2f(m[i] - mx);
         l[i] *= alpha;
 #pragma unroll
@@ -273,49 +307,23 @@ __global__ __launch_bounds__(256) void bsg_kv_attention_kernel(AttnParams p) {
       }
       const float base = (m[i] == -__builtin_inff() ? 0.f : m[i]) - kShift;
       float w[2][4];
+      uint32_t pw[4];
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[a][j] = __builtin_amdgcn_exp2f(s[a][j] - base);
-        l[i] += ((w[a][0] + w[a][1]) + (w[a][2] + w[a][3])) * iv[a];
+        pw[2 * a] = Elem<_Float16>::pack(w[a][0], w[a][1]), pw[2 * a + 1] = Elem<_Float16>::pack(w[a][2], w[a][3]);
+        l[i] = __builtin_fmaf((w[a][0] + w[a][1]) + (w[a][2] + w[a][3]), iv[a], l[i]);
       }
-      pf[i] = __builtin_bit_cast(
-          f16x8, u32x4{Elem<_Float16>::pack(w[0][0], w[0][1]), Elem<_Float16>::pack(w[0][2], w[0][3]),
-                       Elem<_Float16>::pack(w[1][0], w[1][1]), Elem<_Float16>::pack(w[1][2], w[1][3])});
+      pf[i] = __builtin_bit_cast(f16x8, u32x4{pw[0], pw[1], pw[2], pw[3]});
     }
     if (some_nan) {
-      // A NaN among values that some rows do not see: the matrix unit would spread it to all rows
-      // (0 x NaN), so it goes to those that see it by a product of flags and leaves the values.
 #pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        uint32_t f[4];
-#pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int t = t0 + 16 * a + 4 * g + 2 * j;
-            f[2 * a + j] = Elem<_Float16>::pack(t < sees[i] ? 1.f : 0.f, t + 1 < sees[i] ? 1.f : 0.f);
-          }
-        const f16x8 flags = __builtin_bit_cast(f16x8, u32x4{f[0], f[1], f[2], f[3]});
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          f32x4 n = {0.f, 0.f, 0.f, 0.f};
-          n = Elem<_Float16>::mfma(
-              widen<_Float16>(nan_bytes(vr[0][d >> 2][d & 3]), nan_bytes(vr[1][d >> 2][d & 3])), flags, n);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (n[j] > 0.f) acc[i][d][j] = __builtin_nanf("");
-        }
+      for (int c = 0; c < C; ++c) {
+        u32x4 v[2] = {vr[0][c], vr[1][c]};
+        nan_values<RT>(v, t0 + 4 * g, sees, &acc[0][4 * c], DT);
+        vr[0][c] = v[0], vr[1][c] = v[1];
       }
-#pragma unroll
-      for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            const uint32_t n = nan_bytes(vr[a][c][d]);
-            vr[a][c][d] &= ~(n | (n << 1) | (n << 2) | (n >> 1) | (n >> 2) | (n >> 3));
-          }
     }
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
@@ -453,19 +461,341 @@ __global__ __launch_bounds__(256) void bsg_kv_attention_kernel(AttnParams p) {
   }
 }
 
+// Many rows per cached head (prompts).  A work-group of four waves owns 128 rows, 32 of each wave, and walks the
+// tokens they see 64 at a time; a step's keys and values (16 KiB) are brought once, through
+// registers into LDS in the bytes they have in memory, while the step before is at work, and each
+// wave converts what it reads.  Rows do not cross waves, so nothing meets at the end but the parts
+// of a split.  Work-groups of one cached head lie kv_heads apart, that is on the same XCD where the
+// heads are a multiple of 8, and share its L2; one sequence follows the other (all of them side by
+// side: 334 us against 267 for 8 prompts of 2048), its tiles with most tokens first.
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
+  constexpr int C = D / 64, DT = D / 16, RT = 2, ROWS = 128, STEP = 64;
+  typedef typename Elem<T>::x8 x8;
+  __shared__ u32x4 s_kv[2][4][2][C * 64];  // [buffer][16-token tile][keys, values]
+  __shared__ f32x4 s_meta[2][4];           // scale of the scores, log2 and inverse of the values' scale, whether there
+  __shared__ uint32_t s_last;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, g = lane >> 4;
+  const int head = blockIdx.x % p.kv_heads;
+  const int split = blockIdx.y, row = blockIdx.z;
+
+  const int slot = p.slots ? p.slots[row] : row;
+  int64_t from = (int64_t)row * p.max_new, to = from + p.max_new;
+  if (p.cu) from = p.cu[row], to = p.cu[row + 1];
+  if (from < 0 || to > p.tokens || from >= to) return;
+  const int count = (int)(to - from < p.max_new ? to - from : p.max_new);
+  // a sequence's row tiles from its last one on, whatever the longest sequence of the call has
+  const int rt = (count * p.group - 1) / ROWS - (int)(blockIdx.x / p.kv_heads);
+  if (rt < 0) return;
+  const int rows = count * p.group - rt * ROWS;
+  const int used = rows < ROWS ? rows : ROWS;
+  int len = slot >= 0 && slot < p.num_slots ? p.lengths[slot] : 0;
+  const int most = p.max_pages << p.page_shift;
+  len = len < 0 ? 0 : len > most ? most : len;
+  const int first = len - (int)(to - from);
+  const auto sees_until = [&](int r) {  // tokens that row r of the tile sees
+    const int n = first + (rt * ROWS + r) / p.group + 1;
+    return n < 0 ? 0 : n;
+  };
+  const int end = sees_until(used - 1);
+  const int chunks = end <= p.chunk ? 1 : (end + p.chunk - 1) / p.chunk < p.splits ? (end + p.chunk - 1) / p.chunk : p.splits;
+  if (split >= chunks) return;
+  const int t_begin = split * p.chunk;
+  const int t_end = split == chunks - 1 ? end : t_begin + p.chunk;
+  // this wave's rows: 32 wave .. +31
+  const int w_used = used - 32 * wave < 32 ? used - 32 * wave : 32;
+  const int w_end = w_used > 0 ? sees_until(32 * wave + w_used - 1) : 0;  // what its last row sees
+  const int w_all = w_used > 0 ? sees_until(32 * wave) : 0;               // what all of them see
+
+  x8 qf[RT][2 * C];
+  int sees[RT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    const int r = 32 * wave + 16 * i + col;
+    const int rr = rt * ROWS + r, tok = rr / p.group, h = rr - tok * p.group;
+    const bool on = r < used;
+    sees[i] = on ? first + tok + 1 : 0;
+#pragma unroll
+    for (int c = 0; c < 2 * C; ++c) {
+      u32x4 v = {0u, 0u, 0u, 0u};
+      if (on)
+        v = *(const u32x4*)(p.q + (from + tok) * p.q_st + (int64_t)(head * p.group + h) * p.q_sh + 64 * (c >> 1) +
+                            16 * g + 8 * (c & 1));
+      v ^= p.scale2 < 0.f ? 0x80008000u : 0u;  // so that the scores' scale is positive
+      qf[i][c] = __builtin_bit_cast(x8, v);
+    }
+  }
+  const float scale2 = __builtin_fabsf(p.scale2);
+
+  const int32_t* const table = p.table + (int64_t)(slot < 0 || slot >= p.num_slots ? 0 : slot) * p.table_stride;
+  const int64_t head_bytes = (int64_t)2 * D << p.page_shift;
+  const int in_page = (1 << p.page_shift) - 1;
+  const auto page_at = [&](int t0) {  // of the tile that this wave brings
+    const int t = t0 + 16 * wave;
+    return t < t_end ? table[t >> p.page_shift] : -1;
+  };
+  u32x4 kr[C], vr[C];
+  f32x4 meta;
+  const auto fetch = [&](int t0, int page) {
+    const bool there = page >= 0 && page < p.num_pages;
+    const int64_t ph = (int64_t)(there ? page : 0) * p.kv_heads + head;
+    const uint8_t* const at = p.pages + ph * head_bytes + (int64_t)(((t0 + 16 * wave) & in_page) * D) + lane * 16;
+    const f32x2 s = *(const f32x2*)(p.scales + 2 * ph);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      kr[c] = *(const u32x4*)(at + c * 1024);
+      vr[c] = *(const u32x4*)(at + (head_bytes >> 1) + c * 1024);
+    }
+    const float vs = fmaxf(s.y, 0x1p-100f);
+    // a scale of 0 as the least one, so that -inf stays what it is
+    meta = f32x4{fmaxf(s.x * scale2, 0x1p-126f), __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs), there ? 1.f : 0.f};
+  };
+  const auto stage = [&](int buf) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) s_kv[buf][wave][0][c * 64 + lane] = kr[c], s_kv[buf][wave][1][c * 64 + lane] = vr[c];
+    if (lane == 0) s_meta[buf][wave] = meta;
+  };
+
+  f32x4 acc[RT][DT];
+  float m[RT], l[RT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    m[i] = -__builtin_inff(), l[i] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  bool started = false;  // every row has a maximum
+  const auto take = [&](int t0, int buf) {
+    f32x4 s[RT][4], mt[4];
+    bool all_there = true;
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      mt[a] = s_meta[buf][a];
+      all_there = all_there && __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, (float)mt[a].w)) != 0;
+#pragma unroll
+      for (int i = 0; i < RT; ++i) s[i][a] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const u32x4 k = s_kv[buf][a][0][c * 64 + lane];
+        const x8 k0 = widen<T>(k.x, k.y), k1 = widen<T>(k.z, k.w);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          s[i][a] = Elem<T>::mfma(k0, qf[i][2 * c], s[i][a]);
+          s[i][a] = Elem<T>::mfma(k1, qf[i][2 * c + 1], s[i][a]);
+        }
+      }
+    }
+    const bool partial = t0 + STEP > w_all || !all_there;
+    if (partial) {
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        const int t = mt[a].w != 0.f ? t0 + 16 * a + 4 * g : 0x7ffffff0;
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (t + j >= sees[i]) s[i][a][j] = -__builtin_inff();
+      }
+    }
+    // Weights against the maximum so far; only where one of them outgrows fp16 (or a row has no maximum yet) is a
+    // new maximum looked for.  The old one is never above the true one by that.
+    f16x8 pf[RT][2];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      float e[4][4], top = 0.f;
+      const auto weigh = [&]() {
+        const float base = (m[i] == -__builtin_inff() ? 0.f : m[i]) - kShift;
+        top = 0.f;
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          const float off = mt[a].y - base;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            e[a][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][a][j], mt[a].x, off));
+            top = fmaxf(top, e[a][j]);
+          }
+        }
+      };
+      weigh();
+      if (!started || __any(top > kMostWeight)) {
+        float mx = -__builtin_inff();
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          const float t = fmaxf(fmaxf(s[i][a][0], s[i][a][1]), fmaxf(s[i][a][2], s[i][a][3]));
+          mx = fmaxf(mx, __builtin_fmaf(t, mt[a].x, mt[a].y));
+        }
+        mx = fmaxf(m[i], column_max(mx));
+        const float alpha = mx == m[i] ? 1.f : __builtin_amdgcn_exp2f(m[i] - mx);
+        l[i] *= alpha;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[i][d] *= alpha;
+        m[i] = mx;
+        weigh();
+      }
+      uint32_t w[8];
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        l[i] = __builtin_fmaf((e[a][0] + e[a][1]) + (e[a][2] + e[a][3]), mt[a].z, l[i]);
+        w[2 * a] = Elem<_Float16>::pack(e[a][0], e[a][1]), w[2 * a + 1] = Elem<_Float16>::pack(e[a][2], e[a][3]);
+      }
+      pf[i][0] = __builtin_bit_cast(f16x8, u32x4{w[0], w[1], w[2], w[3]});
+      pf[i][1] = __builtin_bit_cast(f16x8, u32x4{w[4], w[5], w[6], w[7]});
+    }
+    started = started || !partial;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        u32x4 v[2] = {s_kv[buf][2 * b][1][c * 64 + lane], s_kv[buf][2 * b + 1][1][c * 64 + lane]};
+        if (partial) {
+          uint32_t nan = 0;
+#pragma unroll
+          for (int a = 0; a < 2; ++a) {
+            v[a] &= mt[2 * b + a].w != 0.f ? byte_mask(t_end - (t0 + 32 * b + 16 * a + 4 * g)) : 0u;
+            nan |= nan_bytes(v[a].x) | nan_bytes(v[a].y) | nan_bytes(v[a].z) | nan_bytes(v[a].w);
+          }
+          if (__any(nan != 0)) nan_values<RT>(v, t0 + 32 * b + 4 * g, sees, &acc[0][4 * c], DT);
+        }
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const f16x8 x = widen<_Float16>(v[0][d], v[1][d]);
+#pragma unroll
+          for (int i = 0; i < RT; ++i) acc[i][4 * c + d] = Elem<_Float16>::mfma(x, pf[i][b], acc[i][4 * c + d]);
+        }
+      }
+    }
+  };
+
+  int page = page_at(t_begin);
+  if (t_begin < t_end) fetch(t_begin, page);
+  page = page_at(t_begin + STEP);
+  int buf = 0;
+  stage(0);
+  __syncthreads();
+  for (int t0 = t_begin; t0 < t_end; t0 += STEP) {
+    const bool more = t0 + STEP < t_end;
+    if (more) {
+      fetch(t0 + STEP, page);
+      page = page_at(t0 + 2 * STEP);
+    }
+    if (t0 < w_end) take(t0, buf);
+    if (more) stage(buf ^ 1);
+    buf ^= 1;
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < RT; ++i) l[i] = column_sum(l[i]);
+
+  const int64_t heads = (int64_t)p.kv_heads * p.group;
+  const auto finish = [&](int r, int d, f32x4 o, float top, float sum) {
+    const int rr = rt * ROWS + r, tok = rr / p.group, h = head * p.group + rr - tok * p.group;
+    const bool nothing = sum == 0.f;
+    const float inv = nothing ? 0.f : 1.f / sum;
+    u32x2* const at = (u32x2*)(p.out + (from + tok) * p.o_st + (int64_t)h * p.o_sh + d);
+    *at = u32x2{Elem<T>::pack(o[0] * inv, o[1] * inv), Elem<T>::pack(o[2] * inv, o[3] * inv)};
+    if (p.lse && d == 0)
+      p.lse[(from + tok) * heads + h] =
+          nothing ? -__builtin_inff() : (top - kShift + __builtin_amdgcn_logf(sum)) * (1.f / kLog2e);
+  };
+  if (chunks == 1) {
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const int r = 32 * wave + 16 * i + col;
+      if (r < used) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d) finish(r, 16 * d + 4 * g, acc[i][d], m[i], l[i]);
+      }
+    }
+    return;
+  }
+
+  const int64_t tile = ((int64_t)row * p.kv_heads + head) * p.row_tiles + rt;
+  constexpr int PART = ROWS * (D + 2);
+  const float* const parts = p.part + tile * p.splits * PART;
+  float* const part = p.part + (tile * p.splits + split) * PART;
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    const int r = 32 * wave + 16 * i + col;
+    if (r < used) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        uint64_t* const at = (uint64_t*)(part + r * D + 16 * d + 4 * g);
+        hand_store(at, __builtin_bit_cast(uint64_t, f32x2{acc[i][d][0], acc[i][d][1]}));
+        hand_store(at + 1, __builtin_bit_cast(uint64_t, f32x2{acc[i][d][2], acc[i][d][3]}));
+      }
+      if (g == 0) hand_store((uint64_t*)(part + ROWS * D) + r, __builtin_bit_cast(uint64_t, f32x2{m[i], l[i]}));
+    }
+  }
+  hand_publish();
+  __syncthreads();
+  if (threadIdx.x == 0) s_last = hand_arrive(p.counters + tile) == (uint32_t)(chunks - 1);
+  __syncthreads();
+  if (!s_last) return;
+  if (threadIdx.x == 0) hand_reset(p.counters + tile);
+  // [row][part] factors and, in the row's first pair, the maximum and the sum
+  float* const s_f = (float*)&s_kv[0][0][0][0];
+  constexpr int FL = 2 * kMaxSplits;
+  static_assert(ROWS * FL * sizeof(float) <= 2 * sizeof(s_kv[0]) || D == 64, "factors in the buffers");
+  constexpr int BLOCK = D == 64 ? 64 : ROWS;  // rows whose factors fit at once
+  for (int r0 = 0; r0 < used; r0 += BLOCK) {
+    const int n = used - r0 < BLOCK ? used - r0 : BLOCK;
+    __syncthreads();
+    for (int e = threadIdx.x; e < n * chunks; e += 256) {
+      const int r = e / chunks, s = e - r * chunks;
+      const f32x2 v = __builtin_bit_cast(f32x2, hand_load((const uint64_t*)(parts + s * PART + ROWS * D) + r0 + r));
+      s_f[r * FL + 2 * s] = v.x, s_f[r * FL + 2 * s + 1] = v.y;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < n) {
+      float* const f = s_f + threadIdx.x * FL;
+      float top = -__builtin_inff(), sum = 0.f;
+      for (int s = 0; s < chunks; ++s) top = fmaxf(top, f[2 * s]);
+      for (int s = 0; s < chunks; ++s) {
+        f[2 * s] = f[2 * s] == top ? 1.f : __builtin_amdgcn_exp2f(f[2 * s] - top);
+        sum += f[2 * s] * f[2 * s + 1];
+      }
+      f[1] = top, f[3] = sum;  // at least two parts
+    }
+    __syncthreads();
+    constexpr int PER = D / 4, BATCH = 8;
+    for (int e = threadIdx.x; e < n * PER; e += 256) {
+      const int r = e / PER, d = (e - r * PER) * 4;
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+      for (int s0 = 0; s0 < chunks; s0 += BATCH) {
+        uint64_t v[BATCH][2];
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+          const float* const q = parts + (s0 + j < chunks ? s0 + j : s0) * PART + (r0 + r) * D + d;
+          v[j][0] = hand_load((const uint64_t*)q), v[j][1] = hand_load((const uint64_t*)q + 1);
+        }
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+          const f32x2 a = __builtin_bit_cast(f32x2, v[j][0]), b = __builtin_bit_cast(f32x2, v[j][1]);
+          if (s0 + j < chunks) o += f32x4{a.x, a.y, b.x, b.y} * s_f[r * FL + 2 * (s0 + j)];
+        }
+      }
+      finish(r0 + r, d, o, s_f[r * FL + 1], s_f[r * FL + 3]);
+    }
+  }
+}
+
 struct Shape {
-  int rt;               // 16-row tiles of a work-group
+  int rows;             // of a work-group
   int32_t row_tiles;    // work-groups over the rows of a cached head
   int32_t splits;
   int32_t chunk;
 };
 
+constexpr int kPrefillRows = 32;  // a cached head's rows past which the prefill kernel runs
+
 // How a call is cut: few rows leave most compute units idle unless the long axis is split.
 Shape shape_of(int32_t rows, int32_t kv_heads, int32_t group, int32_t max_new, int64_t max_len, int32_t cus) {
   Shape s;
   const int64_t per_head = (int64_t)max_new * group;
-  s.rt = per_head <= 16 ? 1 : per_head <= 32 ? 2 : 4;
-  s.row_tiles = (int32_t)ceil_div(per_head, 16 * s.rt);
+  s.rows = per_head <= 16 ? 16 : per_head <= kPrefillRows ? 32 : 128;
+  s.row_tiles = (int32_t)ceil_div(per_head, s.rows);
   const int64_t tiles = (int64_t)rows * kv_heads * s.row_tiles;
   int64_t want = ceil_div((int64_t)2 * cus, tiles > 0 ? tiles : 1);
   if (want > kMaxSplits) want = kMaxSplits;
@@ -478,16 +808,16 @@ Shape shape_of(int32_t rows, int32_t kv_heads, int32_t group, int32_t max_new, i
 }
 
 int64_t workspace_bytes(const Shape& s, int32_t rows, int32_t kv_heads, int32_t d) {
-  if (s.splits <= 1) return 0;
-  return BSG_KV_COUNTER_BYTES + (int64_t)rows * kv_heads * s.row_tiles * s.splits * (16 * s.rt) * (d + 2) * 4;
+  if (s.splits <= 1 || rows == 0) return 0;
+  return BSG_KV_COUNTER_BYTES + (int64_t)rows * kv_heads * s.row_tiles * s.splits * s.rows * (d + 2) * 4;
 }
 
 template <typename T, int D>
 void launch(const AttnParams& p, const Shape& s, dim3 grid, hipStream_t st) {
-  switch (s.rt) {
-    case 1: hipLaunchKernelGGL((bsg_kv_attention_kernel<T, D, 1>), grid, dim3(256), 0, st, p); break;
-    case 2: hipLaunchKernelGGL((bsg_kv_attention_kernel<T, D, 2>), grid, dim3(256), 0, st, p); break;
-    default: hipLaunchKernelGGL((bsg_kv_attention_kernel<T, D, 4>), grid, dim3(256), 0, st, p); break;
+  switch (s.rows) {
+    case 16: hipLaunchKernelGGL((bsg_kv_attention_kernel<T, D, 1>), grid, dim3(256), 0, st, p); break;
+    case 32: hipLaunchKernelGGL((bsg_kv_attention_kernel<T, D, 2>), grid, dim3(256), 0, st, p); break;
+    default: hipLaunchKernelGGL((bsg_kv_prefill_kernel<T, D>), grid, dim3(256), 0, st, p); break;
   }
 }
 
@@ -535,8 +865,8 @@ extern "C" int bsg_kv_attention(const void* q, int64_t q_stride_t, int64_t q_str
     return fail(BSG_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)need);
   if (need > 0 && !is_aligned(ws, 16)) return fail(BSG_ERR_ALIGN, "workspace must be 16-byte aligned");
   const int64_t gx = (int64_t)cache->n_heads * s.row_tiles;
-  if (gx > 0x7fffffff || rows > 65535 || s.splits > 65535)
-    return fail(BSG_ERR_UNSUPPORTED, "grid of %lld x %d x %d", (long long)gx, s.splits, rows);
+  if (gx > 0x7fffffff || rows > 65535 || s.row_tiles > 65535)
+    return fail(BSG_ERR_UNSUPPORTED, "%d sequences of %d tokens", rows, max_new);
   AttnParams p;
   p.q = (const uint16_t*)q;
   p.out = (uint16_t*)out;
