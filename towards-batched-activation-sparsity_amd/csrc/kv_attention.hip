@@ -11,6 +11,8 @@
 // sum w / vs whatever M is.  w is at most 2^14 and goes to the matrix unit as fp16: every weight
 // down to 2^-28 of the largest keeps 11 bits.
 
+#include <utility>
+
 #include "serve.hpp"
 
 using namespace bsgk;
@@ -461,10 +463,31 @@ __global__ __launch_bounds__(256) void bsg_kv_attention_kernel(AttnParams p) {
   }
 }
 
+// The prefill kernel's stages of LDS: arrays of their own, so that a load into one is no reason to wait
+// before a read of another.
+template <int D, int S>
+__device__ __forceinline__ u32x4* prefill_stage() {
+  __shared__ u32x4 stage[4 * 2 * D];  // four 16-token tiles of 32 D bytes
+  return stage;
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t cache_rsrc(const uint8_t* base, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, bytes, 0x00020000);
+}
+// 16 bytes per lane straight into LDS, lane i's at lds + 16 i; out of range: zeros.
+__device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t r, u32x4* lds, int lane_off, int off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, lane_off, off, 0, 0);
+}
+// Wait until at most N vector-memory loads of this wave are outstanding; they complete in order.
+template <int N>
+__device__ __forceinline__ void vmem_wait() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | (0x7 << 4) | (0xF << 8));
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // Many rows per cached head (prompts).  A work-group of four waves owns 128 rows, 32 of each wave, and walks the
-// tokens they see 64 at a time; a step's keys and values (16 KiB) are brought once, through
-// registers into LDS in the bytes they have in memory, while the step before is at work, and each
-// wave converts what it reads.  Rows do not cross waves, so nothing meets at the end but the parts
+// tokens they see 64 at a time; a step's keys and values (16 KiB) are brought once, straight into LDS in
+// the bytes they have in memory, two steps ahead, and each wave converts what it reads.  Rows do not cross waves, so nothing meets at the end but the parts
 // of a split.  Work-groups of one cached head lie kv_heads apart, that is on the same XCD where the
 // heads are a multiple of 8, and share its L2; one sequence follows the other (all of them side by
 // side: 334 us against 267 for 8 prompts of 2048), its tiles with most tokens first.
@@ -472,8 +495,7 @@ template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
   constexpr int C = D / 64, DT = D / 16, RT = 2, ROWS = 128, STEP = 64;
   typedef typename Elem<T>::x8 x8;
-  __shared__ u32x4 s_kv[2][4][2][C * 64];  // [buffer][16-token tile][keys, values]
-  __shared__ f32x4 s_meta[2][4];           // scale of the scores, log2 and inverse of the values' scale, whether there
+  constexpr int TILE = 2 * C * 64, LOADS = 2 * C;  // 16-byte pieces of a 16-token tile, keys then values; a wave's loads
   __shared__ uint32_t s_last;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
@@ -531,30 +553,39 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
   const int32_t* const table = p.table + (int64_t)(slot < 0 || slot >= p.num_slots ? 0 : slot) * p.table_stride;
   const int64_t head_bytes = (int64_t)2 * D << p.page_shift;
   const int in_page = (1 << p.page_shift) - 1;
-  const auto page_at = [&](int t0) {  // of the tile that this wave brings
-    const int t = t0 + 16 * wave;
-    return t < t_end ? table[t >> p.page_shift] : -1;
+  // Lane j keeps the page and scales of the j-th 16-token tile of 16 steps (1024 tokens), from where
+  // they come as scalars; the next 16 steps' are on their way while the last of these are at work.
+  int lane_page = -1, next_page = -1;
+  float lane_ks = 0.f, lane_lv = 0.f, lane_iv = 0.f;
+  f32x2 next_scale = {0.f, 0.f};
+  const auto load_pages = [&](int b0) {
+    const int t = b0 + 16 * lane;
+    const int page = t < t_end ? table[t >> p.page_shift] : -1;
+    next_page = page >= 0 && page < p.num_pages ? page : -1;
   };
-  u32x4 kr[C], vr[C];
-  f32x4 meta;
-  const auto fetch = [&](int t0, int page) {
-    const bool there = page >= 0 && page < p.num_pages;
-    const int64_t ph = (int64_t)(there ? page : 0) * p.kv_heads + head;
-    const uint8_t* const at = p.pages + ph * head_bytes + (int64_t)(((t0 + 16 * wave) & in_page) * D) + lane * 16;
-    const f32x2 s = *(const f32x2*)(p.scales + 2 * ph);
+  const auto load_scales = [&]() {
+    next_scale = *(const f32x2*)(p.scales + 2 * ((int64_t)(next_page < 0 ? 0 : next_page) * p.kv_heads + head));
+  };
+  const auto turn_pages = [&]() {
+    const float vs = fmaxf(next_scale.y, 0x1p-100f);
+    lane_page = next_page;
+    // a scale of 0 as the least one, so that -inf stays what it is
+    lane_ks = fmaxf(next_scale.x * scale2, 0x1p-126f);
+    lane_lv = __builtin_amdgcn_logf(vs), lane_iv = __builtin_amdgcn_rcpf(vs);
+  };
+  // The wave brings the step's tile `wave`; a step past the end, or a page that is not there, loads
+  // zeros, so that every step has the same number of loads to wait by.
+  const auto issue = [&](auto stage, int t0, int page) {
+    const bool there = page >= 0;
+    const __amdgpu_buffer_rsrc_t r = cache_rsrc(p.pages + ((int64_t)(there ? page : 0) * p.kv_heads + head) * head_bytes,
+                                                there ? (int)head_bytes : 0);
+    u32x4* const to = prefill_stage<D, decltype(stage)::value>() + wave * TILE;
+    const int at = ((t0 + 16 * wave) & in_page) * D;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      kr[c] = *(const u32x4*)(at + c * 1024);
-      vr[c] = *(const u32x4*)(at + (head_bytes >> 1) + c * 1024);
+      load_lds(r, to + c * 64, lane * 16, at + c * 1024);
+      load_lds(r, to + (C + c) * 64, lane * 16, at + c * 1024 + (int)(head_bytes >> 1));
     }
-    const float vs = fmaxf(s.y, 0x1p-100f);
-    // a scale of 0 as the least one, so that -inf stays what it is
-    meta = f32x4{fmaxf(s.x * scale2, 0x1p-126f), __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs), there ? 1.f : 0.f};
-  };
-  const auto stage = [&](int buf) {
-#pragma unroll
-    for (int c = 0; c < C; ++c) s_kv[buf][wave][0][c * 64 + lane] = kr[c], s_kv[buf][wave][1][c * 64 + lane] = vr[c];
-    if (lane == 0) s_meta[buf][wave] = meta;
   };
 
   f32x4 acc[RT][DT];
@@ -567,18 +598,24 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
   }
 
   bool started = false;  // every row has a maximum
-  const auto take = [&](int t0, int buf) {
-    f32x4 s[RT][4], mt[4];
-    bool all_there = true;
+  const auto take = [&](auto stage, int t0) {
+    const u32x4* const kv = prefill_stage<D, decltype(stage)::value>() + lane;
+    const int first_tile = (t0 - t_begin) / 16 & 63;
+    f32x4 s[RT][4];
+    float ks[4], lv[4], iv[4];
+    bool there[4], all_there = true;
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
-      mt[a] = s_meta[buf][a];
-      all_there = all_there && __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, (float)mt[a].w)) != 0;
+      there[a] = __builtin_amdgcn_readlane(lane_page, first_tile + a) >= 0;
+      ks[a] = as_float(__builtin_amdgcn_readlane(__builtin_bit_cast(int, lane_ks), first_tile + a));
+      lv[a] = as_float(__builtin_amdgcn_readlane(__builtin_bit_cast(int, lane_lv), first_tile + a));
+      iv[a] = as_float(__builtin_amdgcn_readlane(__builtin_bit_cast(int, lane_iv), first_tile + a));
+      all_there = all_there && there[a];
 #pragma unroll
       for (int i = 0; i < RT; ++i) s[i][a] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        const u32x4 k = s_kv[buf][a][0][c * 64 + lane];
+        const u32x4 k = kv[a * TILE + c * 64];
         const x8 k0 = widen<T>(k.x, k.y), k1 = widen<T>(k.z, k.w);
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
@@ -591,7 +628,7 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
     if (partial) {
 #pragma unroll
       for (int a = 0; a < 4; ++a) {
-        const int t = mt[a].w != 0.f ? t0 + 16 * a + 4 * g : 0x7ffffff0;
+        const int t = there[a] ? t0 + 16 * a + 4 * g : 0x7ffffff0;
 #pragma unroll
         for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -610,10 +647,10 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
         top = 0.f;
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
-          const float off = mt[a].y - base;
+          const float off = lv[a] - base;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            e[a][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][a][j], mt[a].x, off));
+            e[a][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][a][j], ks[a], off));
             top = fmaxf(top, e[a][j]);
           }
         }
@@ -624,7 +661,7 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
           const float t = fmaxf(fmaxf(s[i][a][0], s[i][a][1]), fmaxf(s[i][a][2], s[i][a][3]));
-          mx = fmaxf(mx, __builtin_fmaf(t, mt[a].x, mt[a].y));
+          mx = fmaxf(mx, __builtin_fmaf(t, ks[a], lv[a]));
         }
         mx = fmaxf(m[i], column_max(mx));
         const float alpha = mx == m[i] ? 1.f : __builtin_amdgcn_exp2f(m[i] - mx);
@@ -637,7 +674,7 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
       uint32_t w[8];
 #pragma unroll
       for (int a = 0; a < 4; ++a) {
-        l[i] = __builtin_fmaf((e[a][0] + e[a][1]) + (e[a][2] + e[a][3]), mt[a].z, l[i]);
+        l[i] = __builtin_fmaf((e[a][0] + e[a][1]) + (e[a][2] + e[a][3]), iv[a], l[i]);
         w[2 * a] = Elem<_Float16>::pack(e[a][0], e[a][1]), w[2 * a + 1] = Elem<_Float16>::pack(e[a][2], e[a][3]);
       }
       pf[i][0] = __builtin_bit_cast(f16x8, u32x4{w[0], w[1], w[2], w[3]});
@@ -648,12 +685,12 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
     for (int b = 0; b < 2; ++b) {
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        u32x4 v[2] = {s_kv[buf][2 * b][1][c * 64 + lane], s_kv[buf][2 * b + 1][1][c * 64 + lane]};
+        u32x4 v[2] = {kv[2 * b * TILE + (C + c) * 64], kv[(2 * b + 1) * TILE + (C + c) * 64]};
         if (partial) {
           uint32_t nan = 0;
 #pragma unroll
           for (int a = 0; a < 2; ++a) {
-            v[a] &= mt[2 * b + a].w != 0.f ? byte_mask(t_end - (t0 + 32 * b + 16 * a + 4 * g)) : 0u;
+            v[a] &= there[2 * b + a] ? byte_mask(t_end - (t0 + 32 * b + 16 * a + 4 * g)) : 0u;
             nan |= nan_bytes(v[a].x) | nan_bytes(v[a].y) | nan_bytes(v[a].z) | nan_bytes(v[a].w);
           }
           if (__any(nan != 0)) nan_values<RT>(v, t0 + 32 * b + 4 * g, sees, &acc[0][4 * c], DT);
@@ -668,22 +705,38 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
     }
   };
 
-  int page = page_at(t_begin);
-  if (t_begin < t_end) fetch(t_begin, page);
-  page = page_at(t_begin + STEP);
-  int buf = 0;
-  stage(0);
-  __syncthreads();
-  for (int t0 = t_begin; t0 < t_end; t0 += STEP) {
-    const bool more = t0 + STEP < t_end;
-    if (more) {
-      fetch(t0 + STEP, page);
-      page = page_at(t0 + 2 * STEP);
-    }
-    if (t0 < w_end) take(t0, buf);
-    if (more) stage(buf ^ 1);
-    buf ^= 1;
-    __syncthreads();
+  if (t_begin < t_end) {
+    // page of the tile that this wave brings for step n of the 16 (from 16 on: of the next 16)
+    const auto page_of = [&](int n) {
+      return n < 16 ? __builtin_amdgcn_readlane(lane_page, 4 * n + wave) : __builtin_amdgcn_readlane(next_page, 4 * n - 64 + wave);
+    };
+    load_pages(t_begin);
+    load_scales();
+    turn_pages();
+    issue(std::integral_constant<int, 0>{}, t_begin, page_of(0));
+    issue(std::integral_constant<int, 1>{}, t_begin + STEP, page_of(1));
+    int n = 0;
+    for (int t0 = t_begin; t0 < t_end; t0 += 3 * STEP)
+      [&]<int... I>(std::integer_sequence<int, I...>) {
+        (..., [&](auto stage) {
+          constexpr int S = decltype(stage)::value;
+          const int t = t0 + S * STEP;
+          // this step's pieces have arrived for every wave, and every wave has read the step's before
+          vmem_wait<LOADS>();
+          __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+          asm volatile("" ::: "memory");
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+          __builtin_amdgcn_sched_barrier(0);
+          if (n == 8) load_pages(t + 8 * STEP);
+          if (n == 11) load_scales();
+          issue(std::integral_constant<int, (S + 2) % 3>{}, t + 2 * STEP, t + 2 * STEP < t_end ? page_of(n + 2) : -1);
+          __builtin_amdgcn_sched_barrier(0);
+          if (t < w_end && t < t_end) take(stage, t);
+          if (++n == 16) n = 0, turn_pages();
+        }(std::integral_constant<int, I>{}));
+      }(std::make_integer_sequence<int, 3>{});
+    vmem_wait<0>();  // nothing is on its way into LDS any more
   }
 #pragma unroll
   for (int i = 0; i < RT; ++i) l[i] = column_sum(l[i]);
@@ -735,10 +788,9 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
   if (!s_last) return;
   if (threadIdx.x == 0) hand_reset(p.counters + tile);
   // [row][part] factors and, in the row's first pair, the maximum and the sum
-  float* const s_f = (float*)&s_kv[0][0][0][0];
+  float* const s_f = (float*)prefill_stage<D, 0>();
   constexpr int FL = 2 * kMaxSplits;
-  static_assert(ROWS * FL * sizeof(float) <= 2 * sizeof(s_kv[0]) || D == 64, "factors in the buffers");
-  constexpr int BLOCK = D == 64 ? 64 : ROWS;  // rows whose factors fit at once
+  constexpr int BLOCK = 4 * TILE * 16 / (FL * 4);  // rows whose factors fit a stage at once
   for (int r0 = 0; r0 < used; r0 += BLOCK) {
     const int n = used - r0 < BLOCK ? used - r0 : BLOCK;
     __syncthreads();
