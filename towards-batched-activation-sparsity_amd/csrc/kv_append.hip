@@ -4,8 +4,8 @@
 // page meet once in LDS, for the largest magnitude.  Lane 16 g + t of a tile holds channels
 // 64 c + 16 g .. +15 of token t, two 16-byte loads per c.  For the keys its quantised 16 bytes are
 // the lane's 16 bytes of the tile; for the values the four lanes of a quad exchange their 4 x 4
-// bytes (tokens x channels), after which each holds dwords of four tokens of one channel, which is
-// how the values' tiles are laid out.
+// bytes (tokens x channels), after which each holds dwords of four tokens of one channel, and the
+// four rows of 16 lanes their 4 x 4 dwords, after which these too are the lane's 16 bytes.
 
 #include "serve.hpp"
 
@@ -38,6 +38,20 @@ __device__ __forceinline__ uint32_t quad_transpose(uint32_t w, int i) {
   return lo | (hi << 16);
 }
 
+// The 4 x 4 transpose of four dwords over the four rows of 16 lanes.
+__device__ __forceinline__ void row_transpose(uint32_t w[4]) {
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    const auto r = __builtin_amdgcn_permlane32_swap(w[n], w[n + 2], false, false);
+    w[n] = r[0], w[n + 2] = r[1];
+  }
+#pragma unroll
+  for (int n = 0; n < 4; n += 2) {
+    const auto r = __builtin_amdgcn_permlane16_swap(w[n], w[n + 1], false, false);
+    w[n] = r[0], w[n + 1] = r[1];
+  }
+}
+
 // x / scale to e4m3, rounded to nearest even: the product with a power of two is exact, infinities
 // become the largest value, NaN stays.
 __device__ __forceinline__ float in_range(float x) { return x != x ? x : fminf(fmaxf(x, -448.f), 448.f); }
@@ -53,9 +67,43 @@ __device__ __forceinline__ uint32_t rescale(uint32_t w, float ratio) {
                  __builtin_amdgcn_cvt_f32_fp8((int)w, 2) * ratio, __builtin_amdgcn_cvt_f32_fp8((int)w, 3) * ratio);
 }
 
-__device__ __forceinline__ float finite_magnitude(float x) {
-  x = __builtin_fabsf(x);
-  return x < __builtin_inff() ? x : 0.f;  // false for NaN too
+// The largest finite magnitude in the wave.  Magnitudes of either 16-bit type order as their bits do; only where
+// infinities or NaN are among them are those taken out.
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+template <typename T>
+constexpr uint32_t kInfBits = 0x7c00u;
+template <>
+constexpr uint32_t kInfBits<__bf16> = 0x7f80u;
+
+template <int X>
+__device__ __forceinline__ u16x2 wave_max(u16x2 m) {
+  m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, lane_xor<X>(__builtin_bit_cast(uint32_t, m))));
+  if constexpr (X > 1) m = wave_max<X / 2>(m);
+  return m;
+}
+template <typename T, int C>
+__device__ __forceinline__ float largest_magnitude(const uint32_t x[C][8]) {
+  u16x2 m = {0, 0};
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, x[c][i] & 0x7fff7fffu));
+  m = wave_max<32>(m);
+  uint32_t top = m.x > m.y ? m.x : m.y;
+  if (top >= kInfBits<T>) {
+    m = u16x2{0, 0};
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t w = x[c][i] & 0x7fff7fffu;
+        const uint32_t lo = w & 0xffffu, hi = w >> 16;
+        m = __builtin_elementwise_max(m, u16x2{(unsigned short)(lo < kInfBits<T> ? lo : 0u), (unsigned short)(hi < kInfBits<T> ? hi : 0u)});
+      }
+    m = wave_max<32>(m);
+    top = m.x > m.y ? m.x : m.y;
+  }
+  return low_half<T>(top);
 }
 
 // The least power of two s in [2^-40, 2^80] with a <= 448 s, from the bits of a = 1.m x 2^e:
@@ -72,7 +120,7 @@ __global__ __launch_bounds__(P <= 64 ? 256 : 512) void bsg_kv_append_kernel(Appe
   constexpr int UNITS = P <= 64 ? 4 / W : 1;  // (page, head, K/V) units of a work-group
   constexpr int C = D / 64;
   __shared__ float s_max[UNITS][W];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int unit = wave / W, tile = wave % W;
   // units in the order head, K/V, page of the row, row: neighbours write neighbouring bytes
   const uint32_t u = blockIdx.x * UNITS + unit, per_page = 2 * p.heads;
@@ -80,16 +128,13 @@ __global__ __launch_bounds__(P <= 64 ? 256 : 512) void bsg_kv_append_kernel(Appe
   const int head = hk >> 1, kv = hk & 1;
   const int row = rp / p.pages_per_row, nth = rp - row * p.pages_per_row;
 
-  bool fine = u < (uint32_t)p.units;
-  int slot = -1;
-  int64_t from = 0, to = 0;
-  if (fine) {
-    slot = p.slots ? p.slots[row] : row;
-    from = p.cu ? p.cu[row] : (int64_t)row * p.max_new;
-    to = p.cu ? p.cu[row + 1] : from + p.max_new;
-  }
-  fine = slot >= 0 && slot < p.num_slots && from >= 0 && from < to && to <= p.tokens;
-  int64_t len = fine ? p.lengths[slot] : 0;
+  const bool real = u < (uint32_t)p.units;
+  int64_t from = (int64_t)row * p.max_new, to = from + p.max_new;
+  int slot = real ? row : -1;
+  if (p.slots && real) slot = p.slots[row];
+  int64_t len = slot >= 0 && slot < p.num_slots ? p.lengths[slot] : 0;  // on its way beside the offsets
+  if (p.cu && real) from = p.cu[row], to = p.cu[row + 1];
+  bool fine = slot >= 0 && slot < p.num_slots && from >= 0 && from < to && to <= p.tokens;
   const int64_t start = len - (to - from);  // may be below 0: tokens at negative positions are not written
   const int64_t most = (int64_t)p.max_pages * P;
   if (len > most) len = most;
@@ -104,6 +149,25 @@ __global__ __launch_bounds__(P <= 64 ? 256 : 512) void bsg_kv_append_kernel(Appe
   const int t = lane & 15, g = lane >> 4;
   const int tok = tile * 16 + t;
   const bool is_new = fine && tok >= lo && tok < hi;
+  float* const scale_at = p.scales + ((int64_t)page * p.heads + head) * 2 + kv;
+  const float old = fine && lo > 0 ? *scale_at : 0.f;
+  uint8_t* const dst = p.pages + (((int64_t)page * p.heads + head) * 2 + kv) * (P * D) + (int64_t)tile * 16 * D;
+  // Bytes of the values' dwords (tokens 4q .. 4q+3) that are new, and that hold earlier tokens; what
+  // is there is on its way while the new ones are weighed.
+  uint32_t fresh = 0, held = 0;
+  u32x4 was[C];
+  const int v_off = (t >> 2) * 256 + (4 * g + (t & 3)) * 16;
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    const int k = tile * 16 + (t & 12) + b;
+    if (k >= lo && k < hi) fresh |= 0xffu << (8 * b);
+    if (k < lo) held |= 0xffu << (8 * b);
+  }
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    was[c] = u32x4{0u, 0u, 0u, 0u};
+    if (kv == 1 && fine && fresh != 0xffffffffu && (fresh | held) != 0) was[c] = *(const u32x4*)(dst + c * 1024 + v_off);
+  }
   uint32_t x[C][8];
 #pragma unroll
   for (int c = 0; c < C; ++c)
@@ -126,16 +190,7 @@ __global__ __launch_bounds__(P <= 64 ? 256 : 512) void bsg_kv_append_kernel(Appe
         for (int i = 0; i < 8; ++i) x[c][i] = src[64 * c + 2 * i] | (uint32_t)src[64 * c + 2 * i + 1] << 16;
     }
   }
-  float a = 0.f;
-#pragma unroll
-  for (int c = 0; c < C; ++c)
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      a = fmaxf(a, fmaxf(finite_magnitude(low_half<T>(x[c][i])), finite_magnitude(high_half<T>(x[c][i]))));
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) a = fmaxf(a, __shfl_xor(a, m));
-  float* const scale_at = p.scales + ((int64_t)page * p.heads + head) * 2 + kv;
-  const float old = fine && lo > 0 ? *scale_at : 0.f;
+  float a = largest_magnitude<T, C>(x);
   if constexpr (W > 1) {  // also: every wave has the old scale before one writes the new
     if (lane == 0) s_max[unit][tile] = a;
     __syncthreads();
@@ -154,7 +209,6 @@ __global__ __launch_bounds__(P <= 64 ? 256 : 512) void bsg_kv_append_kernel(Appe
   if (tile * 16 >= hi || (tile * 16 + 16 <= lo && ratio == 1.f)) return;
 
   const float inv = 1.f / scale;
-  uint8_t* const dst = p.pages + (((int64_t)page * p.heads + head) * 2 + kv) * (P * D) + (int64_t)tile * 16 * D;
   uint32_t y[C][4];
 #pragma unroll
   for (int c = 0; c < C; ++c)
@@ -174,30 +228,25 @@ __global__ __launch_bounds__(P <= 64 ? 256 : 512) void bsg_kv_append_kernel(Appe
       }
     }
   } else {
-    // lane i of quad q: channel 4n + i of tokens 4q .. 4q+3
-    const int i = t & 3, q = t >> 2;
-    uint32_t fresh = 0, held = 0;  // bytes of new tokens, and of earlier ones
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const int k = tile * 16 + 4 * q + b;
-      if (k >= lo && k < hi) fresh |= 0xffu << (8 * b);
-      if (k < lo) held |= 0xffu << (8 * b);
-    }
     const bool rounds = held != 0 && ratio != 1.f;
 #pragma unroll
-    for (int c = 0; c < C; ++c)
+    for (int c = 0; c < C; ++c) {
+      uint32_t w[4];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        uint32_t w = quad_transpose(y[c][n], i);
-        uint32_t* const at = (uint32_t*)(dst + c * 1024 + q * 256 + (4 * n + i) * 16 + g * 4);
-        if (fresh != 0xffffffffu) {
-          if (fresh == 0 && !rounds) continue;
-          const uint32_t was = *at;
-          const uint32_t kept = rounds ? (rescale(was, ratio) & held) | (was & ~held) : was;
-          w = (w & fresh) | (kept & ~fresh);
-        }
-        *at = w;
+      for (int n = 0; n < 4; ++n) w[n] = quad_transpose(y[c][n], t & 3);
+      row_transpose(w);  // lane 16 g + 4 q + i: channels 16 n + 4 g + i of tokens 4 q .. 4 q + 3
+      u32x4* const at = (u32x4*)(dst + c * 1024 + v_off);
+      u32x4 v = {w[0], w[1], w[2], w[3]};
+      if (fresh != 0xffffffffu) {
+        if (fresh == 0 && !rounds) continue;
+        u32x4 kept = was[c];
+        if (rounds)
+          kept = (u32x4{rescale(kept.x, ratio), rescale(kept.y, ratio), rescale(kept.z, ratio), rescale(kept.w, ratio)} & held) |
+                 (kept & ~held);
+        v = (v & fresh) | (kept & ~fresh);
       }
+      *at = v;
+    }
   }
 }
 

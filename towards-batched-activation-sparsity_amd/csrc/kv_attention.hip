@@ -146,11 +146,49 @@ __device__ __forceinline__ void nan_values(u32x4 v[2], int t, const int* sees, f
     }
 }
 
+// Sum of a tile's parts: `rows` rows of D numbers in each of `chunks` parts, every part times its
+// factor, s_f[row * FL + 2 * part]; done(row, channel, sum) gets four numbers at a time.  ITEMS x PARTS
+// loads in flight for each thread: many parts of few rows, or few parts of many rows.
+template <int D, int FL, int ITEMS, int PARTS, typename Done>
+__device__ __forceinline__ void sum_parts(__amdgpu_buffer_rsrc_t r, int part_bytes, int row0, int rows, int chunks,
+                                          const float* s_f, const Done& done) {
+  constexpr int PER = D / 4;
+  for (int e0 = threadIdx.x; e0 < rows * PER; e0 += ITEMS * 256) {
+    f32x4 o[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < chunks; s += PARTS) {
+      f32x4 v[PARTS][ITEMS];
+#pragma unroll
+      for (int j = 0; j < PARTS; ++j)
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+          const int e = e0 + 256 * i;
+          // an offset past the buffer loads zeros
+          const int at = e < rows * PER && s + j < chunks ? (s + j) * part_bytes + (row0 * PER + e) * 16 : -1;
+          v[j][i] = hand_load16(r, at);
+        }
+#pragma unroll
+      for (int j = 0; j < PARTS; ++j)
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+          const int e = e0 + 256 * i;
+          if (e < rows * PER && s + j < chunks) o[i] += v[j][i] * s_f[e / PER * FL + 2 * (s + j)];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int e = e0 + 256 * i;
+      if (e < rows * PER) done(row0 + e / PER, e % PER * 4, o[i]);
+    }
+  }
+}
+
 // A work-group of four waves computes RT x 16 rows of one cached head of one sequence over one chunk
 // of its tokens; wave w takes the 32-token steps w, w + 4, ..., each with its own running maximum, and the
 // waves meet in LDS at the end.  Chunks meet in the workspace: the last one to arrive sums them in order.
 template <typename T, int D, int RT>
-__global__ __launch_bounds__(256) void bsg_kv_attention_kernel(AttnParams p) {
+__global__ __launch_bounds__(256, 2) void bsg_kv_attention_kernel(AttnParams p) {
   constexpr int C = D / 64, DT = D / 16, ROWS = 16 * RT, LD = D + 4;
   typedef typename Elem<T>::x8 x8;
   __shared__ float s_acc[ROWS * LD];
@@ -383,9 +421,10 @@ __global__ __launch_bounds__(256) void bsg_kv_attention_kernel(AttnParams p) {
     constexpr int PART = ROWS * (D + 2);
     float* const part = p.part + (tile * p.splits + split) * PART;
     parts = p.part + tile * p.splits * PART;
-    for (int e = threadIdx.x; e < used * (D / 2); e += 256) {
-      const int r = e / (D / 2), d = (e - r * (D / 2)) * 2;
-      hand_store((uint64_t*)(part + r * D + d), __builtin_bit_cast(uint64_t, *(const f32x2*)(s_acc + r * LD + d)));
+    const __amdgpu_buffer_rsrc_t mine_rsrc = hand_buffer(part, PART * 4);
+    for (int e = threadIdx.x; e < used * (D / 4); e += 256) {
+      const int r = e / (D / 4), d = (e - r * (D / 4)) * 4;
+      hand_store16(mine_rsrc, e * 16, *(const f32x4*)(s_acc + r * LD + d));
     }
     if ((int)threadIdx.x < used) {
       const int r = threadIdx.x;
@@ -428,30 +467,8 @@ __global__ __launch_bounds__(256) void bsg_kv_attention_kernel(AttnParams p) {
   }
   __syncthreads();
 
-  constexpr int PER = D / 4;  // a thread writes four channels of a row
-  for (int e = threadIdx.x; e < used * PER; e += 256) {
-    const int r = e / PER, d = (e - r * PER) * 4;
+  const auto finish = [&](int r, int d, f32x4 o) {
     const float top = s_m[0][r], sum = s_l[0][r];
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    if (chunks > 1) {
-      constexpr int PART = ROWS * (D + 2), BATCH = 8;  // parts in flight
-      for (int s0 = 0; s0 < chunks; s0 += BATCH) {
-        uint64_t v[BATCH][2];
-#pragma unroll
-        for (int j = 0; j < BATCH; ++j) {
-          const float* const q = parts + (s0 + j < chunks ? s0 + j : s0) * PART + r * D + d;
-          v[j][0] = hand_load((const uint64_t*)q), v[j][1] = hand_load((const uint64_t*)q + 1);
-        }
-#pragma unroll
-        for (int j = 0; j < BATCH; ++j) {
-          const float f = s0 + j < chunks ? s_acc[r * LD + 2 * (s0 + j)] : 0.f;
-          const f32x2 a = __builtin_bit_cast(f32x2, v[j][0]), b = __builtin_bit_cast(f32x2, v[j][1]);
-          if (s0 + j < chunks) o += f32x4{a.x, a.y, b.x, b.y} * f;
-        }
-      }
-    } else {
-      o = *(const f32x4*)(s_acc + r * LD + d);
-    }
     const int rr = rt * ROWS + r, tok = rr / p.group, h = head * p.group + rr - tok * p.group;
     const bool nothing = sum == 0.f;
     const float inv = nothing ? 0.f : 1.f / sum;
@@ -460,6 +477,13 @@ __global__ __launch_bounds__(256) void bsg_kv_attention_kernel(AttnParams p) {
     if (p.lse && d == 0)
       p.lse[(from + tok) * ((int64_t)p.kv_heads * p.group) + h] =
           nothing ? -__builtin_inff() : (top - kShift + __builtin_amdgcn_logf(sum)) * (1.f / kLog2e);
+  };
+  if (chunks > 1) {
+    constexpr int PART = ROWS * (D + 2);
+    sum_parts<D, LD, 1, 8>(hand_buffer(parts, chunks * PART * 4), PART * 4, 0, used, chunks, s_acc, finish);
+  } else {
+    for (int e = threadIdx.x; e < used * (D / 4); e += 256)
+      finish(e / (D / 4), e % (D / 4) * 4, *(const f32x4*)(s_acc + e / (D / 4) * LD + e % (D / 4) * 4));
   }
 }
 
@@ -768,16 +792,13 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
   constexpr int PART = ROWS * (D + 2);
   const float* const parts = p.part + tile * p.splits * PART;
   float* const part = p.part + (tile * p.splits + split) * PART;
+  const __amdgpu_buffer_rsrc_t mine_rsrc = hand_buffer(part, PART * 4);
 #pragma unroll
   for (int i = 0; i < RT; ++i) {
     const int r = 32 * wave + 16 * i + col;
     if (r < used) {
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        uint64_t* const at = (uint64_t*)(part + r * D + 16 * d + 4 * g);
-        hand_store(at, __builtin_bit_cast(uint64_t, f32x2{acc[i][d][0], acc[i][d][1]}));
-        hand_store(at + 1, __builtin_bit_cast(uint64_t, f32x2{acc[i][d][2], acc[i][d][3]}));
-      }
+      for (int d = 0; d < DT; ++d) hand_store16(mine_rsrc, (r * D + 16 * d + 4 * g) * 4, acc[i][d]);
       if (g == 0) hand_store((uint64_t*)(part + ROWS * D) + r, __builtin_bit_cast(uint64_t, f32x2{m[i], l[i]}));
     }
   }
@@ -811,25 +832,8 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
       f[1] = top, f[3] = sum;  // at least two parts
     }
     __syncthreads();
-    constexpr int PER = D / 4, BATCH = 8;
-    for (int e = threadIdx.x; e < n * PER; e += 256) {
-      const int r = e / PER, d = (e - r * PER) * 4;
-      f32x4 o = {0.f, 0.f, 0.f, 0.f};
-      for (int s0 = 0; s0 < chunks; s0 += BATCH) {
-        uint64_t v[BATCH][2];
-#pragma unroll
-        for (int j = 0; j < BATCH; ++j) {
-          const float* const q = parts + (s0 + j < chunks ? s0 + j : s0) * PART + (r0 + r) * D + d;
-          v[j][0] = hand_load((const uint64_t*)q), v[j][1] = hand_load((const uint64_t*)q + 1);
-        }
-#pragma unroll
-        for (int j = 0; j < BATCH; ++j) {
-          const f32x2 a = __builtin_bit_cast(f32x2, v[j][0]), b = __builtin_bit_cast(f32x2, v[j][1]);
-          if (s0 + j < chunks) o += f32x4{a.x, a.y, b.x, b.y} * s_f[r * FL + 2 * (s0 + j)];
-        }
-      }
-      finish(r0 + r, d, o, s_f[r * FL + 1], s_f[r * FL + 3]);
-    }
+    sum_parts<D, FL, 4, 2>(hand_buffer(parts, chunks * PART * 4), PART * 4, r0, n, chunks, s_f,
+                     [&](int r, int d, f32x4 o) { finish(r, d, o, s_f[(r - r0) * FL + 1], s_f[(r - r0) * FL + 3]); });
   }
 }
 
@@ -842,20 +846,24 @@ struct Shape {
 
 constexpr int kPrefillRows = 32;  // a cached head's rows past which the prefill kernel runs
 
-// How a call is cut: few rows leave most compute units idle unless the long axis is split.
+// How a call is cut.  Few work-groups leave most compute units idle unless the long axis is split, to
+// two for each unit and at least 256 tokens a part.  A part of 128 rows writes and reads 66 KiB, so
+// there only where units would have none at all, and not over less than 1024 tokens (a prompt of 500
+// alone: 23 us, 26 in two parts; 2 x 40 tokens over 1500: 24 us in six, 34 in two).
 Shape shape_of(int32_t rows, int32_t kv_heads, int32_t group, int32_t max_new, int64_t max_len, int32_t cus) {
   Shape s;
   const int64_t per_head = (int64_t)max_new * group;
   s.rows = per_head <= 16 ? 16 : per_head <= kPrefillRows ? 32 : 128;
   s.row_tiles = (int32_t)ceil_div(per_head, s.rows);
   const int64_t tiles = (int64_t)rows * kv_heads * s.row_tiles;
+  if (max_len < 1) max_len = 1;
   int64_t want = ceil_div((int64_t)2 * cus, tiles > 0 ? tiles : 1);
   if (want > kMaxSplits) want = kMaxSplits;
-  const int64_t most = ceil_div(max_len > 0 ? max_len : 1, 256);
-  if (want > most) want = most;
+  if (want > ceil_div(max_len, 256)) want = ceil_div(max_len, 256);
+  if (s.rows == 128 && (tiles >= cus || max_len < 1024)) want = 1;
   if (tiles * 4 > BSG_KV_COUNTER_BYTES) want = 1;
-  s.chunk = (int32_t)(ceil_div(ceil_div(max_len > 0 ? max_len : 1, want), 128) * 128);
-  s.splits = (int32_t)ceil_div(max_len > 0 ? max_len : 1, s.chunk);
+  s.chunk = (int32_t)(ceil_div(ceil_div(max_len, want), 128) * 128);
+  s.splits = (int32_t)ceil_div(max_len, s.chunk);
   return s;
 }
 

@@ -76,34 +76,6 @@ __device__ __forceinline__ float from_order(uint32_t o) {
 }
 __device__ __forceinline__ uint64_t key_of(uint32_t order, uint32_t id) { return (uint64_t)order << 32 | (uint32_t)~id; }
 
-// The value of lane ^ X.
-template <int X>
-__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
-  if constexpr (X == 1) return __builtin_amdgcn_mov_dpp(v, 0xb1, 0xf, 0xf, true);   // quad_perm 1 0 3 2
-  if constexpr (X == 2) return __builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, true);   // quad_perm 2 3 0 1
-  if constexpr (X == 4) {                                                           // 7 - i, then 3 - i in quads
-    v = __builtin_amdgcn_mov_dpp(v, 0x141, 0xf, 0xf, true);
-    return __builtin_amdgcn_mov_dpp(v, 0x1b, 0xf, 0xf, true);
-  }
-  if constexpr (X == 8) return __builtin_amdgcn_mov_dpp(v, 0x128, 0xf, 0xf, true);  // row_ror:8
-  if constexpr (X == 16) {
-    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    return threadIdx.x & 16 ? r[0] : r[1];
-  }
-  if constexpr (X == 32) {
-    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return threadIdx.x & 32 ? r[0] : r[1];
-  }
-}
-template <int X>
-__device__ __forceinline__ float lane_xor(float v) {
-  return as_float(lane_xor<X>(__builtin_bit_cast(uint32_t, v)));
-}
-template <int X>
-__device__ __forceinline__ uint64_t lane_xor(uint64_t v) {
-  return (uint64_t)lane_xor<X>((uint32_t)(v >> 32)) << 32 | lane_xor<X>((uint32_t)v);
-}
-
 // One step of a bitonic network of one value per lane: blocks of N sorted, every second the other
 // way round, the last (N = 64) largest first.
 template <int N, int X, typename V>

@@ -54,6 +54,34 @@ __device__ __forceinline__ float high_half<__bf16>(uint32_t w) {
   return __builtin_bit_cast(float, w & 0xffff0000u);
 }
 
+// The value of lane ^ X.
+template <int X>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+  if constexpr (X == 1) return __builtin_amdgcn_mov_dpp(v, 0xb1, 0xf, 0xf, true);   // quad_perm 1 0 3 2
+  if constexpr (X == 2) return __builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, true);   // quad_perm 2 3 0 1
+  if constexpr (X == 4) {                                                           // 7 - i, then 3 - i in quads
+    v = __builtin_amdgcn_mov_dpp(v, 0x141, 0xf, 0xf, true);
+    return __builtin_amdgcn_mov_dpp(v, 0x1b, 0xf, 0xf, true);
+  }
+  if constexpr (X == 8) return __builtin_amdgcn_mov_dpp(v, 0x128, 0xf, 0xf, true);  // row_ror:8
+  if constexpr (X == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return threadIdx.x & 16 ? r[0] : r[1];
+  }
+  if constexpr (X == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return threadIdx.x & 32 ? r[0] : r[1];
+  }
+}
+template <int X>
+__device__ __forceinline__ float lane_xor(float v) {
+  return as_float(lane_xor<X>(__builtin_bit_cast(uint32_t, v)));
+}
+template <int X>
+__device__ __forceinline__ uint64_t lane_xor(uint64_t v) {
+  return (uint64_t)lane_xor<X>((uint32_t)(v >> 32)) << 32 | lane_xor<X>((uint32_t)v);
+}
+
 // Partials cross work-groups with agent-scope relaxed atomics (device-coherent, with no fence that
 // would write back and invalidate a whole L2): every wave waits for its stores, the work-group
 // meets in a barrier, and one thread counts the arrival.
@@ -68,6 +96,17 @@ __device__ __forceinline__ float hand_load(const float* p) {
 }
 __device__ __forceinline__ uint64_t hand_load(const uint64_t* p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// The same 16 bytes at a time: a buffer's loads and stores with the scope bit of an agent (sc1).
+constexpr int kAgent = 16;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t hand_buffer(const void* base, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
+}
+__device__ __forceinline__ void hand_store16(__amdgpu_buffer_rsrc_t r, int off, f32x4 v) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, off, 0, kAgent);
+}
+__device__ __forceinline__ f32x4 hand_load16(__amdgpu_buffer_rsrc_t r, int off) {
+  return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, kAgent));
 }
 __device__ __forceinline__ void hand_publish() {
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
