@@ -64,7 +64,7 @@ def _ptr(t: Optional[torch.Tensor]) -> int:
 
 def _launch(index: int, fn, *args) -> None:
     """fn(*args, the current stream of device `index`), with that device current."""
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:
         status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):

@@ -25,34 +25,40 @@ struct Pool {
 __device__ __forceinline__ bool is_page(const Pool& p, int32_t id) { return id >= 0 && id < p.num_pages; }
 __device__ __forceinline__ bool is_slot(const Pool& p, int32_t s) { return s >= 0 && s < p.num_slots; }
 
-// One layer of one page, by `threads` threads of which this is `tid`: four 16-byte loads in flight
-// each.
-__device__ __forceinline__ void copy_page(const Pool& p, int64_t layer, int32_t src, int32_t dst, int tid, int threads) {
+// Pages move in pieces of 16 KiB, one for each work-group of 256 threads: four 16-byte loads in flight
+// for each thread, and enough work-groups for the machine from a few pages on.  Against one
+// work-group a page of 128 KiB: 28 copies x 4 layers 10.9 -> 9.8 us, 365 MB in and out 73 -> 66
+// (5.6 TB/s; a plain copy reaches 5.0).
+constexpr int64_t kPiece = 16384;
+constexpr int64_t kCopyGroups = 4096;  // of a data-moving launch: every compute unit several times over
+__host__ __device__ inline int64_t pieces_of(int64_t page_bytes) { return (page_bytes + kPiece - 1) / kPiece; }
+
+__device__ __forceinline__ void copy_piece(const Pool& p, int64_t layer, int32_t src, int32_t dst, int64_t piece) {
   const int64_t base = layer * p.num_pages;
+  const int64_t first = piece * (kPiece / 16) + threadIdx.x, n = p.page_bytes >> 4;
   const u32x4* const from = (const u32x4*)(p.pages + (base + src) * p.page_bytes);
   u32x4* const to = (u32x4*)(p.pages + (base + dst) * p.page_bytes);
-  const int64_t n = p.page_bytes >> 4;
-  for (int64_t i = tid; i < n; i += 4 * threads) {
-    u32x4 v[4];
+  u32x4 v[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (i + k * threads < n) v[k] = __builtin_nontemporal_load(from + i + k * threads);
+  for (int k = 0; k < 4; ++k)
+    if (first + 256 * k < n) v[k] = __builtin_nontemporal_load(from + first + 256 * k);
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (i + k * threads < n) __builtin_nontemporal_store(v[k], to + i + k * threads);
+  for (int k = 0; k < 4; ++k)
+    if (first + 256 * k < n) __builtin_nontemporal_store(v[k], to + first + 256 * k);
+  if (piece == 0) {
+    const float* const sf = p.scales + (base + src) * p.page_scales;
+    float* const st = p.scales + (base + dst) * p.page_scales;
+    for (int64_t i = threadIdx.x; i < p.page_scales; i += 256) st[i] = sf[i];
   }
-  const float* const sf = p.scales + (base + src) * p.page_scales;
-  float* const st = p.scales + (base + dst) * p.page_scales;
-  for (int64_t i = tid; i < p.page_scales; i += threads) st[i] = sf[i];
 }
 
 __global__ __launch_bounds__(256) void bsg_pages_copy_kernel(Pool p, const int32_t* __restrict__ src,
                                                              const int32_t* __restrict__ dst, int32_t n) {
-  for (int64_t item = blockIdx.x; item < (int64_t)n * p.layers; item += gridDim.x) {
-    const int64_t layer = item / n;
-    const int32_t i = (int32_t)(item - layer * n);
+  const int64_t pieces = pieces_of(p.page_bytes), each = p.layers * pieces;
+  for (int64_t item = blockIdx.x; item < n * each; item += gridDim.x) {
+    const int64_t i = item / each, part = item - i * each, layer = part / pieces;
     const int32_t s = src[i], d = dst[i];
-    if (is_page(p, s) && is_page(p, d) && s != d) copy_page(p, layer, s, d, threadIdx.x, 256);
+    if (is_page(p, s) && is_page(p, d) && s != d) copy_piece(p, layer, s, d, part - layer * pieces);
   }
 }
 
@@ -60,46 +66,55 @@ __global__ __launch_bounds__(256) void bsg_pages_copy_kernel(Pool p, const int32
 
 constexpr int kForkCols = 8;  // table columns of one work-group: 1024 pairs x 8 x 4 bytes of LDS
 
-// Every entry that a work-group overwrites lies in its own columns, and it has read all of them
-// (the parents' before the barrier, the child's by the thread that writes it) before it writes.
+// Every entry that a work-group overwrites lies in its own columns, and it has read them all, the
+// parents' and the children's, before a barrier, after which it writes.
 __global__ __launch_bounds__(256) void bsg_pages_fork_kernel(Pool p, const int32_t* __restrict__ parents,
                                                              const int32_t* __restrict__ children, int32_t n) {
-  __shared__ int32_t s_child[BSG_PAGES_MAX_ROWS];
-  __shared__ int32_t s_new[BSG_PAGES_MAX_ROWS * kForkCols];
+  constexpr int PER = BSG_PAGES_MAX_ROWS / 256;
+  __shared__ alignas(16) int32_t s_child[BSG_PAGES_MAX_ROWS + 4];
+  __shared__ int32_t s_parent[BSG_PAGES_MAX_ROWS];
+  __shared__ int32_t s_new[BSG_PAGES_MAX_ROWS * kForkCols], s_old[BSG_PAGES_MAX_ROWS * kForkCols];
   const int tid = threadIdx.x;
   const int c0 = blockIdx.x * kForkCols;
-  for (int i = tid; i < n; i += 256) {
-    const int32_t c = children[i];
-    s_child[i] = is_slot(p, c) && is_slot(p, parents[i]) ? c : -1;
+  for (int i = tid; i < ((n + 3) & ~3); i += 256) {
+    const int32_t c = i < n ? children[i] : -1, a = i < n ? parents[i] : -1;
+    s_child[i] = is_slot(p, c) && is_slot(p, a) ? c : -1;
+    s_parent[i] = a;
   }
-  __syncthreads();
-  // of pairs with the same child the last one counts
-  bool lost[BSG_PAGES_MAX_ROWS / 256];
-#pragma unroll
-  for (int k = 0; k < BSG_PAGES_MAX_ROWS / 256; ++k) {
-    const int i = tid + 256 * k;
-    lost[k] = false;
-    if (i < n && s_child[i] >= 0)
-      for (int j = i + 1; j < n; ++j) lost[k] |= s_child[j] == s_child[i];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < BSG_PAGES_MAX_ROWS / 256; ++k)
-    if (lost[k]) s_child[tid + 256 * k] = -1;
   __syncthreads();
   const bool lengths = c0 >= p.max_pages;  // the work-group past the columns moves the lengths
   const int cols = lengths ? 1 : p.max_pages - c0 < kForkCols ? p.max_pages - c0 : kForkCols;
   for (int e = tid; e < n * cols; e += 256) {
     const int i = e / cols, c = e - i * cols;
-    if (s_child[i] >= 0)
-      s_new[e] = lengths ? p.lengths[parents[i]] : p.table[parents[i] * p.table_stride + c0 + c];
+    if (s_child[i] >= 0) {
+      s_new[e] = lengths ? p.lengths[s_parent[i]] : p.table[s_parent[i] * p.table_stride + c0 + c];
+      s_old[e] = lengths ? p.lengths[s_child[i]] : p.table[s_child[i] * p.table_stride + c0 + c];
+    }
   }
+  // of pairs with the same child the last one counts
+  bool lost[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int i = tid + 256 * k;
+    lost[k] = false;
+    if (i < n && s_child[i] >= 0) {
+      const int32_t c = s_child[i];
+      for (int j = i & ~3; j < n; j += 4) {
+        const int4 v = *(const int4*)(s_child + j);
+        lost[k] |= (v.x == c && j > i) || (v.y == c && j + 1 > i) || (v.z == c && j + 2 > i) || (v.w == c && j + 3 > i);
+      }
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < PER; ++k)
+    if (lost[k]) s_child[tid + 256 * k] = -1;
   __syncthreads();
   for (int e = tid; e < n * cols; e += 256) {
     const int i = e / cols, c = e - i * cols;
     if (s_child[i] < 0) continue;
     int32_t* const at = lengths ? p.lengths + s_child[i] : p.table + s_child[i] * p.table_stride + c0 + c;
-    const int32_t was = *at, now = s_new[e];
+    const int32_t was = s_old[e], now = s_new[e];
     if (was == now) continue;
     *at = now;
     if (lengths) continue;
@@ -170,6 +185,8 @@ __global__ __launch_bounds__(kScan) void bsg_pages_extend_plan_kernel(Pool p, co
                                                                       int32_t* __restrict__ free_ids) {
   __shared__ int32_t s_tail[kScan];
   const int i = threadIdx.x;
+  int32_t v[4];
+  load_counts(p, 4 * i, v);  // the first free pages are mostly here: on their way while the rows are weighed
   const int32_t slot = i < n ? (slots ? slots[i] : i) : -1;
   const bool real = is_slot(p, slot);
   int64_t len = real ? p.lengths[slot] : 0;
@@ -193,8 +210,7 @@ __global__ __launch_bounds__(kScan) void bsg_pages_extend_plan_kernel(Pool p, co
   // the free pages, lowest first, until there are enough
   int found = 0;
   for (int64_t base = 0; base < p.num_pages && found < total; base += 4 * kScan) {
-    int32_t v[4];
-    load_counts(p, base + 4 * i, v);
+    if (base > 0) load_counts(p, base + 4 * i, v);
     const int mine = (v[0] == 0) + (v[1] == 0) + (v[2] == 0) + (v[3] == 0);
     int all;
     int at = found + block_scan(mine, &all);
@@ -234,9 +250,10 @@ __global__ __launch_bounds__(256) void bsg_pages_extend_kernel(Pool p, const Row
       }
     }
   }
+  const int64_t pieces = pieces_of(p.page_bytes);
   if (split)
-    for (int64_t layer = blockIdx.y; layer < p.layers; layer += gridDim.y)
-      copy_page(p, layer, r.copy_from, dst, threadIdx.x, 256);
+    for (int64_t part = blockIdx.y; part < p.layers * pieces; part += gridDim.y)
+      copy_piece(p, part / pieces, r.copy_from, dst, part % pieces);
 }
 
 // ---------------------------------------------------------------------------------------------- compact
@@ -302,10 +319,10 @@ __global__ __launch_bounds__(256) void bsg_pages_compact_kernel(Pool p, const in
     p.refs[free_ids[k]] = p.refs[src[k]];
     p.refs[src[k]] = 0;
   }
-  for (int64_t item = blockIdx.x; item < moved * p.layers; item += gridDim.x) {
-    const int64_t layer = item / moved;
-    const int32_t k = (int32_t)(item - layer * moved);
-    copy_page(p, layer, src[k], free_ids[k], threadIdx.x, 256);
+  const int64_t pieces = pieces_of(p.page_bytes), each = p.layers * pieces;
+  for (int64_t item = blockIdx.x; item < moved * each; item += gridDim.x) {
+    const int64_t k = item / each, part = item - k * each, layer = part / pieces;
+    copy_piece(p, layer, src[k], free_ids[k], part - layer * pieces);
   }
 }
 
@@ -366,8 +383,6 @@ int check_workspace(const bsg_page_pool* q, const void* ws, int64_t ws_bytes) {
   return BSG_OK;
 }
 
-// Work-groups of a data-moving launch: enough for every compute unit several times over.
-constexpr int64_t kCopyGroups = 4096;
 unsigned copy_grid(int64_t items) { return (unsigned)(items < kCopyGroups ? items : kCopyGroups); }
 
 }  // namespace
@@ -383,7 +398,7 @@ extern "C" int bsg_pages_copy(const bsg_page_pool* pool, const int32_t* src, con
   if (n < 0) return fail(BSG_ERR_ARG, "n=%d", n);
   if (n == 0) return BSG_OK;
   if (!src || !dst) return fail(BSG_ERR_ARG, "null pointer (src=%p dst=%p)", (const void*)src, (const void*)dst);
-  hipLaunchKernelGGL(bsg_pages_copy_kernel, dim3(copy_grid(n * pool->layers)), dim3(256), 0, (hipStream_t)stream,
+  hipLaunchKernelGGL(bsg_pages_copy_kernel, dim3(copy_grid(n * pool->layers * pieces_of(pool->page_bytes))), dim3(256), 0, (hipStream_t)stream,
                      device_pool(pool), src, dst, n);
   return launch_status("bsg_pages_copy");
 }
@@ -431,7 +446,9 @@ extern "C" int bsg_pages_extend(const bsg_page_pool* pool, const int32_t* slots,
   const hipStream_t st = (hipStream_t)stream;
   hipLaunchKernelGGL(bsg_pages_extend_plan_kernel, dim3(1), dim3(kScan), 0, st, p, slots, new_tokens, n, served, rows,
                      free_ids);
-  const int64_t gy = pool->layers < 256 ? pool->layers : 256;
+  // few rows need every piece a work-group of its own; many fill the machine with fewer
+  int64_t gy = pool->layers * pieces_of(pool->page_bytes);
+  if (gy > ceil_div(4 * kCopyGroups, n)) gy = ceil_div(4 * kCopyGroups, n);
   hipLaunchKernelGGL(bsg_pages_extend_kernel, dim3((unsigned)n, (unsigned)gy), dim3(256), 0, st, p, rows, free_ids);
   return launch_status("bsg_pages_extend");
 }
