@@ -148,8 +148,8 @@ int bsg_pages_compact(const bsg_page_pool* pool, int32_t* counts, void* ws, int6
  *   top_ids   : int32 [rows][k], top_logprobs: fp32 [rows][k]: the k <= BSG_LOGPROBS_MAX_K likeliest
  *               tokens, by (logit desc, id asc); -0 equals +0 and NaN ranks above every number
  * Rows of nothing but -inf give logprob -inf and entropy 0; a NaN in a row makes every number of the
- * row NaN, as does a +inf but for its ids.  Sums in 32 bits.  Workspace as bsg_kv_attention:
- * BSG_KV_COUNTER_BYTES of counters, zero before the first use and left zero. */
+ * row NaN, as does a +inf but for its ids.  Sums in 32 bits.  The aligned 16-byte granules that a
+ * row begins and ends in are read whole.  Workspace as bsg_kv_attention: BSG_KV_COUNTER_BYTES of counters, zero before the first use and left zero. */
 int64_t bsg_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int32_t k, int dtype, int32_t cu_count);
 int bsg_token_logprobs(const void* logits, int64_t row_stride, int64_t rows, int64_t vocab, const int32_t* tokens,
                        int32_t k, float* logprob, float* entropy, int32_t* top_ids, float* top_logprobs, int dtype,
