@@ -62,6 +62,18 @@ def _ptr(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+_MOLDS: Dict[tuple, torch.Tensor] = {}
+
+
+def _mold(shape, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
+    """A tensor of this shape over one element, for torch.empty_like: a contiguous tensor of the shape
+    at half of what torch.empty costs from Python."""
+    one = _MOLDS.get((dtype, dev))
+    if one is None:
+        one = _MOLDS[dtype, dev] = torch.empty(1, dtype=dtype, device=dev)
+    return one.expand(shape)
+
+
 def _launch(index: int, fn, *args) -> None:
     """fn(*args, the current stream of device `index`), with that device current."""
     if torch._C._cuda_getDevice() == index:
@@ -82,7 +94,7 @@ def _workspace(index: int, nbytes: int, prefix: Optional[str], cleared: bool = T
     prefix's buffer, and calls that may overlap must not share one.  A buffer is never given back while
     a graph may hold it: a larger one is made beside it."""
     key = (index, torch._C._cuda_getCurrentRawStream(index)) if prefix is None else (index, prefix)
-    if torch.cuda.is_current_stream_capturing():
+    if torch._C._cuda_isCurrentStreamCapturing():
         if prefix is None:
             ws = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
             if cleared:
@@ -220,17 +232,17 @@ def kv_attention(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, pag
     call = _CALLS.get(key)
     if call is None:
         call = _remember(key, _attention_call(q, pages, scales, page_table, lengths, cu_seqlens, max_new, slots, max_len, out, lse))
-    index, fn, sizes, rows, most, code, qt, qh, shape, longest, need, cus, scale = call
+    index, fn, sizes, rows, most, code, qt, qh, tokens, heads, out_mold, lse_mold, longest, need, cus, scale = call
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(out_mold)
     if lse is None:
-        lse = torch.empty(shape[:2], dtype=torch.float32, device=q.device)
+        lse = torch.empty_like(lse_mold)
     cache = _lib.KvCache(pages.data_ptr(), scales.data_ptr(), *sizes, page_table.data_ptr(), lengths.data_ptr())
     ws, room = 0, 0
     if need > 0:
         held = _workspace(index, need, workspace_prefix)
         ws, room = held.data_ptr(), held.numel()
-    _launch(index, fn, q.data_ptr(), qt, qh, shape[0], shape[1], cache, _ptr(slots), rows, _ptr(cu_seqlens), most, longest,
+    _launch(index, fn, q.data_ptr(), qt, qh, tokens, heads, cache, _ptr(slots), rows, _ptr(cu_seqlens), most, longest,
             scale if sm_scale is None else sm_scale, out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), code, ws, room, cus)
     return out, lse
 
@@ -253,8 +265,8 @@ def _attention_call(q, pages, scales, page_table, lengths, cu_seqlens, max_new, 
     longest = 0 if max_len is None else max(1, int(max_len))
     cache = _lib.KvCache(pages.data_ptr(), scales.data_ptr(), *sizes, page_table.data_ptr(), lengths.data_ptr())
     need = int(lib.bsg_kv_attention_workspace_bytes(cache, rows, heads, most, longest, cus))
-    return (dev.index, lib.bsg_kv_attention, sizes, rows, most, code, q.stride(0), q.stride(1), tuple(q.shape), longest, need, cus,
-            d ** -0.5)
+    return (dev.index, lib.bsg_kv_attention, sizes, rows, most, code, q.stride(0), q.stride(1), tokens, heads,
+            _mold(q.shape, q.dtype, dev), _mold(q.shape[:2], torch.float32, dev), longest, need, cus, d ** -0.5)
 
 
 def _pool(kind: str, page_table=None, lengths=None, refcounts=None, pages=None, scales=None, *others):
@@ -384,11 +396,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0,
     call = _CALLS.get(key)
     if call is None:
         call = _remember(key, _logprobs_call(logits, tokens, k))
-    index, fn, rows, vocab, stride, k, code, need, cus = call
-    dev = logits.device
-    out = TokenLogprobs(torch.empty(rows, dtype=torch.float32, device=dev), torch.empty(rows, dtype=torch.float32, device=dev),
-                        torch.empty((rows, k), dtype=torch.int32, device=dev),
-                        torch.empty((rows, k), dtype=torch.float32, device=dev))
+    index, fn, rows, vocab, stride, k, code, need, cus, molds = call
+    out = TokenLogprobs(*map(torch.empty_like, molds))
     ws, room = 0, 0
     if need > 0:
         held = _workspace(index, need, workspace_prefix)
@@ -415,7 +424,9 @@ def _logprobs_call(logits: torch.Tensor, tokens: torch.Tensor, k: int) -> tuple:
     code = _LOGIT_DTYPES[logits.dtype]
     lib, cus = load(), _cu_count(dev)
     need = int(lib.bsg_token_logprobs_workspace_bytes(rows, vocab, k, code, cus))
-    return dev.index, lib.bsg_token_logprobs, rows, vocab, logits.stride(0), k, code, need, cus
+    molds = [_mold(s, t, dev) for s, t in (((rows,), torch.float32), ((rows,), torch.float32), ((rows, k), torch.int32),
+                                           ((rows, k), torch.float32))]
+    return dev.index, lib.bsg_token_logprobs, rows, vocab, logits.stride(0), k, code, need, cus, molds
 
 
 def read_pages(pages: torch.Tensor, scales: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -26,7 +26,7 @@ int check_kv_batch(int64_t tokens, int32_t rows, const int32_t* slots, const int
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kMaxSplits = 32;    // parts of one row, which meet in LDS
+constexpr int kMaxSplits = 32;    // parts of one row
 constexpr float kShift = 14.f;  // weights go up to 2^(kShift + kSlack), within fp16
 constexpr float kSlack = 1.5f;  // what a score may exceed the running maximum by before that moves
 constexpr float kMostWeight = 46340.f;  // 2^(kShift + kSlack)
@@ -147,12 +147,12 @@ __device__ __forceinline__ void nan_values(u32x4 v[2], int t, const int* sees, f
 }
 
 // Sum of a tile's parts: `rows` rows of D numbers in each of `chunks` parts, every part times its
-// factor, s_f[row * FL + 2 * part]; done(row, channel, sum) gets four numbers at a time.  ITEMS x PARTS
-// loads in flight for each thread: many parts of few rows, or few parts of many rows.
-template <int D, int FL, int ITEMS, int PARTS, typename Done>
+// factor, s_f[row * FL + 2 * part]; done(row, channel, sum) gets four numbers at a time.  Four rows' and
+// two parts' loads are in flight for each thread.
+template <int D, int FL, typename Done>
 __device__ __forceinline__ void sum_parts(__amdgpu_buffer_rsrc_t r, int part_bytes, int row0, int rows, int chunks,
                                           const float* s_f, const Done& done) {
-  constexpr int PER = D / 4;
+  constexpr int PER = D / 4, ITEMS = 4, PARTS = 2;
   for (int e0 = threadIdx.x; e0 < rows * PER; e0 += ITEMS * 256) {
     f32x4 o[ITEMS];
 #pragma unroll
@@ -414,7 +414,6 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_attention_kernel(AttnParams p) 
   }
 
   const int used = rows < ROWS ? rows : ROWS;
-  // per row: the factor of each part (s_m), and one over the sum of weights (s_l)
   const float* parts = nullptr;
   if (chunks > 1) {
     const int64_t tile = ((int64_t)row * p.kv_heads + head) * p.row_tiles + rt;
@@ -440,35 +439,43 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_attention_kernel(AttnParams p) 
     __syncthreads();
     if (!s_last) return;
     if (threadIdx.x == 0) hand_reset(p.counters + tile);
-    // every part's maximum and sum at once, then their factors, in s_acc ([row][part], two numbers each)
-    for (int e = threadIdx.x; e < used * chunks; e += 256) {
-      const int r = e / chunks, s = e - r * chunks;
-      const f32x2 v = __builtin_bit_cast(f32x2, hand_load((const uint64_t*)(parts + s * PART + ROWS * D) + r));
-      s_acc[r * LD + 2 * s] = v.x, s_acc[r * LD + 2 * s + 1] = v.y;
-    }
-    __syncthreads();
-    if ((int)threadIdx.x < used) {
-      float* const f = s_acc + threadIdx.x * LD;
-      float top = -__builtin_inff(), sum = 0.f;
-      for (int s = 0; s < chunks; ++s) top = fmaxf(top, f[2 * s]);
-      for (int s = 0; s < chunks; ++s) {
-        f[2 * s] = f[2 * s] == top ? 1.f : __builtin_amdgcn_exp2f(f[2 * s] - top);
-        sum += f[2 * s] * f[2 * s + 1];
-      }
-      s_m[0][threadIdx.x] = top, s_l[0][threadIdx.x] = sum;
-    }
-  } else if ((int)threadIdx.x < used) {
-    const int r = threadIdx.x;
-    const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
-    float sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) sum += s_l[w][r] * (s_m[w][r] == top ? 1.f : __builtin_amdgcn_exp2f(s_m[w][r] - top));
-    s_m[0][r] = top, s_l[0][r] = sum;
   }
-  __syncthreads();
 
-  const auto finish = [&](int r, int d, f32x4 o) {
-    const float top = s_m[0][r], sum = s_l[0][r];
+  for (int e = threadIdx.x; e < used * (D / 4); e += 256) {
+    const int r = e / (D / 4), d = e % (D / 4) * 4;
+    float top = -__builtin_inff(), sum = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    if (chunks > 1) {
+      // four numbers of a row from every part, with the part's maximum and sum, eight parts in flight
+      constexpr int PART = ROWS * (D + 2), BATCH = 8;
+      const __amdgpu_buffer_rsrc_t all = hand_buffer(parts, chunks * PART * 4);
+      for (int s = 0; s < chunks; s += BATCH) {
+        f32x4 v[BATCH];
+        f32x2 ml[BATCH];
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+          const int at = s + j < chunks ? (s + j) * PART * 4 : 0x40000000;  // past the buffer: zeros
+          v[j] = hand_load16(all, at + e * 16);
+          ml[j] = hand_load8(all, at + (ROWS * D + 2 * r) * 4);
+        }
+        float high = top;
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) high = s + j < chunks ? fmaxf(high, ml[j].x) : high;
+        const float f = top == high ? 1.f : __builtin_amdgcn_exp2f(top - high);
+        o *= f, sum *= f, top = high;
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j)
+          if (s + j < chunks) {
+            const float w = ml[j].x == top ? 1.f : __builtin_amdgcn_exp2f(ml[j].x - top);
+            o += v[j] * w, sum += ml[j].y * w;
+          }
+      }
+    } else {
+      top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+#pragma unroll
+      for (int w = 0; w < 4; ++w) sum += s_l[w][r] * (s_m[w][r] == top ? 1.f : __builtin_amdgcn_exp2f(s_m[w][r] - top));
+      o = *(const f32x4*)(s_acc + r * LD + d);
+    }
     const int rr = rt * ROWS + r, tok = rr / p.group, h = head * p.group + rr - tok * p.group;
     const bool nothing = sum == 0.f;
     const float inv = nothing ? 0.f : 1.f / sum;
@@ -477,13 +484,6 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_attention_kernel(AttnParams p) 
     if (p.lse && d == 0)
       p.lse[(from + tok) * ((int64_t)p.kv_heads * p.group) + h] =
           nothing ? -__builtin_inff() : (top - kShift + __builtin_amdgcn_logf(sum)) * (1.f / kLog2e);
-  };
-  if (chunks > 1) {
-    constexpr int PART = ROWS * (D + 2);
-    sum_parts<D, LD, 1, 8>(hand_buffer(parts, chunks * PART * 4), PART * 4, 0, used, chunks, s_acc, finish);
-  } else {
-    for (int e = threadIdx.x; e < used * (D / 4); e += 256)
-      finish(e / (D / 4), e % (D / 4) * 4, *(const f32x4*)(s_acc + e / (D / 4) * LD + e % (D / 4) * 4));
   }
 }
 
@@ -832,7 +832,7 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
       f[1] = top, f[3] = sum;  // at least two parts
     }
     __syncthreads();
-    sum_parts<D, FL, 4, 2>(hand_buffer(parts, chunks * PART * 4), PART * 4, r0, n, chunks, s_f,
+    sum_parts<D, FL>(hand_buffer(parts, chunks * PART * 4), PART * 4, r0, n, chunks, s_f,
                      [&](int r, int d, f32x4 o) { finish(r, d, o, s_f[(r - r0) * FL + 1], s_f[(r - r0) * FL + 3]); });
   }
 }

@@ -107,15 +107,18 @@ __device__ __forceinline__ V sort_steps(V v) {
   if constexpr (N > 2) v = sort_steps<N / 2>(v);
   return merge_steps<N, N / 2>(v);
 }
+// Sorted, the largest in lane 0, or in lane 63.
 template <typename V>
-__device__ __forceinline__ V sorted(V v) {
+__device__ __forceinline__ V sorted_down(V v) {
   return sort_steps<64>(v);
 }
-// The 64 largest of two lists, both largest first.
-__device__ __forceinline__ uint64_t merged(uint64_t a, uint64_t b) {
-  // b the other way round: lane 63 - i
-  b = lane_xor<32>(lane_xor<16>(lane_xor<8>(lane_xor<4>(lane_xor<2>(lane_xor<1>(b))))));
-  return merge_steps<64, 32>(a > b ? a : b);
+template <typename V>
+__device__ __forceinline__ V sorted_up(V v) {
+  return (V)~sort_steps<64>((V)~v);
+}
+// The 64 largest of two lists, the first largest first, the second largest last; largest first.
+__device__ __forceinline__ uint64_t merged(uint64_t down, uint64_t up) {
+  return merge_steps<64, 32>(down > up ? down : up);
 }
 
 struct Sums {
@@ -171,7 +174,7 @@ struct Best {
     } else {
       if (waiting > 64 && lane < waiting - 64) wait[lane] = rest;
       waiting = waiting > 64 ? waiting - 64 : 0;
-      list = merged(list, sorted(v));
+      list = merged(list, sorted_up(v));
     }
     const uint32_t kth = (uint32_t)__builtin_amdgcn_readlane((int)(list >> 32), k - 1);
     bar = bar > kth ? bar : kth;
@@ -222,33 +225,40 @@ __device__ __forceinline__ uint32_t clip_tile(u32x4 raw[kVectors], int64_t id0, 
 }
 
 // A tile into the sums and the alternatives; there: a bit for each of the lane's logits that is one of
-// the row (the others are -inf).
+// the row (the others are -inf); used: the vectors that any lane has.
 template <typename T>
-__device__ __forceinline__ void take_tile(const u32x4 raw[kVectors], uint32_t there, int64_t id0, int k, bool first, Sums& sum,
+__device__ __forceinline__ void take_tile(const u32x4 raw[kVectors], uint32_t there, int used, int64_t id0, int k, bool first, Sums& sum,
                                           Best& best) {
   typedef Logit<T> L;
   constexpr int N = L::N;
   const int lane = threadIdx.x & 63;
-  float top = -__builtin_inff(), low = __builtin_inff();
+  float top = -__builtin_inff(), low = __builtin_inff(), tops[kVectors];
 #pragma unroll
-  for (int i = 0; i < kVectors; ++i)
+  for (int i = 0; i < kVectors; ++i) {
+    tops[i] = -__builtin_inff();
+    if (i < used) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const float v = L::at(raw[i], j);
-      top = fmaxf(top, v);
-      low = fminf(low, v);
+      for (int j = 0; j < N; ++j) {
+        const float v = L::at(raw[i], j);
+        tops[i] = fmaxf(tops[i], v);
+        low = fminf(low, v);
+      }
     }
+    top = fmaxf(top, tops[i]);
+  }
   float l = 0.f, t = 0.f;
   if (!__any(top > sum.m + kSlack || low < kLow || !(__builtin_fabsf(sum.m) < kHuge))) {
     const float base = sum.m * kLog2e;
 #pragma unroll
     for (int i = 0; i < kVectors; ++i)
+      if (i < used) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float d = __builtin_fmaf(L::at(raw[i], j), kLog2e, -base);
-        const float e = __builtin_amdgcn_exp2f(d);
-        l += e;
-        t = __builtin_fmaf(e, d, t);
+        for (int j = 0; j < N; ++j) {
+          const float d = __builtin_fmaf(L::at(raw[i], j), kLog2e, -base);
+          const float e = __builtin_amdgcn_exp2f(d);
+          l += e;
+          t = __builtin_fmaf(e, d, t);
+        }
       }
     sum.l += l, sum.t += t;
   } else {  // a new reference, or numbers that need care
@@ -258,12 +268,14 @@ __device__ __forceinline__ void take_tile(const u32x4 raw[kVectors], uint32_t th
     const float c = huge ? 0.f : -(m * kLog2e), u = huge ? m : 0.f;
 #pragma unroll
     for (int i = 0; i < kVectors; ++i)
+      if (i < used) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float d = __builtin_fmaf(L::at(raw[i], j) - u, kLog2e, c);
-        const float e = __builtin_amdgcn_exp2f(d);
-        l += e;
-        t = __builtin_fmaf(e, fmaxf(d, kFloor), t);
+        for (int j = 0; j < N; ++j) {
+          const float d = __builtin_fmaf(L::at(raw[i], j) - u, kLog2e, c);
+          const float e = __builtin_amdgcn_exp2f(d);
+          l += e;
+          t = __builtin_fmaf(e, fmaxf(d, kFloor), t);
+        }
       }
     sum = join(sum, Sums{top, l, t});
   }
@@ -274,30 +286,34 @@ __device__ __forceinline__ void take_tile(const u32x4 raw[kVectors], uint32_t th
     if (l != l) {  // a NaN or +inf among them
 #pragma unroll
       for (int i = 0; i < kVectors; ++i)
+        if (i < used) {
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-          if (L::at(raw[i], j) != L::at(raw[i], j)) mine = 0xffffffffu;
+          for (int j = 0; j < N; ++j)
+            if (L::at(raw[i], j) != L::at(raw[i], j)) mine = 0xffffffffu;
+        }
     }
     // what equals the bar enters too: of the k at or above it the ids are not known
-    const uint32_t kth = (uint32_t)__builtin_amdgcn_readlane((int)sorted(mine), k - 1);
+    const uint32_t kth = (uint32_t)__builtin_amdgcn_readlane((int)sorted_down(mine), k - 1);
     best.bar = kth < 2 ? 0 : kth - (kth == 0x80000000u ? 2 : 1);  // below +0 comes -0, its equal
   }
   // The bar as a number; what is above it enters, and a NaN.  No number is above a bar of +inf, every
   // one above a bar of NaN, which stands for fewer than k keys so far.
   const float bar = best.bar == 0 ? __builtin_nanf("") : best.bar >= 0xff800000u ? __builtin_inff() : from_order(best.bar);
-  if (!__any(!(top <= bar) || l != l)) return;
+  const bool nan = l != l;
+  if (!__any(!(top <= bar) || nan)) return;
 
   // Few enter; each lane takes its own one at a time, by position, from a copy of the tile in LDS.
   uint32_t mask = 0;
-#pragma unroll
-  for (int i = 0; i < kVectors; ++i)
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (!(L::at(raw[i], j) <= bar)) mask |= 1u << (i * N + j);
-  mask &= there;
   u32x4* const copy = (u32x4*)(best.wait + 128);
 #pragma unroll
-  for (int i = 0; i < kVectors; ++i) copy[64 * i + lane] = raw[i];
+  for (int i = 0; i < kVectors; ++i)
+    if (i < used && __any(!(tops[i] <= bar) || nan)) {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (!(L::at(raw[i], j) <= bar)) mask |= 1u << (i * N + j);
+      copy[64 * i + lane] = raw[i];
+    }
+  mask &= there;
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   for (bool more = __any(mask != 0); more;) {
     const int bit = mask != 0 ? __builtin_ctz(mask) : 0;
@@ -354,7 +370,8 @@ __global__ __launch_bounds__(64 * kWaves) void bsg_token_logprobs_kernel(ScorePa
     const int64_t id0 = v0 * N - skip;
     uint32_t there = 0xffffffffu;
     if (id0 < 0 || v0 + STEP > v_end || id0 + STEP * N > p.vocab) there = clip_tile<T>(raw, id0, v_end - v0, p.vocab);
-    take_tile<T>(raw, there, id0, k, v0 == v_begin, sum, best);
+    const int used = v0 + STEP <= v_end ? kVectors : (int)((v_end - v0 + 63) >> 6);
+    take_tile<T>(raw, there, used, id0, k, v0 == v_begin, sum, best);
   }
   sum = join_lanes<1>(sum);
 
@@ -367,7 +384,7 @@ __global__ __launch_bounds__(64 * kWaves) void bsg_token_logprobs_kernel(ScorePa
       }
       __syncthreads();
       if ((part & (2 * step - 1)) == 0) {
-        if (k > 0) best.list = merged(best.list, s_wait[wave + step][lane]);
+        if (k > 0) best.list = merged(best.list, s_wait[wave + step][63 - lane]);
         sum = join(sum, s_sum[wave + step]);
       }
     }
@@ -404,7 +421,7 @@ __global__ __launch_bounds__(64 * kWaves) void bsg_token_logprobs_kernel(ScorePa
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll 1
-      for (int i = 0; part + i * W < p.splits; ++i) best.list = merged(best.list, lists[64 * i + lane]);
+      for (int i = 0; part + i * W < p.splits; ++i) best.list = merged(best.list, lists[64 * i + 63 - lane]);
     }
     meet();
   }
@@ -431,13 +448,14 @@ struct Shape {
 };
 
 // Waves of a row: enough rows fill the machine with one wave each (16 per compute unit); fewer take up
-// to the four of a work-group, and long ones several work-groups, which leave each wave kSplitTiles tiles: 64
-// rows of 32000 with 8 alternatives take 14.9 us so, 15.8 in twice the work-groups.
+// to the four of a work-group, with two vectors a lane at least (2000 rows of 1000, 5 alternatives: 8.0
+// us, 10.9 with one), and long ones several work-groups, which leave each wave kSplitTiles tiles (64 rows of
+// 32000 with 8 alternatives: 14.9 us so, 15.8 in twice the work-groups).
 Shape shape_of(int64_t rows, int64_t vocab, int per_vector, int32_t cus) {
   const int64_t vectors = ceil_div(vocab, per_vector) + 1;  // a row may begin inside a vector
   Shape s;
   s.log_waves = 0;
-  while ((1 << s.log_waves) < kWaves && (rows << s.log_waves) < 16 * (int64_t)cus && (64 << s.log_waves) < vectors)
+  while ((1 << s.log_waves) < kWaves && (rows << s.log_waves) < 16 * (int64_t)cus && (128 << s.log_waves) < vectors)
     ++s.log_waves;
   int64_t want = vectors / (64 * kWaves * kVectors * kSplitTiles);
   if (rows > 0 && want > 2 * cus / rows) want = 2 * cus / rows;

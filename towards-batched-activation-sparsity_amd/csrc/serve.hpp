@@ -85,14 +85,8 @@ __device__ __forceinline__ uint64_t lane_xor(uint64_t v) {
 // Partials cross work-groups with agent-scope relaxed atomics (device-coherent, with no fence that
 // would write back and invalidate a whole L2): every wave waits for its stores, the work-group
 // meets in a barrier, and one thread counts the arrival.
-__device__ __forceinline__ void hand_store(float* p, float v) {
-  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
 __device__ __forceinline__ void hand_store(uint64_t* p, uint64_t v) {
   __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ float hand_load(const float* p) {
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 __device__ __forceinline__ uint64_t hand_load(const uint64_t* p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -107,6 +101,9 @@ __device__ __forceinline__ void hand_store16(__amdgpu_buffer_rsrc_t r, int off, 
 }
 __device__ __forceinline__ f32x4 hand_load16(__amdgpu_buffer_rsrc_t r, int off) {
   return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, kAgent));
+}
+__device__ __forceinline__ f32x2 hand_load8(__amdgpu_buffer_rsrc_t r, int off) {
+  return __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, kAgent));
 }
 __device__ __forceinline__ void hand_publish() {
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
