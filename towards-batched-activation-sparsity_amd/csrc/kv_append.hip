@@ -144,30 +144,10 @@ __global__ __launch_bounds__(P <= 64 ? 256 : 512) void bsg_kv_append_kernel(Appe
   fine = fine && lo < hi && j < p.max_pages;
   int32_t page = -1;
   if (fine) page = p.table[(int64_t)slot * p.table_stride + j];
-  fine = fine && page >= 0 && page < p.num_pages;
 
   const int t = lane & 15, g = lane >> 4;
   const int tok = tile * 16 + t;
   const bool is_new = fine && tok >= lo && tok < hi;
-  float* const scale_at = p.scales + ((int64_t)page * p.heads + head) * 2 + kv;
-  const float old = fine && lo > 0 ? *scale_at : 0.f;
-  uint8_t* const dst = p.pages + (((int64_t)page * p.heads + head) * 2 + kv) * (P * D) + (int64_t)tile * 16 * D;
-  // Bytes of the values' dwords (tokens 4q .. 4q+3) that are new, and that hold earlier tokens; what
-  // is there is on its way while the new ones are weighed.
-  uint32_t fresh = 0, held = 0;
-  u32x4 was[C];
-  const int v_off = (t >> 2) * 256 + (4 * g + (t & 3)) * 16;
-#pragma unroll
-  for (int b = 0; b < 4; ++b) {
-    const int k = tile * 16 + (t & 12) + b;
-    if (k >= lo && k < hi) fresh |= 0xffu << (8 * b);
-    if (k < lo) held |= 0xffu << (8 * b);
-  }
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    was[c] = u32x4{0u, 0u, 0u, 0u};
-    if (kv == 1 && fine && fresh != 0xffffffffu && (fresh | held) != 0) was[c] = *(const u32x4*)(dst + c * 1024 + v_off);
-  }
   uint32_t x[C][8];
 #pragma unroll
   for (int c = 0; c < C; ++c)
@@ -189,6 +169,27 @@ __global__ __launch_bounds__(P <= 64 ? 256 : 512) void bsg_kv_append_kernel(Appe
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[c][i] = src[64 * c + 2 * i] | (uint32_t)src[64 * c + 2 * i + 1] << 16;
     }
+  }
+  // The new numbers were asked for beside the page; what the page decides comes now.
+  fine = fine && page >= 0 && page < p.num_pages;
+  float* const scale_at = p.scales + ((int64_t)page * p.heads + head) * 2 + kv;
+  const float old = fine && lo > 0 ? *scale_at : 0.f;
+  uint8_t* const dst = p.pages + (((int64_t)page * p.heads + head) * 2 + kv) * (P * D) + (int64_t)tile * 16 * D;
+  // Bytes of the values' dwords (tokens 4q .. 4q+3) that are new, and that hold earlier tokens; what
+  // is there is on its way while the new ones are weighed.
+  uint32_t fresh = 0, held = 0;
+  u32x4 was[C];
+  const int v_off = (t >> 2) * 256 + (4 * g + (t & 3)) * 16;
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    const int k = tile * 16 + (t & 12) + b;
+    if (k >= lo && k < hi) fresh |= 0xffu << (8 * b);
+    if (k < lo) held |= 0xffu << (8 * b);
+  }
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    was[c] = u32x4{0u, 0u, 0u, 0u};
+    if (kv == 1 && fine && fresh != 0xffffffffu && (fresh | held) != 0) was[c] = *(const u32x4*)(dst + c * 1024 + v_off);
   }
   float a = largest_magnitude<T, C>(x);
   if constexpr (W > 1) {  // also: every wave has the old scale before one writes the new

@@ -272,8 +272,6 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_attention_kernel(AttnParams p) 
         }
       }
     }
-    const float lane_ks = lane_scale.x * p.scale2, lane_vs = fmaxf(lane_scale.y, 0x1p-100f);
-    const float lane_lv = __builtin_amdgcn_logf(lane_vs), lane_iv = 1.f / lane_vs;
     const auto fetch = [&](int n, Step& s) {
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
@@ -288,6 +286,7 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_attention_kernel(AttnParams p) 
         }
       }
     };
+    float lane_ks = 0.f, lane_lv = 0.f, lane_iv = 0.f;
     const auto take = [&](int n, Step& s) {
     const int t0 = b0 + 128 * n;
     auto& kr = s.k;
@@ -374,6 +373,9 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_attention_kernel(AttnParams p) 
     };
     Step even, odd;
     fetch(0, even);
+    // the scales were asked for before the step, and are only looked at now
+    const float lane_vs = fmaxf(lane_scale.y, 0x1p-100f);
+    lane_ks = lane_scale.x * p.scale2, lane_lv = __builtin_amdgcn_logf(lane_vs), lane_iv = __builtin_amdgcn_rcpf(lane_vs);
     for (int n = 0; n < steps; n += 2) {
       if (n + 1 < steps) fetch(n + 1, odd);
       take(n, even);
@@ -736,9 +738,10 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
     };
     load_pages(t_begin);
     load_scales();
-    turn_pages();
+    lane_page = next_page;
     issue(std::integral_constant<int, 0>{}, t_begin, page_of(0));
     issue(std::integral_constant<int, 1>{}, t_begin + STEP, page_of(1));
+    turn_pages();
     int n = 0;
     for (int t0 = t_begin; t0 < t_end; t0 += 3 * STEP)
       [&]<int... I>(std::integer_sequence<int, I...>) {
