@@ -14,9 +14,9 @@
 // largest of the lanes' own maxima is a bound that at least k logits reach.  Waves of a row meet in
 // LDS, two lists at a time; no barrier before that.
 //
-// 4000 x 32000 bf16 (256 MB): 51 us without alternatives (5.0 TB/s, the rate of a copy), 57 with one, 69 with 8,
-// 92 with 50 (fp16): what is left of the sorts, of which every wave runs two.  64 x 32000: 8.6 us without, 14.9
-// with 8, a chain of loads, sort, merge and the meeting of three work-groups.
+// 4000 x 32000 bf16 (256 MB): 52 us without alternatives (4.9 TB/s, the rate of a copy), 57 with one, 68 with 8,
+// 90 with 50 (fp16): what is left of the sorts, of which every wave runs two.  64 x 32000 fp16: 9.2 us without,
+// 14.1 with 8, bound by the chain of loads, sort, insertions and the three meetings of eight waves.
 
 #include "serve.hpp"
 
@@ -26,8 +26,9 @@ namespace {
 
 constexpr int kVectors = 4;     // 16-byte vectors of a lane and tile
 constexpr int kAhead = 1;       // tiles in flight beside the one at work
-constexpr int kWaves = 4;       // of a work-group
-constexpr int kInsert = 8;      // keys up to which inserting one by one is quicker than a sort
+constexpr int kWaves = 4;       // of a work-group of several rows, or of a row's split
+constexpr int kMostWaves = 8;   // of a work-group that has a row to itself
+constexpr int kInsert = 16;     // keys up to which inserting one by one is quicker than a sort
 constexpr int kSplitTiles = 2;  // tiles of a wave that a split of a long row leaves
 constexpr int kMaxSplits = 32;  // of a row
 constexpr int kMaxK = BSG_LOGPROBS_MAX_K;
@@ -325,16 +326,16 @@ __device__ __forceinline__ void take_tile(const u32x4 raw[kVectors], uint32_t th
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(64 * kWaves) void bsg_token_logprobs_kernel(ScoreParams p) {
+template <typename T, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void bsg_token_logprobs_kernel(ScoreParams p) {
   typedef Logit<T> L;
   constexpr int N = L::N;
-  __shared__ alignas(16) uint64_t s_wait[kWaves][128 + 2 * 64 * kVectors];
-  __shared__ Sums s_sum[kWaves];
+  __shared__ alignas(16) uint64_t s_wait[WAVES][128 + 2 * 64 * kVectors];
+  __shared__ Sums s_sum[WAVES];
   __shared__ uint32_t s_last;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int W = 1 << p.log_waves, part = wave & (W - 1);
-  const int64_t row = (int64_t)blockIdx.y * (blockDim.x >> (6 + p.log_waves)) + (wave >> p.log_waves);
+  const int64_t row = (int64_t)blockIdx.y * (WAVES >> p.log_waves) + (wave >> p.log_waves);
   const bool real = row < p.rows;
   const T* const x = (const T*)p.x + (real ? row : 0) * p.stride;
   const int k = p.k;
@@ -412,7 +413,7 @@ __global__ __launch_bounds__(64 * kWaves) void bsg_token_logprobs_kernel(ScorePa
     sum = join_lanes<1>(sum);
     best.list = 0;
     if (k > 0) {
-      constexpr int MANY = kMaxSplits / kWaves;
+      constexpr int MANY = kMaxSplits / WAVES;
       uint64_t* const lists = s_wait[wave];
 #pragma unroll
       for (int i = 0; i < MANY; ++i) {
@@ -449,24 +450,33 @@ struct Shape {
 
 // Waves of a row: enough rows fill the machine with one wave each (16 per compute unit); fewer take up
 // to the four of a work-group, with two vectors a lane at least (2000 rows of 1000, 5 alternatives: 8.0
-// us, 10.9 with one), and long ones several work-groups, which leave each wave kSplitTiles tiles (64 rows of
-// 32000 with 8 alternatives: 14.9 us so, 15.8 in twice the work-groups).
+// us, 10.9 with one).  Long ones take several work-groups, which leave each wave kSplitTiles tiles (7 rows of
+// 100003 fp32, 20 alternatives: 16.9 us so, 17.7 in half as many of eight waves), and where that
+// makes no second work-group, one of eight waves (64 rows of 32000 fp16, 8 alternatives: 14.1 us so, 15.4 of
+// four, 14.6 of sixteen, 15.8 in two work-groups; 256 rows: 14.9 against 16.1; 64 rows of 512: 5.5 against 5.0).
 Shape shape_of(int64_t rows, int64_t vocab, int per_vector, int32_t cus) {
   const int64_t vectors = ceil_div(vocab, per_vector) + 1;  // a row may begin inside a vector
   Shape s;
-  s.log_waves = 0;
-  while ((1 << s.log_waves) < kWaves && (rows << s.log_waves) < 16 * (int64_t)cus && (128 << s.log_waves) < vectors)
-    ++s.log_waves;
   int64_t want = vectors / (64 * kWaves * kVectors * kSplitTiles);
   if (rows > 0 && want > 2 * cus / rows) want = 2 * cus / rows;
   if (want > kMaxSplits) want = kMaxSplits;
   if (want < 1 || rows * 4 > BSG_KV_COUNTER_BYTES) want = 1;
   s.split_vectors = ceil_div(vectors, want);
   s.splits = (int32_t)ceil_div(vectors, s.split_vectors);
+  const int most = s.splits > 1 ? kWaves : kMostWaves;
+  s.log_waves = 0;
+  while ((1 << s.log_waves) < most && (rows << s.log_waves) < 16 * (int64_t)cus && (128 << s.log_waves) < vectors)
+    ++s.log_waves;
   return s;
 }
 
 int per_vector(int dtype) { return dtype == BSG_F32 ? 4 : 8; }
+
+template <typename T>
+void launch(const ScoreParams& p, dim3 grid, bool wide, hipStream_t st) {
+  if (wide) hipLaunchKernelGGL((bsg_token_logprobs_kernel<T, kMostWaves>), grid, dim3(64 * kMostWaves), 0, st, p);
+  else hipLaunchKernelGGL((bsg_token_logprobs_kernel<T, kWaves>), grid, dim3(64 * kWaves), 0, st, p);
+}
 
 int64_t workspace_bytes(const Shape& s, int64_t rows, int32_t k) {
   return s.splits <= 1 || rows == 0 ? 0 : BSG_KV_COUNTER_BYTES + rows * s.splits * (16 + 8 * (int64_t)k);
@@ -519,7 +529,8 @@ extern "C" int bsg_token_logprobs(const void* logits, int64_t row_stride, int64_
   const hipStream_t st = (hipStream_t)stream;
   const size_t es = dtype == BSG_F32 ? 4 : 2;
   // one launch takes 65535 work-groups of rows
-  const int64_t group = kWaves >> s.log_waves, most = 65535 * group;
+  const bool wide = (1 << s.log_waves) > kWaves;
+  const int64_t group = (wide ? kMostWaves : kWaves) >> s.log_waves, most = 65535 * group;
   p.log_waves = s.log_waves;
   for (int64_t r = 0; r < rows; r += most) {
     const int64_t n = rows - r < most ? rows - r : most;
@@ -530,13 +541,10 @@ extern "C" int bsg_token_logprobs(const void* logits, int64_t row_stride, int64_
     p.entropy = entropy + r;
     p.top_ids = k > 0 ? top_ids + r * k : nullptr;
     p.top_logprobs = k > 0 ? top_logprobs + r * k : nullptr;
-    const dim3 grid((unsigned)s.splits, (unsigned)ceil_div(n, group)), block(64 * kWaves);
-    if (dtype == BSG_F16)
-      hipLaunchKernelGGL(bsg_token_logprobs_kernel<_Float16>, grid, block, 0, st, p);
-    else if (dtype == BSG_BF16)
-      hipLaunchKernelGGL(bsg_token_logprobs_kernel<__bf16>, grid, block, 0, st, p);
-    else
-      hipLaunchKernelGGL(bsg_token_logprobs_kernel<float>, grid, block, 0, st, p);
+    const dim3 grid((unsigned)s.splits, (unsigned)ceil_div(n, group));
+    if (dtype == BSG_F16) launch<_Float16>(p, grid, wide, st);
+    else if (dtype == BSG_BF16) launch<__bf16>(p, grid, wide, st);
+    else launch<float>(p, grid, wide, st);
   }
   return launch_status("bsg_token_logprobs");
 }
