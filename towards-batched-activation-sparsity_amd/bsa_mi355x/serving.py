@@ -47,8 +47,8 @@ _CALLS: Dict[tuple, tuple] = {}
 _CALLS_MAX = 4096
 
 
-def _sig(t: Optional[torch.Tensor]):
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+def _sigs(*tensors: Optional[torch.Tensor]) -> tuple:
+    return tuple([t if t is None else (t.shape, t.stride(), t.dtype, t.get_device()) for t in tensors])
 
 
 def _remember(key: tuple, call: tuple) -> tuple:
@@ -194,8 +194,7 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, scales: tor
     magnitude to 448 or below, and no less than the scale of tokens that the page held before (which
     are rounded again where it grows).  Infinities become +-448 x scale, NaN stays NaN.  max_new bounds
     the tokens of one sequence (default: all of them; a tight one makes a smaller launch)."""
-    key = ("append", _sig(k), _sig(v), _sig(pages), _sig(scales), _sig(page_table), _sig(lengths), _sig(cu_seqlens), _sig(slots),
-           max_new)
+    key = ("append", _sigs(k, v, pages, scales, page_table, lengths, cu_seqlens, slots), max_new)
     call = _CALLS.get(key)
     if call is None:
         dev, sizes = _layer(pages, scales, page_table, lengths)
@@ -227,8 +226,7 @@ def kv_attention(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, pag
     1 / sqrt(head_dim) by default.  max_len, the longest sequence (default: what a table row holds),
     decides how the long axis is split and bounds nothing.  q rows must be 16-byte aligned, out rows
     8-byte aligned."""
-    key = ("attend", _sig(q), _sig(pages), _sig(scales), _sig(page_table), _sig(lengths), _sig(cu_seqlens), _sig(slots), _sig(out),
-           _sig(lse), max_new, max_len)
+    key = ("attend", _sigs(q, pages, scales, page_table, lengths, cu_seqlens, slots, out, lse), max_new, max_len)
     call = _CALLS.get(key)
     if call is None:
         call = _remember(key, _attention_call(q, pages, scales, page_table, lengths, cu_seqlens, max_new, slots, max_len, out, lse))
@@ -269,10 +267,15 @@ def _attention_call(q, pages, scales, page_table, lengths, cu_seqlens, max_new, 
             _mold(q.shape, q.dtype, dev), _mold(q.shape[:2], torch.float32, dev), longest, need, cus, d ** -0.5)
 
 
-def _pool(kind: str, page_table=None, lengths=None, refcounts=None, pages=None, scales=None, *others):
-    """The device index of what a page call is given, and its bsg_page_pool; `others` are int32 tensors
-    of the call."""
-    key = (kind, _sig(page_table), _sig(lengths), _sig(refcounts), _sig(pages), _sig(scales), *[_sig(t) for t in others])
+# The int32 tensors of each page call beside the cache's own.
+_PAGE_CALLS = {"copy": ("src", "dst"), "fork": ("parents", "children"), "extend": ("new_tokens", "slots", "served"),
+               "free": ("slots",), "compact": ("counts",)}
+
+
+def _pool(kind: str, page_table, lengths, refcounts, pages, scales, *others) -> tuple:
+    """What a page call needs beside `others`, its own int32 tensors: the device index, the library's
+    function, the bsg_page_pool and the bytes of a plan's lists."""
+    key = (kind, _sigs(page_table, lengths, refcounts, pages, scales, *others))
     call = _CALLS.get(key)
     if call is None:
         dev = (page_table if page_table is not None else pages).device
@@ -293,27 +296,22 @@ def _pool(kind: str, page_table=None, lengths=None, refcounts=None, pages=None, 
             _i32(lengths, dev, "lengths", slots)
             _i32(refcounts, dev, "refcounts", None if pages is None else pages.shape[1])
             count = refcounts.numel()
-        for i, t in enumerate(others):
-            _i32(t, dev, f"argument {i}")
-        call = _remember(key, (dev.index, (layers, count, page_bytes, page_scales, page_size, slots, each, stride)))
-    index, sizes = call
-    pool = _lib.PagePool(_ptr(pages), _ptr(scales), *sizes, _ptr(page_table), _ptr(lengths), _ptr(refcounts))
-    return index, pool
-
-
-def _same(n: int, **others) -> None:
-    for what, t in others.items():
-        if t is not None and t.numel() != n:
-            raise ValueError(f"{what} has {t.numel()} entries, needs {n}")
+        n = 2 if kind == "compact" else others[0].numel()
+        for what, t in zip(_PAGE_CALLS[kind], others):
+            _i32(t, dev, what, n)
+        need = int(load().bsg_pages_workspace_bytes(count)) if kind in ("extend", "compact") else 0
+        call = _remember(key, (dev.index, getattr(load(), "bsg_pages_" + kind),
+                               (layers, count, page_bytes, page_scales, page_size, slots, each, stride), need))
+    index, fn, sizes, need = call
+    return index, fn, _lib.PagePool(_ptr(pages), _ptr(scales), *sizes, _ptr(page_table), _ptr(lengths), _ptr(refcounts)), need
 
 
 def pages_copy(pages: torch.Tensor, scales: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
     """Copy pages src[i] -> dst[i] (int32) with their scales in every layer of pages [layers, pages,
     heads, 2, page_size, head_dim].  Pairs with an id out of range are skipped.  No page may be
     written twice, or both read and written, in one call."""
-    index, pool = _pool("copy", None, None, None, pages, scales, src, dst)
-    _same(src.numel(), dst=dst)
-    _launch(index, load().bsg_pages_copy, pool, src.data_ptr(), dst.data_ptr(), src.numel())
+    index, fn, pool, _ = _pool("copy", None, None, None, pages, scales, src, dst)
+    _launch(index, fn, pool, src.data_ptr(), dst.data_ptr(), src.numel())
 
 
 def pages_fork(page_table: torch.Tensor, lengths: torch.Tensor, refcounts: torch.Tensor, parents: torch.Tensor,
@@ -322,9 +320,8 @@ def pages_fork(page_table: torch.Tensor, lengths: torch.Tensor, refcounts: torch
     share, and its length, and releases what it held.  All pairs at once, so that a reordering of
     beams is one call.  Pairs with a slot out of range are skipped; of pairs with the same child the
     last one counts.  At most 1024 pairs."""
-    index, pool = _pool("fork", page_table, lengths, refcounts, None, None, parents, children)
-    _same(parents.numel(), children=children)
-    _launch(index, load().bsg_pages_fork, pool, parents.data_ptr(), children.data_ptr(), parents.numel())
+    index, fn, pool, _ = _pool("fork", page_table, lengths, refcounts, None, None, parents, children)
+    _launch(index, fn, pool, parents.data_ptr(), children.data_ptr(), parents.numel())
 
 
 def pages_extend(pages: torch.Tensor, scales: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
@@ -341,24 +338,24 @@ def pages_extend(pages: torch.Tensor, scales: torch.Tensor, page_table: torch.Te
     n = new_tokens.numel()
     if served is None:
         served = torch.empty(n, dtype=torch.int32, device=new_tokens.device)
-    index, pool = _pool("extend", page_table, lengths, refcounts, pages, scales, new_tokens, slots, served)
-    _same(n, slots=slots, served=served)
-    ws = _plan_workspace(index, pool.num_pages, workspace_prefix)
-    _launch(index, load().bsg_pages_extend, pool, _ptr(slots), new_tokens.data_ptr(), n, served.data_ptr(), ws.data_ptr(), ws.numel())
+    index, fn, pool, need = _pool("extend", page_table, lengths, refcounts, pages, scales, new_tokens, slots, served)
+    held, ws, room = _plan_workspace(index, need, workspace_prefix)
+    _launch(index, fn, pool, _ptr(slots), new_tokens.data_ptr(), n, served.data_ptr(), ws, room)
     return served
 
 
-def _plan_workspace(index: int, num_pages: int, prefix: Optional[str]) -> torch.Tensor:
-    """Room for a plan's lists, past the counters that other calls need zero."""
-    need = int(load().bsg_pages_workspace_bytes(num_pages))
-    return _workspace(index, COUNTER_BYTES + need, prefix, cleared=False)[COUNTER_BYTES:]
+def _plan_workspace(index: int, need: int, prefix: Optional[str]) -> Tuple[torch.Tensor, int, int]:
+    """A workspace, with the address and bytes of its room for a plan's lists, past the counters that
+    other calls need zero."""
+    held = _workspace(index, COUNTER_BYTES + need, prefix, cleared=False)
+    return held, held.data_ptr() + COUNTER_BYTES, held.numel() - COUNTER_BYTES
 
 
 def pages_free(page_table: torch.Tensor, lengths: torch.Tensor, refcounts: torch.Tensor, slots: torch.Tensor) -> None:
     """Release every page of the given slots (int32): their table rows become -1, their lengths 0.
     Slots out of range are skipped, one named twice is released once.  At most 1024 slots."""
-    index, pool = _pool("free", page_table, lengths, refcounts, None, None, slots)
-    _launch(index, load().bsg_pages_free, pool, slots.data_ptr(), slots.numel())
+    index, fn, pool, _ = _pool("free", page_table, lengths, refcounts, None, None, slots)
+    _launch(index, fn, pool, slots.data_ptr(), slots.numel())
 
 
 def pages_compact(pages: torch.Tensor, scales: torch.Tensor, page_table: torch.Tensor, refcounts: torch.Tensor,
@@ -367,10 +364,9 @@ def pages_compact(pages: torch.Tensor, scales: torch.Tensor, page_table: torch.T
     ids before, and every entry of page_table (all slots) follows.  Returns counts, int32 [live, moved]."""
     if counts is None:
         counts = torch.empty(2, dtype=torch.int32, device=page_table.device)
-    index, pool = _pool("compact", page_table, None, refcounts, pages, scales, counts)
-    _same(2, counts=counts)
-    ws = _plan_workspace(index, pool.num_pages, workspace_prefix)
-    _launch(index, load().bsg_pages_compact, pool, counts.data_ptr(), ws.data_ptr(), ws.numel())
+    index, fn, pool, need = _pool("compact", page_table, None, refcounts, pages, scales, counts)
+    held, ws, room = _plan_workspace(index, need, workspace_prefix)
+    _launch(index, fn, pool, counts.data_ptr(), ws, room)
     return counts
 
 
@@ -392,7 +388,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0,
     A token outside the vocabulary gives NaN.  A row of nothing but -inf gives -inf, entropy 0 and the
     lowest ids; a NaN or +inf in a row makes its numbers NaN (NaN ranks first among the ids, -0 equals
     +0)."""
-    key = ("logprobs", _sig(logits), _sig(tokens), k)
+    key = ("logprobs", _sigs(logits, tokens), k)
     call = _CALLS.get(key)
     if call is None:
         call = _remember(key, _logprobs_call(logits, tokens, k))

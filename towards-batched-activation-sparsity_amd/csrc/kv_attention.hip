@@ -7,9 +7,9 @@
 // operand that O^T needs: nothing is shuffled between the two products.
 //
 // Scales and softmax in one exponent: with s2 = log2(e) sm_scale ks (q . k8) and lv = log2(vs), the weight of a
-// token is w = 2^(s2 + lv - M + 14) against the running maximum M of s2 + lv, so that O = sum w v8 /
-// sum w / vs whatever M is.  w is at most 2^14 and goes to the matrix unit as fp16: every weight
-// down to 2^-28 of the largest keeps 11 bits.
+// token is w = 2^(s2 + lv - M + 14) against a maximum M of s2 + lv that a later one may pass by kSlack
+// octaves, so that O = sum w v8 / sum w / vs whatever M is.  w is at most 2^15.5 and goes to the matrix
+// unit as fp16: every weight down to 2^-28 of the largest keeps 11 bits.  Its sum is taken in fp32 before.
 
 #include <utility>
 
@@ -187,6 +187,13 @@ __device__ __forceinline__ void sum_parts(__amdgpu_buffer_rsrc_t r, int part_byt
 // A work-group of four waves computes RT x 16 rows of one cached head of one sequence over one chunk
 // of its tokens; wave w takes the 32-token steps w, w + 4, ..., each with its own running maximum, and the
 // waves meet in LDS at the end.  Chunks meet in the workspace: the last one to arrive sums them in order.
+//
+// Steps are interleaved over the waves, so that a work-group reads on as one stream; a step of a wave is
+// 8 KiB (D = 128), straight into registers in the order the matrix unit wants, and one more is on its
+// way, which with two work-groups on a compute unit covers HBM's latency.  64 sequences of up to 4096 tokens x 32
+// heads of 128, fp16 (1.44 GB): 232 us, 6.2 TB/s.  64 x 4 new tokens over 1500: 84 us (5.8 TB/s); 5 x 32 heads over
+// 60001 tokens of 8 cached heads, bf16: 81 us (5.5 TB/s): bound by HBM, past the rate of a copy
+// (5.0).  One sequence of 777 tokens: 8.9 us, the chain length, page, scale and tile, then the parts' meeting.
 template <typename T, int D, int RT>
 __global__ __launch_bounds__(256, 2) void bsg_kv_attention_kernel(AttnParams p) {
   constexpr int C = D / 64, DT = D / 16, ROWS = 16 * RT, LD = D + 4;
@@ -513,10 +520,16 @@ __device__ __forceinline__ void vmem_wait() {
 
 // Many rows per cached head (prompts).  A work-group of four waves owns 128 rows, 32 of each wave, and walks the
 // tokens they see 64 at a time; a step's keys and values (16 KiB) are brought once, straight into LDS in
-// the bytes they have in memory, two steps ahead, and each wave converts what it reads.  Rows do not cross waves, so nothing meets at the end but the parts
-// of a split.  Work-groups of one cached head lie kv_heads apart, that is on the same XCD where the
-// heads are a multiple of 8, and share its L2; one sequence follows the other (all of them side by
-// side: 334 us against 267 for 8 prompts of 2048), its tiles with most tokens first.
+// the bytes they have in memory, two steps ahead, and each wave converts what it reads (converted once
+// for all four, LDS holds twice the bytes: 645 us against 584 for a prompt of 8192).  Rows do not cross waves,
+// so nothing meets at the end but the parts of a split.  Work-groups of one cached head lie kv_heads
+// apart, that is on the same XCD where the heads are a multiple of 8, and share its L2; one sequence
+// follows the other (all of them side by side: 334 us against 267 for 8 prompts of 2048), its tiles with
+// most tokens first.
+//
+// 3 prompts of up to 2000 tokens over up to 2800, 32 heads on 8 of 128, fp16: 159 us, 720 TFLOP/s; a prompt of
+// 8192: 584 us, 940 TFLOP/s, 0.78 of a library product of 8192^3 (1210).  For each MFMA of 16 cycles
+// there are two conversions and a share of the softmax to issue; these, the MFMAs and the step's barrier bound it.
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
   constexpr int C = D / 64, DT = D / 16, RT = 2, ROWS = 128, STEP = 64;
