@@ -228,8 +228,8 @@ __global__ __launch_bounds__(kScan) void bsg_pages_extend_plan_kernel(Pool p, co
   }
 }
 
-// Work-group (i, chunk): a part of the copied page's layers; the first chunk also writes row i.  64 rows, 28
-// pages of 128 KiB split in 4 layers each (29 MB in and out): 8-10 us after a plan of 5.3, a chain of length,
+// Work-group (i, chunk): a part of the copied page's layers; the first chunk also writes row i.  64 rows, some
+// 22 pages of 128 KiB copied in 4 layers each (23 MB in and out): 8-10 us after a plan of 5.3, a chain of length,
 // entry, count and two scans in one work-group.
 __global__ __launch_bounds__(256) void bsg_pages_extend_kernel(Pool p, const Row* __restrict__ rows,
                                                                const int32_t* __restrict__ free_ids) {
