@@ -77,7 +77,7 @@ int bsg_kv_append(const void* k, int64_t k_stride_t, int64_t k_stride_h, const v
  *              is computed rightly)
  * A token that sees nothing gives zeros and -inf, as do the tokens of a sequence whose slot is out of
  * range; rows of q that cu gives to no sequence are not computed.  Tokens on a page id out of range are not seen.  Products of 16-bit operands (keys and
- * values converted exactly, probabilities in fp16 after a shift by 2^14), sums, maxima and
+ * values converted exactly, probabilities in fp16 after a shift by 2^13), sums, maxima and
  * exponentials in 32 bits.  Workspace: 16-byte aligned, its first BSG_KV_COUNTER_BYTES zero before
  * the first use and left zero; calls that may overlap must not share one. */
 #define BSG_KV_COUNTER_BYTES 65536

@@ -7,9 +7,9 @@
 // operand that O^T needs: nothing is shuffled between the two products.
 //
 // Scales and softmax in one exponent: with s2 = log2(e) sm_scale ks (q . k8) and lv = log2(vs), the weight of a
-// token is w = 2^(s2 + lv - M + 14) against a maximum M of s2 + lv that a later one may pass by kSlack
-// octaves, so that O = sum w v8 / sum w / vs whatever M is.  w is at most 2^15.5 and goes to the matrix
-// unit as fp16: every weight down to 2^-28 of the largest keeps 11 bits.  Its sum is taken in fp32 before.
+// token is w = 2^(s2 + lv - M + 13) against a maximum M of s2 + lv that a later one may pass by an octave or
+// more, so that O = sum w v8 / sum w / vs whatever M is.  w stays within fp16, as which it goes to the matrix
+// unit: every weight down to 2^-27 of the largest keeps 11 bits.  Its sum is taken in fp32 before.
 
 #include <utility>
 
@@ -27,9 +27,9 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxSplits = 32;    // parts of one row
-constexpr float kShift = 14.f;  // weights go up to 2^(kShift + kSlack), within fp16
-constexpr float kSlack = 1.5f;  // what a score may exceed the running maximum by before that moves
-constexpr float kMostWeight = 46340.f;  // 2^(kShift + kSlack)
+constexpr float kShift = 13.f;  // weights go up to 2^(kShift + kSlack), within fp16
+constexpr float kSlack = 1.5f;  // octaves by which, in the first kernel, a score may exceed the running maximum before that moves
+constexpr float kMostWeight = 65504.f;  // of fp16; four weights at the maximum make half of it
 
 struct AttnParams {
   const uint16_t* q;
@@ -592,38 +592,44 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
   const int32_t* const table = p.table + (int64_t)(slot < 0 || slot >= p.num_slots ? 0 : slot) * p.table_stride;
   const int64_t head_bytes = (int64_t)2 * D << p.page_shift;
   const int in_page = (1 << p.page_shift) - 1;
-  // Lane j keeps the page and scales of the j-th 16-token tile of 16 steps (1024 tokens), from where
+  // Lane j keeps where the j-th 16-token tile of 16 steps (1024 tokens) lies and its scales, from where
   // they come as scalars; the next 16 steps' are on their way while the last of these are at work.
-  int lane_page = -1, next_page = -1;
-  float lane_ks = 0.f, lane_lv = 0.f, lane_iv = 0.f;
+  struct Tiles {
+    int64_t at;  // bytes into the pages; below 0: not there
+    float ks, lv, iv;
+  } tiles = {-1, 0.f, 0.f, 0.f};
+  int next_page = -1;
+  int64_t next_at = -1;
   f32x2 next_scale = {0.f, 0.f};
-  const auto load_pages = [&](int b0) {
+  const auto load_pages = [&](int b0) {  // not looked at before load_scales
     const int t = b0 + 16 * lane;
-    const int page = t < t_end ? table[t >> p.page_shift] : -1;
-    next_page = page >= 0 && page < p.num_pages ? page : -1;
+    next_page = t < t_end ? table[t >> p.page_shift] : -1;
   };
-  const auto load_scales = [&]() {
-    next_scale = *(const f32x2*)(p.scales + 2 * ((int64_t)(next_page < 0 ? 0 : next_page) * p.kv_heads + head));
+  const auto load_scales = [&](int b0) {
+    const bool there = next_page >= 0 && next_page < p.num_pages;
+    const int64_t block = (int64_t)(there ? next_page : 0) * p.kv_heads + head;
+    next_at = there ? block * head_bytes + (int64_t)(((b0 + 16 * lane) & in_page) * D) : -1;
+    next_scale = *(const f32x2*)(p.scales + 2 * block);
   };
   const auto turn_pages = [&]() {
     const float vs = fmaxf(next_scale.y, 0x1p-100f);
-    lane_page = next_page;
     // a scale of 0 as the least one, so that -inf stays what it is
-    lane_ks = fmaxf(next_scale.x * scale2, 0x1p-126f);
-    lane_lv = __builtin_amdgcn_logf(vs), lane_iv = __builtin_amdgcn_rcpf(vs);
+    tiles = Tiles{next_at, fmaxf(next_scale.x * scale2, 0x1p-126f), __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs)};
   };
-  // The wave brings the step's tile `wave`; a step past the end, or a page that is not there, loads
-  // zeros, so that every step has the same number of loads to wait by.
-  const auto issue = [&](auto stage, int t0, int page) {
-    const bool there = page >= 0;
-    const __amdgpu_buffer_rsrc_t r = cache_rsrc(p.pages + ((int64_t)(there ? page : 0) * p.kv_heads + head) * head_bytes,
-                                                there ? (int)head_bytes : 0);
+  // The wave brings the tile `wave` of step n of the 16 (from 16 on: of the next 16); one that is not
+  // there, or past the end, loads zeros, so that every step has the same number of loads to wait by.
+  const auto issue = [&](auto stage, int n) {
+    const int64_t from = n < 16 ? tiles.at : next_at;
+    const int at = 4 * n + wave & 63;
+    const int lo = __builtin_amdgcn_readlane((int)from, at), hi = __builtin_amdgcn_readlane((int)(from >> 32), at);
+    const int64_t off = hi < 0 ? 0 : (int64_t)hi << 32 | (uint32_t)lo;
+    const int half = (int)(head_bytes >> 1);
+    const __amdgpu_buffer_rsrc_t r = cache_rsrc(p.pages + off, hi >= 0 ? half + 1024 * C : 0);
     u32x4* const to = prefill_stage<D, decltype(stage)::value>() + wave * TILE;
-    const int at = ((t0 + 16 * wave) & in_page) * D;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      load_lds(r, to + c * 64, lane * 16, at + c * 1024);
-      load_lds(r, to + (C + c) * 64, lane * 16, at + c * 1024 + (int)(head_bytes >> 1));
+      load_lds(r, to + c * 64, lane * 16, c * 1024);
+      load_lds(r, to + (C + c) * 64, lane * 16, c * 1024 + half);
     }
   };
 
@@ -645,10 +651,10 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
     bool there[4], all_there = true;
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
-      there[a] = __builtin_amdgcn_readlane(lane_page, first_tile + a) >= 0;
-      ks[a] = as_float(__builtin_amdgcn_readlane(__builtin_bit_cast(int, lane_ks), first_tile + a));
-      lv[a] = as_float(__builtin_amdgcn_readlane(__builtin_bit_cast(int, lane_lv), first_tile + a));
-      iv[a] = as_float(__builtin_amdgcn_readlane(__builtin_bit_cast(int, lane_iv), first_tile + a));
+      there[a] = __builtin_amdgcn_readlane((int)(tiles.at >> 32), first_tile + a) >= 0;
+      ks[a] = as_float(__builtin_amdgcn_readlane(__builtin_bit_cast(int, tiles.ks), first_tile + a));
+      lv[a] = as_float(__builtin_amdgcn_readlane(__builtin_bit_cast(int, tiles.lv), first_tile + a));
+      iv[a] = as_float(__builtin_amdgcn_readlane(__builtin_bit_cast(int, tiles.iv), first_tile + a));
       all_there = all_there && there[a];
 #pragma unroll
       for (int i = 0; i < RT; ++i) s[i][a] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -675,12 +681,13 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
             if (t + j >= sees[i]) s[i][a][j] = -__builtin_inff();
       }
     }
-    // Weights against the maximum so far; only where one of them outgrows fp16 (or a row has no maximum yet) is a
-    // new maximum looked for.  The old one is never above the true one by that.
+    // Weights against the maximum so far; only where four of them together outgrow fp16 (or a row has no
+    // maximum yet) is a new one looked for.  The sums are wanted anyway: asking each weight took 590 us
+    // instead of 566 for a prompt of 8192.
     f16x8 pf[RT][2];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-      float e[4][4], top = 0.f;
+      float e[4][4], sum[4], top = 0.f;
       const auto weigh = [&]() {
         const float base = (m[i] == -__builtin_inff() ? 0.f : m[i]) - kShift;
         top = 0.f;
@@ -688,10 +695,9 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
         for (int a = 0; a < 4; ++a) {
           const float off = lv[a] - base;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            e[a][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][a][j], ks[a], off));
-            top = fmaxf(top, e[a][j]);
-          }
+          for (int j = 0; j < 4; ++j) e[a][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][a][j], ks[a], off));
+          sum[a] = (e[a][0] + e[a][1]) + (e[a][2] + e[a][3]);
+          top = fmaxf(top, sum[a]);
         }
       };
       weigh();
@@ -713,7 +719,7 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
       uint32_t w[8];
 #pragma unroll
       for (int a = 0; a < 4; ++a) {
-        l[i] = __builtin_fmaf((e[a][0] + e[a][1]) + (e[a][2] + e[a][3]), iv[a], l[i]);
+        l[i] = __builtin_fmaf(sum[a], iv[a], l[i]);
         w[2 * a] = Elem<_Float16>::pack(e[a][0], e[a][1]), w[2 * a + 1] = Elem<_Float16>::pack(e[a][2], e[a][3]);
       }
       pf[i][0] = __builtin_bit_cast(f16x8, u32x4{w[0], w[1], w[2], w[3]});
@@ -745,15 +751,11 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
   };
 
   if (t_begin < t_end) {
-    // page of the tile that this wave brings for step n of the 16 (from 16 on: of the next 16)
-    const auto page_of = [&](int n) {
-      return n < 16 ? __builtin_amdgcn_readlane(lane_page, 4 * n + wave) : __builtin_amdgcn_readlane(next_page, 4 * n - 64 + wave);
-    };
     load_pages(t_begin);
-    load_scales();
-    lane_page = next_page;
-    issue(std::integral_constant<int, 0>{}, t_begin, page_of(0));
-    issue(std::integral_constant<int, 1>{}, t_begin + STEP, page_of(1));
+    load_scales(t_begin);
+    tiles.at = next_at;
+    issue(std::integral_constant<int, 0>{}, 0);
+    issue(std::integral_constant<int, 1>{}, 1);
     turn_pages();
     int n = 0;
     for (int t0 = t_begin; t0 < t_end; t0 += 3 * STEP)
@@ -769,8 +771,8 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
           asm volatile("" ::: "memory");
           __builtin_amdgcn_sched_barrier(0);
           if (n == 8) load_pages(t + 8 * STEP);
-          if (n == 11) load_scales();
-          issue(std::integral_constant<int, (S + 2) % 3>{}, t + 2 * STEP, t + 2 * STEP < t_end ? page_of(n + 2) : -1);
+          if (n == 11) load_scales(t + 5 * STEP);
+          issue(std::integral_constant<int, (S + 2) % 3>{}, n + 2);
           __builtin_amdgcn_sched_barrier(0);
           if (t < w_end && t < t_end) take(stage, t);
           if (++n == 16) n = 0, turn_pages();
