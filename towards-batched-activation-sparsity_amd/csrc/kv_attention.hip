@@ -527,9 +527,9 @@ __device__ __forceinline__ void vmem_wait() {
 // follows the other (all of them side by side: 334 us against 267 for 8 prompts of 2048), its tiles with
 // most tokens first.
 //
-// 3 prompts of up to 2000 tokens over up to 2800, 32 heads on 8 of 128, fp16: 159 us, 720 TFLOP/s; a prompt of
-// 8192: 584 us, 940 TFLOP/s, 0.78 of a library product of 8192^3 (1210).  For each MFMA of 16 cycles
-// there are two conversions and a share of the softmax to issue; these, the MFMAs and the step's barrier bound it.
+// 3 prompts of up to 2000 tokens over up to 2800, 32 heads on 8 of 128, fp16: 150 us, 767 TFLOP/s; a prompt of
+// 8192: 555 us, 990 TFLOP/s, 0.82 of a library product of 8192^3 (1210).  The conversions hide behind the
+// MFMAs; the softmax between the two products, with two waves on a SIMD, and the step's barrier do not.
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
   constexpr int C = D / 64, DT = D / 16, RT = 2, ROWS = 128, STEP = 64;
