@@ -46,7 +46,7 @@ typedef struct bsg_kv_cache {
   int32_t page_size;         /* 16, 32, 64 or 128 */
   int32_t head_dim;          /* 64 or 128 */
   int32_t num_slots;         /* rows of page_table, entries of lengths */
-  int32_t max_pages;         /* columns of page_table */
+  int32_t max_pages;         /* columns of page_table; max_pages x page_size <= 2^30 */
   int64_t table_stride;      /* elements between its rows, >= max_pages */
   const int32_t* page_table;
   const int32_t* lengths;    /* tokens of each slot, the new ones of a call among them */

@@ -78,6 +78,14 @@ def test_bad_caches_are_refused(bad, code):
     assert _lib.last_error()
 
 
+def test_rows_of_more_than_2_30_tokens_are_refused():
+    """Positions are 32-bit in the attention, and go past a row's end by up to a few thousand."""
+    over, most = (_cache(max_pages=n, table_stride=n) for n in ((1 << 26) + 1, 1 << 26))
+    assert _append(over) == _lib.BSG_ERR_UNSUPPORTED and _attend(over) == _lib.BSG_ERR_UNSUPPORTED
+    need = bsa.load().bsg_kv_attention_workspace_bytes
+    assert need(ctypes.byref(over), 4, 4, 1, 0, 256) == -1 and need(ctypes.byref(most), 4, 4, 1, 0, 256) > 0
+
+
 def test_bad_batches_are_refused():
     c = _cache()
     assert _append(c, k=None) == _lib.BSG_ERR_ARG

@@ -287,7 +287,8 @@ int check_kv_cache(const bsg_kv_cache* c) {
     return fail(BSG_ERR_UNSUPPORTED, "cache: head_dim=%d (64 or 128)", c->head_dim);
   if (!is_aligned(c->pages, 16) || !is_aligned(c->scales, 8))
     return fail(BSG_ERR_ALIGN, "cache: pages must be 16-byte and scales 8-byte aligned");
-  if ((int64_t)c->max_pages * c->page_size > 0x7fffffff)
+  // the attention's positions are 32-bit and go past a row's end by up to 4096
+  if ((int64_t)c->max_pages * c->page_size > 1 << 30)
     return fail(BSG_ERR_UNSUPPORTED, "cache: %d pages of %d tokens in a row", c->max_pages, c->page_size);
   return BSG_OK;
 }
