@@ -121,6 +121,12 @@ def _pool(**kw):
     return ctypes.byref(_lib.PagePool(*a.values()))
 
 
+def test_append_of_too_much_work_is_refused():
+    """A bound on the new tokens near 2^31 is counted in 64 bits."""
+    for most in (2 ** 31 - 1, 2 ** 31 - 14):
+        assert _append(_cache(), cu=FAKE, max_new=most) == _lib.BSG_ERR_UNSUPPORTED
+
+
 def test_bad_pools_are_refused():
     lib = bsa.load()
     need = lib.bsg_pages_workspace_bytes(100)

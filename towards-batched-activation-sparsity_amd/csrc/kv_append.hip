@@ -317,7 +317,7 @@ extern "C" int bsg_kv_append(const void* k, int64_t k_stride_t, int64_t k_stride
   if (!k || !v) return fail(BSG_ERR_ARG, "null pointer (k=%p v=%p)", k, v);
   if (!is_aligned(k, 2) || !is_aligned(v, 2)) return fail(BSG_ERR_ALIGN, "k and v must be 2-byte aligned");
   const int P = cache->page_size;
-  const int64_t per_row = (max_new + P - 2) / P + 1;  // pages that max_new tokens can touch
+  const int64_t per_row = ((int64_t)max_new + P - 2) / P + 1;  // pages that max_new tokens can touch
   const int64_t units = per_row * rows * cache->n_heads * 2;
   if (units > 0x7fffffff) return fail(BSG_ERR_UNSUPPORTED, "%lld tiles of work", (long long)units);
   AppendParams p;
