@@ -174,7 +174,7 @@ def _batch(x: torch.Tensor, what: str, heads: int, d: int, dev: torch.device, ro
         if max_new is not None and int(max_new) != per:
             raise ValueError(f"max_new={max_new}, but each of {rows} sequences has {per} tokens")
         return per
-    return x.shape[0] if max_new is None else int(max_new)
+    return x.shape[0] if max_new is None else min(int(max_new), x.shape[0])
 
 
 def _rows(slots: Optional[torch.Tensor], cu: Optional[torch.Tensor], lengths: torch.Tensor) -> int:
@@ -459,15 +459,16 @@ class KVCache:
         self.lengths = torch.zeros(max_slots, dtype=torch.int32, device=dev)
         self.refcounts = torch.zeros(num_pages, dtype=torch.int32, device=dev)
         self.page_size, self.head_dim, self.heads = page_size, head_dim, heads
+        self._layers = list(zip(self.pages, self.scales))  # views: indexing costs a call more than its checks do
 
     def extend(self, new_tokens: torch.Tensor, slots: Optional[torch.Tensor] = None, **kw) -> torch.Tensor:
         return pages_extend(self.pages, self.scales, self.page_table, self.lengths, self.refcounts, new_tokens, slots, **kw)
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, **kw) -> None:
-        kv_append(k, v, self.pages[layer], self.scales[layer], self.page_table, self.lengths, **kw)
+        kv_append(k, v, *self._layers[layer], self.page_table, self.lengths, **kw)
 
     def attend(self, layer: int, q: torch.Tensor, **kw) -> Tuple[torch.Tensor, torch.Tensor]:
-        return kv_attention(q, self.pages[layer], self.scales[layer], self.page_table, self.lengths, **kw)
+        return kv_attention(q, *self._layers[layer], self.page_table, self.lengths, **kw)
 
     def fork(self, parents: torch.Tensor, children: torch.Tensor) -> None:
         pages_fork(self.page_table, self.lengths, self.refcounts, parents, children)
