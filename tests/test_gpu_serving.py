@@ -633,3 +633,31 @@ def test_nothing_to_do(dev):
     assert bsa.pages_extend(pages, scales, tab, n, refs, none).numel() == 0
     bsa.pages_copy(pages, scales, none, none)
     assert bsa.token_logprobs(torch.zeros(0, 5, device=dev), none, 2).top_ids.shape == (0, 2)
+
+
+def test_sizes_given_as_tensors_are_read_at_each_call(dev):
+    """max_new, max_len and k as tensors that change between calls."""
+    rng = np.random.default_rng(14)
+    raw, sc, table, pages, scales, tab = _cache(rng, dev, [40], 2, 16, 64)
+    n, cu = _i32([40], dev), _i32([0, 3], dev)
+    q = torch.randn(3, 2, 64, device=dev, dtype=torch.float16)
+    want = bsa.kv_attention(q, pages, scales, tab, n, cu_seqlens=cu, max_new=3)[0]
+    most = torch.tensor(1)
+    one = bsa.kv_attention(q, pages, scales, tab, n, cu_seqlens=cu, max_new=most, max_len=most, out=torch.zeros_like(q))[0]
+    assert torch.equal(one[:1], want[:1]) and not one[1:].any()
+    most.fill_(3)
+    assert torch.equal(bsa.kv_attention(q, pages, scales, tab, n, cu_seqlens=cu, max_new=most, max_len=most, out=torch.zeros_like(q))[0], want)
+    most.fill_(1)
+    kept = pages.view(torch.uint8).clone()
+    x = torch.ones(3, 2, 64, device=dev, dtype=torch.float16)
+    bsa.kv_append(x, x, pages, scales, tab, n, cu_seqlens=cu, max_new=most)
+    most.fill_(3)
+    bsa.kv_append(x, x, pages, scales, tab, n, cu_seqlens=cu, max_new=most)
+    again = kept.clone().view(F8)
+    bsa.kv_append(x, x, again, scales, tab, n, cu_seqlens=cu, max_new=3)
+    assert torch.equal(pages.view(torch.uint8), again.view(torch.uint8))
+    k = torch.tensor(2)
+    logits, tokens = torch.randn(2, 30, device=dev), _i32([0, 1], dev)
+    assert bsa.token_logprobs(logits, tokens, k).top_ids.shape == (2, 2)
+    k.fill_(5)
+    assert bsa.token_logprobs(logits, tokens, k).top_ids.shape == (2, 5)

@@ -171,10 +171,10 @@ def _batch(x: torch.Tensor, what: str, heads: int, d: int, dev: torch.device, ro
         if rows and x.shape[0] % rows:
             raise ValueError(f"without cu_seqlens {what}'s {x.shape[0]} tokens must divide over {rows} sequences")
         per = x.shape[0] // rows if rows else 0
-        if max_new is not None and int(max_new) != per:
+        if max_new is not None and max_new != per:
             raise ValueError(f"max_new={max_new}, but each of {rows} sequences has {per} tokens")
         return per
-    return x.shape[0] if max_new is None else min(int(max_new), x.shape[0])
+    return x.shape[0] if max_new is None else min(max_new, x.shape[0])
 
 
 def _rows(slots: Optional[torch.Tensor], cu: Optional[torch.Tensor], lengths: torch.Tensor) -> int:
@@ -194,6 +194,8 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, scales: tor
     magnitude to 448 or below, and no less than the scale of tokens that the page held before (which
     are rounded again where it grows).  Infinities become +-448 x scale, NaN stays NaN.  max_new bounds
     the tokens of one sequence (default: all of them; a tight one makes a smaller launch)."""
+    if max_new is not None:
+        max_new = int(max_new)  # a number, not a tensor that may change, in the signature
     key = ("append", _sigs(k, v, pages, scales, page_table, lengths, cu_seqlens, slots), max_new)
     call = _CALLS.get(key)
     if call is None:
@@ -226,6 +228,10 @@ def kv_attention(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, pag
     1 / sqrt(head_dim) by default.  max_len, the longest sequence (default: what a table row holds),
     decides how the long axis is split and bounds nothing.  q rows must be 16-byte aligned, out rows
     8-byte aligned."""
+    if max_new is not None:
+        max_new = int(max_new)
+    if max_len is not None:
+        max_len = int(max_len)
     key = ("attend", _sigs(q, pages, scales, page_table, lengths, cu_seqlens, slots, out, lse), max_new, max_len)
     call = _CALLS.get(key)
     if call is None:
@@ -260,7 +266,7 @@ def _attention_call(q, pages, scales, page_table, lengths, cu_seqlens, max_new, 
     _i32(cu_seqlens, dev, "cu_seqlens", rows + 1)
     _i32(slots, dev, "slots")
     lib, cus = load(), _cu_count(dev)
-    longest = 0 if max_len is None else max(1, int(max_len))
+    longest = 0 if max_len is None else max(1, max_len)
     cache = _lib.KvCache(pages.data_ptr(), scales.data_ptr(), *sizes, page_table.data_ptr(), lengths.data_ptr())
     need = int(lib.bsg_kv_attention_workspace_bytes(cache, rows, heads, most, longest, cus))
     return (dev.index, lib.bsg_kv_attention, sizes, rows, most, code, q.stride(0), q.stride(1), tokens, heads,
@@ -388,6 +394,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0,
     A token outside the vocabulary gives NaN.  A row of nothing but -inf gives -inf, entropy 0 and the
     lowest ids; a NaN or +inf in a row makes its numbers NaN (NaN ranks first among the ids, -0 equals
     +0)."""
+    k = int(k)
     key = ("logprobs", _sigs(logits, tokens), k)
     call = _CALLS.get(key)
     if call is None:
@@ -413,7 +420,6 @@ def _logprobs_call(logits: torch.Tensor, tokens: torch.Tensor, k: int) -> tuple:
     rows, vocab = logits.shape
     if logits.stride(1) != 1 and vocab > 1:
         raise ValueError(f"logits rows must be contiguous, strides {logits.stride()}")
-    k = int(k)
     if not 0 <= k <= min(MAX_ALTERNATIVES, vocab):
         raise ValueError(f"k={k} (0 to {min(MAX_ALTERNATIVES, vocab)})")
     _i32(tokens, dev, "tokens", rows)
