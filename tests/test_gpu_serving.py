@@ -534,6 +534,43 @@ def test_logprobs_hard_rows(dev, dtype, vocab):
         _check_logprobs(got, orc.token_logprobs(t.double().numpy(), tokens, 20))
 
 
+@pytest.mark.parametrize("vocab", [40, 5000, 40000])
+@pytest.mark.parametrize("dtype,mask", [("fp16", -6e4), *[(t, m) for t in ("bf16", "fp32")
+                                                          for m in (-1e6, -1e9, -1e10, -1e12, -1e20, -1e30, -3e38, -np.inf)]])
+def test_logprobs_masks_of_any_size(dev, dtype, mask, vocab):
+    """Rows of which a few logits, every other one, one or none is no mask, tokens under the mask and beside it."""
+    rng = np.random.default_rng(vocab)
+    x = rng.standard_normal((8, vocab)).astype(np.float32)
+    lowest = max(mask, float(torch.finfo(DT[dtype]).min))
+    x[0, 5:] = mask
+    x[1, : vocab - 5] = mask
+    x[2, ::2] = mask
+    x[3] = mask
+    x[4, np.arange(vocab) != vocab // 2] = mask
+    x[5, : vocab // 2], x[5, vocab // 2:] = mask, lowest / 2
+    x[6, 7:] = mask
+    x[7, rng.random(vocab) < 0.9] = mask
+    tokens = np.array([0, 3, 2, vocab - 1, vocab // 2, vocab - 1, vocab - 1, 5])
+    t = torch.from_numpy(x).to(DT[dtype])
+    for k in (0, 20):
+        got = bsa.token_logprobs(t.to(dev), _i32(tokens, dev), k)
+        _check_logprobs(got, orc.token_logprobs(t.double().numpy(), tokens, k))
+
+
+@pytest.mark.parametrize("vocab", [40, 5000, 40000])
+@pytest.mark.parametrize("middle", [2.0 ** 20, -(2.0 ** 20), 2.0 ** 21, 1e6, 1e8, -1e10, 1e30])
+def test_logprobs_far_from_zero(dev, middle, vocab):
+    """Logits that are far from zero, or on either side of where that begins, and close to each other."""
+    rng = np.random.default_rng(3)
+    x = (middle + 3 * rng.standard_normal((4, vocab))).astype(np.float32)
+    x[1] = np.float32(middle) + np.spacing(np.float32(middle)) * rng.integers(-9, 9, vocab)
+    x[2, rng.random(vocab) < 0.5] = 0
+    x[3] = np.float32(middle) * rng.standard_normal(vocab)
+    tokens = rng.integers(0, vocab, 4)
+    got = bsa.token_logprobs(torch.from_numpy(x).to(dev), _i32(tokens, dev), 6)
+    _check_logprobs(got, orc.token_logprobs(x.astype(np.float64), tokens, 6))
+
+
 @pytest.mark.parametrize("dtype", ["fp16", "fp32"])
 @pytest.mark.parametrize("offset,width", [(1, 1003), (3, 1009), (7, 1024)])
 def test_logprobs_unaligned_rows(dev, dtype, offset, width):

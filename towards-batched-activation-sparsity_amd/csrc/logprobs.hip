@@ -4,7 +4,8 @@
 // With a reference M near the row's maximum, d = (x - M) log2(e), l = sum 2^d and t = sum 2^d d:
 //   logprob = ln 2 (d_token - log2 l),  entropy = ln 2 (log2 l - t / l).
 // Any M gives the same, so a lane keeps its first tile's maximum until a logit is kSlack above it,
-// and what log2(e) M is rounded to cancels: d is one fused multiply-add.
+// and where |M| is below kFar what log2(e) M is rounded to cancels: d is one fused multiply-add.  From there on
+// (masks are logits too, and a lane may have nothing else) the rounding alone would be octaves, so x - M comes first.
 //
 // The alternatives are found beside it.  A logit's key is its order among fp32 numbers (upper half) and
 // its id's complement (lower half), so that keys are distinct and (logit desc, id asc) is key desc.
@@ -34,7 +35,8 @@ constexpr int kMaxSplits = 32;  // of a row
 constexpr int kMaxK = BSG_LOGPROBS_MAX_K;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 20.f;  // a lane's weights stay below 2^29
-constexpr float kHuge = 2e38f;  // past it log2(e) x overflows: differences before products there
+constexpr float kFar = 0x1p20f;  // references from here on: log2(e) M is off by 2^-4 octaves and more, differences before products
+constexpr float kHuge = 1e38f;  // logits from here on: log2(e) (x - M) may overflow where x - M does not
 constexpr float kLow = -1e30f;  // below it (masks) 2^d d is not formed from d as it is
 constexpr float kFloor = -1e4f;  // exponents below it weigh nothing; keeps 0 x -inf out of t
 
@@ -125,19 +127,23 @@ __device__ __forceinline__ uint64_t merged(uint64_t down, uint64_t up) {
 struct Sums {
   float m, l, t;  // l and t against the reference m; -inf: nothing yet
 };
+__device__ __forceinline__ bool is_far(float m) { return !(__builtin_fabsf(m) < kFar); }
 // (x - m) log2(e)
 __device__ __forceinline__ float octaves(float x, float m) {
-  return __builtin_fabsf(m) < kHuge ? __builtin_fmaf(x, kLog2e, -(m * kLog2e)) : (x - m) * kLog2e;
+  return is_far(m) ? (x - m) * kLog2e : __builtin_fmaf(x, kLog2e, -(m * kLog2e));
+}
+// Octaves from reference m to a, each as sums against it have it: rounded after the product where it is not far.
+__device__ __forceinline__ float between(float a, float m) {
+#pragma clang fp contract(off)
+  const float pa = a * kLog2e, pm = m * kLog2e;
+  if (is_far(m)) return is_far(a) ? (a - m) * kLog2e : __builtin_fmaf(-m, kLog2e, pa);
+  return is_far(a) ? __builtin_fmaf(a, kLog2e, -pm) : pa - pm;
 }
 __device__ __forceinline__ Sums join(Sums a, Sums b) {
-  // between references as they are rounded, each product by itself, so that what cancels in the sums
-  // cancels here
 #pragma clang fp contract(off)
   const float m = fmaxf(a.m, b.m);
   if (m == -__builtin_inff()) return Sums{m, a.l + b.l, a.t + b.t};
-  const bool huge = !(__builtin_fabsf(m) < kHuge);
-  const float da = fmaxf(huge ? (a.m - m) * kLog2e : a.m * kLog2e - m * kLog2e, kFloor);
-  const float db = fmaxf(huge ? (b.m - m) * kLog2e : b.m * kLog2e - m * kLog2e, kFloor);
+  const float da = fmaxf(between(a.m, m), kFloor), db = fmaxf(between(b.m, m), kFloor);
   const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
   return Sums{m, a.l * fa + b.l * fb, fa * (a.t + a.l * da) + fb * (b.t + b.l * db)};
 }
@@ -248,7 +254,7 @@ __device__ __forceinline__ void take_tile(const u32x4 raw[kVectors], uint32_t th
     top = fmaxf(top, tops[i]);
   }
   float l = 0.f, t = 0.f;
-  if (!__any(top > sum.m + kSlack || low < kLow || !(__builtin_fabsf(sum.m) < kHuge))) {
+  if (!__any(top > sum.m + kSlack || low < kLow || is_far(sum.m))) {
     const float base = sum.m * kLog2e;
 #pragma unroll
     for (int i = 0; i < kVectors; ++i)
@@ -264,9 +270,9 @@ __device__ __forceinline__ void take_tile(const u32x4 raw[kVectors], uint32_t th
     sum.l += l, sum.t += t;
   } else {  // a new reference, or numbers that need care
     const float m = top == -__builtin_inff() ? 0.f : top;
-    // (x - m) log2(e) as s x + c, or as s (x - c)
-    const bool huge = !(__builtin_fabsf(m) < kHuge);
-    const float c = huge ? 0.f : -(m * kLog2e), u = huge ? m : 0.f;
+    // (x - m) log2(e), with the difference first or last
+    const bool far = is_far(m);
+    const float c = far ? 0.f : -(m * kLog2e), u = far ? m : 0.f;
 #pragma unroll
     for (int i = 0; i < kVectors; ++i)
       if (i < used) {
@@ -431,7 +437,10 @@ __global__ __launch_bounds__(64 * WAVES) void bsg_token_logprobs_kernel(ScorePar
   // a NaN is in l even where it was never the maximum; nothing but -inf has l = 0
   const float log_l = __builtin_amdgcn_logf(sum.l);
   const float top = sum.m == -__builtin_inff() ? 0.f : sum.m;
-  const auto logprob = [&](float v) { return sum.l == 0.f ? v : (octaves(v, top) - log_l) * kLn2; };
+  const auto logprob = [&](float v) {
+    if (sum.l == 0.f) return v;
+    return __builtin_fabsf(v) < kHuge ? (octaves(v, top) - log_l) * kLn2 : (v - top) - log_l * kLn2;
+  };
   if (lane < k) {
     p.top_ids[row * k + lane] = (int32_t)~(uint32_t)best.list;
     p.top_logprobs[row * k + lane] = logprob(from_order((uint32_t)(best.list >> 32)));
