@@ -571,6 +571,28 @@ def test_logprobs_far_from_zero(dev, middle, vocab):
     _check_logprobs(got, orc.token_logprobs(x.astype(np.float64), tokens, 6))
 
 
+@pytest.mark.parametrize("rows,vocab", [(4200, 8192), (300, 32000), (3, 100003)])
+@pytest.mark.parametrize("dtype", ["fp16", "fp32"])
+def test_logprobs_confident_rows(dev, dtype, rows, vocab):
+    """One logit 2 to 26 above the others, anywhere in its row, so that the entropy is small beside log2 l and
+    t / l where the reference lies far below it.  Against 64 bits: weights of at most 3 octaves, so that
+    the exponent, its logarithm and the quotient are each off by at most 2^-22, and sums whose
+    roundings are independent, 2^-21: together below 2^-19 of 1 + |value|."""
+    g = torch.Generator(device=dev).manual_seed(vocab)
+    x = torch.randn(rows, vocab, generator=g, device=dev)
+    at = torch.randint(0, vocab, (rows,), generator=g, device=dev)
+    x[torch.arange(rows, device=dev), at] = x.amax(1) + torch.linspace(2, 26, rows, device=dev)
+    x = x.to(DT[dtype])
+    got = bsa.token_logprobs(x, at.int(), 1)
+    assert torch.equal(got.top_ids[:, 0], at.int())
+    for r in range(0, rows, 300):
+        d = x[r:r + 300].double()
+        d -= d.amax(1, keepdim=True)
+        d -= d.exp().sum(1, keepdim=True).log()
+        for a, b in ((got.logprob, d.amax(1)), (got.top_logprobs[:, 0], d.amax(1)), (got.entropy, -(d.exp() * d).sum(1))):
+            assert ((a[r:r + 300].double() - b).abs() <= 2.0 ** -19 * (1 + b.abs())).all()
+
+
 @pytest.mark.parametrize("dtype", ["fp16", "fp32"])
 @pytest.mark.parametrize("offset,width", [(1, 1003), (3, 1009), (7, 1024)])
 def test_logprobs_unaligned_rows(dev, dtype, offset, width):

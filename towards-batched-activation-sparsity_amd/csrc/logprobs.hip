@@ -3,9 +3,10 @@
 //
 // With a reference M near the row's maximum, d = (x - M) log2(e), l = sum 2^d and t = sum 2^d d:
 //   logprob = ln 2 (d_token - log2 l),  entropy = ln 2 (log2 l - t / l).
-// Any M gives the same, so a lane keeps its first tile's maximum until a logit is kSlack above it,
-// and where |M| is below kFar what log2(e) M is rounded to cancels: d is one fused multiply-add.  From there on
-// (masks are logits too, and a lane may have nothing else) the rounding alone would be octaves, so x - M comes first.
+// Any M gives the same, so a wave keeps its first tile's maximum until a logit is kSlack above it: close to the
+// row's, since the entropy is what log2 l and t / l differ by, and they are as large as the maximum lies above M.
+// Where |M| is below kFar what log2(e) M is rounded to cancels: d is one fused multiply-add.  From there on (masks are
+// logits too, and a wave may have nothing else) the rounding alone would be octaves, so x - M comes first.
 //
 // The alternatives are found beside it.  A logit's key is its order among fp32 numbers (upper half) and
 // its id's complement (lower half), so that keys are distinct and (logit desc, id asc) is key desc.
@@ -34,7 +35,7 @@ constexpr int kSplitTiles = 2;  // tiles of a wave that a split of a long row le
 constexpr int kMaxSplits = 32;  // of a row
 constexpr int kMaxK = BSG_LOGPROBS_MAX_K;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kSlack = 20.f;  // a lane's weights stay below 2^29
+constexpr float kSlack = 2.f;  // weights stay below 2^3
 constexpr float kFar = 0x1p20f;  // references from here on: log2(e) M is off by 2^-4 octaves and more, differences before products
 constexpr float kHuge = 1e38f;  // logits from here on: log2(e) (x - M) may overflow where x - M does not
 constexpr float kLow = -1e30f;  // below it (masks) 2^d d is not formed from d as it is
@@ -125,7 +126,7 @@ __device__ __forceinline__ uint64_t merged(uint64_t down, uint64_t up) {
 }
 
 struct Sums {
-  float m, l, t;  // l and t against the reference m; -inf: nothing yet
+  float m, l, t;  // l and t against the reference m, which a wave's lanes share while they read; -inf: nothing yet
 };
 __device__ __forceinline__ bool is_far(float m) { return !(__builtin_fabsf(m) < kFar); }
 // (x - m) log2(e)
@@ -146,6 +147,18 @@ __device__ __forceinline__ Sums join(Sums a, Sums b) {
   const float da = fmaxf(between(a.m, m), kFloor), db = fmaxf(between(b.m, m), kFloor);
   const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
   return Sums{m, a.l * fa + b.l * fb, fa * (a.t + a.l * da) + fb * (b.t + b.l * db)};
+}
+template <int X>
+__device__ __forceinline__ float max_lanes(float v) {
+  v = fmaxf(v, lane_xor<X>(v));
+  if constexpr (X < 32) v = max_lanes<2 * X>(v);
+  return v;
+}
+template <int X>
+__device__ __forceinline__ float add_lanes(float v) {
+  v += lane_xor<X>(v);
+  if constexpr (X < 32) v = add_lanes<2 * X>(v);
+  return v;
 }
 template <int X>
 __device__ __forceinline__ Sums join_lanes(Sums s) {
@@ -267,9 +280,10 @@ __device__ __forceinline__ void take_tile(const u32x4 raw[kVectors], uint32_t th
           t = __builtin_fmaf(e, d, t);
         }
       }
-    sum.l += l, sum.t += t;
   } else {  // a new reference, or numbers that need care
-    const float m = top == -__builtin_inff() ? 0.f : top;
+    const float high = max_lanes<1>(top);
+    if (high > sum.m) sum = join(sum, Sums{high, 0.f, 0.f});
+    const float m = sum.m == -__builtin_inff() ? 0.f : sum.m;
     // (x - m) log2(e), with the difference first or last
     const bool far = is_far(m);
     const float c = far ? 0.f : -(m * kLog2e), u = far ? m : 0.f;
@@ -284,8 +298,8 @@ __device__ __forceinline__ void take_tile(const u32x4 raw[kVectors], uint32_t th
           t = __builtin_fmaf(e, fmaxf(d, kFloor), t);
         }
       }
-    sum = join(sum, Sums{top, l, t});
   }
+  sum.l += l, sum.t += t;
   if (k == 0) return;
 
   if (first) {
@@ -380,7 +394,7 @@ __global__ __launch_bounds__(64 * WAVES) void bsg_token_logprobs_kernel(ScorePar
     const int used = v0 + STEP <= v_end ? kVectors : (int)((v_end - v0 + 63) >> 6);
     take_tile<T>(raw, there, used, id0, k, v0 == v_begin, sum, best);
   }
-  sum = join_lanes<1>(sum);
+  sum.l = add_lanes<1>(sum.l), sum.t = add_lanes<1>(sum.t);
 
   // the waves of a row, two at a time; the lists go through the waves' own LDS
   const auto meet = [&]() {
