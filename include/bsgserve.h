@@ -126,7 +126,9 @@ int bsg_pages_fork(const bsg_page_pool* pool, const int32_t* parents, const int3
  * of range, its table row is too short, or the free pages do not reach: rows are served in order
  * until the first that they do not reach; of the later ones only those that need no page and write
  * to no shared one are.  Slots must be distinct.  n <= BSG_PAGES_MAX_ROWS.
- * Workspace: bsg_pages_workspace_bytes(num_pages), no initialisation. */
+ * Workspace: bsg_pages_workspace_bytes(num_pages), no initialisation.  The call is two launches, the
+ * first of which leaves the second its plan there: nothing else may write to it on the stream in
+ * between, so threads that share a stream need one each. */
 int64_t bsg_pages_workspace_bytes(int64_t num_pages);
 int bsg_pages_extend(const bsg_page_pool* pool, const int32_t* slots, const int32_t* new_tokens, int32_t n,
                      int32_t* served, void* ws, int64_t ws_bytes, void* stream);

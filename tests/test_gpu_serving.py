@@ -12,6 +12,8 @@ Tolerances, from the arithmetic:
 """
 from __future__ import annotations
 
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -424,6 +426,43 @@ def test_pages_copy(dev):
     for a, b in zip(src[:3], dst[:3]):
         want[0][:, b], want[1][:, b] = want[0][:, a], want[1][:, a]
     assert torch.equal(pages, want[0]) and torch.equal(scales, want[1])
+
+
+def test_threads_on_one_stream(dev):
+    """Two threads, each with a cache of its own, on one stream: extensions, compactions and split attention
+    give each what it asked for."""
+    slots, count, p, rounds = 40, 900, 16, 60
+    results = {}
+
+    def work(seed):
+        rng = np.random.default_rng(seed)
+        pool, pages, scales, tab, lengths, refs = _random_pool(rng, dev, slots, 12, count, p)
+        was = pages.clone(), scales.clone()
+        f8 = pages.view(F8)
+        raw, sc, table, kv, kv_scales, kv_tab = _cache(rng, dev, [3000], 2, 16, 64)
+        q, n = torch.randn(1, 4, 64, device=dev, dtype=torch.float16), _i32([3000], dev)
+        ok = []
+        first = bsa.kv_attention(q, kv, kv_scales, kv_tab, n)[0]
+        for _ in range(rounds):
+            gone = rng.integers(0, slots, 8)
+            pool.free(gone.tolist())
+            bsa.pages_free(tab, lengths, refs, _i32(gone, dev))
+            new = rng.integers(0, 20, slots)
+            served = bsa.pages_extend(f8, scales, tab, lengths, refs, _i32(new, dev))
+            out = bsa.kv_attention(q, kv, kv_scales, kv_tab, n)[0]
+            counts = bsa.pages_compact(f8, scales, tab, refs)
+            ok.append((served, pool.extend(new.tolist()), counts, pool.compact(), torch.equal(out, first)))
+        for got, want, counts, moved, same in ok:
+            assert got.tolist() == want and counts.tolist() == moved and same
+        _same_pool(pool, tab, lengths, refs, pages, scales, was)
+        results[seed] = True
+
+    threads = [threading.Thread(target=work, args=(s,)) for s in (21, 22)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert results == {21: True, 22: True}
 
 
 def test_cache_class_and_graph(dev):

@@ -7,6 +7,7 @@ import os
 import re
 import shutil
 import subprocess
+import threading
 
 import numpy as np
 import pytest
@@ -186,6 +187,47 @@ def test_python_layer_refuses_host_tensors():
         bsa.kv_attention(torch.zeros(1, 1, 64, dtype=torch.float16), pages, torch.ones(2, 1, 2), tab, n)
     with pytest.raises(ValueError):
         bsa.pages_free(tab, n, n, n)
+
+
+class _Device:
+    """torch's current device, streams and capture as a test sets them; workspaces are host tensors."""
+
+    def __init__(self, monkeypatch):
+        self.current, self.capturing = 0, set()
+        monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: self.current, raising=False)
+        monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 1000 * index, raising=False)
+        monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: self.current in self.capturing, raising=False)
+        for name in ("zeros", "empty"):
+            def make(*a, real=getattr(torch, name), device=None, **kw):
+                return real(*a, **kw)
+            monkeypatch.setattr(serving.torch, name, make)
+        outer = self
+
+        class Guard:
+            def __init__(self, index):
+                self.index = index
+
+            def __enter__(self):
+                self.was, outer.current = outer.current, self.index
+
+            def __exit__(self, *_):
+                outer.current = self.was
+
+        monkeypatch.setattr(torch.cuda, "device", Guard)
+
+
+def test_threads_on_one_stream_have_workspaces_of_their_own(monkeypatch):
+    """extend and compact hand a plan from one launch to the next in the workspace: what another thread
+    enqueues on the same stream in between must not write there."""
+    _Device(monkeypatch)
+    mine = serving._workspace(0, 5000, None)
+    assert serving._workspace(0, 5000, None) is mine
+    theirs = []
+    threads = [threading.Thread(target=lambda: theirs.append(serving._workspace(0, 5000, None))) for _ in range(2)]
+    for t in threads:
+        t.start()
+        t.join()
+    assert len({t.data_ptr() for t in (mine, *theirs)}) == 3
 
 
 def test_oracle_e4m3_is_torchs():

@@ -23,6 +23,7 @@ int32 [pages] how many table entries name a page.
 """
 from __future__ import annotations
 
+import threading
 from typing import Dict, NamedTuple, Optional, Tuple
 
 import torch
@@ -38,7 +39,8 @@ MAX_ROWS = 1024  # BSG_PAGES_MAX_ROWS
 MAX_ALTERNATIVES = 64  # BSG_LOGPROBS_MAX_K
 
 _F8 = torch.float8_e4m3fn
-_WORKSPACES: Dict[tuple, list] = {}
+_WORKSPACES: Dict[tuple, list] = {}  # by (device, prefix)
+_OF_THREAD = threading.local()  # its attributes by (device, stream)
 
 
 # What a call's shapes, strides, types and devices decide (the checks, the sizes, the library's
@@ -88,23 +90,27 @@ def _launch(index: int, fn, *args) -> None:
 def _workspace(index: int, nbytes: int, prefix: Optional[str], cleared: bool = True) -> torch.Tensor:
     """At least `nbytes`, the first COUNTER_BYTES of them zero (the kernels leave them zero).
 
-    Without a prefix an eager call takes the buffer of its stream, which calls on that stream use in
-    turn, and a captured one a buffer of its own in the graph's memory, its counters cleared by the
-    graph (where `cleared`): graphs may then replay beside each other.  With a prefix both take the
-    prefix's buffer, and calls that may overlap must not share one.  A buffer is never given back while
-    a graph may hold it: a larger one is made beside it."""
-    key = (index, torch._C._cuda_getCurrentRawStream(index)) if prefix is None else (index, prefix)
+    Without a prefix an eager call takes the buffer that its thread has for its stream, which the
+    thread's calls on that stream use in turn (another thread's could come between the two launches of
+    a page plan), and a captured one a buffer of its own in the graph's memory, its counters cleared by
+    the graph (where `cleared`): graphs may then replay beside each other.  With a prefix both take the
+    prefix's buffer, and calls of several threads, or that may overlap, must not share one.  A buffer is
+    never given back while a graph may hold it: a larger one is made beside it."""
+    if prefix is None:
+        key, all_held = (index, torch._C._cuda_getCurrentRawStream(index)), _OF_THREAD.__dict__
+    else:
+        key, all_held = (index, prefix), _WORKSPACES
     if torch._C._cuda_isCurrentStreamCapturing():
         if prefix is None:
             ws = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
             if cleared:
                 ws[:COUNTER_BYTES].zero_()
             return ws
-        held = _WORKSPACES.get(key)
+        held = all_held.get(key)
         if not held or held[-1].numel() < nbytes:
             raise RuntimeError(f"workspace {prefix!r} is too small for this call: run it once before capturing it")
         return held[-1]
-    held = _WORKSPACES.setdefault(key, [])
+    held = all_held.setdefault(key, [])
     if not held or held[-1].numel() < nbytes:
         held.append(torch.zeros(1 << max(20, (nbytes - 1).bit_length()), dtype=torch.uint8, device=torch.device("cuda", index)))
     return held[-1]
