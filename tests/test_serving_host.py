@@ -230,6 +230,21 @@ def test_threads_on_one_stream_have_workspaces_of_their_own(monkeypatch):
     assert len({t.data_ptr() for t in (mine, *theirs)}) == 3
 
 
+def test_workspace_asks_the_tensors_device_for_a_capture(monkeypatch):
+    """Not the current one: a call on device 1 from device 0."""
+    d = _Device(monkeypatch)
+    eager = serving._workspace(1, 5000, None)
+    d.capturing = {1}
+    first, second = (serving._workspace(1, 5000, None) for _ in range(2))
+    assert first is not eager and second is not first and first.numel() == 5000
+    assert serving._workspace(0, 5000, None) is serving._workspace(0, 5000, None)
+    d.capturing = {0}
+    assert serving._workspace(1, 5000, None) is eager
+    with pytest.raises(RuntimeError):
+        serving._workspace(0, 5000, "not used before")
+    assert serving._workspace(1, 5000, "not used before") is not None and d.current == 0
+
+
 def test_oracle_e4m3_is_torchs():
     table = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).double().numpy()
     np.testing.assert_array_equal(orc.E4M3, table)

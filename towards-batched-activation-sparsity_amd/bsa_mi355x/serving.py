@@ -96,6 +96,9 @@ def _workspace(index: int, nbytes: int, prefix: Optional[str], cleared: bool = T
     the graph (where `cleared`): graphs may then replay beside each other.  With a prefix both take the
     prefix's buffer, and calls of several threads, or that may overlap, must not share one.  A buffer is
     never given back while a graph may hold it: a larger one is made beside it."""
+    if torch._C._cuda_getDevice() != index:  # the capture asked for below is the current device's
+        with torch.cuda.device(index):
+            return _workspace(index, nbytes, prefix, cleared)
     if prefix is None:
         key, all_held = (index, torch._C._cuda_getCurrentRawStream(index)), _OF_THREAD.__dict__
     else:
