@@ -522,6 +522,47 @@ def test_cache_class_and_graph(dev):
     assert int(cache.lengths[2]) == 48 and torch.isfinite(k).all()
 
 
+def test_cache_grown_by_larger_tensors(dev):
+    """All calls work on the tensors that the cache has now; layers are indexed as a list's entries are."""
+    heads, d, layers = 2, 64, 3
+    cache = bsa.KVCache(layers, 4, heads, d, page_size=16, max_slots=2, max_pages=8, device=dev)
+    assert cache.extend(_i32([20, 9], dev)).tolist() == [1, 1]
+    x = [torch.randn(29, heads, d, device=dev, dtype=torch.float16) for _ in range(layers)]
+    cu = _i32([0, 20, 29], dev)
+    for layer in range(layers):
+        cache.append(layer, x[layer], -x[layer], cu_seqlens=cu)
+    old = cache.pages
+    cache.pages = torch.zeros(layers, 40, heads, 2, 16, d, dtype=torch.uint8, device=dev).view(F8)
+    cache.pages.view(torch.uint8)[:, :4] = old.view(torch.uint8)
+    cache.scales = torch.cat([cache.scales, torch.ones(layers, 36, heads, 2, device=dev)], 1)
+    cache.refcounts = torch.cat([cache.refcounts, cache.refcounts.new_zeros(36)])
+    old.view(torch.uint8).fill_(0x7F)
+    assert cache.extend(_i32([60, 50], dev)).tolist() == [1, 1]
+    new = [torch.randn(110, heads, d, device=dev, dtype=torch.float16) for _ in range(layers)]
+    cu = _i32([0, 60, 110], dev)
+    for layer in (0, 2, -2):
+        cache.append(layer, new[layer], -new[layer], cu_seqlens=cu)
+        q = torch.randn(2, heads, d, device=dev, dtype=torch.float16)
+        out, lse = cache.attend(layer, q)
+        ref = orc.attention(q.double().cpu().numpy(), orc.Layer(_raw(cache.pages[layer]), cache.scales[layer].cpu().numpy()),
+                            cache.page_table.cpu().numpy(), cache.lengths.cpu().numpy(), [0, 1, 2])
+        _check_attention(out, lse, ref, torch.float16, d)
+        k, v = cache.read(layer, 0)
+        want = torch.cat([x[layer][:20], new[layer][:60]]).transpose(0, 1).float()
+        assert (k - want).abs().max() <= 0.3 and (v + want).abs().max() <= 0.3  # of at most 6: 2^-4 of a number
+    for layer in (3, -4):
+        with pytest.raises(IndexError):
+            cache.append(layer, new[0], new[0], cu_seqlens=cu)
+        with pytest.raises(IndexError):
+            cache.attend(layer, q)
+    with pytest.raises(TypeError):
+        cache.attend(0.5, q)
+    with pytest.raises(ValueError):
+        bsa.kv_attention(q, cache.pages, cache.scales, cache.page_table, cache.lengths)
+    with pytest.raises(ValueError):
+        bsa.kv_attention(q, cache.pages[0], cache.scales[0], cache.page_table, cache.lengths, layer=0)
+
+
 # ---------------------------------------------------------------------------------------- log probabilities
 
 

@@ -23,6 +23,7 @@ int32 [pages] how many table entries name a page.
 """
 from __future__ import annotations
 
+import operator
 import threading
 from typing import Dict, NamedTuple, Optional, Tuple
 
@@ -158,14 +159,29 @@ def _storage(pages: torch.Tensor, scales: torch.Tensor, dims: int) -> torch.devi
     return dev
 
 
-def _layer(pages: torch.Tensor, scales: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor):
-    """The device of one layer's tensors, and the sizes of its bsg_kv_cache."""
-    dev = _storage(pages, scales, 5)
+def _layer(pages: torch.Tensor, scales: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, layer: Optional[int]):
+    """The device of one layer's tensors, the sizes of its bsg_kv_cache, and of pages and scales of
+    several layers their number and the bytes from one to the next."""
+    dev = _storage(pages, scales, 5 if layer is None else 6)
     _table(page_table, dev)
-    n, h, _, p, d = pages.shape
+    n, h, _, p, d = pages.shape[-5:]
     slots, each = page_table.shape
     _i32(lengths, dev, "lengths", slots)
-    return dev, (n, h, p, d, slots, each, page_table.stride(0) if slots > 1 else each)
+    steps = (1, 0, 0) if layer is None else (pages.shape[0], n * h * 2 * p * d, n * h * 2 * 4)
+    return dev, (n, h, p, d, slots, each, page_table.stride(0) if slots > 1 else each), steps
+
+
+def _kv_cache(pages: torch.Tensor, scales: torch.Tensor, layer: Optional[int], steps: tuple, sizes: tuple,
+              page_table: torch.Tensor, lengths: torch.Tensor) -> _lib.KvCache:
+    at, scales_at = pages.data_ptr(), scales.data_ptr()
+    if layer is not None:
+        layers, page_step, scale_step = steps
+        i = operator.index(layer)
+        if not -layers <= i < layers:
+            raise IndexError(f"layer {i} of {layers}")
+        i %= layers
+        at, scales_at = at + i * page_step, scales_at + i * scale_step
+    return _lib.KvCache(at, scales_at, *sizes, page_table.data_ptr(), lengths.data_ptr())
 
 
 def _batch(x: torch.Tensor, what: str, heads: int, d: int, dev: torch.device, rows: int, cu, max_new) -> int:
@@ -194,7 +210,7 @@ def _rows(slots: Optional[torch.Tensor], cu: Optional[torch.Tensor], lengths: to
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, page_table: torch.Tensor,
               lengths: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None, max_new: Optional[int] = None,
-              slots: Optional[torch.Tensor] = None) -> None:
+              slots: Optional[torch.Tensor] = None, layer: Optional[int] = None) -> None:
     """Write the new keys and values of a batch, [tokens, heads, head_dim] fp16/bf16, into one
     layer's pages.  Row b (slot slots[b], or b) has the tokens cu_seqlens[b] .. cu_seqlens[b+1], or an
     equal share of them; they are the last of its lengths, which already count them.
@@ -202,13 +218,14 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, scales: tor
     Each page, head and K/V has one scale: the least power of two that brings its largest finite
     magnitude to 448 or below, and no less than the scale of tokens that the page held before (which
     are rounded again where it grows).  Infinities become +-448 x scale, NaN stays NaN.  max_new bounds
-    the tokens of one sequence (default: all of them; a tight one makes a smaller launch)."""
+    the tokens of one sequence (default: all of them; a tight one makes a smaller launch).  With
+    `layer`, pages and scales are those of all layers, of which it names one."""
     if max_new is not None:
         max_new = int(max_new)  # a number, not a tensor that may change, in the signature
-    key = ("append", _sigs(k, v, pages, scales, page_table, lengths, cu_seqlens, slots), max_new)
+    key = ("append", _sigs(k, v, pages, scales, page_table, lengths, cu_seqlens, slots), max_new, layer is None)
     call = _CALLS.get(key)
     if call is None:
-        dev, sizes = _layer(pages, scales, page_table, lengths)
+        dev, sizes, steps = _layer(pages, scales, page_table, lengths, layer)
         rows = _rows(slots, cu_seqlens, lengths)
         most = _batch(k, "k", sizes[1], sizes[3], dev, rows, cu_seqlens, max_new)
         _batch(v, "v", sizes[1], sizes[3], dev, rows, cu_seqlens, None if cu_seqlens is None else most)
@@ -217,9 +234,9 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, scales: tor
         _i32(cu_seqlens, dev, "cu_seqlens", rows + 1)
         _i32(slots, dev, "slots")
         call = _remember(key, (dev.index, load().bsg_kv_append, sizes, rows, most, _dtype_code(k), k.stride(0), k.stride(1),
-                               v.stride(0), v.stride(1), k.shape[0]))
-    index, fn, sizes, rows, most, code, kt, kh, vt, vh, tokens = call
-    cache = _lib.KvCache(pages.data_ptr(), scales.data_ptr(), *sizes, page_table.data_ptr(), lengths.data_ptr())
+                               v.stride(0), v.stride(1), k.shape[0], steps))
+    index, fn, sizes, rows, most, code, kt, kh, vt, vh, tokens, steps = call
+    cache = _kv_cache(pages, scales, layer, steps, sizes, page_table, lengths)
     _launch(index, fn, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, tokens, cache, _ptr(slots), rows, _ptr(cu_seqlens), most, code)
 
 
@@ -227,13 +244,14 @@ def kv_attention(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, pag
                  lengths: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None, max_new: Optional[int] = None,
                  slots: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None, max_len: Optional[int] = None,
                  out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
-                 workspace_prefix: Optional[str] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+                 workspace_prefix: Optional[str] = None,
+                 layer: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Attention of a batch's new tokens q, [tokens, query heads, head_dim] fp16/bf16, over one
     layer's cached tokens, their own (appended before) among them: token i of a sequence's n new ones sees the
     first length - n + i + 1 tokens.  Query head h reads cached head h // (query heads / heads).
     Returns (out like q, lse fp32 [tokens, query heads]); a token that sees nothing gets zeros and -inf.
 
-    Rows, cu_seqlens and max_new as kv_append (tokens past max_new are not computed); sm_scale is
+    Rows, cu_seqlens, max_new and layer as kv_append (tokens past max_new are not computed); sm_scale is
     1 / sqrt(head_dim) by default.  max_len, the longest sequence (default: what a table row holds),
     decides how the long axis is split and bounds nothing.  q rows must be 16-byte aligned, out rows
     8-byte aligned."""
@@ -241,16 +259,16 @@ def kv_attention(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, pag
         max_new = int(max_new)
     if max_len is not None:
         max_len = int(max_len)
-    key = ("attend", _sigs(q, pages, scales, page_table, lengths, cu_seqlens, slots, out, lse), max_new, max_len)
+    key = ("attend", _sigs(q, pages, scales, page_table, lengths, cu_seqlens, slots, out, lse), max_new, max_len, layer is None)
     call = _CALLS.get(key)
     if call is None:
-        call = _remember(key, _attention_call(q, pages, scales, page_table, lengths, cu_seqlens, max_new, slots, max_len, out, lse))
-    index, fn, sizes, rows, most, code, qt, qh, tokens, heads, out_mold, lse_mold, longest, need, cus, scale = call
+        call = _remember(key, _attention_call(q, pages, scales, page_table, lengths, cu_seqlens, max_new, slots, max_len, out, lse, layer))
+    index, fn, sizes, rows, most, code, qt, qh, tokens, heads, out_mold, lse_mold, longest, need, cus, scale, steps = call
     if out is None:
         out = torch.empty_like(out_mold)
     if lse is None:
         lse = torch.empty_like(lse_mold)
-    cache = _lib.KvCache(pages.data_ptr(), scales.data_ptr(), *sizes, page_table.data_ptr(), lengths.data_ptr())
+    cache = _kv_cache(pages, scales, layer, steps, sizes, page_table, lengths)
     ws, room = 0, 0
     if need > 0:
         held = _workspace(index, need, workspace_prefix)
@@ -260,9 +278,9 @@ def kv_attention(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, pag
     return out, lse
 
 
-def _attention_call(q, pages, scales, page_table, lengths, cu_seqlens, max_new, slots, max_len, out, lse) -> tuple:
+def _attention_call(q, pages, scales, page_table, lengths, cu_seqlens, max_new, slots, max_len, out, lse, layer) -> tuple:
     """The checks of kv_attention and what follows from its arguments' shapes."""
-    dev, sizes = _layer(pages, scales, page_table, lengths)
+    dev, sizes, steps = _layer(pages, scales, page_table, lengths, layer)
     rows = _rows(slots, cu_seqlens, lengths)
     most = _batch(q, "q", 0, sizes[3], dev, rows, cu_seqlens, max_new)
     code = _dtype_code(q)
@@ -279,7 +297,7 @@ def _attention_call(q, pages, scales, page_table, lengths, cu_seqlens, max_new, 
     cache = _lib.KvCache(pages.data_ptr(), scales.data_ptr(), *sizes, page_table.data_ptr(), lengths.data_ptr())
     need = int(lib.bsg_kv_attention_workspace_bytes(cache, rows, heads, most, longest, cus))
     return (dev.index, lib.bsg_kv_attention, sizes, rows, most, code, q.stride(0), q.stride(1), tokens, heads,
-            _mold(q.shape, q.dtype, dev), _mold(q.shape[:2], torch.float32, dev), longest, need, cus, d ** -0.5)
+            _mold(q.shape, q.dtype, dev), _mold(q.shape[:2], torch.float32, dev), longest, need, cus, d ** -0.5, steps)
 
 
 # The int32 tensors of each page call beside the cache's own.
@@ -474,16 +492,15 @@ class KVCache:
         self.lengths = torch.zeros(max_slots, dtype=torch.int32, device=dev)
         self.refcounts = torch.zeros(num_pages, dtype=torch.int32, device=dev)
         self.page_size, self.head_dim, self.heads = page_size, head_dim, heads
-        self._layers = list(zip(self.pages, self.scales))  # views: indexing costs a call more than its checks do
 
     def extend(self, new_tokens: torch.Tensor, slots: Optional[torch.Tensor] = None, **kw) -> torch.Tensor:
         return pages_extend(self.pages, self.scales, self.page_table, self.lengths, self.refcounts, new_tokens, slots, **kw)
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, **kw) -> None:
-        kv_append(k, v, *self._layers[layer], self.page_table, self.lengths, **kw)
+        kv_append(k, v, self.pages, self.scales, self.page_table, self.lengths, layer=layer, **kw)
 
     def attend(self, layer: int, q: torch.Tensor, **kw) -> Tuple[torch.Tensor, torch.Tensor]:
-        return kv_attention(q, *self._layers[layer], self.page_table, self.lengths, **kw)
+        return kv_attention(q, self.pages, self.scales, self.page_table, self.lengths, layer=layer, **kw)
 
     def fork(self, parents: torch.Tensor, children: torch.Tensor) -> None:
         pages_fork(self.page_table, self.lengths, self.refcounts, parents, children)
