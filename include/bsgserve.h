@@ -35,6 +35,7 @@ extern "C" {
 #define BSG_F32 2                     /* logits only */
 #define BSG_KV_SCALE_MIN_EXP (-40)    /* scales lie in [2^-40, 2^80] */
 #define BSG_KV_SCALE_MAX_EXP 80
+#define BSG_KV_MAX_TOKENS (1 << 30)   /* max_pages x page_size of a table */
 #define BSG_PAGES_MAX_ROWS 1024       /* slots of one fork, extend or free call */
 #define BSG_LOGPROBS_MAX_K 64
 
@@ -46,7 +47,7 @@ typedef struct bsg_kv_cache {
   int32_t page_size;         /* 16, 32, 64 or 128 */
   int32_t head_dim;          /* 64 or 128 */
   int32_t num_slots;         /* rows of page_table, entries of lengths */
-  int32_t max_pages;         /* columns of page_table; max_pages x page_size <= 2^30 */
+  int32_t max_pages;         /* columns of page_table; max_pages x page_size <= BSG_KV_MAX_TOKENS */
   int64_t table_stride;      /* elements between its rows, >= max_pages */
   const int32_t* page_table;
   const int32_t* lengths;    /* tokens of each slot, the new ones of a call among them */
@@ -101,7 +102,7 @@ typedef struct bsg_page_pool {
   int64_t page_scales;    /* floats of one layer's page */
   int32_t page_size;
   int32_t num_slots;
-  int32_t max_pages;
+  int32_t max_pages;      /* as in bsg_kv_cache */
   int64_t table_stride;
   int32_t* page_table;
   int32_t* lengths;

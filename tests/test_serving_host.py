@@ -87,6 +87,17 @@ def test_rows_of_more_than_2_30_tokens_are_refused():
     assert need(ctypes.byref(over), 4, 4, 1, 0, 256) == -1 and need(ctypes.byref(most), 4, 4, 1, 0, 256) > 0
 
 
+def test_page_calls_refuse_the_rows_that_append_and_attention_refuse():
+    lib = bsa.load()
+    over, most = (dict(max_pages=n, table_stride=n) for n in ((1 << 26) + 1, 1 << 26))
+    need = lib.bsg_pages_workspace_bytes(100)
+    for sizes, code in ((over, _lib.BSG_ERR_UNSUPPORTED), (most, _lib.BSG_ERR_WORKSPACE)):
+        assert lib.bsg_pages_extend(_pool(**sizes), FAKE, FAKE, 4, FAKE, FAKE, need - 1, None) == code
+        assert lib.bsg_pages_compact(_pool(**sizes), FAKE, FAKE, need - 1, None) == code
+    assert lib.bsg_pages_fork(_pool(**over), FAKE, FAKE, 4, None) == _lib.BSG_ERR_UNSUPPORTED
+    assert lib.bsg_pages_free(_pool(**over), FAKE, 4, None) == _lib.BSG_ERR_UNSUPPORTED
+
+
 def test_bad_batches_are_refused():
     c = _cache()
     assert _append(c, k=None) == _lib.BSG_ERR_ARG

@@ -288,7 +288,7 @@ int check_kv_cache(const bsg_kv_cache* c) {
   if (!is_aligned(c->pages, 16) || !is_aligned(c->scales, 8))
     return fail(BSG_ERR_ALIGN, "cache: pages must be 16-byte and scales 8-byte aligned");
   // the attention's positions are 32-bit and go past a row's end by up to 4096
-  if ((int64_t)c->max_pages * c->page_size > 1 << 30)
+  if ((int64_t)c->max_pages * c->page_size > BSG_KV_MAX_TOKENS)
     return fail(BSG_ERR_UNSUPPORTED, "cache: %d pages of %d tokens in a row", c->max_pages, c->page_size);
   return BSG_OK;
 }

@@ -348,7 +348,8 @@ int check_pool(const bsg_page_pool* q, bool data, bool table, bool refs) {
     if (q->page_size < 1 || q->num_slots < 1 || q->max_pages < 1 || q->table_stride < q->max_pages)
       return fail(BSG_ERR_ARG, "pool: page_size=%d num_slots=%d max_pages=%d table_stride=%lld", q->page_size,
                   q->num_slots, q->max_pages, (long long)q->table_stride);
-    if ((int64_t)q->max_pages * q->page_size > 0x7fffffff)
+    // what append and attention take of a row
+    if ((int64_t)q->max_pages * q->page_size > BSG_KV_MAX_TOKENS)
       return fail(BSG_ERR_UNSUPPORTED, "pool: %d pages of %d tokens in a row", q->max_pages, q->page_size);
   }
   if (refs && !q->refcounts) return fail(BSG_ERR_ARG, "pool: refcounts is null");
