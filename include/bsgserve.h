@@ -58,7 +58,7 @@ typedef struct bsg_kv_cache {
  *   slots    : the slot of each of `rows` sequences, or NULL for 0 .. rows-1; others are skipped
  *   cu       : rows + 1 token offsets, or NULL when every sequence has max_new tokens
  *              (tokens == rows * max_new)
- *   max_new  : at least the most tokens of one sequence (later ones are not written)
+ *   max_new  : at least the most tokens of one sequence (later ones are neither written nor weighed)
  * Row b's new tokens are the last cu[b+1] - cu[b] of its lengths[slot].  Per page, head and K/V:
  * a = the largest finite magnitude among the new tokens, scale = the least power of two >= a / 448,
  * and no less than the page's scale if it holds earlier tokens, which are rounded again when the scale grows

@@ -79,15 +79,15 @@ class Layer:
 
 
 def append(layer: Layer, k: np.ndarray, v: np.ndarray, table: np.ndarray, lengths: np.ndarray, cu: List[int],
-           slots: Optional[List[int]] = None) -> None:
+           slots: Optional[List[int]] = None, max_new: Optional[int] = None) -> None:
     p, n = layer.p, layer.values.shape[0]
     for b in range(len(cu) - 1):
         slot = b if slots is None else slots[b]
         new = cu[b + 1] - cu[b]
         if not 0 <= slot < len(lengths) or new == 0:
             continue
-        end = min(int(lengths[slot]), table.shape[1] * p)
         start = int(lengths[slot]) - new
+        end = min(start + (new if max_new is None else min(new, max_new)), table.shape[1] * p)
         for j in range(max(start, 0) // p, -(-end // p)):
             page = int(table[slot, j])
             if not 0 <= page < n:

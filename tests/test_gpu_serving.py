@@ -154,6 +154,22 @@ def test_append_edges(dev, case):
     _same_pages(pages, scales, layer)
 
 
+@pytest.mark.parametrize("p", [16, 128])
+@pytest.mark.parametrize("max_new", [1, 3, 17, 40])
+def test_append_writes_max_new_tokens(dev, p, max_new):
+    """Tokens past max_new are not written, wherever a page ends, and do not weigh in a scale."""
+    rng = np.random.default_rng([p, max_new])
+    new, lengths = [5, 1, 0, 40, 12], [21, 1, 7, 150, 9]  # the last one's first three have no place
+    raw, sc, table, pages, scales, tab = _cache(rng, dev, lengths, 2, p, 64)
+    cu = np.concatenate([[0], np.cumsum(new)])
+    k, v = (torch.from_numpy(rng.standard_normal((cu[-1], 2, 64)) * 2.0 ** np.arange(cu[-1])[:, None, None] ** 0.5).half().to(dev)
+            for _ in range(2))
+    layer = orc.Layer(raw, sc)
+    orc.append(layer, k.float().cpu().numpy(), v.float().cpu().numpy(), table, np.array(lengths), list(cu), max_new=max_new)
+    bsa.kv_append(k, v, pages, scales, tab, _i32(lengths, dev), cu_seqlens=_i32(cu, dev), max_new=max_new)
+    _same_pages(pages, scales, layer)
+
+
 # ---------------------------------------------------------------------------------------- attention
 
 

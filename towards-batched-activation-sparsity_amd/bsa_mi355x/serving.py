@@ -218,7 +218,8 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, scales: tor
     Each page, head and K/V has one scale: the least power of two that brings its largest finite
     magnitude to 448 or below, and no less than the scale of tokens that the page held before (which
     are rounded again where it grows).  Infinities become +-448 x scale, NaN stays NaN.  max_new bounds
-    the tokens of one sequence (default: all of them; a tight one makes a smaller launch).  With
+    the tokens of one sequence (default: all of them; a tight one makes a smaller launch); the ones past
+    it are not written.  With
     `layer`, pages and scales are those of all layers, of which it names one."""
     if max_new is not None:
         max_new = int(max_new)  # a number, not a tensor that may change, in the signature

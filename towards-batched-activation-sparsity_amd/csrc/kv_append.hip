@@ -138,15 +138,16 @@ __global__ __launch_bounds__(P <= 64 ? 256 : 512) void bsg_kv_append_kernel(Appe
   int64_t from = (int64_t)row * p.max_new, to = from + p.max_new;
   int slot = real ? row : -1;
   if (p.slots && real) slot = p.slots[row];
-  int64_t len = slot >= 0 && slot < p.num_slots ? p.lengths[slot] : 0;  // on its way beside the offsets
+  const int64_t len = slot >= 0 && slot < p.num_slots ? p.lengths[slot] : 0;  // on its way beside the offsets
   if (p.cu && real) from = p.cu[row], to = p.cu[row + 1];
   bool fine = slot >= 0 && slot < p.num_slots && from >= 0 && from < to && to <= p.tokens;
   const int64_t start = len - (to - from);  // may be below 0: tokens at negative positions are not written
   const int64_t most = (int64_t)p.max_pages * P;
-  if (len > most) len = most;
+  int64_t end = to - from > p.max_new ? start + p.max_new : len;  // of the tokens that are written
+  if (end > most) end = most;
   const int64_t j = (start > 0 ? start : 0) / P + nth;
   const int64_t lo = start > j * P ? start - j * P : 0;                 // first new token of the page
-  const int64_t hi = len < (j + 1) * P ? len - j * P : P;               // end of its tokens
+  const int64_t hi = end < (j + 1) * P ? end - j * P : P;               // end of its tokens
   fine = fine && lo < hi && j < p.max_pages;
   int32_t page = -1;
   if (fine) page = p.table[(int64_t)slot * p.table_stride + j];
