@@ -231,6 +231,107 @@ def test_attention_split(dev, lengths, max_len):
     _attend(dev, rng, lengths, [3] * len(lengths), 4, 2, 64, 64, torch.bfloat16, max_len=max_len)
 
 
+# ---- prompts (more than 32 rows of a cached head) over more tokens than one turn of the kernel's page numbers
+# (1024), in one part and in several, which take other paths at their ends
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("hq,heads,p,d", [(2, 2, 16, 64), (4, 2, 64, 128), (3, 1, 128, 64), (1, 1, 16, 128)])
+@pytest.mark.parametrize("lengths,new,max_len", [([1100], [40], None), ([2049, 70, 1025], [130, 65, 33], None),
+                                                 ([5000], [200], 700), ([5000, 1300], [35, 60], 1100), ([4099], [300], None)])
+def test_prompt_over_long_caches(dev, dtype, hq, heads, p, d, lengths, new, max_len):
+    rng = np.random.default_rng([hq, p, d, len(new), lengths[0]])
+    _attend(dev, rng, lengths, new, hq, heads, p, d, DT[dtype], max_len=max_len)
+
+
+@pytest.mark.parametrize("max_len", [None, 500])
+@pytest.mark.parametrize("p", [16, 64, 128])
+def test_prompt_pages_out_of_range(dev, p, max_len):
+    """Pages that do not exist before and after token 1024, and a whole turn of them."""
+    rng = np.random.default_rng(p)
+    lengths, new = [3300, 2500], [70, 40]
+    raw, sc, table, pages, scales, tab = _cache(rng, dev, lengths, 2, p, 64, poison=True)
+    table[0, 300 // p], table[0, 1040 // p], table[0, 2064 // p], table[0, 3299 // p] = -1, 10 ** 7, -3, 2 ** 31 - 1
+    table[1, 1024 // p: 2176 // p] = -1
+    cu = np.concatenate([[0], np.cumsum(new)])
+    q = torch.from_numpy(rng.standard_normal((cu[-1], 4, 64)).astype(np.float32)).half().to(dev)
+    ref = orc.attention(q.double().cpu().numpy(), orc.Layer(raw, sc), table, np.array(lengths), list(cu))
+    out, lse = bsa.kv_attention(q, pages, scales, _i32(table, dev), _i32(lengths, dev), cu_seqlens=_i32(cu, dev), max_new=70,
+                                max_len=max_len)
+    _check_attention(out, lse, ref, torch.float16, 64)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("max_len", [None, 500])
+@pytest.mark.parametrize("new", [3, 50])
+@pytest.mark.parametrize("kind", ["keys_grow", "keys_shrink", "sink", "value_scales", "values_grow", "values_shrink"])
+def test_attention_maximum_moves(dev, kind, new, max_len, dtype):
+    """Scores and value scales that outgrow, late and by many octaves, what was the maximum at first, or
+    never come near it again."""
+    rng = np.random.default_rng(len(kind) + new)
+    p, d, length, dt = 16, 64, 2200, DT[dtype]
+    raw, sc, table, pages, scales, tab = _cache(rng, dev, [length, 700], 2, p, d)
+    for row, n in ((0, length), (1, 700)):
+        ids, at = table[row, : -(-n // p)], np.arange(-(-n // p))[:, None]
+        if kind == "keys_grow":
+            sc[ids, :, 0] = 2.0 ** (at * 8 // len(at) - 8)
+        elif kind == "keys_shrink":
+            sc[ids, :, 0] = 2.0 ** (-1 - at * 8 // len(at))
+        elif kind == "sink":
+            sc[ids[:1], :, 0] = 1.0
+        elif kind == "value_scales":
+            sc[ids, :, 1] = 2.0 ** rng.integers(-38, 20, (len(ids), 2))
+        else:
+            steps = at * 40 // len(at) - 20
+            sc[ids, :, 1] = 2.0 ** (steps if kind == "values_grow" else -steps)
+    q = torch.from_numpy(rng.standard_normal((2 * new, 4, d)).astype(np.float32)).to(dt).to(dev)
+    ref = orc.attention(q.double().cpu().numpy(), orc.Layer(raw, sc), table, np.array([length, 700]), [0, new, 2 * new])
+    out, lse = bsa.kv_attention(q, pages, torch.from_numpy(sc).to(dev), tab, _i32([length, 700], dev), max_len=max_len)
+    if dt == torch.float16:  # outputs past its range are infinite (the ones about 65520 may be either)
+        past = np.abs(ref[0]) >= 65520 * (1 - 2.0 ** -7)
+        sure = np.abs(ref[0]) >= 65520 * (1 + 2.0 ** -7)
+        assert (out.double().cpu().numpy()[sure] == np.copysign(np.inf, ref[0][sure])).all()
+        out = torch.where(torch.from_numpy(past).to(dev), 0, out)
+        ref = (np.where(past, 0.0, ref[0]), *ref[1:])
+    _check_attention(out, lse, ref, dt, d)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("new", [2, 60])
+@pytest.mark.parametrize("sm_scale", [-0.125, -1.0, 0.0, -0.0, 1e-30, -1e-30, 2.0])
+def test_attention_scales_of_any_sign(dev, sm_scale, new, dtype):
+    rng = np.random.default_rng(new)
+    lengths = [1500, 61]
+    raw, sc, table, pages, scales, tab = _cache(rng, dev, lengths, 2, 32, 64, poison=True)
+    q = torch.from_numpy(rng.standard_normal((2 * new, 4, 64)).astype(np.float32)).to(DT[dtype]).to(dev)
+    ref = orc.attention(q.double().cpu().numpy(), orc.Layer(raw, sc), table, np.array(lengths), [0, new, 2 * new], sm_scale=sm_scale)
+    for max_len in (None, 500):
+        out, lse = bsa.kv_attention(q, pages, scales, tab, _i32(lengths, dev), sm_scale=sm_scale, max_len=max_len)
+        _check_attention(out, lse, ref, DT[dtype], 64)
+
+
+def test_prompt_split_graph_and_repeats(dev):
+    """A prompt in several parts: the same numbers at every call, eager or replayed."""
+    rng = np.random.default_rng(16)
+    raw, sc, table, pages, scales, tab = _cache(rng, dev, [3000, 1900], 2, 16, 128)
+    n = _i32([3000, 1900], dev)
+    q = torch.randn(300, 4, 128, device=dev, dtype=torch.bfloat16)
+    want, want_l = (x.clone() for x in bsa.kv_attention(q, pages, scales, tab, n))
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out, lse = bsa.kv_attention(q, pages, scales, tab, n)
+    for _ in range(4):
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(lse, want_l)
+        eager = bsa.kv_attention(q, pages, scales, tab, n)
+        assert torch.equal(eager[0], want) and torch.equal(eager[1], want_l)
+    ref = orc.attention(q.double().cpu().numpy(), orc.Layer(raw, sc), table, np.array([3000, 1900]), [0, 150, 300])
+    _check_attention(want, want_l, ref, torch.bfloat16, 128)
+
+
 def test_attention_empty_rows(dev):
     """Sequences without tokens, new tokens that have no place, slots out of range: zeros and -inf."""
     rng = np.random.default_rng(2)
