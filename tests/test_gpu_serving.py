@@ -332,6 +332,50 @@ def test_prompt_split_graph_and_repeats(dev):
     _check_attention(want, want_l, ref, torch.bfloat16, 128)
 
 
+@pytest.mark.parametrize("octaves", [10, 20, 24, 26, 27, 28, 30, 40, 70])
+@pytest.mark.parametrize("new,hq", [(1, 2), (3, 2), (30, 4)])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_attention_far_scores(dev, dtype, new, hq, octaves):
+    """Scores of up to 2^octaves that differ by as much: the values of the largest are averaged.  Queries and
+    keys are small integers, so the products are exact; the outputs are rounded once (2^-11 or 2^-8) after weights
+    that are equal or vanish, and the lse carries a few roundings of its own size."""
+    rng = np.random.default_rng(octaves)
+    p, d, lengths = 16, 64, [1300, 70]
+    raw, sc, table, pages, scales, tab = _cache(rng, dev, lengths, 1, p, d)
+    ints = torch.from_numpy(rng.integers(-1, 2, raw[:, :, 0].shape).astype(np.float32)).to(F8)
+    raw[:, :, 0] = ints.view(torch.uint8).numpy()
+    sc[..., 0], sc[..., 1] = 2.0 ** octaves, 0.125
+    q = torch.from_numpy(rng.integers(-2, 3, (2 * new, hq, d)).astype(np.float32)).to(DT[dtype]).to(dev)
+    o, l, *_ = orc.attention(q.double().cpu().numpy(), orc.Layer(raw, sc), table, np.array(lengths), [0, new, 2 * new], sm_scale=0.25)
+    out, lse = bsa.kv_attention(q, torch.from_numpy(raw).to(dev).view(F8), torch.from_numpy(sc).to(dev), tab, _i32(lengths, dev),
+                                sm_scale=0.25)
+    u = 2.0 ** -10 if dtype == "fp16" else 2.0 ** -7
+    assert (np.abs(out.double().cpu().numpy() - o) <= u * np.abs(o) + 2.0 ** -10).all()
+    assert (np.abs(lse.double().cpu().numpy() - l) <= 2.0 ** -21 * np.abs(l)).all()
+
+
+def test_prompt_scores_of_minus_infinity_first(dev):
+    """A prompt whose first tokens' scores pass the end of 32 bits: the later ones are seen as if alone."""
+    rng = np.random.default_rng(17)
+    p, d, length, new = 16, 64, 300, 40
+    raw, sc, table, pages, scales, tab = _cache(rng, dev, [length], 1, p, d)
+    sc[:] = 1.0
+    minus = torch.tensor([-448.0, -8.0]).to(F8).view(torch.uint8).numpy()
+    for t in range(length):
+        tile = raw[table[0, t // p], 0, 0].reshape(-1)
+        for x in range(d):
+            tile[orc.key_offset(t % p, x, d)] = 0
+        tile[orc.key_offset(t % p, 0, d)] = minus[0] if t < 128 else 0
+        tile[orc.key_offset(t % p, 1, d)] = minus[1]
+    q = torch.zeros(new, 1, d)
+    q[..., 0], q[..., 1] = 1e38, 128
+    q = q.bfloat16().to(dev)
+    ref = orc.attention(q.double().cpu().numpy(), orc.Layer(raw, sc), table, np.array([length]), [0, new])
+    out, lse = bsa.kv_attention(q, torch.from_numpy(raw).to(dev).view(F8), torch.from_numpy(sc).to(dev), tab, _i32([length], dev))
+    assert np.allclose(ref[1][:, 0], np.log(length - 128 - new + 1 + np.arange(new)) - 128, atol=1e-9)
+    _check_attention(out, lse, (*ref[:3], np.full_like(ref[3], 128.0), *ref[4:]), torch.bfloat16, d)
+
+
 def test_attention_empty_rows(dev):
     """Sequences without tokens, new tokens that have no place, slots out of range: zeros and -inf."""
     rng = np.random.default_rng(2)

@@ -7,9 +7,11 @@
 // operand that O^T needs: nothing is shuffled between the two products.
 //
 // Scales and softmax in one exponent: with s2 = log2(e) sm_scale ks (q . k8) and lv = log2(vs), the weight of a
-// token is w = 2^(s2 + lv - M + 13) against a maximum M of s2 + lv that a later one may pass by an octave or
-// more, so that O = sum w v8 / sum w / vs whatever M is.  w stays within fp16, as which it goes to the matrix
+// token is w = 2^(s2 + lv - B), where B = M - 13 for a maximum M of s2 + lv that a later one may pass by an octave or
+// more, so that O = sum w v8 / sum w / vs whatever B is.  w stays within fp16, as which it goes to the matrix
 // unit: every weight down to 2^-27 of the largest keeps 11 bits.  Its sum is taken in fp32 before.
+// From 2^22 octaves on s2 + lv and M - 13 are rounded by octaves themselves, so there B = M, and the difference is
+// taken between rounded sums, which is exact near the maximum.
 
 #include <utility>
 
@@ -28,6 +30,7 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxSplits = 32;    // parts of one row
 constexpr float kShift = 13.f;  // weights go up to 2^(kShift + kSlack), within fp16
+constexpr float kFarScore = 0x1p22f;  // octaves from which on a score's last bit is half an octave or more
 constexpr float kSlack = 1.5f;  // octaves by which, in the first kernel, a score may exceed the running maximum before that moves
 constexpr float kMostWeight = 65504.f;  // of fp16; four weights at the maximum make half of it
 
@@ -85,6 +88,9 @@ __device__ __forceinline__ typename Elem<T>::x8 widen(uint32_t lo, uint32_t hi) 
   return __builtin_bit_cast(typename Elem<T>::x8, u32x4{Elem<T>::word(lo, false), Elem<T>::word(lo, true),
                                                         Elem<T>::word(hi, false), Elem<T>::word(hi, true)});
 }
+
+// The base B for a maximum, both in octaves.
+__device__ __forceinline__ float base_of(float m) { return __builtin_fabsf(m) < kFarScore ? m - kShift : m; }
 
 // Over the four lanes that hold one column: lanes l, l ^ 16, l ^ 32, l ^ 48.
 __device__ __forceinline__ float column_max(float v) {
@@ -248,10 +254,10 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_attention_kernel(AttnParams p) 
   }
 
   f32x4 acc[RT][DT];
-  float m[RT], l[RT];
+  float base[RT], l[RT];  // -inf: no token seen
 #pragma unroll
   for (int i = 0; i < RT; ++i) {
-    m[i] = -__builtin_inff(), l[i] = 0.f;
+    base[i] = -__builtin_inff(), l[i] = 0.f;
 #pragma unroll
     for (int d = 0; d < DT; ++d) acc[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -343,21 +349,22 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_attention_kernel(AttnParams p) 
       }
       float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                        fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-      mx = fmaxf(m[i], column_max(mx));
-      if (__any(mx > m[i] + kSlack)) {
-        const float alpha = mx == m[i] ? 1.f : __builtin_amdgcn_exp2f(m[i] - mx);
+      mx = column_max(mx);
+      if (__any(mx - base[i] > kShift + kSlack)) {
+        const float next = fmaxf(base[i], base_of(mx));
+        const float alpha = next == base[i] ? 1.f : __builtin_amdgcn_exp2f(base[i] - next);
         l[i] *= alpha;
 #pragma unroll
         for (int d = 0; d < DT; ++d) acc[i][d] *= alpha;
-        m[i] = mx;
+        base[i] = next;
       }
-      const float base = (m[i] == -__builtin_inff() ? 0.f : m[i]) - kShift;
+      const float from = base[i] == -__builtin_inff() ? 0.f : base[i];
       float w[2][4];
       uint32_t pw[4];
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[a][j] = __builtin_amdgcn_exp2f(s[a][j] - base);
+        for (int j = 0; j < 4; ++j) w[a][j] = __builtin_amdgcn_exp2f(s[a][j] - from);
         pw[2 * a] = Elem<_Float16>::pack(w[a][0], w[a][1]), pw[2 * a + 1] = Elem<_Float16>::pack(w[a][2], w[a][3]);
         l[i] = __builtin_fmaf((w[a][0] + w[a][1]) + (w[a][2] + w[a][3]), iv[a], l[i]);
       }
@@ -392,11 +399,11 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_attention_kernel(AttnParams p) 
     }
   }
 
-  // the waves' parts under a common maximum
+  // the waves' parts under a common base
 #pragma unroll
   for (int i = 0; i < RT; ++i) {
     l[i] = column_sum(l[i]);
-    if (g == 0) s_m[wave][16 * i + col] = m[i], s_l[wave][16 * i + col] = l[i];
+    if (g == 0) s_m[wave][16 * i + col] = base[i], s_l[wave][16 * i + col] = l[i];
   }
   __syncthreads();
   float f[RT];
@@ -404,7 +411,7 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_attention_kernel(AttnParams p) 
   for (int i = 0; i < RT; ++i) {
     const int r = 16 * i + col;
     const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
-    f[i] = m[i] == top ? 1.f : __builtin_amdgcn_exp2f(m[i] - top);
+    f[i] = base[i] == top ? 1.f : __builtin_amdgcn_exp2f(base[i] - top);
   }
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
@@ -492,7 +499,7 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_attention_kernel(AttnParams p) 
     *at = u32x2{Elem<T>::pack(o[0] * inv, o[1] * inv), Elem<T>::pack(o[2] * inv, o[3] * inv)};
     if (p.lse && d == 0)
       p.lse[(from + tok) * ((int64_t)p.kv_heads * p.group) + h] =
-          nothing ? -__builtin_inff() : (top - kShift + __builtin_amdgcn_logf(sum)) * (1.f / kLog2e);
+          nothing ? -__builtin_inff() : (top + __builtin_amdgcn_logf(sum)) * (1.f / kLog2e);
   }
 }
 
@@ -634,15 +641,15 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
   };
 
   f32x4 acc[RT][DT];
-  float m[RT], l[RT];
+  float base[RT], l[RT];  // -inf: no token seen
 #pragma unroll
   for (int i = 0; i < RT; ++i) {
-    m[i] = -__builtin_inff(), l[i] = 0.f;
+    base[i] = -__builtin_inff(), l[i] = 0.f;
 #pragma unroll
     for (int d = 0; d < DT; ++d) acc[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  bool started = false;  // every row has a maximum
+  bool started = false;  // every row has a base, and one that is not far
   const auto take = [&](auto stage, int t0) {
     const u32x4* const kv = prefill_stage<D, decltype(stage)::value>() + lane;
     const int first_tile = (t0 - t_begin) / 16 & 63;
@@ -681,26 +688,29 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
             if (t + j >= sees[i]) s[i][a][j] = -__builtin_inff();
       }
     }
-    // Weights against the maximum so far; only where four of them together outgrow fp16 (or a row has no
-    // maximum yet) is a new one looked for.  The sums are wanted anyway: asking each weight took 590 us
-    // instead of 566 for a prompt of 8192.
+    // Weights against the base so far; only where four of them together outgrow fp16 (or a row has no
+    // base yet, or a far one) is a new one looked for.  The sums are wanted anyway: asking each weight took 590 us
+    // instead of 566 for a prompt of 8192.  Against a new base the score is rounded first, so that the maximum's
+    // weight is 2^13 or 1 however far it is; otherwise both come in one step.
     f16x8 pf[RT][2];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
       float e[4][4], sum[4], top = 0.f;
-      const auto weigh = [&]() {
-        const float base = (m[i] == -__builtin_inff() ? 0.f : m[i]) - kShift;
+      const auto weigh = [&](auto exactly) {
+        const float from = base[i] == -__builtin_inff() ? 0.f : base[i];
         top = 0.f;
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
-          const float off = lv[a] - base;
+          const float off = lv[a] - from;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) e[a][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][a][j], ks[a], off));
+          for (int j = 0; j < 4; ++j)
+            e[a][j] = __builtin_amdgcn_exp2f(decltype(exactly)::value ? __builtin_fmaf(s[i][a][j], ks[a], lv[a]) - from
+                                                                      : __builtin_fmaf(s[i][a][j], ks[a], off));
           sum[a] = (e[a][0] + e[a][1]) + (e[a][2] + e[a][3]);
           top = fmaxf(top, sum[a]);
         }
       };
-      weigh();
+      weigh(std::false_type{});
       if (!started || __any(top > kMostWeight)) {
         float mx = -__builtin_inff();
 #pragma unroll
@@ -708,13 +718,15 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
           const float t = fmaxf(fmaxf(s[i][a][0], s[i][a][1]), fmaxf(s[i][a][2], s[i][a][3]));
           mx = fmaxf(mx, __builtin_fmaf(t, ks[a], lv[a]));
         }
-        mx = fmaxf(m[i], column_max(mx));
-        const float alpha = mx == m[i] ? 1.f : __builtin_amdgcn_exp2f(m[i] - mx);
+        mx = column_max(mx);
+        const float next = fmaxf(base[i], base_of(mx));
+        const float alpha = next == base[i] ? 1.f : __builtin_amdgcn_exp2f(base[i] - next);
         l[i] *= alpha;
 #pragma unroll
         for (int d = 0; d < DT; ++d) acc[i][d] *= alpha;
-        m[i] = mx;
-        weigh();
+        base[i] = next;
+        started = false;
+        weigh(std::true_type{});
       }
       uint32_t w[8];
 #pragma unroll
@@ -725,7 +737,8 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
       pf[i][0] = __builtin_bit_cast(f16x8, u32x4{w[0], w[1], w[2], w[3]});
       pf[i][1] = __builtin_bit_cast(f16x8, u32x4{w[4], w[5], w[6], w[7]});
     }
-    started = started || !partial;
+    if (!started)
+      started = !partial && !__any(!(__builtin_fabsf(base[0]) < kFarScore) || !(__builtin_fabsf(base[1]) < kFarScore));
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
 #pragma unroll
@@ -792,7 +805,7 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
     *at = u32x2{Elem<T>::pack(o[0] * inv, o[1] * inv), Elem<T>::pack(o[2] * inv, o[3] * inv)};
     if (p.lse && d == 0)
       p.lse[(from + tok) * heads + h] =
-          nothing ? -__builtin_inff() : (top - kShift + __builtin_amdgcn_logf(sum)) * (1.f / kLog2e);
+          nothing ? -__builtin_inff() : (top + __builtin_amdgcn_logf(sum)) * (1.f / kLog2e);
   };
   if (chunks == 1) {
 #pragma unroll
@@ -800,7 +813,7 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
       const int r = 32 * wave + 16 * i + col;
       if (r < used) {
 #pragma unroll
-        for (int d = 0; d < DT; ++d) finish(r, 16 * d + 4 * g, acc[i][d], m[i], l[i]);
+        for (int d = 0; d < DT; ++d) finish(r, 16 * d + 4 * g, acc[i][d], base[i], l[i]);
       }
     }
     return;
@@ -817,7 +830,7 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
     if (r < used) {
 #pragma unroll
       for (int d = 0; d < DT; ++d) hand_store16(mine_rsrc, (r * D + 16 * d + 4 * g) * 4, acc[i][d]);
-      if (g == 0) hand_store((uint64_t*)(part + ROWS * D) + r, __builtin_bit_cast(uint64_t, f32x2{m[i], l[i]}));
+      if (g == 0) hand_store((uint64_t*)(part + ROWS * D) + r, __builtin_bit_cast(uint64_t, f32x2{base[i], l[i]}));
     }
   }
   hand_publish();
@@ -826,7 +839,7 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
   __syncthreads();
   if (!s_last) return;
   if (threadIdx.x == 0) hand_reset(p.counters + tile);
-  // [row][part] factors and, in the row's first pair, the maximum and the sum
+  // [row][part] factors and, in the row's first pair, the base and the sum
   float* const s_f = (float*)prefill_stage<D, 0>();
   constexpr int FL = 2 * kMaxSplits;
   constexpr int BLOCK = 4 * TILE * 16 / (FL * 4);  // rows whose factors fit a stage at once
