@@ -66,6 +66,35 @@ def test_step_as_a_graph(dev):
         assert bool(served.all())
 
 
+@pytest.mark.parametrize("left", [0, 2, 5, 9])
+def test_a_beam_without_room_writes_nothing(dev, left):
+    """With `left` pages left, the beams that got none leave every page that they read as it was, and
+    others go on in their places."""
+    dec = BeamDecoder(device=dev, **SMALL)
+    prompts = torch.randint(0, 500, (3, 21), device=dev, dtype=torch.int32, generator=torch.Generator(device=dev).manual_seed(5))
+    dec.prefill(prompts)
+    cache = dec.cache
+    free = (cache.refcounts == 0).nonzero()[:, 0]
+    cache.refcounts[free[left:]] = 1  # taken by someone else
+    table, lengths = cache.page_table.clone(), cache.lengths.clone()
+    pages, scales = cache.pages.view(torch.uint8).clone(), cache.scales.clone()
+    tokens, parents, served = dec.step()
+    got = served.tolist()
+    # of four readers of a prompt's last page three need a copy, and the last one keeps it
+    assert sum(got) == (12 if left >= 9 else left // 3 * 4 + left % 3)
+    for beam, ok in enumerate(got):
+        if not ok:
+            ids = table[beam, : -(-int(lengths[beam]) // cache.page_size)].long()
+            assert torch.equal(cache.pages.view(torch.uint8)[:, ids], pages[:, ids]) and torch.equal(cache.scales[:, ids], scales[:, ids])
+    for prompt in range(3):
+        some = [b for b in range(4 * prompt, 4 * prompt + 4) if got[b]]
+        if some:
+            assert set(parents[4 * prompt:4 * prompt + 4].tolist()) <= set(some)
+            assert (cache.lengths[4 * prompt:4 * prompt + 4] == 22).all() and dec.scores[prompt].isfinite().all()
+        else:
+            assert (cache.lengths[4 * prompt:4 * prompt + 4] == 21).all() and dec.scores[prompt].isneginf().all()
+
+
 def test_refuses_what_it_has_no_room_for(dev):
     dec = BeamDecoder(device=dev, **dict(SMALL, max_len=32))
     with pytest.raises(ValueError):

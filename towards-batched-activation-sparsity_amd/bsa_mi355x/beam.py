@@ -119,12 +119,16 @@ class BeamDecoder:
         self.history = [(self.tokens.clone(), self.slots.clone())]
 
     def step(self) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-        """One token of every beam; returns (tokens, parents, served) of the beams that go on."""
+        """One token of every beam; returns (tokens, parents, served) of the beams that go on.  A beam
+        that found no room (served 0) has its token written nowhere and does not go on."""
         served = self.cache.extend(self.ones)
         pos = self.cache.lengths - 1
-        logits = self.forward(self.tokens, pos, True)
+        room = served > 0
+        # without room the newest place is an older token's, on a page that other beams may read
+        logits = self.forward(self.tokens, pos, True, slots=torch.where(room, self.slots, -1))
         got = token_logprobs(logits, self.tokens, k=self.width)
         total = self.scores[:, :, None] + got.top_logprobs.view(self.prompts, self.width, self.width)
+        total = torch.where(room.view(self.prompts, self.width, 1), total, -torch.inf)
         best, at = total.view(self.prompts, -1).topk(self.width, dim=1)
         parents = (self.base + at // self.width).reshape(-1)
         self.scores.copy_(best)
