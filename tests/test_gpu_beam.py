@@ -95,6 +95,52 @@ def test_a_beam_without_room_writes_nothing(dev, left):
             assert (cache.lengths[4 * prompt:4 * prompt + 4] == 21).all() and dec.scores[prompt].isneginf().all()
 
 
+def test_decoders_beside_each_other(dev):
+    """Two decoders of one shape on two streams, one as a replayed graph: each has workspaces of its own, gives
+    what it gives alone, and leaves nothing behind."""
+    from bsa_mi355x import runtime
+
+    small = dict(SMALL, density=0.5)
+    prompts = [torch.randint(0, 500, (3, 21), device=dev, dtype=torch.int32, generator=torch.Generator(device=dev).manual_seed(i))
+               for i in (6, 7)]
+    decs = [BeamDecoder(device=dev, **small) for _ in prompts]
+
+    def buffers(dec):
+        return {b.data_ptr() for k, b in runtime._WORKSPACE_CACHE["bufs"].items() if k[0] == dec._prefix}
+
+    want = []
+    for dec, p in zip(decs, prompts):
+        dec.prefill(p)
+        want.append([])
+        for _ in range(8):
+            dec.step()
+            want[-1].append((dec.tokens.clone(), dec.scores.clone()))
+        dec.prefill(p)
+    assert buffers(decs[0]) and buffers(decs[1]) and not buffers(decs[0]) & buffers(decs[1])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        decs[0].step()
+    decs[0].prefill(prompts[0])
+    streams = [torch.cuda.Stream() for _ in decs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(8):
+        for i, dec in enumerate(decs):
+            with torch.cuda.stream(streams[i]):
+                graph.replay() if i == 0 else dec.step()
+                got[i].append((dec.tokens.clone(), dec.scores.clone()))
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        for (t, s), (u, v) in zip(a, b):
+            assert torch.equal(t, u) and torch.equal(s, v)
+    names = [d._prefix for d in decs]
+    del dec, decs, graph
+    import gc
+    gc.collect()
+    assert not [k for k in runtime._WORKSPACE_CACHE["bufs"] if k[0] in names]
+
+
 def test_refuses_what_it_has_no_room_for(dev):
     dec = BeamDecoder(device=dev, **dict(SMALL, max_len=32))
     with pytest.raises(ValueError):

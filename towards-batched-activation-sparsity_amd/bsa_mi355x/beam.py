@@ -16,14 +16,19 @@ the choice among width^2 candidates are plain torch.
 from __future__ import annotations
 
 import argparse
+import itertools
 import time
+import weakref
 from typing import List, Optional, Tuple
 
 import torch
 
-from .runtime import gemm_packed, n_keep_for_density, nblk_of, pack_weight
+from .runtime import _release_workspaces, gemm_packed, n_keep_for_density, nblk_of, pack_weight
 from .select import select_gemm_packed
 from .serving import KVCache, token_logprobs
+
+
+_NUMBER = itertools.count()
 
 
 def _rms(x: torch.Tensor) -> torch.Tensor:
@@ -41,7 +46,10 @@ def _rotate(x: torch.Tensor, pos: torch.Tensor) -> torch.Tensor:
 
 
 class BeamDecoder:
-    """A decoder of `layers` layers for `prompts` x `width` beams of up to max_len tokens each."""
+    """A decoder of `layers` layers for `prompts` x `width` beams of up to max_len tokens each.
+
+    Its linears' workspaces are its own, so decoders may run beside each other on several streams; one
+    decoder's eager steps and replayed graphs come one after the other."""
 
     def __init__(self, hidden: int = 4096, intermediate: int = 11008, heads: int = 32, kv_heads: int = 32, layers: int = 8,
                  vocab: int = 32000, prompts: int = 8, width: int = 8, max_len: int = 1024, page_size: int = 16,
@@ -50,6 +58,8 @@ class BeamDecoder:
         self.hidden, self.heads, self.kv_heads, self.vocab = hidden, heads, kv_heads, vocab
         self.prompts, self.width, self.density = prompts, width, density
         self.head_dim = hidden // heads
+        self._prefix = f"beam {next(_NUMBER)}"
+        weakref.finalize(self, _release_workspaces, self._prefix)
         g = torch.Generator(device=self.device).manual_seed(seed)
 
         def weight(k: int, n: int, spread: float = 0.02) -> Tuple[torch.Tensor, int, int]:
@@ -77,9 +87,9 @@ class BeamDecoder:
         packed, k, n = w
         y = torch.empty(x.shape[0], n, dtype=x.dtype, device=x.device)
         if sparse:
-            select_gemm_packed(x, packed, n, n_keep_for_density(self.density, nblk_of(k)), y, workspace_prefix="beam")
+            select_gemm_packed(x, packed, n, n_keep_for_density(self.density, nblk_of(k)), y, workspace_prefix=self._prefix)
         else:
-            gemm_packed(x, packed, n, None, y, workspace_prefix="beam")
+            gemm_packed(x, packed, n, None, y, workspace_prefix=self._prefix)
         return y
 
     def forward(self, tokens: torch.Tensor, pos: torch.Tensor, sparse: bool, last: Optional[torch.Tensor] = None, **batch) -> torch.Tensor:

@@ -263,6 +263,13 @@ def _workspace(prefix: str, device: torch.device, nbytes: int, layout: tuple = (
     return buf
 
 
+def _release_workspaces(prefix: str) -> None:
+    """Drop a prefix's workspaces: its owner is gone, and so are the graphs that it may have captured."""
+    cache = _WORKSPACE_CACHE["bufs"]
+    for key in [k for k in list(cache) if k[0] == prefix]:
+        cache.pop(key, None)
+
+
 # ---------------------------------------------------------------------------------------
 # GEMM entry points
 
