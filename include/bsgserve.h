@@ -74,6 +74,7 @@ int bsg_kv_append(const void* k, int64_t k_stride_t, int64_t k_stride_h, const v
  *   q, out   : [tokens][q_heads][head_dim], q_heads a multiple of n_heads; query head h reads
  *              cached head h / (q_heads / n_heads); rows 16-byte (q) and 8-byte (out) aligned
  *   lse      : [tokens][q_heads], or NULL
+ *   sm_scale : finite, as log2(e) times it
  *   max_len  : at least the longest sequence, for the split over the long axis only (any length
  *              is computed rightly)
  * A token that sees nothing gives zeros and -inf, as do the tokens of a sequence whose slot is out of

@@ -133,6 +133,15 @@ def _pool(**kw):
     return ctypes.byref(_lib.PagePool(*a.values()))
 
 
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), float("-inf"), 3e38])
+@pytest.mark.parametrize("new", [1, 40])
+def test_attention_refuses_a_scale_that_is_no_number(scale, new):
+    """The prompt kernel would read NaN as 0."""
+    rc = bsa.load().bsg_kv_attention(FAKE, 512, 128, 4 * new, 4, ctypes.byref(_cache()), None, 4, None, new, 0, scale, FAKE, 512, 128,
+                                     None, 0, FAKE, 1 << 40, 256, None)
+    assert rc == _lib.BSG_ERR_ARG and "sm_scale" in _lib.last_error()
+
+
 def test_append_of_too_much_work_is_refused():
     """A bound on the new tokens near 2^31 is counted in 64 bits."""
     for most in (2 ** 31 - 1, 2 ** 31 - 14):

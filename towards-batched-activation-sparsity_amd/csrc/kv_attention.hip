@@ -938,6 +938,7 @@ extern "C" int bsg_kv_attention(const void* q, int64_t q_stride_t, int64_t q_str
   if (const int rc = check_heads(cache, q_heads)) return rc;
   if (const int rc = check_kv_batch(tokens, rows, slots, cu, max_new, cache, dtype)) return rc;
   if (cu_count < 1) return fail(BSG_ERR_ARG, "cu_count=%d", cu_count);
+  if (!(__builtin_fabsf(sm_scale * kLog2e) < __builtin_inff())) return fail(BSG_ERR_ARG, "sm_scale=%g", sm_scale);
   if (tokens == 0 || rows == 0 || max_new == 0) return BSG_OK;
   if (!q || !out) return fail(BSG_ERR_ARG, "null pointer (q=%p out=%p)", q, out);
   if (!is_aligned(q, 16) || ((q_stride_t | q_stride_h) & 7) != 0)
