@@ -560,6 +560,52 @@ def test_pages_random_steps(dev, slots, each, count, p):
         _same_pool(pool, tab, lengths, refs, pages, scales, was)
 
 
+def test_pages_of_a_large_pool(dev):
+    """70001 pages (the plans walk them 4096 at a time), 4.6 GB of data: the free ids in the middle, then last."""
+    slots, each, count, p = 300, 200, 70001, 32
+    pool = orc.Pool([[-1] * each] * slots, [0] * slots, [0] * count, p, range(count))
+    rng = np.random.default_rng(18)
+    pool.extend(rng.integers(150 * p, each * p, slots).tolist())
+    # the live pages lie in two blocks, the second one at the pool's end
+    for s in range(slots):
+        pool.table[s] = [x if x < 20000 or x < 0 else count - 1 - (x - 20000) for x in pool.table[s]]
+    refs = [0] * count
+    for row in pool.table:
+        for x in row:
+            if x >= 0:
+                refs[x] = 1
+    pool.refs = refs
+    g = torch.Generator(device=dev).manual_seed(1)
+    pages = torch.randint(0, 127, (2, count, 4, 2, p, 128), generator=g, device=dev, dtype=torch.uint8)
+    scales = torch.rand(2, count, 4, 2, generator=g, device=dev)
+    was = pages.clone(), scales.clone()
+    tab, lengths, refs = _i32(pool.table, dev), _i32(pool.lengths, dev), _i32(pool.refs, dev)
+    f8 = pages.view(F8)
+
+    def check():
+        assert torch.equal(tab, _i32(pool.table, dev)) and torch.equal(lengths, _i32(pool.lengths, dev))
+        assert torch.equal(refs, _i32(pool.refs, dev))
+        some = [i for i, r in enumerate(pool.refs) if r > 0]
+        some = some[:500] + some[len(some) // 2 - 500: len(some) // 2 + 500] + some[-500:]
+        src = [pool.data[i] for i in some]
+        assert torch.equal(pages[:, some], was[0][:, src]) and torch.equal(scales[:, some], was[1][:, src])
+
+    for step in range(3):
+        parents, children = rng.integers(0, slots, 40), rng.permutation(slots)[:40]
+        pool.fork(parents.tolist(), children.tolist())
+        bsa.pages_fork(tab, lengths, refs, _i32(parents, dev), _i32(children, dev))
+        new = rng.integers(0, 40, slots)
+        served = bsa.pages_extend(f8, scales, tab, lengths, refs, _i32(new, dev))
+        assert served.cpu().tolist() == pool.extend(new.tolist())
+        check()
+        counts = bsa.pages_compact(f8, scales, tab, refs)
+        assert counts.cpu().tolist() == pool.compact()
+        check()
+        gone = rng.integers(0, slots, 30)
+        pool.free(gone.tolist())
+        bsa.pages_free(tab, lengths, refs, _i32(gone, dev))
+
+
 def test_pages_extend_shared_tail_without_room(dev):
     """Readers of one partly filled page when the free pages do not reach: nobody writes to a page
     that another still reads."""
