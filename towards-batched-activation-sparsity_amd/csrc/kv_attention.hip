@@ -301,89 +301,89 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_attention_kernel(AttnParams p) 
     };
     float lane_ks = 0.f, lane_lv = 0.f, lane_iv = 0.f;
     const auto take = [&](int n, Step& s) {
-    const int t0 = b0 + 128 * n;
-    auto& kr = s.k;
-    auto& vr = s.v;
-    float ks[2], lv[2], iv[2];
-    bool there[2];
-#pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      there[a] = __builtin_amdgcn_readlane(lane_page, 2 * n + a) >= 0;
-      ks[a] = as_float(__builtin_amdgcn_readlane(__builtin_bit_cast(int, lane_ks), 2 * n + a));
-      lv[a] = as_float(__builtin_amdgcn_readlane(__builtin_bit_cast(int, lane_lv), 2 * n + a));
-      iv[a] = as_float(__builtin_amdgcn_readlane(__builtin_bit_cast(int, lane_iv), 2 * n + a));
-    }
-    const bool partial = t0 + 32 > all_see || !there[0] || !there[1];
-    uint32_t nan = 0;
-    if (partial) {
-      // tokens past the tile's end may be anything
+      const int t0 = b0 + 128 * n;
+      auto& kr = s.k;
+      auto& vr = s.v;
+      float ks[2], lv[2], iv[2];
+      bool there[2];
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
-        const uint32_t mask = there[a] ? byte_mask(t_end - (t0 + 16 * a + 4 * g)) : 0u;
+        there[a] = __builtin_amdgcn_readlane(lane_page, 2 * n + a) >= 0;
+        ks[a] = as_float(__builtin_amdgcn_readlane(__builtin_bit_cast(int, lane_ks), 2 * n + a));
+        lv[a] = as_float(__builtin_amdgcn_readlane(__builtin_bit_cast(int, lane_lv), 2 * n + a));
+        iv[a] = as_float(__builtin_amdgcn_readlane(__builtin_bit_cast(int, lane_iv), 2 * n + a));
+      }
+      const bool partial = t0 + 32 > all_see || !there[0] || !there[1];
+      uint32_t nan = 0;
+      if (partial) {
+        // tokens past the tile's end may be anything
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-          vr[a][c] &= mask;
-          nan |= nan_bytes(vr[a][c].x) | nan_bytes(vr[a][c].y) | nan_bytes(vr[a][c].z) | nan_bytes(vr[a][c].w);
+        for (int a = 0; a < 2; ++a) {
+          const uint32_t mask = there[a] ? byte_mask(t_end - (t0 + 16 * a + 4 * g)) : 0u;
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            vr[a][c] &= mask;
+            nan |= nan_bytes(vr[a][c].x) | nan_bytes(vr[a][c].y) | nan_bytes(vr[a][c].z) | nan_bytes(vr[a][c].w);
+          }
         }
       }
-    }
-    const bool some_nan = partial && __any(nan != 0);
+      const bool some_nan = partial && __any(nan != 0);
 
-    f16x8 pf[RT];
+      f16x8 pf[RT];
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      f32x4 s[2];
+      for (int i = 0; i < RT; ++i) {
+        f32x4 s[2];
 #pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        s[a] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int a = 0; a < 2; ++a) {
+          s[a] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            s[a] = Elem<T>::mfma(widen<T>(kr[a][c].x, kr[a][c].y), qf[i][2 * c], s[a]);
+            s[a] = Elem<T>::mfma(widen<T>(kr[a][c].z, kr[a][c].w), qf[i][2 * c + 1], s[a]);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            s[a][j] = s[a][j] * ks[a] + lv[a];
+            if (partial && (!there[a] || t0 + 16 * a + 4 * g + j >= sees[i])) s[a][j] = -__builtin_inff();
+          }
+        }
+        float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                         fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        mx = column_max(mx);
+        if (__any(mx - base[i] > kShift + kSlack)) {
+          const float next = fmaxf(base[i], base_of(mx));
+          const float alpha = next == base[i] ? 1.f : __builtin_amdgcn_exp2f(base[i] - next);
+          l[i] *= alpha;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) acc[i][d] *= alpha;
+          base[i] = next;
+        }
+        const float from = base[i] == -__builtin_inff() ? 0.f : base[i];
+        float w[2][4];
+        uint32_t pw[4];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[a][j] = __builtin_amdgcn_exp2f(s[a][j] - from);
+          pw[2 * a] = Elem<_Float16>::pack(w[a][0], w[a][1]), pw[2 * a + 1] = Elem<_Float16>::pack(w[a][2], w[a][3]);
+          l[i] = __builtin_fmaf((w[a][0] + w[a][1]) + (w[a][2] + w[a][3]), iv[a], l[i]);
+        }
+        pf[i] = __builtin_bit_cast(f16x8, u32x4{pw[0], pw[1], pw[2], pw[3]});
+      }
+      if (some_nan) {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-          s[a] = Elem<T>::mfma(widen<T>(kr[a][c].x, kr[a][c].y), qf[i][2 * c], s[a]);
-          s[a] = Elem<T>::mfma(widen<T>(kr[a][c].z, kr[a][c].w), qf[i][2 * c + 1], s[a]);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s[a][j] = s[a][j] * ks[a] + lv[a];
-          if (partial && (!there[a] || t0 + 16 * a + 4 * g + j >= sees[i])) s[a][j] = -__builtin_inff();
+          u32x4 v[2] = {vr[0][c], vr[1][c]};
+          nan_values<RT>(v, t0 + 4 * g, sees, &acc[0][4 * c], DT);
+          vr[0][c] = v[0], vr[1][c] = v[1];
         }
       }
-      float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                       fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-      mx = column_max(mx);
-      if (__any(mx - base[i] > kShift + kSlack)) {
-        const float next = fmaxf(base[i], base_of(mx));
-        const float alpha = next == base[i] ? 1.f : __builtin_amdgcn_exp2f(base[i] - next);
-        l[i] *= alpha;
 #pragma unroll
-        for (int d = 0; d < DT; ++d) acc[i][d] *= alpha;
-        base[i] = next;
+      for (int d = 0; d < DT; ++d) {
+        const f16x8 v = widen<_Float16>(vr[0][d >> 2][d & 3], vr[1][d >> 2][d & 3]);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) acc[i][d] = Elem<_Float16>::mfma(v, pf[i], acc[i][d]);
       }
-      const float from = base[i] == -__builtin_inff() ? 0.f : base[i];
-      float w[2][4];
-      uint32_t pw[4];
-#pragma unroll
-      for (int a = 0; a < 2; ++a) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[a][j] = __builtin_amdgcn_exp2f(s[a][j] - from);
-        pw[2 * a] = Elem<_Float16>::pack(w[a][0], w[a][1]), pw[2 * a + 1] = Elem<_Float16>::pack(w[a][2], w[a][3]);
-        l[i] = __builtin_fmaf((w[a][0] + w[a][1]) + (w[a][2] + w[a][3]), iv[a], l[i]);
-      }
-      pf[i] = __builtin_bit_cast(f16x8, u32x4{pw[0], pw[1], pw[2], pw[3]});
-    }
-    if (some_nan) {
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        u32x4 v[2] = {vr[0][c], vr[1][c]};
-        nan_values<RT>(v, t0 + 4 * g, sees, &acc[0][4 * c], DT);
-        vr[0][c] = v[0], vr[1][c] = v[1];
-      }
-    }
-#pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      const f16x8 v = widen<_Float16>(vr[0][d >> 2][d & 3], vr[1][d >> 2][d & 3]);
-#pragma unroll
-      for (int i = 0; i < RT; ++i) acc[i][d] = Elem<_Float16>::mfma(v, pf[i], acc[i][d]);
-    }
     };
     Step even, odd;
     fetch(0, even);
