@@ -23,8 +23,8 @@ int32 [pages] how many table entries name a page.
 """
 from __future__ import annotations
 
-import operator
 import threading
+from operator import index as _index
 from typing import Dict, NamedTuple, Optional, Tuple
 
 import torch
@@ -171,17 +171,10 @@ def _layer(pages: torch.Tensor, scales: torch.Tensor, page_table: torch.Tensor, 
     return dev, (n, h, p, d, slots, each, page_table.stride(0) if slots > 1 else each), steps
 
 
-def _kv_cache(pages: torch.Tensor, scales: torch.Tensor, layer: Optional[int], steps: tuple, sizes: tuple,
-              page_table: torch.Tensor, lengths: torch.Tensor) -> _lib.KvCache:
-    at, scales_at = pages.data_ptr(), scales.data_ptr()
-    if layer is not None:
-        layers, page_step, scale_step = steps
-        i = operator.index(layer)
-        if not -layers <= i < layers:
-            raise IndexError(f"layer {i} of {layers}")
-        i %= layers
-        at, scales_at = at + i * page_step, scales_at + i * scale_step
-    return _lib.KvCache(at, scales_at, *sizes, page_table.data_ptr(), lengths.data_ptr())
+def _from_end(i: int, layers: int) -> int:
+    if not -layers <= i < layers:
+        raise IndexError(f"layer {i} of {layers}")
+    return i % layers
 
 
 def _batch(x: torch.Tensor, what: str, heads: int, d: int, dev: torch.device, rows: int, cu, max_new) -> int:
@@ -235,9 +228,15 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, scales: tor
         _i32(cu_seqlens, dev, "cu_seqlens", rows + 1)
         _i32(slots, dev, "slots")
         call = _remember(key, (dev.index, load().bsg_kv_append, sizes, rows, most, _dtype_code(k), k.stride(0), k.stride(1),
-                               v.stride(0), v.stride(1), k.shape[0], steps))
-    index, fn, sizes, rows, most, code, kt, kh, vt, vh, tokens, steps = call
-    cache = _kv_cache(pages, scales, layer, steps, sizes, page_table, lengths)
+                               v.stride(0), v.stride(1), k.shape[0], *steps))
+    index, fn, sizes, rows, most, code, kt, kh, vt, vh, tokens, layers, page_step, scale_step = call
+    at, scales_at = pages.data_ptr(), scales.data_ptr()
+    if layer is not None:
+        i = _index(layer)
+        if not 0 <= i < layers:
+            i = _from_end(i, layers)
+        at, scales_at = at + i * page_step, scales_at + i * scale_step
+    cache = _lib.KvCache(at, scales_at, *sizes, page_table.data_ptr(), lengths.data_ptr())
     _launch(index, fn, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, tokens, cache, _ptr(slots), rows, _ptr(cu_seqlens), most, code)
 
 
@@ -264,12 +263,18 @@ def kv_attention(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, pag
     call = _CALLS.get(key)
     if call is None:
         call = _remember(key, _attention_call(q, pages, scales, page_table, lengths, cu_seqlens, max_new, slots, max_len, out, lse, layer))
-    index, fn, sizes, rows, most, code, qt, qh, tokens, heads, out_mold, lse_mold, longest, need, cus, scale, steps = call
+    index, fn, sizes, rows, most, code, qt, qh, tokens, heads, out_mold, lse_mold, longest, need, cus, scale, layers, page_step, scale_step = call
     if out is None:
         out = torch.empty_like(out_mold)
     if lse is None:
         lse = torch.empty_like(lse_mold)
-    cache = _kv_cache(pages, scales, layer, steps, sizes, page_table, lengths)
+    at, scales_at = pages.data_ptr(), scales.data_ptr()
+    if layer is not None:
+        i = _index(layer)
+        if not 0 <= i < layers:
+            i = _from_end(i, layers)
+        at, scales_at = at + i * page_step, scales_at + i * scale_step
+    cache = _lib.KvCache(at, scales_at, *sizes, page_table.data_ptr(), lengths.data_ptr())
     ws, room = 0, 0
     if need > 0:
         held = _workspace(index, need, workspace_prefix)
@@ -298,7 +303,7 @@ def _attention_call(q, pages, scales, page_table, lengths, cu_seqlens, max_new, 
     cache = _lib.KvCache(pages.data_ptr(), scales.data_ptr(), *sizes, page_table.data_ptr(), lengths.data_ptr())
     need = int(lib.bsg_kv_attention_workspace_bytes(cache, rows, heads, most, longest, cus))
     return (dev.index, lib.bsg_kv_attention, sizes, rows, most, code, q.stride(0), q.stride(1), tokens, heads,
-            _mold(q.shape, q.dtype, dev), _mold(q.shape[:2], torch.float32, dev), longest, need, cus, d ** -0.5, steps)
+            _mold(q.shape, q.dtype, dev), _mold(q.shape[:2], torch.float32, dev), longest, need, cus, d ** -0.5, *steps)
 
 
 # The int32 tensors of each page call beside the cache's own.
