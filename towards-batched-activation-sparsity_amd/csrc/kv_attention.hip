@@ -534,8 +534,8 @@ __device__ __forceinline__ void vmem_wait() {
 // follows the other (all of them side by side: 334 us against 267 for 8 prompts of 2048), its tiles with
 // most tokens first.
 //
-// 3 prompts of up to 2000 tokens over up to 2800, 32 heads on 8 of 128, fp16: 150 us, 767 TFLOP/s; a prompt of
-// 8192: 555 us, 990 TFLOP/s, 0.82 of a library product of 8192^3 (1210).  The conversions hide behind the
+// 3 prompts of up to 2000 tokens over up to 2800, 32 heads on 8 of 128, fp16: 152 us, 758 TFLOP/s; a prompt of
+// 8192: 556 us, 989 TFLOP/s, 0.82 of a library product of 8192^3 (1210).  The conversions hide behind the
 // MFMAs; the softmax between the two products, with two waves on a SIMD, and the step's barrier do not.
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
@@ -880,7 +880,7 @@ constexpr int kPrefillRows = 32;  // a cached head's rows past which the prefill
 // How a call is cut.  Few work-groups leave most compute units idle unless the long axis is split, to
 // two for each unit and at least 256 tokens a part.  A part of 128 rows writes and reads 66 KiB, so
 // there only where units would have none at all, and not over less than 1024 tokens (a prompt of 500
-// alone: 23 us, 26 in two parts; 2 x 40 tokens over 1500: 24 us in six, 34 in two).
+// alone: 21.0 us, 23.8 in two parts; 2 x 40 tokens over 1500: 22.4 us in six, 31.5 in two).
 Shape shape_of(int32_t rows, int32_t kv_heads, int32_t group, int32_t max_new, int64_t max_len, int32_t cus) {
   Shape s;
   const int64_t per_head = (int64_t)max_new * group;

@@ -16,9 +16,9 @@
 // largest of the lanes' own maxima is a bound that at least k logits reach.  Waves of a row meet in
 // LDS, two lists at a time; no barrier before that.
 //
-// 4000 x 32000 bf16 (256 MB): 52 us without alternatives (4.9 TB/s, the rate of a copy), 57 with one, 68 with 8,
-// 90 with 50 (fp16): what is left of the sorts, of which every wave runs two.  64 x 32000 fp16: 9.2 us without,
-// 14.1 with 8, bound by the chain of loads, sort, insertions and the three meetings of eight waves.
+// 4000 x 32000 bf16 (256 MB): 49 us without alternatives (5.3 TB/s, past the rate of a copy), 52 with one, 63 with
+// 8, 87 with 50 (fp16): what is left of the sorts, of which every wave runs two.  64 x 32000 fp16: 8.3 us without,
+// 13.0 with 8, bound by the chain of loads, sort, insertions and the three meetings of eight waves.
 
 #include "serve.hpp"
 
@@ -472,11 +472,11 @@ struct Shape {
 };
 
 // Waves of a row: enough rows fill the machine with one wave each (16 per compute unit); fewer take up
-// to the four of a work-group, with two vectors a lane at least (2000 rows of 1000, 5 alternatives: 8.0
-// us, 10.9 with one).  Long ones take several work-groups, which leave each wave kSplitTiles tiles (7 rows of
-// 100003 fp32, 20 alternatives: 16.9 us so, 17.7 in half as many of eight waves), and where that
-// makes no second work-group, one of eight waves (64 rows of 32000 fp16, 8 alternatives: 14.1 us so, 15.4 of
-// four, 14.6 of sixteen, 15.8 in two work-groups; 256 rows: 14.9 against 16.1; 64 rows of 512: 5.5 against 5.0).
+// to the four of a work-group, with two vectors a lane at least.  Long ones take several work-groups, which leave
+// each wave kSplitTiles tiles (7 rows of 100003 fp32, 20 alternatives: 15.9 us so, 16.6 in half as many of
+// eight waves), and where that makes no second work-group, one of eight waves (64 rows of 32000 fp16, 8
+// alternatives: 13.0 us so, 14.5 of four, 13.1 of sixteen, 14.9 in two work-groups, 28.7 with one wave; 256 rows: 13.3,
+// 14.9 of four, 30.3 with one).
 Shape shape_of(int64_t rows, int64_t vocab, int per_vector, int32_t cus) {
   const int64_t vectors = ceil_div(vocab, per_vector) + 1;  // a row may begin inside a vector
   Shape s;
