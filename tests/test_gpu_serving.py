@@ -170,6 +170,44 @@ def test_append_writes_max_new_tokens(dev, p, max_new):
     _same_pages(pages, scales, layer)
 
 
+def test_append_of_many_sequences_without_a_bound(dev):
+    """300 sequences of 1 to 2000 new tokens with no max_new: a grid past what one launch takes."""
+    rng = np.random.default_rng(19)
+    heads, p, d, n = 24, 16, 64, 300
+    new = rng.integers(1, 600, n)
+    new[::60] = 2000
+    lengths = new + rng.integers(0, 40, n)
+    per = -(-lengths // p)
+    table = np.full((n, per.max()), -1)
+    ids = rng.permutation(int(per.sum()))
+    for b, at in enumerate(np.cumsum(per) - per):
+        table[b, : per[b]] = ids[at: at + per[b]]
+    cu = np.concatenate([[0], np.cumsum(new)])
+    g = torch.Generator(device=dev).manual_seed(1)
+    k, v = (torch.randn(int(cu[-1]), heads, d, generator=g, device=dev, dtype=torch.float16) for _ in range(2))
+    got = []
+    for most in (2000, None):
+        pages = torch.zeros(len(ids), heads, 2, p, d, dtype=torch.uint8, device=dev).view(F8)
+        scales = torch.ones(len(ids), heads, 2, device=dev)
+        bsa.kv_append(k, v, pages, scales, _i32(table, dev), _i32(lengths, dev), cu_seqlens=_i32(cu, dev), max_new=most)
+        got.append((pages.view(torch.uint8), scales))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    some = [0, 1, 137, n - 1]  # the first call against the oracle
+    part = np.concatenate([table[b, : per[b]] for b in some])
+    raw = np.zeros((len(part), heads, 2, p, d), np.uint8)
+    layer = orc.Layer(raw, np.ones((len(part), heads, 2), np.float32))
+    own = np.full((len(some), per.max()), -1)
+    own_cu = np.concatenate([[0], np.cumsum(new[some])])
+    at = 0
+    for i, b in enumerate(some):
+        own[i, : per[b]] = np.arange(at, at + per[b])
+        at += per[b]
+    rows = np.concatenate([np.arange(cu[b], cu[b + 1]) for b in some])
+    orc.append(layer, k[rows].float().cpu().numpy(), v[rows].float().cpu().numpy(), own, lengths[some], list(own_cu))
+    index = torch.from_numpy(part).to(dev)
+    _same_pages(got[0][0][index].view(F8), got[0][1][index], layer)
+
+
 # ---------------------------------------------------------------------------------------- attention
 
 

@@ -29,7 +29,7 @@ struct AppendParams {
   const int32_t* slots;
   const int32_t* cu;
   int64_t table_stride, tokens;
-  int32_t num_pages, heads, num_slots, max_pages, max_new, pages_per_row, units, wide;
+  int32_t num_pages, heads, num_slots, max_pages, max_new, pages_per_row, first_unit, units, wide;
 };
 
 // Bytes b of the four dwords a quad's lanes hold, to lane b of the quad: the 4 x 4 byte transpose.
@@ -129,7 +129,7 @@ __global__ __launch_bounds__(P <= 64 ? 256 : 512) void bsg_kv_append_kernel(Appe
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int unit = wave / W, tile = wave % W;
   // units in the order head, K/V, page of the row, row: neighbours write neighbouring bytes
-  const uint32_t u = blockIdx.x * UNITS + unit, per_page = 2 * p.heads;
+  const uint32_t u = p.first_unit + blockIdx.x * UNITS + unit, per_page = 2 * p.heads;
   const uint32_t rp = u / per_page, hk = u - rp * per_page;
   const int head = hk >> 1, kv = hk & 1;
   const int row = rp / p.pages_per_row, nth = rp - row * p.pages_per_row;
@@ -258,14 +258,22 @@ __global__ __launch_bounds__(P <= 64 ? 256 : 512) void bsg_kv_append_kernel(Appe
   }
 }
 
+// One launch takes fewer than 2^32 threads; a batch without a bound on its sequences' new tokens has every sequence
+// take as many pages as all tokens fill.
+constexpr int64_t kLaunchUnits = 1 << 22;  // a multiple of a work-group's, of at most 512 threads each
+
 template <typename T, int D>
-void launch(const AppendParams& p, int page_size, int64_t units, hipStream_t st) {
-  const auto grid = [&](int per) { return dim3((unsigned)ceil_div(units, per)); };
-  switch (page_size) {
-    case 16: hipLaunchKernelGGL((bsg_kv_append_kernel<T, D, 16>), grid(4), dim3(256), 0, st, p); break;
-    case 32: hipLaunchKernelGGL((bsg_kv_append_kernel<T, D, 32>), grid(2), dim3(256), 0, st, p); break;
-    case 64: hipLaunchKernelGGL((bsg_kv_append_kernel<T, D, 64>), grid(1), dim3(256), 0, st, p); break;
-    default: hipLaunchKernelGGL((bsg_kv_append_kernel<T, D, 128>), grid(1), dim3(512), 0, st, p); break;
+void launch(AppendParams p, int page_size, hipStream_t st) {
+  for (int64_t first = 0; first < p.units; first += kLaunchUnits) {
+    const int64_t units = p.units - first < kLaunchUnits ? p.units - first : kLaunchUnits;
+    const auto grid = [&](int per) { return dim3((unsigned)ceil_div(units, per)); };
+    p.first_unit = (int32_t)first;
+    switch (page_size) {
+      case 16: hipLaunchKernelGGL((bsg_kv_append_kernel<T, D, 16>), grid(4), dim3(256), 0, st, p); break;
+      case 32: hipLaunchKernelGGL((bsg_kv_append_kernel<T, D, 32>), grid(2), dim3(256), 0, st, p); break;
+      case 64: hipLaunchKernelGGL((bsg_kv_append_kernel<T, D, 64>), grid(1), dim3(256), 0, st, p); break;
+      default: hipLaunchKernelGGL((bsg_kv_append_kernel<T, D, 128>), grid(1), dim3(512), 0, st, p); break;
+    }
   }
 }
 
@@ -343,8 +351,8 @@ extern "C" int bsg_kv_append(const void* k, int64_t k_stride_t, int64_t k_stride
            ((k_stride_t | k_stride_h | v_stride_t | v_stride_h) & 7) == 0;
   const hipStream_t st = (hipStream_t)stream;
   if (dtype == BSG_F16)
-    cache->head_dim == 64 ? launch<_Float16, 64>(p, P, units, st) : launch<_Float16, 128>(p, P, units, st);
+    cache->head_dim == 64 ? launch<_Float16, 64>(p, P, st) : launch<_Float16, 128>(p, P, st);
   else
-    cache->head_dim == 64 ? launch<__bf16, 64>(p, P, units, st) : launch<__bf16, 128>(p, P, units, st);
+    cache->head_dim == 64 ? launch<__bf16, 64>(p, P, st) : launch<__bf16, 128>(p, P, st);
   return launch_status("bsg_kv_append");
 }
