@@ -142,6 +142,14 @@ def test_attention_refuses_a_scale_that_is_no_number(scale, new):
     assert rc == _lib.BSG_ERR_ARG and "sm_scale" in _lib.last_error()
 
 
+def test_launches_of_too_many_threads_are_refused():
+    """The machine cuts a launch of 2^32 threads short without an error."""
+    wide = _cache(n_heads=4096)
+    assert _attend(wide, heads=4096, rows=1, tokens=1 << 19, max_new=1 << 19) == _lib.BSG_ERR_UNSUPPORTED
+    flat = _pool(page_size=1, max_pages=1 << 28, table_stride=1 << 28)
+    assert bsa.load().bsg_pages_fork(flat, FAKE, FAKE, 4, None) == _lib.BSG_ERR_UNSUPPORTED
+
+
 def test_append_of_too_much_work_is_refused():
     """A bound on the new tokens near 2^31 is counted in 64 bits."""
     for most in (2 ** 31 - 1, 2 ** 31 - 14):

@@ -258,9 +258,9 @@ __global__ __launch_bounds__(P <= 64 ? 256 : 512) void bsg_kv_append_kernel(Appe
   }
 }
 
-// One launch takes fewer than 2^32 threads; a batch without a bound on its sequences' new tokens has every sequence
-// take as many pages as all tokens fill.
-constexpr int64_t kLaunchUnits = 1 << 22;  // a multiple of a work-group's, of at most 512 threads each
+// Of one launch: a multiple of a work-group's units, and with up to 512 threads each within what a launch takes.  A
+// batch without a bound on its sequences' new tokens has every sequence take as many pages as all tokens fill.
+constexpr int64_t kLaunchUnits = 1 << 22;
 
 template <typename T, int D>
 void launch(AppendParams p, int page_size, hipStream_t st) {

@@ -957,7 +957,7 @@ extern "C" int bsg_kv_attention(const void* q, int64_t q_stride_t, int64_t q_str
     return fail(BSG_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)need);
   if (need > 0 && !is_aligned(ws, 16)) return fail(BSG_ERR_ALIGN, "workspace must be 16-byte aligned");
   const int64_t gx = (int64_t)cache->n_heads * s.row_tiles;
-  if (gx > 0x7fffffff || rows > 65535 || s.row_tiles > 65535)
+  if (gx > kLaunchGroups || rows > 65535 || s.row_tiles > 65535)
     return fail(BSG_ERR_UNSUPPORTED, "%d sequences of %d tokens", rows, max_new);
   AttnParams p;
   p.q = (const uint16_t*)q;

@@ -416,8 +416,9 @@ extern "C" int bsg_pages_fork(const bsg_page_pool* pool, const int32_t* parents,
   if (n == 0) return BSG_OK;
   if (!parents || !children)
     return fail(BSG_ERR_ARG, "null pointer (parents=%p children=%p)", (const void*)parents, (const void*)children);
-  const unsigned groups = (unsigned)ceil_div(pool->max_pages, kForkCols) + 1;
-  hipLaunchKernelGGL(bsg_pages_fork_kernel, dim3(groups), dim3(256), 0, (hipStream_t)stream, device_pool(pool), parents,
+  const int64_t groups = ceil_div(pool->max_pages, kForkCols) + 1;
+  if (groups > kLaunchGroups) return fail(BSG_ERR_UNSUPPORTED, "pool: max_pages=%d", pool->max_pages);
+  hipLaunchKernelGGL(bsg_pages_fork_kernel, dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, device_pool(pool), parents,
                      children, n);
   return launch_status("bsg_pages_fork");
 }

@@ -17,6 +17,9 @@ inline int launch_status(const char* what) {
   return e == hipSuccess ? BSG_OK : fail(BSG_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
 
+// One launch takes fewer than 2^32 threads in x; past that it is cut short without an error.
+constexpr int64_t kLaunchGroups = (1 << 24) - 1;  // of 256 threads
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline bool is_aligned(const void* p, unsigned n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
