@@ -1,0 +1,695 @@
+"""Parity of the operators of drafted tokens with oracle/drafts.py (64 bits, from the definitions) on the GPU: sizes,
+trees, masks and numbers at which they can go wrong, streams and graphs, and a step of all of them.
+
+Tolerances, from the arithmetic:
+- kv_append_rotated: a channel is two products and a sum, each off by half a step, 2^-24, of their magnitudes: 3 x 2^-24 of
+  |a cos| + |b sin|, and 4 is allowed.  A norm adds a sum of 128 squares (chains of at most 40 terms, halved by the root),
+  the root's own step, and two products: another 30 x 2^-24.  Then one rounding: half a step of the type, or of e4m3.
+- kv_tree_attention: as kv_attention in test_gpu_serving.py.
+- verify_drafts, pages_keep: none; both answers are exact.
+"""
+from __future__ import annotations
+
+import threading
+
+import numpy as np
+import pytest
+import torch
+
+import bsa_mi355x as bsa
+from oracle import drafts as dft
+from oracle import serving as orc
+from test_gpu_serving import DT, F8, _cache, _check_attention, _i32, _raw, _same_pages
+
+pytestmark = pytest.mark.gpu
+
+
+def _parents(rng, n, kind="any"):
+    """A tree of n nodes: chain, star, or any; the first node a root, now and then another one."""
+    if kind == "chain":
+        return [i - 1 for i in range(n)]
+    if kind == "star":
+        return ([-1] + [0] * n)[:n]
+    return [-1] + [int(rng.integers(-1, i)) if rng.random() < 0.1 else int(rng.integers(max(0, i - 6), i)) for i in range(1, n)]
+
+
+def _cu(new):
+    return [0, *np.cumsum(new).tolist()]
+
+
+def _angles(positions, dims):
+    a = np.arange(positions)[:, None] * 10000.0 ** (-np.arange(dims // 2) / (dims // 2))
+    return np.cos(a).astype(np.float32), np.sin(a).astype(np.float32)
+
+
+# ---------------------------------------------------------------------------------------- rotation into the cache
+
+
+def _step8(x):
+    """The step of e4m3 at x."""
+    return 2.0 ** np.maximum(np.floor(np.log2(np.maximum(np.abs(x), 2.0 ** -9))) - 3, -9)
+
+
+def _check_rotated(out, pages, scales, layer0, ref_q, mag_q, k, mag_k, v, table, lengths, cu, dtype, normed, slots=None, max_new=None):
+    """out and the cache against the turned q and k (64 bits) and their magnitudes."""
+    eps = (34 if normed else 4) * 2.0 ** -24
+    u = 2.0 ** -11 if dtype == torch.float16 else 2.0 ** -8
+    got = out.double().cpu().numpy()
+    mine = np.zeros(len(got), bool)  # tokens whose queries the call writes
+    for b in range(len(cu) - 1):
+        if 0 <= (b if slots is None else slots[b]) < len(lengths):
+            mine[cu[b]:min(cu[b + 1], cu[b] + (max_new or cu[b + 1]))] = True
+    bound = eps * mag_q + u * (np.abs(ref_q) + eps * mag_q) + 2.0 ** -25
+    np.testing.assert_array_equal(np.isnan(got[mine]), np.isnan(ref_q[mine]))
+    fine = mine[:, None, None] & np.isfinite(ref_q)
+    assert (np.abs(got - ref_q)[fine] <= bound[fine]).all(), np.max((np.abs(got - ref_q) / bound)[fine])
+    want = layer0
+    orc.append(want, k, v, table, np.asarray(lengths), cu, slots, max_new)
+    np.testing.assert_array_equal(scales.cpu().numpy().astype(np.float64), want.scales)
+    # the keys' bound, placed as the keys are
+    err = orc.Layer(np.zeros_like(_raw(pages)), np.ones(scales.shape, np.float32))
+    err.values[:] = 0.0
+    for b in range(len(cu) - 1):
+        slot, n = b if slots is None else slots[b], cu[b + 1] - cu[b]
+        if not 0 <= slot < len(lengths):
+            continue
+        for i in range(n):
+            pos = int(lengths[slot]) - n + i
+            page = table[slot][pos // err.p] if 0 <= pos < len(table[slot]) * err.p else -1
+            if 0 <= page < err.values.shape[0]:
+                err.values[page, :, 0, pos % err.p] = np.nan_to_num(eps * mag_k[cu[b] + i])
+    err.values /= want.scales[..., None, None]
+    values = orc.E4M3[_raw(pages)]
+    tiled = want.tiled()
+    np.testing.assert_array_equal(np.isnan(values), np.isnan(tiled))
+    off = np.abs(np.nan_to_num(values) - np.nan_to_num(tiled))
+    # a number that its error carries over a border between two values is off by one step more than not at all
+    slack = np.where(err.tiled() > 0, _step8(np.maximum(np.abs(np.nan_to_num(tiled)), np.abs(np.nan_to_num(values)))), 0.0)
+    assert (off <= slack).all()
+    # and few are: a border within the error is 2 err / step likely; ten times that, and ten
+    assert np.count_nonzero(off) <= 10 + 10 * (2 * err.tiled() / _step8(np.nan_to_num(tiled))).sum()
+    return mine
+
+
+def _rotated(dev, rng, lengths, new, hq, heads, p, d, dims, dtype, interleaved=False, norm=False, mode="place", slots=None, **kw):
+    raw, sc, table, pages, scales, tab = _cache(rng, dev, lengths, heads, p, d)
+    cu = _cu(new)
+    q, k, v = (torch.from_numpy((rng.standard_normal((cu[-1], h, d)) * np.exp(rng.standard_normal((cu[-1], h, 1)))).astype(np.float32)).to(dtype).to(dev)
+               for h in (hq, heads, heads))
+    cos, sin = _angles(max(lengths) + 3, dims)
+    wq, wk = ((torch.from_numpy((1 + 0.3 * rng.standard_normal(d)).astype(np.float32)).to(dtype).to(dev) for _ in range(2)) if norm
+              else (None, None))
+    given, places = {}, {}
+    if mode == "positions":
+        places["positions"] = rng.integers(0, max(lengths) + 3, cu[-1])
+    if mode == "tree":
+        places["parents"] = [x for n in new for x in _parents(rng, n)]
+    given = {name: _i32(x, dev) for name, x in places.items()}
+    if slots is not None:
+        given["slots"] = _i32(slots, dev)
+    out = bsa.kv_append_rotated(q, k, v, torch.from_numpy(cos).to(dev), torch.from_numpy(sin).to(dev), pages, scales, tab, _i32(lengths, dev),
+                                cu_seqlens=_i32(cu, dev), max_new=max(new), q_norm=wq, k_norm=wk, eps=1e-5, interleaved=interleaved,
+                                **given, **kw)
+    host = [None if x is None else x.double().cpu().numpy() for x in (q, wq, k, wk)]
+    rq, mq = dft.turned(host[0], host[1], 1e-5, cos, sin, interleaved, lengths, cu, slots, **places)
+    rk, mk = dft.turned(host[2], host[3], 1e-5, cos, sin, interleaved, lengths, cu, slots, **places)
+    _check_rotated(out, pages, scales, orc.Layer(raw, sc), rq, mq, rk, mk, v.double().cpu().numpy(), table, lengths, cu, dtype, norm, slots)
+    return out
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("p,d,dims", [(16, 64, 64), (16, 128, 128), (32, 128, 64), (64, 64, 32), (64, 128, 32), (128, 128, 16), (16, 64, 16)])
+@pytest.mark.parametrize("interleaved,norm,mode", [(False, False, "place"), (True, True, "tree"), (False, True, "positions"), (True, False, "place")])
+def test_rotated(dev, dtype, p, d, dims, interleaved, norm, mode):
+    rng = np.random.default_rng([p, d, dims, interleaved, norm])
+    _rotated(dev, rng, [1, 21, 38, 300], [1, 5, 33, 64], 6, 3, p, d, dims, DT[dtype], interleaved, norm, mode)
+
+
+@pytest.mark.parametrize("hq,heads", [(1, 1), (7, 1), (32, 4), (40, 8)])
+@pytest.mark.parametrize("new", [[1, 1, 1], [3, 0, 1], [40, 129, 17]])
+def test_rotated_batches(dev, hq, heads, new):
+    rng = np.random.default_rng([hq, *new])
+    lengths = [n + o for n, o in zip(new, [5, 16, 131])]
+    _rotated(dev, rng, lengths, new, hq, heads, 32, 128, 128, torch.bfloat16, norm=True)
+    _rotated(dev, rng, lengths, new, hq, heads, 16, 64, 64, torch.float16)
+
+
+def test_rotated_by_nothing_is_append(dev):
+    """Angles of 0: the bytes that kv_append writes, and q as it is."""
+    rng = np.random.default_rng(3)
+    lengths, new = [40, 17, 200], [7, 17, 64]
+    _, _, _, pages, scales, tab = _cache(rng, dev, lengths, 2, 16, 128)
+    cu = _i32(_cu(new), dev)
+    q, k, v = (torch.randn(88, h, 128, device=dev).half() for h in (4, 2, 2))
+    k[3, 1, 5], k[9], v[20, 0, 7], v[21, 1] = float("inf"), 0.0, float("nan"), 60000.0
+    pages2, scales2 = pages.view(torch.uint8).clone().view(F8), scales.clone()
+    one, zero = torch.ones(210, 64, device=dev), torch.zeros(210, 64, device=dev)
+    # an infinity times 0 is NaN, so the infinite pair does not turn but in the keys that have none
+    k[3, 1, 5] = 3.0
+    out = bsa.kv_append_rotated(q, k, v, one, zero, pages, scales, tab, _i32(lengths, dev), cu_seqlens=cu, max_new=64)
+    bsa.kv_append(k, v, pages2, scales2, tab, _i32(lengths, dev), cu_seqlens=cu, max_new=64)
+    assert torch.equal(pages.view(torch.uint8), pages2.view(torch.uint8)) and torch.equal(scales, scales2) and torch.equal(out, q)
+
+
+@pytest.mark.parametrize("case", ["fused", "odd_stride", "in_place", "slots", "bad_pages", "short", "nan_inf", "rows_behind", "max_new",
+                                  "layer", "position_out"])
+def test_rotated_edges(dev, case):
+    rng = np.random.default_rng(len(case))
+    lengths, new, hq, heads, p, d = [37, 20, 16], [5, 20, 1], 4, 2, 16, 64
+    raw, sc, table, pages, scales, tab = _cache(rng, dev, lengths, heads, p, d)
+    cu, slots, max_new, dtype = _cu(new), None, 20, torch.float16
+    total = cu[-1] + (4 if case == "rows_behind" else 0)
+    qkv = torch.randn(total, hq + 2 * heads, d, device=dev).to(dtype)
+    q, k, v = (x.contiguous() for x in qkv.split([hq, heads, heads], 1))
+    cos, sin = _angles(40, d)
+    kw, positions = {}, None
+    if case == "fused":
+        q, k, v = qkv.split([hq, heads, heads], 1)
+    elif case == "odd_stride":
+        k, v = (torch.randn(total, heads, d + 1, device=dev).to(dtype)[..., :d] for _ in range(2))
+    elif case == "slots":
+        slots = [2, 9, 0]
+        lengths = [37, 20, 16]
+        new = [5, 3, 1]
+        cu, total = _cu(new), 9
+        q, k, v = q[:9].contiguous(), k[:9].contiguous(), v[:9].contiguous()
+    elif case == "bad_pages":
+        table[1, 0], table[0, 2] = 10 ** 7, -1
+        tab = _i32(table, dev)
+    elif case == "short":
+        lengths = [3, 20, 16]  # fewer tokens than the new ones: the first have no place
+    elif case == "nan_inf":
+        k[0, 0, 3], k[8, 1, 7], q[1, 2, 5], v[3, 0, 2], v[4, 1, 1] = float("nan"), float("inf"), float("inf"), float("inf"), float("nan")
+    elif case == "max_new":
+        max_new = 6
+    elif case == "position_out":
+        positions = np.arange(26) + 30
+        positions[5] = -2
+    if positions is not None:
+        kw["positions"] = _i32(positions, dev)
+    if slots is not None:
+        kw["slots"] = _i32(slots, dev)
+    host = [x.double().cpu().numpy() for x in (q, k, v)]
+    out = torch.full(q.shape, 7.0, dtype=dtype, device=dev)
+    if case == "in_place":
+        out = q
+    args = [pages, scales]
+    if case == "layer":
+        both = torch.stack([pages.view(torch.uint8)] * 3).view(F8), torch.stack([scales] * 3)
+        args, kw["layer"] = list(both), -2
+    got = bsa.kv_append_rotated(q, k, v, torch.from_numpy(cos).to(dev), torch.from_numpy(sin).to(dev), *args, tab, _i32(lengths, dev),
+                                cu_seqlens=_i32(cu, dev), max_new=max_new, out=out, **kw)
+    assert got is out
+    if case == "layer":
+        for i in (0, 2):
+            assert torch.equal(both[0][i].view(torch.uint8), pages.view(torch.uint8)) and torch.equal(both[1][i], scales)
+        pages, scales = both[0][1], both[1][1]
+    with np.errstate(invalid="ignore"):
+        (rq, mq), (rk, mk) = (dft.turned(x, None, 1e-6, cos, sin, False, lengths, cu, slots, positions) for x in host[:2])
+        mine = _check_rotated(out, pages, scales, orc.Layer(raw, sc), rq, mq, rk, np.nan_to_num(mk, posinf=0.0), host[2], table, lengths, cu,
+                              dtype, False, slots, max_new if case == "max_new" else None)
+    assert mine.sum() == {"slots": 6, "max_new": 12}.get(case, 26)
+    if case != "in_place":
+        assert (out.cpu()[torch.from_numpy(~mine)] == 7.0).all()  # nobody's rows
+
+
+def test_rotated_graph_and_streams(dev):
+    """Captured and replayed with new inputs in the same tensors, and on another stream: the eager numbers."""
+    rng = np.random.default_rng(5)
+    lengths, new = [40, 9], [6, 3]
+    _, _, _, pages, scales, tab = _cache(rng, dev, lengths, 2, 16, 128)
+    n, cu, par = _i32(lengths, dev), _i32(_cu(new), dev), _i32([-1, 0, 0, 1, 2, 2, -1, 0, 0], dev)
+    cos, sin = (torch.from_numpy(x).to(dev) for x in _angles(64, 128))
+    q, k, v = (torch.randn(9, h, 128, device=dev).half() for h in (4, 2, 2))
+    was, was_s = pages.view(torch.uint8).clone(), scales.clone()
+
+    def reset():
+        pages.view(torch.uint8).copy_(was)
+        scales.copy_(was_s)
+
+    def call():
+        return bsa.kv_append_rotated(q, k, v, cos, sin, pages, scales, tab, n, cu_seqlens=cu, max_new=6, parents=par)
+
+    call()
+    reset()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for i in range(3):
+        for x in (q, k, v):
+            x.copy_(torch.randn_like(x))
+        reset()
+        want = call()
+        bytes_want, scales_want = pages.view(torch.uint8).clone(), scales.clone()
+        reset()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(pages.view(torch.uint8), bytes_want) and torch.equal(scales, scales_want)
+        reset()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = call()
+        side.synchronize()
+        assert torch.equal(got, want) and torch.equal(pages.view(torch.uint8), bytes_want)
+
+
+# ---------------------------------------------------------------------------------------- attention of a tree
+
+
+def _attend(dev, rng, lengths, new, hq, heads, p, d, dtype, kind="any", **kw):
+    raw, sc, table, pages, scales, tab = _cache(rng, dev, lengths, heads, p, d, poison=True)
+    cu = _cu(new)
+    parents = [x for n in new for x in _parents(rng, n, kind)]
+    q = torch.from_numpy(rng.standard_normal((cu[-1], hq, d)).astype(np.float32)).to(dtype).to(dev)
+    ref = dft.tree_attention(q.double().cpu().numpy(), parents, orc.Layer(raw, sc), table, np.array(lengths), cu)
+    out, lse = bsa.kv_tree_attention(q, _i32(parents, dev), pages, scales, tab, _i32(lengths, dev), cu_seqlens=_i32(cu, dev),
+                                     max_new=max(new), **kw)
+    _check_attention(out, lse, ref, dtype, d)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("kind", ["any", "star", "chain"])
+@pytest.mark.parametrize("new", [1, 2, 7, 16, 17, 33, 64])
+@pytest.mark.parametrize("hq,heads,p,d", [(2, 2, 16, 128), (6, 2, 32, 64), (8, 1, 64, 128)])
+def test_tree(dev, dtype, kind, new, hq, heads, p, d):
+    rng = np.random.default_rng([new, hq, len(kind)])
+    _attend(dev, rng, [new, new + 1, 64 + new, 200], [new] * 4, hq, heads, p, d, DT[dtype], kind)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("hq,heads,p,d", [(3, 3, 16, 64), (4, 1, 128, 128), (12, 2, 64, 128), (20, 1, 16, 128)])
+@pytest.mark.parametrize("lengths,new", [([150, 257, 64, 31], [64, 13, 1, 30]), ([1100, 2049], [40, 64]), ([33, 47, 48, 49, 63, 64, 65], [32, 32, 17, 18, 31, 64, 33])])
+def test_tree_of_several_sizes(dev, dtype, hq, heads, p, d, lengths, new):
+    rng = np.random.default_rng([hq, p, len(new)])
+    _attend(dev, rng, lengths, new, hq, heads, p, d, DT[dtype])
+
+
+@pytest.mark.parametrize("hq,heads,nodes", [(2, 2, 5), (4, 2, 16), (2, 1, 30), (4, 1, 64)])
+@pytest.mark.parametrize("lengths,max_len", [([5000], None), ([5000, 90, 2049], 5000), ([5000, 1200], 700), ([4099], 1)])
+def test_tree_split(dev, hq, heads, nodes, lengths, max_len):
+    rng = np.random.default_rng(nodes)
+    _attend(dev, rng, lengths, [nodes] * len(lengths), hq, heads, 16, 128, torch.float16, max_len=max_len)
+    _attend(dev, rng, lengths, [nodes] * len(lengths), hq, heads, 64, 64, torch.bfloat16, max_len=max_len)
+
+
+@pytest.mark.parametrize("nodes,hq", [(9, 2), (30, 2), (40, 4)])
+def test_tree_odd_parents_and_slots(dev, nodes, hq):
+    """Parents that are no earlier node make roots; slots out of range and trees of more nodes than the sequence has
+    tokens; sequences without tokens."""
+    rng = np.random.default_rng(nodes)
+    lengths, slots = [60, 0, nodes - 2, 200], [3, 17, 2, -1, 0, 1]
+    raw, sc, table, pages, scales, tab = _cache(rng, dev, lengths, 2, 16, 64, poison=True)
+    new = [nodes, 3, nodes, 2, 0, 4]
+    cu = _cu(new)
+    parents = rng.integers(-3, nodes + 3, cu[-1]).tolist()
+    parents[1], parents[2] = 1, 2 ** 31 - 1
+    q = torch.randn(cu[-1] + 2, 2 * hq, 64, device=dev).bfloat16()
+    out = torch.full_like(q, 5.0)
+    with np.errstate(invalid="ignore"):
+        ref = dft.tree_attention(q[:cu[-1]].double().cpu().numpy(), parents, orc.Layer(raw, sc), table, np.array(lengths), cu, slots)
+    got, lse = bsa.kv_tree_attention(q, _i32(parents + [0, 0], dev), pages, scales, tab, _i32(lengths, dev), cu_seqlens=_i32(cu, dev),
+                                     max_new=nodes, slots=_i32(slots, dev), out=out)
+    assert (got[cu[-1]:] == 5.0).all()
+    _check_attention(got[:cu[-1]], lse[:cu[-1]], ref, torch.bfloat16, 64)
+
+
+@pytest.mark.parametrize("nodes,hq", [(5, 2), (20, 4), (64, 2)])
+def test_tree_nan_in_unseen_nodes(dev, nodes, hq):
+    """A NaN of a node reaches its descendants and nobody else; pages out of range are not seen."""
+    rng = np.random.default_rng(nodes)
+    p, d, length = 16, 64, 150
+    raw, sc, table, pages, scales, tab = _cache(rng, dev, [length], 1, p, d)
+    parents = _parents(rng, nodes)
+    at_v, at_k = length - nodes + nodes // 2, length - 1
+    raw[table[0, at_v // p], 0, 1].reshape(-1)[orc.value_offset(at_v % p, 7, d)] = 0xFF
+    raw[table[0, at_k // p], 0, 0].reshape(-1)[orc.key_offset(at_k % p, 3, d)] = 0x7F
+    table[0, 1], table[0, 3] = -1, 10 ** 8
+    q = torch.randn(nodes, hq, d, device=dev).half()
+    with np.errstate(invalid="ignore"):
+        ref = dft.tree_attention(q.double().cpu().numpy(), parents, orc.Layer(raw, sc), table, np.array([length]), [0, nodes])
+    out, lse = bsa.kv_tree_attention(q, _i32(parents, dev), torch.from_numpy(raw).to(dev).view(F8), scales, _i32(table, dev), _i32([length], dev))
+    bad = np.isnan(ref[1])
+    assert bad[-1].all() and not bad.all() and np.isnan(ref[0][nodes // 2, :, 7]).all()
+    assert np.isnan(lse.cpu().numpy()[bad]).all()
+    _check_attention(out, torch.where(torch.from_numpy(bad).to(dev), 0.0, lse), (ref[0], np.where(bad, 0.0, ref[1]), *[np.nan_to_num(x) for x in ref[2:]]),
+                     torch.float16, d)
+
+
+def test_tree_graph_streams_and_threads(dev):
+    """Split trees: the same numbers eager, replayed, on streams and from threads side by side."""
+    rng = np.random.default_rng(2)
+    raw, sc, table, pages, scales, tab = _cache(rng, dev, [3000, 1900], 2, 16, 128)
+    n = _i32([3000, 1900], dev)
+    for nodes in (8, 24, 60):
+        q = torch.randn(2 * nodes, 4, 128, device=dev).bfloat16()
+        parents = _i32(_parents(rng, nodes) + _parents(rng, nodes), dev)
+        want, want_l = (x.clone() for x in bsa.kv_tree_attention(q, parents, pages, scales, tab, n))
+        torch.cuda.synchronize()
+        graphs = []
+        for _ in range(2):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                graphs.append((graph, *bsa.kv_tree_attention(q, parents, pages, scales, tab, n)))
+        for _ in range(3):
+            for g, out, lse in graphs:
+                out.fill_(float("nan"))
+                g.replay()
+            eager = bsa.kv_tree_attention(q, parents, pages, scales, tab, n)
+            torch.cuda.synchronize()
+            for _, out, lse in [*graphs, (None, *eager)]:
+                assert torch.equal(out, want) and torch.equal(lse, want_l)
+        got = []
+
+        def run():
+            with torch.cuda.stream(torch.cuda.Stream()):
+                got.append(bsa.kv_tree_attention(q, parents, pages, scales, tab, n))
+                torch.cuda.current_stream().synchronize()
+
+        threads = [threading.Thread(target=run) for _ in range(3)]
+        [t.start() for t in threads]
+        [t.join() for t in threads]
+        assert len(got) == 3 and all(torch.equal(o, want) and torch.equal(l, want_l) for o, l in got)
+
+
+# ---------------------------------------------------------------------------------------- verification
+
+
+def _same_verdict(got, want, most):
+    accepted, path, tokens = (x.cpu().tolist() for x in got)
+    for b, (count, nodes, said) in enumerate(want):
+        assert accepted[b] == count, (b, accepted[b], count)
+        assert path[b] == nodes + [-1] * (most - len(nodes)), b
+        assert tokens[b] == said + [-1] * (most - len(said)), (b, tokens[b], said)
+
+
+def _drafts(rng, new, vocab, tree, spread=2.0):
+    """Logits with a few likely tokens, trees of them, numbers."""
+    total = sum(new)
+    x = rng.standard_normal((total, vocab)) * spread
+    for _ in range(2):
+        x[np.arange(total), rng.integers(0, vocab, total)] += 8.0
+    parents = [p for n in new for p in (_parents(rng, n) if tree else _parents(rng, n, "chain"))]
+    tokens = rng.integers(0, vocab, total)
+    at = 0
+    for n in new:
+        for i in range(1, n):
+            p = dft.tree_parent(parents[at:at + n], i)
+            if p >= 0 and rng.random() < 0.8:
+                tokens[at + i] = np.argsort(-x[at + p])[min(rng.integers(0, 3), vocab - 1)]
+        at += n
+    return x, parents, tokens, rng.random(total).astype(np.float32)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("vocab", [1, 2, 33, 500, 2048, 2049, 5003, 32000])
+@pytest.mark.parametrize("temperature", [0.0, 0.3, 1.0])
+def test_verify_trees(dev, dtype, vocab, temperature):
+    rng = np.random.default_rng([vocab, int(10 * temperature)])
+    new = [1, 2, 5, 16, 3, 9] + ([64] if vocab < 6000 else [])
+    x, parents, tokens, u = _drafts(rng, new, vocab, True)
+    logits = torch.from_numpy(x.astype(np.float32)).to(DT[dtype]).to(dev)
+    want = dft.verify(logits.double().cpu().numpy(), tokens, u, parents, None, temperature, _cu(new))
+    got = bsa.verify_drafts(logits, _i32(tokens, dev), torch.from_numpy(u).to(dev), parents=_i32(parents, dev), temperature=temperature,
+                            cu_seqlens=_i32(_cu(new), dev), max_new=max(new))
+    _same_verdict(got, want, max(new))
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("vocab", [2, 33, 2048, 5003, 32000])
+@pytest.mark.parametrize("temperature", [0.0, 0.6, 1.0])
+@pytest.mark.parametrize("noise", [0.0, 0.5, 3.0])
+def test_verify_chains_of_drawn_drafts(dev, dtype, vocab, temperature, noise):
+    rng = np.random.default_rng([vocab, int(10 * temperature), int(10 * noise)])
+    new = [1, 2, 5, 8, 3, 12]
+    x, _, tokens, u = _drafts(rng, new, vocab, False)
+    logits = torch.from_numpy(x.astype(np.float32)).to(DT[dtype]).to(dev)
+    draft = (logits.float() + noise * torch.from_numpy(rng.standard_normal(x.shape).astype(np.float32)).to(dev)).to(DT[dtype])
+    want = dft.verify(logits.double().cpu().numpy(), tokens, u, None, draft.double().cpu().numpy(), temperature, _cu(new))
+    got = bsa.verify_drafts(logits, _i32(tokens, dev), torch.from_numpy(u).to(dev), draft_logits=draft, temperature=temperature,
+                            cu_seqlens=_i32(_cu(new), dev), max_new=12)
+    _same_verdict(got, want, 12)
+    if noise == 0 and temperature > 0:  # what the target would have drawn is accepted whatever the number
+        assert [w[0] for w in want] == new
+
+
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("vocab", [40, 5000])
+def test_verify_hard_rows(dev, vocab, draft):
+    """Masks, infinities and NaN in rows; tokens that do not exist, twice the same token among siblings, numbers at the
+    ends of their range; a temperature for each sequence; sequences without nodes."""
+    rng = np.random.default_rng([vocab, draft])
+    new = [4, 4, 4, 4, 4, 4, 0, 4, 5, 5, 3]
+    cu = _cu(new)
+    x, _, tokens, u = _drafts(rng, new, vocab, False)
+    parents = [p for n in new for p in ([i - 1 for i in range(n)] if draft else ([-1] + [0] * n)[:n])]
+    x[cu[0]] = -np.inf                             # nothing
+    x[cu[1], 3] = np.nan
+    x[cu[2], 5] = np.inf
+    x[cu[3]] = -np.inf
+    x[cu[3], 7] = 2.0                              # one token only
+    tokens[cu[3] + 1] = 7
+    x[cu[4]] = np.where(np.arange(vocab) % 3 == 0, x[cu[4]], -np.inf)
+    x[cu[5]] = np.where(np.arange(vocab) % 3 == 0, x[cu[5]], -6e4)
+    tokens[cu[7] + 1], tokens[cu[7] + 2] = -1, vocab
+    tokens[cu[8] + 1:cu[8] + 5] = int(np.argmax(x[cu[8]]))  # siblings of the same token
+    u[cu[8] + 1], u[cu[8] + 2] = 1 - 2.0 ** -24, 0.0
+    x[cu[9]] = 0.0                                 # every token alike; the last of them, or the first
+    u[cu[9]] = 1 - 2.0 ** -24
+    x[cu[10]], u[cu[10]] = 0.0, 0.0
+    tokens[cu[10] + 1:] = vocab + 3
+    temperature = np.array([1, 1, 1, 0.5, 1, 2, 1, 0.01, 1, 1, -1], np.float32)
+    logits = torch.from_numpy(x.astype(np.float32)).to(dev)
+    drafted = None
+    if draft:
+        d = x + 0.5 * rng.standard_normal(x.shape)
+        d[cu[5]] = np.nan
+        d[cu[9], : vocab // 2] = -np.inf
+        drafted = torch.from_numpy(d.astype(np.float32)).to(dev)
+    with np.errstate(invalid="ignore"):
+        want = dft.verify(logits.double().cpu().numpy(), tokens, u, None if draft else parents,
+                          None if drafted is None else drafted.double().cpu().numpy(), temperature, cu)
+    got = bsa.verify_drafts(logits, _i32(tokens, dev), torch.from_numpy(u).to(dev), None if draft else _i32(parents, dev), drafted,
+                            torch.from_numpy(temperature).to(dev), _i32(cu, dev), 5)
+    _same_verdict(got, want, 5)
+    assert [w[2][-1] for w in want[:3]] == [-1, -1, -1] and want[6] == (0, [], [])
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+def test_verify_ties_take_the_first(dev, dtype):
+    rng = np.random.default_rng(1)
+    x = rng.integers(0, 4, (24, 9000)).astype(np.float32)  # thousands of equal maxima
+    x[:, :2300] = np.minimum(x[:, :2300], 2)
+    logits = torch.from_numpy(x).to(DT[dtype]).to(dev)
+    tokens = np.concatenate([[0], np.argmax(x, 1)[:-1]])
+    tokens[10] += 1
+    want = dft.verify(x, tokens, np.zeros(24), None, None, 0.0, [0, 8, 16, 24])
+    got = bsa.verify_drafts(logits, _i32(tokens, dev), torch.zeros(24, device=dev), temperature=0.0, max_new=8)
+    _same_verdict(got, want, 8)
+    assert want[0][0] == 8 and want[1][0] == 2
+
+
+@pytest.mark.parametrize("offset,width,dtype", [(0, 5010, "fp16"), (3, 5007, "bf16"), (1, 2500, "fp32"), (5, 40, "fp16")])
+def test_verify_strided_logits(dev, offset, width, dtype):
+    rng = np.random.default_rng(width)
+    new = [6, 3, 11]
+    x, parents, tokens, u = _drafts(rng, new, width, True)
+    wide = torch.full((20, width + 13), float("nan"), device=dev, dtype=DT[dtype])
+    logits = wide[:, offset:offset + width]
+    logits.copy_(torch.from_numpy(x.astype(np.float32)))
+    want = dft.verify(logits.double().cpu().numpy(), tokens, u, parents, None, 0.9, _cu(new))
+    got = bsa.verify_drafts(logits, _i32(tokens, dev), torch.from_numpy(u).to(dev), _i32(parents, dev), None, 0.9, _i32(_cu(new), dev), 11)
+    _same_verdict(got, want, 11)
+
+
+def test_verify_max_new_bounds_the_nodes(dev):
+    rng = np.random.default_rng(4)
+    new = [9, 2, 7]
+    x, parents, tokens, u = _drafts(rng, new, 300, True)
+    logits = torch.from_numpy(x).float().to(dev)
+    want = dft.verify(logits.double().cpu().numpy(), tokens, u, parents, None, 1.0, _cu(new), max_new=4)
+    got = bsa.verify_drafts(logits, _i32(tokens, dev), torch.from_numpy(u).to(dev), _i32(parents, dev), cu_seqlens=_i32(_cu(new), dev), max_new=4)
+    _same_verdict(got, want, 4)
+
+
+@pytest.mark.parametrize("kind", ["drawn", "likeliest"])
+def test_verify_leaves_the_targets_distribution(dev, kind):
+    """The first token that comes out is distributed as the target's first row says, whatever was drafted: of 16000
+    sequences each token's share is within 5 standard deviations."""
+    g = torch.Generator(device=dev).manual_seed(9)
+    rows, vocab = 16000, 11
+    p = torch.randn(3, vocab, generator=g, device=dev)
+    q = p + torch.randn(3, vocab, generator=g, device=dev)
+    logits = p.repeat(rows, 1).contiguous()
+    u = torch.rand(3 * rows, generator=g, device=dev)
+    if kind == "drawn":
+        first = torch.multinomial(q[0].softmax(0), rows, replacement=True, generator=g)
+        second = torch.multinomial(q[1].softmax(0), rows, replacement=True, generator=g)
+        got = bsa.verify_drafts(logits, torch.stack([torch.zeros_like(first), first, second], 1).reshape(-1).int(), u,
+                                draft_logits=q.repeat(rows, 1).contiguous(), max_new=3)
+    else:
+        best = q[0].topk(2)[1]
+        tokens = torch.stack([torch.zeros_like(best[0]), best[0], best[1]]).repeat(rows).int()
+        got = bsa.verify_drafts(logits, tokens, u, parents=_i32([-1, 0, 0] * rows, dev), max_new=3)
+    share = torch.bincount(got.tokens[:, 0].long(), minlength=vocab).double() / rows
+    want = p[0].double().softmax(0)
+    assert (got.accepted > 1).float().mean() > 0.2
+    assert ((share - want).abs() <= 5 * (want * (1 - want) / rows).sqrt()).all()
+
+
+def test_verify_graph_threads_and_prefix(dev):
+    rng = np.random.default_rng(8)
+    new = [5, 3, 8, 1]
+    x, _, tokens, u = _drafts(rng, new, 32000, False)
+    logits = torch.from_numpy(x).half().to(dev)
+    draft = (logits.float() + 0.5 * torch.randn(logits.shape, device=dev)).half()
+    ids, nums, cu = _i32(tokens, dev), torch.from_numpy(u).to(dev), _i32(_cu(new), dev)
+
+    def call(prefix=None):
+        return bsa.verify_drafts(logits, ids, nums, draft_logits=draft, cu_seqlens=cu, max_new=8, workspace_prefix=prefix)
+
+    call("verify test")
+    torch.cuda.synchronize()
+    graphs = []
+    for prefix in (None, None, "verify test"):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs.append((graph, call(prefix)))
+    for i in range(4):
+        nums.copy_(torch.rand_like(nums))
+        want = dft.verify(logits.double().cpu().numpy(), tokens, nums.cpu().numpy(), None, draft.double().cpu().numpy(), 1.0, _cu(new))
+        for graph, out in graphs:
+            for t in out:
+                t.fill_(99)
+            graph.replay()
+        eager = call()
+        torch.cuda.synchronize()
+        for out in [eager] + [o for _, o in graphs]:
+            _same_verdict(out, want, 8)
+    got = []
+
+    def run():
+        for _ in range(5):
+            got.append(call())
+
+    threads = [threading.Thread(target=run) for _ in range(3)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    torch.cuda.synchronize()
+    assert len(got) == 15
+    for out in got:
+        _same_verdict(out, want, 8)
+
+
+# ---------------------------------------------------------------------------------------- what stays
+
+
+def _kept(dev, rng, lengths, news, path, accepted, p, d, heads=2, layers=2, slots=None, spread=4, shared=()):
+    most = len(path[0])
+    made = [_cache(np.random.default_rng([rng.integers(1 << 30), 0]), dev, lengths, heads, p, d) for _ in range(layers)]
+    table = made[0][2]
+    refs = np.zeros(made[0][0].shape[0], np.int64)
+    for b, n in enumerate(lengths):
+        for j in range(-(-n // p)):
+            refs[table[b, j]] += 1
+    for page in shared:
+        refs[table[page]] += 1
+    scs = [2.0 ** rng.integers(-6 - spread, -6 + spread, m[1].shape).astype(np.float32) for m in made]
+    pages = torch.stack([torch.from_numpy(m[0]) for m in made]).to(dev).view(F8)
+    scales = torch.from_numpy(np.stack(scs)).to(dev)
+    pool = orc.Pool(table, lengths, refs, p)
+    ref = [orc.Layer(m[0], s) for m, s in zip(made, scs)]
+    dft.keep(ref, pool, path, accepted, news, slots)
+    tab, n, r = _i32(table, dev), _i32(lengths, dev), _i32(refs, dev)
+    cu = _i32(_cu(news), dev)
+    bsa.pages_keep(pages, scales, tab, n, r, _i32(path, dev), _i32(accepted, dev), cu_seqlens=cu, slots=None if slots is None else _i32(slots, dev))
+    assert tab.cpu().tolist() == pool.table and n.cpu().tolist() == pool.lengths and r.cpu().tolist() == pool.refs
+    for i in range(layers):
+        _same_pages(pages[i], scales[i], ref[i])
+    del most
+
+
+@pytest.mark.parametrize("p,d", [(16, 64), (16, 128), (32, 128), (64, 64), (128, 128)])
+@pytest.mark.parametrize("nodes", [1, 2, 7, 20, 64])
+def test_keep(dev, p, d, nodes):
+    """Paths of every kind over pages whose scales differ by octaves: moves within a page and from page to page."""
+    rng = np.random.default_rng([p, d, nodes])
+    lengths = [nodes, nodes + 1, nodes + 14, 2 * nodes + 33, 200 + nodes]
+    news = [nodes] * 5
+    path, accepted = [], []
+    for b in range(5):
+        count = int(rng.integers(0, nodes + 1)) if b else nodes
+        accepted.append(count)
+        path.append(sorted(rng.choice(nodes, count, replace=False).tolist()) + [-1] * (nodes - count))
+    _kept(dev, rng, lengths, news, path, accepted, p, d)
+
+
+@pytest.mark.parametrize("spread", [1, 12])
+def test_keep_scales_grow(dev, spread):
+    """A page takes tokens of later pages of much larger, or smaller, scales."""
+    rng = np.random.default_rng(spread)
+    path = [[5, 20, 33, 40, 47] + [-1] * 43, list(range(0, 48, 2)) + [-1] * 24, [47] + [-1] * 47]
+    _kept(dev, rng, [61, 62, 50], [48, 48, 48], path, [5, 24, 1], 16, 64, heads=5, layers=3, spread=spread)
+
+
+def test_keep_odd_paths_and_slots(dev):
+    """What does not ascend or exist ends a path; slots out of range and sequences shorter than their new tokens are
+    left as they are; counts of pages that others read."""
+    rng = np.random.default_rng(3)
+    lengths = [40, 5, 33, 64, 18, 30, 20]
+    path = [[0, 2, 2, 3], [0, 1, 2, 3], [1, 3, 9, 2], [-1, 2, 3, 1], [0, 1, 2, 3], [2, 3, 1, 0], [3, 4, 5, 6]]
+    accepted = [4, 3, 4, 2, 9, -3, 4]
+    news = [7, 8, 4, 5, 4, 4, 4]
+    slots = [0, 1, 2, 3, 9, 5, 6]
+    _kept(dev, rng, lengths, news, path, accepted, 16, 64, slots=slots, shared=[(2, 2), (0, 0)])
+    _kept(dev, rng, lengths, [4] * 7, path, accepted, 16, 128, slots=[3, 2, 6, 0, 1, -1, 4])
+
+
+def test_keep_nan_and_bad_pages(dev):
+    rng = np.random.default_rng(4)
+    raw, sc, table, pages, scales, tab = _cache(rng, dev, [40, 40], 1, 16, 64)
+    at = orc.key_offset(38 % 16, 5, 64)
+    raw[table[0, 38 // 16], 0, 0].reshape(-1)[at] = 0xFF
+    sc[table[0, 2], 0, 0], sc[table[0, 1], 0, 0] = 2.0, 0.25
+    table[1, 1] = 10 ** 7
+    layer, pool = orc.Layer(raw, sc), orc.Pool(table, [40, 40], [1] * raw.shape[0], 16)
+    path = [[0, 8, -1, -1], [2, 7, 8, -1]]
+    dft.keep([layer], pool, path, [2, 3], [10, 10])
+    pages, scales = torch.from_numpy(raw)[None].to(dev).view(F8), torch.from_numpy(sc)[None].to(dev)
+    tab, n, refs = _i32(table, dev), _i32([40, 40], dev), torch.ones(raw.shape[0], dtype=torch.int32, device=dev)
+    bsa.pages_keep(pages, scales, tab, n, refs, _i32(path, dev), _i32([2, 3], dev), cu_seqlens=_i32([0, 10, 20], dev))
+    assert tab.cpu().tolist() == pool.table and refs.cpu().tolist() == pool.refs
+    _same_pages(pages[0], scales[0], layer)
+
+
+def test_keep_graph(dev):
+    rng = np.random.default_rng(6)
+    _, _, table, pages, scales, tab = _cache(rng, dev, [50, 23], 2, 16, 64)
+    pages, scales = torch.stack([pages.view(torch.uint8)] * 2).view(F8), torch.stack([scales] * 2)
+    n, refs = _i32([50, 23], dev), torch.ones(pages.shape[1], dtype=torch.int32, device=dev)
+    path, accepted = _i32([[0, 3, 9, -1], [1, -1, -1, -1]], dev), _i32([3, 1], dev)
+    cu = _i32([0, 12, 16], dev)
+    state = (pages.view(torch.uint8), scales, tab, n, refs)
+    before = [x.clone() for x in state]
+
+    def reset():
+        for x, was in zip(state, before):
+            x.copy_(was)
+
+    def call():
+        bsa.pages_keep(pages, scales, tab, n, refs, path, accepted, cu_seqlens=cu)
+
+    call()
+    want = [x.clone() for x in state]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    reset()
+    with torch.cuda.graph(graph):
+        call()
+    for _ in range(3):
+        reset()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, w) for x, w in zip(state, want))
+    assert n.tolist() == [41, 20]

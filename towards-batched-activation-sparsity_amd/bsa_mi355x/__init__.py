@@ -9,6 +9,7 @@ layer that mirrors the reference's Python entry points
 """
 from ._lib import BLOCK_K, MAX_NBLK, BsgArgError, BsgDtypeError, BsgError, BsgUnsupported, Plan, load
 from .autotune import set_autotune
+from .drafts import Verified, kv_append_rotated, kv_tree_attention, pages_keep, verify_drafts
 from .runtime import (INDEX_BLOCK_META_SIZE, TiledPackedWeight, TileConfig, _build_active_k_bitmap, _get_prepacked_weight_block_major,
                       _prepacked_block_sparse_gemm_from_active_blocks,
                       _prepacked_block_sparse_gemm_from_active_blocks_bitmap_preload,
@@ -47,4 +48,5 @@ __all__ = [
     "_get_cached_active_n_blocks_delta", "gemm_2d_packed", "scatter_nblocks", "nmask_blocks",
     "KVCache", "TokenLogprobs", "kv_append", "kv_attention", "pages_copy", "pages_fork", "pages_extend", "pages_free",
     "pages_compact", "read_pages", "token_logprobs",
+    "Verified", "kv_append_rotated", "kv_tree_attention", "verify_drafts", "pages_keep",
 ]

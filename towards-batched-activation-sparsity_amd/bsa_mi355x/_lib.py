@@ -137,6 +137,24 @@ class PagePool(ctypes.Structure):
     ]
 
 
+class Rotary(ctypes.Structure):
+    """bsg_rotary (include/bsgdraft.h)."""
+
+    _fields_ = [
+        ("cos", ctypes.c_void_p),
+        ("sin", ctypes.c_void_p),
+        ("stride", ctypes.c_int64),
+        ("positions", ctypes.c_int32),
+        ("dims", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("q_norm", ctypes.c_void_p),
+        ("k_norm", ctypes.c_void_p),
+        ("token_positions", ctypes.c_void_p),
+        ("parents", ctypes.c_void_p),
+    ]
+
+
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
@@ -145,8 +163,9 @@ _f32 = ctypes.c_float
 _pplan = ctypes.POINTER(Plan)
 _pkv = ctypes.POINTER(KvCache)
 _ppool = ctypes.POINTER(PagePool)
+_protary = ctypes.POINTER(Rotary)
 
-# name -> (restype, argtypes); every function declared in include/bsgemm.h and include/bsgserve.h
+# name -> (restype, argtypes); every function declared in include/bsgemm.h, bsgserve.h and bsgdraft.h
 SIGNATURES = {
     "bsg_version": (ctypes.c_char_p, []),
     "bsg_last_error": (ctypes.c_char_p, []),
@@ -190,6 +209,16 @@ SIGNATURES = {
     "bsg_pages_compact": (_int, [_ppool, _vp, _vp, _i64, _vp]),
     "bsg_token_logprobs_workspace_bytes": (_i64, [_i64, _i64, _i32, _int, _i32]),
     "bsg_token_logprobs": (_int, [_vp, _i64, _i64, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _int, _vp, _i64, _i32, _vp]),
+    # include/bsgdraft.h
+    "bsg_kv_append_rotated": (_int, [_vp, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _protary,
+                                     _pkv, _vp, _i32, _vp, _i32, _int, _vp]),
+    "bsg_kv_tree_attention_workspace_bytes": (_i64, [_pkv, _i32, _i32, _i32, _i64, _i32]),
+    "bsg_kv_tree_attention": (_int, [_vp, _i64, _i64, _i64, _i32, _vp, _pkv, _vp, _i32, _vp, _i32, _i64, _f32, _vp, _i64, _i64,
+                                     _vp, _int, _vp, _i64, _i32, _vp]),
+    "bsg_verify_drafts_workspace_bytes": (_i64, [_i64, _i32, _i64, _i32, _int, _i32]),
+    "bsg_verify_drafts": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i32, _i32, _f32, _vp, _vp, _vp, _vp,
+                                 _int, _vp, _i64, _vp]),
+    "bsg_pages_keep": (_int, [_ppool, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i32, _vp]),
     # include/bsgemm_timeline.h
     "bsg_timeline_attach": (_int, [_vp, _i64, _i64]),
     "bsg_timeline_clock_khz": (_i64, []),

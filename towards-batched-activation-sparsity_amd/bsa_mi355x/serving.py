@@ -14,6 +14,7 @@ attention that reads it, the bookkeeping of its pages, and the log probabilities
 All of it runs on the device with no host round trip (csrc/kv_append.hip, kv_attention.hip, pages.hip,
 logprobs.hip through include/bsgserve.h), on torch's current stream, and can be captured.  The
 reference leaves attention and cache to the model's own library, so these have no counterpart there.
+drafts.py has the calls of a step whose new tokens are a tree of drafts.
 
 Layout.  pages is [layers, pages, heads, 2, page_size, head_dim] in torch.float8_e4m3fn, keys then
 values, in tile order inside [page_size, head_dim] (include/bsgserve.h; `read_pages` gives plain
@@ -483,7 +484,8 @@ class KVCache:
 
     A slot is a sequence: `extend` gives it pages for new tokens (once for all layers), `append`
     writes a layer's keys and values, `attend` reads them, `fork` lets slots go on from others, `free`
-    releases them, `compact` makes the pool dense."""
+    releases them, `compact` makes the pool dense.  Where the new tokens are drafts, `append_rotated` and
+    `attend_tree` take them as a tree, and `keep` leaves the accepted ones (drafts.py)."""
 
     def __init__(self, layers: int, num_pages: int, heads: int, head_dim: int = 128, page_size: int = 16,
                  max_slots: int = 64, max_pages: int = 256, device: Optional[torch.device] = None):
@@ -508,6 +510,16 @@ class KVCache:
     def attend(self, layer: int, q: torch.Tensor, **kw) -> Tuple[torch.Tensor, torch.Tensor]:
         return kv_attention(q, self.pages, self.scales, self.page_table, self.lengths, layer=layer, **kw)
 
+    def append_rotated(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                       **kw) -> torch.Tensor:
+        return drafts.kv_append_rotated(q, k, v, cos, sin, self.pages, self.scales, self.page_table, self.lengths, layer=layer, **kw)
+
+    def attend_tree(self, layer: int, q: torch.Tensor, parents: torch.Tensor, **kw) -> Tuple[torch.Tensor, torch.Tensor]:
+        return drafts.kv_tree_attention(q, parents, self.pages, self.scales, self.page_table, self.lengths, layer=layer, **kw)
+
+    def keep(self, path: torch.Tensor, accepted: torch.Tensor, **kw) -> None:
+        drafts.pages_keep(self.pages, self.scales, self.page_table, self.lengths, self.refcounts, path, accepted, **kw)
+
     def fork(self, parents: torch.Tensor, children: torch.Tensor) -> None:
         pages_fork(self.page_table, self.lengths, self.refcounts, parents, children)
 
@@ -526,3 +538,6 @@ class KVCache:
         ids = self.page_table[slot, : -(-n // self.page_size)].long()
         k, v = read_pages(self.pages[layer].view(torch.uint8)[ids].view(_F8), self.scales[layer][ids])
         return tuple(x.transpose(0, 1).reshape(self.heads, -1, self.head_dim)[:, :n] for x in (k, v))
+
+
+from . import drafts  # noqa: E402  (which takes its helpers from here)

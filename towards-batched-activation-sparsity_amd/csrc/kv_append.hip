@@ -13,7 +13,7 @@
 // 16: 6.8 us, a chain of three dependent loads from cold caches (length, page, what the page holds) between
 // launch and store.
 
-#include "serve.hpp"
+#include "kv_quant.hpp"
 
 using namespace bsgk;
 
@@ -31,47 +31,6 @@ struct AppendParams {
   int64_t table_stride, tokens;
   int32_t num_pages, heads, num_slots, max_pages, max_new, pages_per_row, first_unit, units, wide;
 };
-
-// Bytes b of the four dwords a quad's lanes hold, to lane b of the quad: the 4 x 4 byte transpose.
-__device__ __forceinline__ uint32_t quad_transpose(uint32_t w, int i) {
-  const uint32_t w0 = __builtin_amdgcn_mov_dpp(w, 0x00, 0xf, 0xf, true);
-  const uint32_t w1 = __builtin_amdgcn_mov_dpp(w, 0x55, 0xf, 0xf, true);
-  const uint32_t w2 = __builtin_amdgcn_mov_dpp(w, 0xaa, 0xf, 0xf, true);
-  const uint32_t w3 = __builtin_amdgcn_mov_dpp(w, 0xff, 0xf, 0xf, true);
-  const uint32_t sel = (uint32_t)i * 0x0101u + 0x0400u;  // byte i of each of two words
-  const uint32_t lo = __builtin_amdgcn_perm(w1, w0, sel) & 0xffffu;
-  const uint32_t hi = __builtin_amdgcn_perm(w3, w2, sel) & 0xffffu;
-  return lo | (hi << 16);
-}
-
-// The 4 x 4 transpose of four dwords over the four rows of 16 lanes.
-__device__ __forceinline__ void row_transpose(uint32_t w[4]) {
-#pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    const auto r = __builtin_amdgcn_permlane32_swap(w[n], w[n + 2], false, false);
-    w[n] = r[0], w[n + 2] = r[1];
-  }
-#pragma unroll
-  for (int n = 0; n < 4; n += 2) {
-    const auto r = __builtin_amdgcn_permlane16_swap(w[n], w[n + 1], false, false);
-    w[n] = r[0], w[n + 1] = r[1];
-  }
-}
-
-// x / scale to e4m3, rounded to nearest even: the product with a power of two is exact, infinities
-// become the largest value, NaN stays.
-__device__ __forceinline__ float in_range(float x) { return x != x ? x : fminf(fmaxf(x, -448.f), 448.f); }
-
-__device__ __forceinline__ uint32_t to_e4m3(float a, float b, float c, float d) {
-  int r = __builtin_amdgcn_cvt_pk_fp8_f32(in_range(a), in_range(b), 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(in_range(c), in_range(d), r, true);
-}
-
-// Four cached numbers under a new, larger scale.
-__device__ __forceinline__ uint32_t rescale(uint32_t w, float ratio) {
-  return to_e4m3(__builtin_amdgcn_cvt_f32_fp8((int)w, 0) * ratio, __builtin_amdgcn_cvt_f32_fp8((int)w, 1) * ratio,
-                 __builtin_amdgcn_cvt_f32_fp8((int)w, 2) * ratio, __builtin_amdgcn_cvt_f32_fp8((int)w, 3) * ratio);
-}
 
 // The largest finite magnitude in the wave.  Magnitudes of either 16-bit type order as their bits do; only where
 // infinities or NaN are among them are those taken out.
@@ -110,14 +69,6 @@ __device__ __forceinline__ float largest_magnitude(const uint32_t x[C][8]) {
     top = m.x > m.y ? m.x : m.y;
   }
   return low_half<T>(top);
-}
-
-// The least power of two s in [2^-40, 2^80] with a <= 448 s, from the bits of a = 1.m x 2^e:
-// 448 = 1.75 x 2^8.
-__device__ __forceinline__ float scale_for(float a) {
-  const int e = (int)((__builtin_bit_cast(uint32_t, a) + 0x1fffffu) >> 23) - 127 - 8;
-  const int c = e < BSG_KV_SCALE_MIN_EXP ? BSG_KV_SCALE_MIN_EXP : e > BSG_KV_SCALE_MAX_EXP ? BSG_KV_SCALE_MAX_EXP : e;
-  return __builtin_bit_cast(float, (uint32_t)(c + 127) << 23);
 }
 
 template <typename T, int D, int P>
