@@ -202,19 +202,26 @@ def test_no_spills_and_no_packed_floats(asm):
 
 
 def test_tree_steps_issue_their_loads(asm):
-    """As for prompts: tiles of 128 rows wait for a step's keys and values by the count of loads a step."""
+    """As for prompts: a step's keys and values are waited for by the count of loads, so between two barriers of the
+    pipeline each wave issues exactly that many, in one run of instructions."""
     found = 0
-    for name, body in _functions(asm["kv_tree.hip"], r"_ZN12_GLOBAL__N_121bsg_kv_prefill_kernel"):
+    for name, body in _functions(asm["kv_tree.hip"], r"_ZN12_GLOBAL__N_118bsg_kv_tree_kernel"):
         loads = 2 * int(re.search(r"Li(\d+)E", name).group(1)) // 64
-        at = [i for i, line in enumerate(body) if line.strip().startswith("s_barrier")]
-        steps = [body[a:b] for a, b in zip(at, at[1:]) if any("mfma" in line for line in body[a:b])]
-        assert len(steps) == 3, (name, len(steps))
-        for step in steps:
-            lines = [i for i, line in enumerate(step) if " lds" in line]
+        steps = 0
+        for i, line in enumerate(body):
+            if not line.strip().startswith("s_barrier"):
+                continue
+            # what comes before the step's first product, or the next barrier
+            after = next((j for j in range(i + 1, len(body)) if "mfma" in body[j] or body[j].strip().startswith("s_barrier")), len(body))
+            lines = [j for j in range(i, after) if body[j].rstrip().endswith(" lds") or " lds" in body[j]]
+            if after == len(body) or "mfma" not in body[after] or not lines:
+                continue
             assert len(lines) == loads, name
-            assert not any(re.match(r"\s*(s_cbranch|\.LBB)", line) for line in step[lines[0]:lines[-1]]), name
+            assert not any(re.match(r"\s*(s_cbranch|\.LBB)", x) for x in body[lines[0]:lines[-1]]), name
+            steps += 1
+        assert steps == 3, (name, steps)
         found += 1
-    assert found == 4  # two types x two head sizes
+    assert found == 8  # two types x two head sizes x two tiles
 
 
 # ---------------------------------------------------------------------------------------- the oracle
