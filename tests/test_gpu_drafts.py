@@ -503,6 +503,43 @@ def test_verify_strided_logits(dev, offset, width, dtype):
     _same_verdict(got, want, 11)
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("vocab", [300, 5003, 32000])
+def test_verify_numbers_next_to_their_border(dev, dtype, vocab):
+    """The 32-bit number below a child's border accepts it, the one above does not, after none, one and two rejected
+    siblings: no nearer than 2^-25 of it, and 64-bit sums tell them apart.  The new token's number likewise."""
+    rng = np.random.default_rng(vocab)
+    new = [4] * 12
+    x, _, _, u = _drafts(rng, new, vocab, False)
+    logits = torch.from_numpy(x.astype(np.float32)).to(DT[dtype]).to(dev)
+    host = logits.double().cpu().numpy()
+    tokens, parents = np.zeros(48, np.int64), [-1, 0, 0, 0] * 12
+    for b in range(12):
+        best = np.argsort(-host[4 * b], kind="stable")
+        tokens[4 * b + 1:4 * b + 4] = best[[5, 2, 3]]
+        p = np.exp(host[4 * b] - host[4 * b].max())
+        p /= p.sum()
+        u[4 * b + 1:4 * b + 4] = 1 - 2.0 ** -24
+        asked, up = b % 3, b // 3 % 2 == 0
+        border = p[tokens[4 * b + 1 + asked]] / (1 - sum(p[tokens[4 * b + 1 + i]] for i in range(asked)))
+        near = np.float32(border)
+        near = near if (float(near) >= border) == up else np.nextafter(near, np.float32(2 if up else 0))
+        u[4 * b + 1 + asked] = near
+        assert (float(near) < border) != up and abs(float(near) / border - 1) < 2.0 ** -22
+        # the new token's, between two tokens of the tail of what is left of its row
+        at = 4 * b + (0 if up else 1 + asked)
+        q = np.exp(host[at] - host[at].max())
+        if up:
+            q[tokens[4 * b + 1:4 * b + 4]] = 0
+        sums = np.cumsum(q) / q.sum()
+        u[4 * b] = np.float32(sums[(7919 * b) % vocab])
+        assert u[4 * b] < 1
+    want = dft.verify(host, tokens, u, parents, None, 1.0, _cu(new))
+    got = bsa.verify_drafts(logits, _i32(tokens, dev), torch.from_numpy(u).to(dev), _i32(parents, dev), max_new=4)
+    _same_verdict(got, want, 4)
+    assert [w[0] for w in want] == [1, 1, 1, 2, 2, 2] * 2
+
+
 def test_verify_max_new_bounds_the_nodes(dev):
     rng = np.random.default_rng(4)
     new = [9, 2, 7]

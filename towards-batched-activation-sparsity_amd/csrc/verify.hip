@@ -2,15 +2,18 @@
 //
 // Answers are whole numbers next to borders: a number u against a ratio of probabilities, and the first running sum past
 // u of the whole.  So weights w = 2^((x - m) k), k = log2(e) / temperature, and their sums are 64-bit.  2^t is
-// 2^n times the Taylor polynomial of e^(f ln 2), t = n + f, |f| <= 1/2, to the 12th power (relative error
-// (ln 2 / 2)^13 / 13! = 1.7e-16).
+// 2^n times a polynomial of the 9th degree in f, t = n + f, |f| <= 1/2, which interpolates 2^f in the Chebyshev points of
+// that interval (relative error 2^-46).
 //
-// First launch: a wave has kPiece consecutive logits of one node's row in registers and leaves their maximum and
-// the sum of their weights against it (or, greedy, where the first maximum is).  The last work-group of a sequence to arrive
-// has all of them: it walks the tree (a node in each lane; nodes in order, each asked if its parent is the last accepted
-// one) and draws the new token from the last row, whose pieces' sums it already has: the piece by them, the token by reading
-// that piece again.  Second launch, where drafts come with probabilities: the sums of max(p - q, 0) over the pieces of
-// a row whose child was rejected, and the draw from those.
+// First launch: of the rows of nodes that have children a wave has kPiece logits in registers and leaves their maximum
+// and the sum of their weights against it (or, greedy, where the first maximum is).  Second launch: the work-groups
+// of a sequence each put the rows together and walk the tree (a node in each lane; nodes in order, each asked if its
+// parent is the last accepted one); then each makes the sums of some pieces of what is left of the last row, and the last
+// to arrive draws the new token, first a piece, then a number of it.
+//
+// Of a row without draft_logits the walk only asks on which side of a number its sum lies, so that the first launch adds its
+// weights in 32 bits, kNear off at most; where a number is as near as that to its border the wave adds the row again in
+// 64.  Against draft_logits the last row's sums are wanted exactly, and both are 64-bit from the start.
 
 #include "bsgdraft.h"
 #include "draft_tree.hpp"
@@ -19,20 +22,18 @@ using namespace bsgk;
 
 namespace {
 
-constexpr int kPiece = 2048;  // logits of a wave
+constexpr int kPiece = 1024;  // logits of a wave
 constexpr int kWaves = 4;     // of a work-group
-constexpr int kMostPieces = 512;  // of a row
+constexpr int kMostVocab = 1 << 20;
 constexpr double kLog2e = 1.4426950408889634;
+// The 32-bit sum of a row: a weight of t octaves is off by 0.7 x 3 |t| 2^-24 (the difference, k, their product) and 2^-22 of
+// itself; |t|, averaged by the weights, is at most the logarithm of the vocabulary, 20.  Sums of 32 numbers add 2^-19.
+constexpr double kNear = 0x1p-17;
 
 struct Piece {  // of a row
   double sum;   // of its weights; NaN: a logit is NaN or +inf
   float top;
   int32_t at;   // of the first maximum
-};
-struct Verdict {  // what the first launch leaves the second
-  double total[2];  // of p's and q's row, against the maxima
-  float top[2];
-  int32_t node, count, residual, pad;  // residual: the row whose max(p - q, 0) is drawn from is node's
 };
 
 struct VerifyParams {
@@ -49,30 +50,25 @@ struct VerifyParams {
   int32_t* accepted;
   int32_t* path;
   int32_t* out;
-  uint32_t* counters;  // [rows]: the first launch's, then the second's
-  Verdict* verdicts;   // [rows]
+  uint32_t* counters;  // [rows]: of the second launch
   Piece* stats;        // [tokens][1 + drafts][pieces]
-  double* left;        // [rows][pieces]
+  Piece* last;         // [rows][pieces], of the last row
 };
 
-// 2^t for t <= 0, and 0 far below.
-__device__ __forceinline__ double exp2_64(double t) {
-  t = t < -1100.0 ? -1100.0 : t;
+// The weight of a logit against a maximum: 2^((x - top) k), 0 far below and for -inf (and NaN, which its row is known by).
+__device__ __forceinline__ double weight(float x, float top, double k) {
+  const double t = __builtin_fmax(((double)x - (double)top) * k, -1100.0);
   const double n = __builtin_rint(t), f = t - n;
-  // (ln 2)^i / i!
-  double y = 2.5678435993488206e-11;
-  y = __builtin_fma(y, f, 4.4455382718708115e-10);
-  y = __builtin_fma(y, f, 7.0549116208011234e-09);
-  y = __builtin_fma(y, f, 1.0178086009239699e-07);
-  y = __builtin_fma(y, f, 1.3215486790144309e-06);
-  y = __builtin_fma(y, f, 1.5252733804059841e-05);
-  y = __builtin_fma(y, f, 0.00015403530393381609);
-  y = __builtin_fma(y, f, 0.0013333558146428443);
-  y = __builtin_fma(y, f, 0.0096181291076284772);
-  y = __builtin_fma(y, f, 0.055504108664821580);
-  y = __builtin_fma(y, f, 0.24022650695910071);
-  y = __builtin_fma(y, f, 0.69314718055994531);
-  y = __builtin_fma(y, f, 1.0);
+  double y = 1.0205905413765595e-07;
+  y = __builtin_fma(y, f, 1.325964524488711e-06);
+  y = __builtin_fma(y, f, 1.5252672924850737e-05);
+  y = __builtin_fma(y, f, 0.0001540343375125101);
+  y = __builtin_fma(y, f, 0.0013333558200794592);
+  y = __builtin_fma(y, f, 0.009618129193934313);
+  y = __builtin_fma(y, f, 0.05550410866465167);
+  y = __builtin_fma(y, f, 0.2402265069564034);
+  y = __builtin_fma(y, f, 0.6931471805599462);
+  y = __builtin_fma(y, f, 1.0000000000000135);
   return __builtin_ldexp(y, (int)n);
 }
 
@@ -97,30 +93,91 @@ struct Logit<__bf16> {
   static __device__ __forceinline__ float one(const void* x, int64_t at) { return as_float((uint32_t)((const uint16_t*)x)[at] << 16); }
 };
 
-// A wave's piece of a row: vector v of lane l holds the logits piece * kPiece + (64 v + l) PER .. of the row, -inf past its
-// end.  Rows that 16 bytes do not divide come number by number.
+// Numbers of a row in registers.  A row is cut at addresses that 16 bytes divide, so that every load is whole (the granules in
+// which it begins and ends are read whole); `shift` is how many numbers of the first granule lie before the row.  What
+// lies outside the row is -inf.
 template <typename T>
-struct PieceOf {
-  static constexpr int PER = Logit<T>::PER, VECTORS = kPiece / 64 / PER;
+__device__ __forceinline__ int shift_of(const void* x, int64_t row_at) {
+  return (int)(((uintptr_t)((const T*)x + row_at) & 15) / sizeof(T));
+}
+template <typename T, int BYTES>
+struct Numbers {
+  typedef T vec __attribute__((ext_vector_type(Logit<T>::PER)));
+  static constexpr int PER = Logit<T>::PER, VECTORS = BYTES / 16, N = PER * VECTORS;
   u32x4 v[VECTORS];
-  __device__ __forceinline__ void load(const void* x, int64_t row_at, int64_t vocab, int piece, int lane) {
-    const T* const row = (const T*)x + row_at;
-    const bool wide = ((uintptr_t)row & 15) == 0;
-#pragma unroll
+  // f(number of the vector, vector) for one after the other, in a loop: a wave comes by here once or twice, and code
+  // that is not in the instruction cache yet costs more than the loop.
+  template <typename F>
+  __device__ __forceinline__ void each(const F& f) {
+#pragma unroll 1
     for (int k = 0; k < VECTORS; ++k) {
-      const int64_t at = (int64_t)piece * kPiece + (64 * k + lane) * PER;
-      if (wide && at + PER <= vocab) {
-        v[k] = *(const u32x4*)(row + at);
-      } else {
-        typedef T vec __attribute__((ext_vector_type(PER)));
-        vec w;
+      u32x4 first = v[0];
+      f(k, first);
 #pragma unroll
-        for (int e = 0; e < PER; ++e) w[e] = at + e < vocab ? row[at + e] : (T)-__builtin_inff();
-        v[k] = __builtin_bit_cast(u32x4, w);
-      }
+      for (int i = 0; i + 1 < VECTORS; ++i) v[i] = v[i + 1];
+      v[VECTORS - 1] = first;
     }
   }
-  __device__ __forceinline__ float get(int k, int e) const { return Logit<T>::of(v[k], e); }
+  // Vector k from number at(k) of a row on.  shift: the cut's, which is the row's own but where it goes beside another row.
+  template <typename At>
+  __device__ __forceinline__ void load(const void* x, int64_t row_at, int n, int shift, bool inside, const At& at) {
+    const T* const row = (const T*)x + row_at;
+    const bool own = shift_of<T>(x, row_at) == shift;
+    // all loads before one is looked at; what lies outside loads the first granule
+    if (own) {
+#pragma unroll
+      for (int k = 0; k < VECTORS; ++k) v[k] = *(const u32x4*)(row + (at(k) < n ? at(k) : -shift));
+      if (inside) return;
+    }
+    each([&](int k, u32x4& a) {
+      vec w = __builtin_bit_cast(vec, a);
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        const bool in = at(k) + e >= 0 && at(k) + e < n;
+        if (!own) w[e] = row[in ? at(k) + e : 0];
+        w[e] = in ? w[e] : (T)-__builtin_inff();
+      }
+      a = __builtin_bit_cast(u32x4, w);
+    });
+  }
+  // The number that the row has at `place` weighs nothing any more, if it is one of the lane's.
+  template <typename At>
+  __device__ __forceinline__ void drop(int place, const At& at) {
+    each([&](int k, u32x4& a) {
+      vec w = __builtin_bit_cast(vec, a);
+#pragma unroll
+      for (int e = 0; e < PER; ++e) w[e] = at(k) + e == place ? (T)-__builtin_inff() : w[e];
+      a = __builtin_bit_cast(u32x4, w);
+    });
+  }
+};
+// A wave's piece: vector k of lane l from number (64 k + l) PER of it on.
+template <typename T>
+struct PieceOf : Numbers<T, (int)(kPiece / 64 * sizeof(T))> {
+  static constexpr int PER = Logit<T>::PER;
+  __device__ __forceinline__ void load(const void* x, int64_t row_at, int64_t vocab, int shift, int piece, int lane) {
+    const int first = piece * kPiece - shift, n = (int)vocab;
+    Numbers<T, (int)(kPiece / 64 * sizeof(T))>::load(x, row_at, n, shift, first >= 0 && first + kPiece <= n,
+                                                     [&](int k) { return first + (64 * k + lane) * PER; });
+  }
+  __device__ __forceinline__ void drop(int place, int shift, int piece, int lane) {
+    Numbers<T, (int)(kPiece / 64 * sizeof(T))>::drop(place, [&](int k) { return piece * kPiece - shift + (64 * k + lane) * PER; });
+  }
+};
+// A wave's share of the piece that the new token is drawn from: lane l has the numbers 8 l .. 8 l + 7 of it.
+constexpr int kShare = 512;
+template <typename T>
+struct ShareOf : Numbers<T, (int)(kShare / 64 * sizeof(T))> {
+  static constexpr int PER = Logit<T>::PER, N = kShare / 64;
+  __device__ __forceinline__ void load(const void* x, int64_t row_at, int64_t vocab, int shift, int first, int lane) {
+    const int n = (int)vocab;
+    Numbers<T, (int)(kShare / 64 * sizeof(T))>::load(x, row_at, n, shift, first >= 0 && first + kShare <= n,
+                                                       [&](int k) { return first + lane * N + k * PER; });
+  }
+  __device__ __forceinline__ void drop(int place, int first, int lane) {
+    Numbers<T, (int)(kShare / 64 * sizeof(T))>::drop(place, [&](int k) { return first + lane * N + k * PER; });
+  }
+  __device__ __forceinline__ float get(int i) const { return Logit<T>::of(this->v[i / PER], i % PER); }
 };
 
 template <int X>
@@ -156,11 +213,6 @@ __device__ __forceinline__ double wave_scan(double v, int lane) {
   return v;
 }
 
-// The weight of a logit against a maximum; 0 for -inf.
-__device__ __forceinline__ double weight(float x, float top, double k) {
-  return x == -__builtin_inff() ? 0.0 : exp2_64(((double)x - (double)top) * k);
-}
-
 // A sequence, as every wave of it sees it.
 struct Tree {
   int64_t from;
@@ -179,37 +231,77 @@ __device__ __forceinline__ Tree tree_of(const VerifyParams& p, int row, int lane
   t.parent = load_parent(p.parents, t.from, t.count, lane);
   return t;
 }
-
-__device__ __forceinline__ const Piece* piece_at(const VerifyParams& p, int64_t token, int which) {
-  return p.stats + (token * (1 + p.drafts) + which) * p.pieces;
-}
-__device__ __forceinline__ Piece load_piece(const Piece* at) {
-  Piece v;
-  v.sum = __builtin_bit_cast(double, hand_load((const uint64_t*)at));
-  const uint64_t b = hand_load((const uint64_t*)at + 1);
-  v.top = as_float((uint32_t)b), v.at = (int32_t)(b >> 32);
+// The nodes that have children.
+__device__ __forceinline__ uint64_t inner_of(const Tree& t) {
+  uint64_t v = t.parent >= 0 ? 1ull << t.parent : 0;
+  v |= lane_xor<1>(v), v |= lane_xor<2>(v), v |= lane_xor<4>(v);
+  v |= lane_xor<8>(v), v |= lane_xor<16>(v), v |= lane_xor<32>(v);
   return v;
 }
 
-// A row's maximum, the sum of its weights against it and where the first maximum is, from its pieces: a wave's work.
-struct Row {
-  double total;
-  float top;
-  int32_t at;
-};
-__device__ __forceinline__ Row row_of(const Piece* pieces, int n, double k, int lane) {
-  Row r = {0.0, -__builtin_inff(), 0x7fffffff};
-  for (int c0 = 0; c0 < n; c0 += 64) {
-    Piece v = {0.0, -__builtin_inff(), 0x7fffffff};
-    if (c0 + lane < n) v = load_piece(pieces + c0 + lane);
-    const float top = fmaxf(r.top, wave_max<32>(v.top));
-    const int at = wave_min<32>(v.top == top ? v.at : 0x7fffffff);
-    if (top > r.top || c0 == 0) r.at = at;
-    const double sum = wave_sum<32>(v.sum == v.sum ? v.sum * weight(v.top, top, k) : v.sum);
-    r.total = (r.top == -__builtin_inff() ? r.total : r.total * weight(r.top, top, k)) + sum;
-    r.top = top;
+// What a piece is to its row: its maximum, the sum of its weights against that, and greedy the place of the first
+// maximum.  first: the place of the piece's first number.
+template <typename T>
+__device__ __forceinline__ Piece piece_of(PieceOf<T>& x, bool greedy, bool exact, double k, int first, int lane) {
+  constexpr int PER = PieceOf<T>::PER;
+  bool bad = false;
+  float top = -__builtin_inff();
+  x.each([&](int, u32x4& v) {
+#pragma unroll
+    for (int e = 0; e < PER; ++e) top = fmaxf(top, Logit<T>::of(v, e)), bad = bad || !(Logit<T>::of(v, e) < __builtin_inff());
+  });
+  Piece mine = {0.0, wave_max<32>(top), 0x7fffffff};
+  if (greedy) {
+    x.each([&](int i, u32x4& v) {
+#pragma unroll
+      for (int e = PER - 1; e >= 0; --e)
+        if (Logit<T>::of(v, e) == mine.top && first + (64 * i + lane) * PER + e < mine.at) mine.at = first + (64 * i + lane) * PER + e;
+    });
+    mine.at = wave_min<32>(mine.at);
+  } else if (exact) {
+    x.each([&](int, u32x4& v) {
+#pragma unroll
+      for (int e = 0; e < PER; ++e) mine.sum += weight(Logit<T>::of(v, e), mine.top, k);
+    });
+    mine.sum = wave_sum<32>(mine.sum);
+  } else {
+    // a piece of nothing but -inf has no maximum to be weighed against
+    const float by = (float)k, from = mine.top == -__builtin_inff() ? 0.f : mine.top;
+    float sum = 0.f;
+    x.each([&](int, u32x4& v) {
+#pragma unroll
+      for (int e = 0; e < PER; ++e) sum += __builtin_amdgcn_exp2f((Logit<T>::of(v, e) - from) * by);
+    });
+    mine.sum = wave_sum<32>((double)sum);
   }
-  return r;
+  if (__any(bad)) mine.sum = __builtin_nan("");
+  return mine;
+}
+
+// The rows of the nodes that have children, by pieces: of a sequence's the blockIdx.y-th, and every gridDim.y-th from there.
+// 64 chains of up to 5 drawn drafts, 32000 fp16 logits of two models: 18 us, of which the 64-bit weights are some 12 (18
+// instructions each, all at the rate of a fused multiply-add); 64 trees of up to 16 nodes: 13 us with 32-bit weights, 21 with
+// 64-bit ones.
+template <typename T>
+__global__ __launch_bounds__(64 * kWaves) void bsg_verify_rows_kernel(VerifyParams p) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int which = blockIdx.x / p.groups, piece = (blockIdx.x - which * p.groups) * kWaves + wave;
+  const Tree t = tree_of(p, blockIdx.z, lane);
+  const bool greedy = !(t.temperature > 0.f);
+  if (piece >= p.pieces || (greedy && which)) return;
+  uint64_t left = inner_of(t);
+  for (int skip = blockIdx.y; left; skip = gridDim.y - 1) {
+    for (; skip > 0 && left; --skip) left &= left - 1;
+    if (!left) return;
+    const int node = __builtin_amdgcn_readfirstlane(__builtin_ctzll(left));
+    left &= left - 1;
+    const int64_t at = (t.from + node) * p.stride[which];
+    const int shift = shift_of<T>(p.x[which], at);
+    PieceOf<T> x;
+    x.load(p.x[which], at, p.vocab, shift, piece, lane);
+    const Piece mine = piece_of<T>(x, greedy, p.drafts != 0, kLog2e / (double)t.temperature, piece * kPiece - shift, lane);
+    if (lane == 0) p.stats[((t.from + node) * (1 + p.drafts) + which) * p.pieces + piece] = mine;
+  }
 }
 
 __device__ __forceinline__ double read_lane(double v, int lane) {
@@ -218,262 +310,289 @@ __device__ __forceinline__ double read_lane(double v, int lane) {
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
-// The first piece of a row whose running sum passes `goal`, the last one of any weight if none does; `before` gets the
-// sum before it.
-template <typename Sum>
-__device__ __forceinline__ int pick_piece(int n, double goal, int lane, double* before, const Sum& sum) {
-  double run = 0.0, last_before = 0.0;
-  int last = -1;
-  for (int c0 = 0; c0 < n; c0 += 64) {
-    const double v = c0 + lane < n ? sum(c0 + lane) : 0.0;
-    const double upto = run + wave_scan(v, lane);
-    const uint64_t past = __ballot(upto > goal && v > 0.0), some = __ballot(v > 0.0);
-    const int at = past ? __builtin_ctzll(past) : some ? 63 - __builtin_clzll(some) : -1;
-    if (at >= 0) {
-      last = c0 + at;
-      last_before = read_lane(upto - v, at);
-      if (past) break;
-    }
-    run = read_lane(upto, 63);
-  }
-  *before = last_before;
-  return last;
-}
-
-// The first token of a piece whose running sum, from `before` on, passes `goal`; the last one of any weight if none does.
-template <typename T, typename Weight>
-__device__ __forceinline__ int pick_token(int piece, double before, double goal, int lane, const Weight& weight_of) {
-  constexpr int PER = PieceOf<T>::PER, VECTORS = PieceOf<T>::VECTORS;
-  int found = -1, last = -1;
-#pragma unroll
-  for (int k = 0; k < VECTORS; ++k) {
-    if (found >= 0) continue;
-    double v[PER], sum = 0.0;
-#pragma unroll
-    for (int e = 0; e < PER; ++e) v[e] = weight_of(k, e), sum += v[e];
-    const double upto = before + wave_scan(sum, lane);
-    double run = upto - sum;
-    int hit = -1, any = -1;
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      run += v[e];
-      if (v[e] > 0.0) {
-        any = e;
-        if (hit < 0 && run > goal) hit = e;
-      }
-    }
-    // what passes by the scan's sum passes here, where the lane's own may be short of it by a last bit
-    if (hit < 0 && any >= 0 && upto > goal) hit = any;
-    const uint64_t past = __ballot(hit >= 0), some = __ballot(any >= 0);
-    const int base = piece * kPiece + 64 * k * PER;
-    if (past) {
-      const int at = __builtin_ctzll(past);
-      found = base + at * PER + __builtin_amdgcn_readlane(hit, at);
-    }
-    if (some) {
-      const int at = 63 - __builtin_clzll(some);
-      last = base + at * PER + __builtin_amdgcn_readlane(any, at);
-    }
-    before = read_lane(upto, 63);
-  }
-  return found >= 0 ? found : last;
-}
-
-// The sequence's answer: the accepted nodes (a bit for each), the new token.  A wave's work.
-__device__ __forceinline__ void answer(const VerifyParams& p, int row, const Tree& t, uint64_t taken, int token, int lane) {
+// The sequence's answer: the accepted nodes (a bit for each), and the new token.  id: of node `lane`.  A wave's work.
+__device__ __forceinline__ void answer(const VerifyParams& p, int row, uint64_t taken, int id, int token, int lane) {
   const int count = __builtin_popcountll(taken);
   int32_t* const path = p.path + (int64_t)row * p.max_new;
   int32_t* const out = p.out + (int64_t)row * p.max_new;
   const int place = __builtin_popcountll(taken & ((1ull << lane) - 1));
   const bool mine = taken >> lane & 1;
   if (mine) path[place] = lane;
-  if (mine && place > 0) out[place - 1] = p.ids[t.from + lane];
+  if (mine && place > 0) out[place - 1] = id;
   if (lane == 0 && count > 0) out[count - 1] = token;
   for (int i = count + lane; i < p.max_new; i += 64) path[i] = -1, out[i] = -1;
   if (lane == 0) p.accepted[row] = count;
 }
 
+// The piece of a row that `u` of its whole falls into: the first one whose running sum passes that, the last one of any
+// weight if none does, -1 without any.  load(i) gives piece i, weighed against its own maximum, or, WEIGHED,
+// against the row's.  A lane has `each` pieces that follow each other.
+struct Picked {
+  int piece;
+  float top;             // of the row
+  double whole, before;  // sums of the row, and of the pieces before
+};
+template <bool WEIGHED, typename Load>
+__device__ __forceinline__ Picked pick_piece(int pieces, double u, double k, int lane, const Load& load) {
+  const int each = (pieces + 63) / 64;
+  Picked r = {-1, -__builtin_inff(), 0.0, 0.0};
+  Piece v = {0.0, -__builtin_inff(), 0};
+  if constexpr (!WEIGHED) {
+    for (int i = 0; i < each; ++i)
+      if (lane * each + i < pieces) v = load(lane * each + i), r.top = fmaxf(r.top, v.top);
+    r.top = wave_max<32>(r.top);
+  }
+  const auto sum_of = [&](int i) {
+    if (lane * each + i >= pieces) return 0.0;
+    if (WEIGHED || each > 1) v = load(lane * each + i);
+    return WEIGHED || v.sum != v.sum ? v.sum : v.sum * weight(v.top, r.top, k);
+  };
+  double mine = 0.0;
+  for (int i = 0; i < each; ++i) mine += sum_of(i);
+  const double upto = wave_scan(mine, lane);
+  r.whole = read_lane(upto, 63);
+  const double goal = u * r.whole;
+  const uint64_t past = __ballot(upto > goal && mine > 0.0), some = __ballot(mine > 0.0);
+  if (!some) return r;
+  const int at = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+  double run = upto - mine, before = run;
+  int hit = -1;
+  if (each == 1) {
+    hit = 0;
+  } else {
+    bool found = false;
+    for (int i = 0; i < each; ++i) {
+      const double w = sum_of(i);
+      if (!found && w > 0.0) hit = i, before = run, found = run + w > goal;
+      run += w;
+    }
+  }
+  r.piece = at * each + __builtin_amdgcn_readlane(hit, at), r.before = read_lane(before, at);
+  return r;
+}
+
+// The place in its piece of the first number whose running sum, from `before` on, passes `goal`; the last one of any weight if
+// none does; -1 without any.  A work-group's work: each wave has a share of the piece, or nothing, a lane N consecutive numbers.
+template <int N>
+__device__ __forceinline__ int pick_number(const double (&w)[N], double before, double goal, int lane, int wave) {
+  __shared__ double s_sum[kWaves];
+  __shared__ int2 s_hit[kWaves];  // the first number past the goal, the last of any weight
+  double sum = 0.0;
+  int any = -1;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    sum += w[i];
+    if (w[i] > 0.0) any = i;
+  }
+  const double scan = wave_scan(sum, lane);
+  if (lane == 63) s_sum[wave] = scan;
+  __syncthreads();
+  for (int i = 0; i < wave; ++i) before += s_sum[i];
+  const double upto = before + scan;
+  double run = upto - sum;
+  int hit = -1;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    run += w[i];
+    if (hit < 0 && w[i] > 0.0 && run > goal) hit = i;
+  }
+  // the lane's own sum may be short of the scan's by a last bit
+  if (hit < 0 && any >= 0 && upto > goal) hit = any;
+  const uint64_t past = __ballot(hit >= 0), some = __ballot(any >= 0);
+  if (lane == 0) s_hit[wave] = make_int2(-1, -1);
+  if (past && lane == __builtin_ctzll(past)) s_hit[wave].x = wave * kShare + lane * N + hit;
+  if (some && lane == 63 - __builtin_clzll(some)) s_hit[wave].y = wave * kShare + lane * N + any;
+  __syncthreads();
+  int at = -1;
+  for (int i = 0; i < kWaves; ++i)
+    if (s_hit[i].y >= 0) at = s_hit[i].y;
+  for (int i = kWaves - 1; i >= 0; --i)
+    if (s_hit[i].x >= 0) at = s_hit[i].x;
+  return at;
+}
+
+__device__ __forceinline__ Piece load_piece(const Piece* at) {
+  Piece v;
+  v.sum = __builtin_bit_cast(double, hand_load((const uint64_t*)at));
+  const uint64_t b = hand_load((const uint64_t*)at + 1);
+  v.top = as_float((uint32_t)b), v.at = (int32_t)(b >> 32);
+  return v;
+}
+__device__ __forceinline__ void store_piece(Piece* at, const Piece& v) {
+  hand_store((uint64_t*)at, __builtin_bit_cast(uint64_t, v.sum));
+  hand_store((uint64_t*)at + 1, (uint64_t)(uint32_t)v.at << 32 | __builtin_bit_cast(uint32_t, v.top));
+}
+
+// A row's maximum, the sum of its weights against it and the place of the first maximum, from its pieces, by a segment of
+// `seg` lanes (16, 32 or 64), each of which gets them.
+struct Row {
+  double total;
+  float top;
+  int32_t at;
+};
+template <typename Load>
+__device__ __forceinline__ Row row_of(int pieces, double k, int seg, int lane, const Load& load) {
+  Row r = {0.0, -__builtin_inff(), 0x7fffffff};
+  const int sub = lane & (seg - 1);
+  Piece v = {0.0, -__builtin_inff(), 0x7fffffff};
+  for (int c = sub; c < pieces; c += seg) {
+    v = load(c);
+    r.top = fmaxf(r.top, v.top);
+  }
+  if (seg > 32) r.top = fmaxf(r.top, lane_xor<32>(r.top));
+  if (seg > 16) r.top = fmaxf(r.top, lane_xor<16>(r.top));
+  r.top = wave_max<8>(r.top);
+  for (int c = sub; c < pieces; c += seg) {
+    if (pieces > seg) v = load(c);
+    if (v.top == r.top && v.at < r.at) r.at = v.at;
+    r.total += v.sum == v.sum ? v.sum * weight(v.top, r.top, k) : v.sum;
+  }
+  const auto join = [&](double total, int32_t at) { r.total += total, r.at = at < r.at ? at : r.at; };
+  if (seg > 32) join(lane_xor64<32>(r.total), (int32_t)lane_xor<32>((uint32_t)r.at));
+  if (seg > 16) join(lane_xor64<16>(r.total), (int32_t)lane_xor<16>((uint32_t)r.at));
+  r.total = wave_sum<8>(r.total), r.at = wave_min<8>(r.at);
+  return r;
+}
+
 template <typename T>
-__global__ __launch_bounds__(64 * kWaves) void bsg_verify_rows_kernel(VerifyParams p) {
+__global__ __launch_bounds__(64 * kWaves) void bsg_verify_walk_kernel(VerifyParams p) {
+  constexpr int PER = PieceOf<T>::PER, N = ShareOf<T>::N;
   __shared__ double s_total[2][BSG_TREE_NODES];
   __shared__ float s_top[2][BSG_TREE_NODES];
   __shared__ int32_t s_at[BSG_TREE_NODES];
   __shared__ uint32_t s_last;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int which = blockIdx.x / p.groups, group = blockIdx.x - which * p.groups;
-  const int node = blockIdx.y, row = blockIdx.z;
+  const int row = blockIdx.y, group = blockIdx.x;
   const Tree t = tree_of(p, row, lane);
-  if (node >= t.count) {
-    if (t.count == 0 && node == 0 && blockIdx.x == 0 && wave == 0) answer(p, row, t, 0, -1, lane);
+  if (t.count == 0) {
+    if (group == 0 && wave == 0) answer(p, row, 0, -1, -1, lane);
     return;
   }
-  const bool greedy = !(t.temperature > 0.f);
+  const bool greedy = !(t.temperature > 0.f), drafts = p.drafts != 0 && !greedy;
   const double k = greedy ? 1.0 : kLog2e / (double)t.temperature;
-  const int piece = group * kWaves + wave;
-  if (piece < p.pieces && !(greedy && which)) {
-    PieceOf<T> x;
-    x.load(p.x[which], (t.from + node) * p.stride[which], p.vocab, piece, lane);
-    float top = -__builtin_inff();
-    bool bad = false;
-#pragma unroll
-    for (int v = 0; v < PieceOf<T>::VECTORS; ++v)
-#pragma unroll
-      for (int e = 0; e < PieceOf<T>::PER; ++e) {
-        const float y = x.get(v, e);
-        top = fmaxf(top, y);
-        bad = bad || !(y < __builtin_inff());
-      }
-    top = wave_max<32>(top);
-    Piece mine = {0.0, top, 0x7fffffff};
-    if (greedy) {
-#pragma unroll
-      for (int v = PieceOf<T>::VECTORS - 1; v >= 0; --v)
-#pragma unroll
-        for (int e = PieceOf<T>::PER - 1; e >= 0; --e)
-          if (x.get(v, e) == top) mine.at = piece * kPiece + (64 * v + lane) * PieceOf<T>::PER + e;
-      mine.at = wave_min<32>(mine.at);
-    } else if (top > -__builtin_inff()) {
-#pragma unroll
-      for (int v = 0; v < PieceOf<T>::VECTORS; ++v)
-#pragma unroll
-        for (int e = 0; e < PieceOf<T>::PER; ++e) mine.sum += exp2_64(((double)x.get(v, e) - (double)top) * k);
-      mine.sum = wave_sum<32>(mine.sum);
-    }
-    if (__any(bad)) mine.sum = __builtin_nan("");
-    if (lane == 0) {
-      uint64_t* const at = (uint64_t*)(piece_at(p, t.from + node, which) + piece);
-      hand_store(at, __builtin_bit_cast(uint64_t, mine.sum));
-      hand_store(at + 1, (uint64_t)(uint32_t)mine.at << 32 | __builtin_bit_cast(uint32_t, mine.top));
-    }
-  }
-  hand_publish();
-  __syncthreads();
-  const uint32_t arrivals = (uint32_t)t.count * p.groups * (1 + p.drafts);
-  if (threadIdx.x == 0) s_last = hand_arrive(p.counters + row) == arrivals - 1;
-  __syncthreads();
-  if (!s_last) return;
-  if (threadIdx.x == 0) hand_reset(p.counters + row);
-
-  // this work-group has the sequence: its rows' maxima and sums
-  const bool drafts = p.drafts != 0 && !greedy;
-  for (int r = wave; r < (drafts ? 2 * t.count : t.count); r += kWaves) {
-    const int w = r >= t.count, i = w ? r - t.count : r;
-    const Row v = row_of(piece_at(p, t.from + i, w), p.pieces, k, lane);
-    if (lane == 0) {
-      s_total[w][i] = v.total, s_top[w][i] = v.top;
-      if (!w) s_at[i] = v.at;
-    }
-  }
-  __syncthreads();
-  if (wave != 0) return;
-
-  // node `lane`: its token's weight in its parent's row, and in the drafts'
-  const int up = t.parent < 0 ? 0 : t.parent;
+  // node `lane`: its token, its number, and the token's logits in its parent's rows
   const int id = lane < t.count ? p.ids[t.from + lane] : -1;
   const double u = lane < t.count ? (double)p.uniforms[t.from + lane] : 0.0;
-  const bool child = t.parent >= 0, known = child && id >= 0 && id < p.vocab;
+  const int up = t.parent < 0 ? 0 : t.parent;
+  const bool known = t.parent >= 0 && id >= 0 && id < p.vocab;
+  float x0 = 0.f, x1 = 0.f;
+  if (known && !greedy) {
+    x0 = Logit<T>::one(p.x[0], (t.from + up) * p.stride[0] + id);
+    if (drafts) x1 = Logit<T>::one(p.x[1], (t.from + up) * p.stride[1] + id);
+  }
+
+  const uint64_t inner = inner_of(t);
+  const auto stats = [&](int node, int which) { return p.stats + ((t.from + node) * (1 + p.drafts) + which) * p.pieces; };
+  {
+    const int seg = p.pieces <= 16 ? 16 : p.pieces <= 32 ? 32 : 64, each = 64 / seg;
+    const int rows = __builtin_popcountll(inner);
+    for (int i0 = wave * each; i0 < (drafts ? 2 * rows : rows); i0 += kWaves * each) {
+      const int i = i0 + lane / seg, which = i >= rows;
+      // the (i or i - rows)-th of the nodes that have children
+      int nth = which ? i - rows : i, node = 0;
+      for (uint64_t m = inner; m && nth >= 0; m &= m - 1, --nth) node = __builtin_ctzll(m);
+      const bool on = i < (drafts ? 2 * rows : rows);
+      const Piece* const at = stats(on ? node : __builtin_ctzll(inner), on ? which : 0);
+      const Row r = row_of(p.pieces, k, seg, lane, [&](int c) { return at[c]; });
+      if (on && (lane & (seg - 1)) == 0) {
+        s_total[which][node] = r.total, s_top[which][node] = r.top;
+        if (!which) s_at[node] = r.at;
+      }
+    }
+  }
+  __syncthreads();
+
+  // Of a node's row, against its maximum: by each wave for itself, seldom.
+  const auto exact_total = [&](int node) {
+    const int64_t from = (t.from + node) * p.stride[0];
+    const int off = shift_of<T>(p.x[0], from);
+    double sum = 0.0;
+#pragma unroll 1
+    for (int c = 0; c < p.pieces; ++c) {
+      PieceOf<T> x;
+      x.load(p.x[0], from, p.vocab, off, c, lane);
+      x.each([&](int, u32x4& v) {
+#pragma unroll
+        for (int e = 0; e < PER; ++e) sum += weight(Logit<T>::of(v, e), s_top[0][node], k);
+      });
+    }
+    return wave_sum<32>(sum);
+  };
+
+  // every wave walks
   double mine = 0.0, theirs = 0.0;
   if (known && !greedy) {
-    mine = weight(Logit<T>::one(p.x[0], (t.from + up) * p.stride[0] + id), s_top[0][up], k);
-    if (drafts) {
-      mine /= s_total[0][up];
-      theirs = weight(Logit<T>::one(p.x[1], (t.from + up) * p.stride[1] + id), s_top[1][up], k) / s_total[1][up];
-    }
+    mine = weight(x0, s_top[0][up], k);
+    if (drafts) mine /= s_total[0][up], theirs = weight(x1, s_top[1][up], k) / s_total[1][up];
   }
   int at = 0;
   uint64_t taken = 1, refused = 0;  // refused: the rejected children of `at`, of each token one
   double out = 0.0;                 // their weights
+  double total = inner != 0 ? s_total[0][0] : 0.0;
+  bool exact = drafts;              // total is
   for (uint64_t left = ~1ull;;) {
-    const uint64_t asked = left & __ballot(child && t.parent == at);
+    const uint64_t asked = left & __ballot(t.parent >= 0 && t.parent == at);
     if (!asked) break;
     const int j = __builtin_ctzll(asked);
     left = j == 63 ? 0 : left & ~0ull << (j + 1);
     const bool same = (refused & __ballot(id == __builtin_amdgcn_readlane(id, j))) != 0;  // has no weight left
-    const bool ok = greedy ? id == s_at[at] && s_total[0][at] == s_total[0][at] : drafts ? u * theirs < mine : u * (s_total[0][at] - out) < mine;
-    if (!same && (__ballot(ok && known) >> j & 1) != 0) {
+    const double u_j = read_lane(u, j), w_j = read_lane(mine, j);
+    bool ok = (__ballot(known) >> j & 1) != 0 && !same;
+    if (greedy) {
+      ok = ok && __builtin_amdgcn_readlane(id, j) == s_at[at] && total == total;
+    } else if (drafts) {
+      ok = ok && u_j * read_lane(theirs, j) < w_j;
+    } else if (ok) {
+      if (!exact && __builtin_fabs(u_j * (total - out) - w_j) <= kNear * total * u_j) {
+        total = exact_total(at), exact = true;
+      }
+      ok = u_j * (total - out) < w_j;
+    }
+    if (ok) {
       at = j, taken |= 1ull << j, refused = 0, out = 0.0;
+      total = inner >> j & 1 ? s_total[0][j] : 0.0, exact = drafts;
     } else if (!same) {
-      refused |= 1ull << j, out += read_lane(mine, j);
+      refused |= 1ull << j, out += w_j;
     }
   }
 
-  // the new token
-  const double total = s_total[0][at];
-  const float top = s_top[0][at];
-  const bool residual = drafts && refused != 0;
-  int token = -1;
-  if (greedy) {
-    if (total == total && top > -__builtin_inff()) token = s_at[at];
-  } else if (total > 0.0 && !residual) {
-    // what is left of the row: the rejected tokens' weights go out of their pieces
-    double rest = total - out;
-    if (!(rest > 0.0)) rest = total, refused = 0;
-    const double goal = read_lane(u, 0) * rest;
-    const Piece* const pieces = piece_at(p, t.from + at, 0);
-    double before;
-    const int c = pick_piece(p.pieces, goal, lane, &before, [&](int i) {
-      const Piece v = load_piece(pieces + i);
-      double sum = v.sum * weight(v.top, top, k);
-      for (uint64_t m = refused; m; m &= m - 1) {
-        const int j = __builtin_ctzll(m), gone = __builtin_amdgcn_readlane(id, j);
-        if (gone >= 0 && gone / kPiece == i) sum -= read_lane(mine, j);
-      }
-      return sum;
-    });
-    if (c >= 0) {
-      PieceOf<T> x;
-      x.load(p.x[0], (t.from + at) * p.stride[0], p.vocab, c, lane);
-      uint32_t gone = 0;  // of the lane's numbers, as bits
-      for (uint64_t m = refused; m; m &= m - 1) {
-        const int off = __builtin_amdgcn_readlane(id, __builtin_ctzll(m)) - c * kPiece;
-        if (off >= 0 && off < kPiece && off / PieceOf<T>::PER % 64 == lane)
-          gone |= 1u << (off / PieceOf<T>::PER / 64 * PieceOf<T>::PER + off % PieceOf<T>::PER);
-      }
-      token = pick_token<T>(c, before, goal, lane, [&](int v, int e) {
-        return gone >> (v * PieceOf<T>::PER + e) & 1 ? 0.0 : weight(x.get(v, e), top, k);
-      });
-    }
+  const bool leaf = (inner >> at & 1) == 0, residual = drafts && refused != 0;
+  float top = leaf ? 0.f : s_top[0][at];
+  // known by now: greedy of a row that the first launch had; none of a row that has no probabilities
+  if (!leaf && (greedy || !(total > 0.0))) {
+    const bool some = greedy && total == total && top > -__builtin_inff();
+    if (group == 0 && wave == 0) answer(p, row, taken, id, some ? s_at[at] : -1, lane);
+    return;
   }
-  answer(p, row, t, taken, token, lane);
-  if (p.drafts && lane == 0) {
-    Verdict v;
-    v.total[0] = total, v.total[1] = s_total[1][at];
-    v.top[0] = top, v.top[1] = s_top[1][at];
-    v.node = at, v.count = __builtin_popcountll(taken), v.residual = residual && total > 0.0, v.pad = 0;
-    p.verdicts[row] = v;
-  }
-}
 
-// The new token of the sequences whose last row's child was rejected, from max(p - q, 0); from p where nothing is left.
-template <typename T>
-__global__ __launch_bounds__(64 * kWaves) void bsg_verify_residual_kernel(VerifyParams p) {
-  __shared__ uint32_t s_last;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int row = blockIdx.y;
-  const Tree t = tree_of(p, row, lane);
-  if (t.count == 0 || !(t.temperature > 0.f)) return;
-  const Verdict v = p.verdicts[row];
-  if (!v.residual) return;
-  const double k = kLog2e / (double)t.temperature;
-  const double by[2] = {1.0 / v.total[0], 1.0 / v.total[1]};
-  const int64_t at[2] = {(t.from + v.node) * p.stride[0], (t.from + v.node) * p.stride[1]};
-  double* const left = p.left + (int64_t)row * p.pieces;
-  const auto of = [&](const PieceOf<T>& x, const PieceOf<T>& y, int i, int e) {
-    const double d = weight(x.get(i, e), v.top[0], k) * by[0] - weight(y.get(i, e), v.top[1], k) * by[1];
-    return d > 0.0 ? d : 0.0;
-  };
-  PieceOf<T> x, y;
-  const int piece = blockIdx.x * kWaves + wave;
+  // what is left of the last row: the row without the rejected tokens, or what it has over its drafts
+  const int64_t x_at = (t.from + at) * p.stride[0], y_at = (t.from + at) * p.stride[1];
+  const int shift = shift_of<T>(p.x[0], x_at);
+  const double by[2] = {1.0 / total, residual ? 1.0 / s_total[1][at] : 0.0};
+  const float y_top = residual ? s_top[1][at] : 0.f;
+  const auto surplus = [&](double x, double y) { return __builtin_fmax(x * by[0] - y * by[1], 0.0); };
+  Piece* const last = p.last + (int64_t)row * p.pieces;
+  const int piece = group * kWaves + wave;
   if (piece < p.pieces) {
-    x.load(p.x[0], at[0], p.vocab, piece, lane);
-    y.load(p.x[1], at[1], p.vocab, piece, lane);
-    double sum = 0.0;
+    PieceOf<T> x;
+    x.load(p.x[0], x_at, p.vocab, shift, piece, lane);
+    Piece v = {0.0, 0.f, 0};
+    if (residual) {
+      PieceOf<T> y;
+      y.load(p.x[1], y_at, p.vocab, shift, piece, lane);
+      x.each([&](int, u32x4& a) {
+        const u32x4 b = y.v[0];
 #pragma unroll
-    for (int i = 0; i < PieceOf<T>::VECTORS; ++i)
+        for (int e = 0; e < PER; ++e) v.sum += surplus(weight(Logit<T>::of(a, e), top, k), weight(Logit<T>::of(b, e), y_top, k));
 #pragma unroll
-      for (int e = 0; e < PieceOf<T>::PER; ++e) sum += of(x, y, i, e);
-    sum = wave_sum<32>(sum);
-    if (lane == 0) hand_store((uint64_t*)left + piece, __builtin_bit_cast(uint64_t, sum));
+        for (int i = 0; i + 1 < PieceOf<T>::VECTORS; ++i) y.v[i] = y.v[i + 1];
+      });
+      v.sum = wave_sum<32>(v.sum);
+    } else {
+      for (uint64_t m = refused; m; m &= m - 1) x.drop(__builtin_amdgcn_readlane(id, __builtin_ctzll(m)), shift, piece, lane);
+      v = piece_of<T>(x, greedy, true, k, piece * kPiece - shift, lane);
+    }
+    if (lane == 0) store_piece(last + piece, v);
   }
   hand_publish();
   __syncthreads();
@@ -481,41 +600,57 @@ __global__ __launch_bounds__(64 * kWaves) void bsg_verify_residual_kernel(Verify
   __syncthreads();
   if (!s_last) return;
   if (threadIdx.x == 0) hand_reset(p.counters + row);
-  if (wave != 0) return;
 
-  double total = 0.0;
-  for (int c = lane; c < p.pieces; c += 64) total += __builtin_bit_cast(double, hand_load((const uint64_t*)left + c));
-  total = wave_sum<32>(total);
-  const bool some = total > 0.0;
-  const Piece* const pieces = piece_at(p, t.from + v.node, 0);
-  const double goal = (double)p.uniforms[t.from] * (some ? total : v.total[0]);
-  double before;
-  const int c = pick_piece(p.pieces, goal, lane, &before, [&](int i) {
-    if (some) return __builtin_bit_cast(double, hand_load((const uint64_t*)left + i));
-    const Piece w = load_piece(pieces + i);
-    return w.sum * weight(w.top, v.top[0], k);
-  });
   int token = -1;
-  if (c >= 0) {
-    x.load(p.x[0], at[0], p.vocab, c, lane);
-    y.load(p.x[1], at[1], p.vocab, c, lane);
-    token = pick_token<T>(c, before, goal, lane, [&](int i, int e) {
-      return some ? of(x, y, i, e) : weight(x.get(i, e), v.top[0], k);
-    });
+  if (greedy) {
+    const Row r = row_of(p.pieces, k, 64, lane, [&](int c) { return load_piece(last + c); });
+    if (r.total == r.total && r.top > -__builtin_inff()) token = r.at;
+  } else {
+    const double draw = read_lane(u, 0);
+    bool over = residual;  // something is left of the row over its drafts; else from the row
+    Picked c;
+    if (residual) c = pick_piece<true>(p.pieces, draw, k, lane, [&](int i) { return load_piece(last + i); });
+    over = residual && c.whole > 0.0;
+    if (!over) {
+      const Piece* const own = stats(at, 0);
+      c = pick_piece<false>(p.pieces, draw, k, lane, [&](int i) { return residual ? own[i] : load_piece(last + i); });
+      top = c.top;
+    }
+    if (c.whole > 0.0) {
+      double w[N];
+      const int first = c.piece * kPiece + wave * kShare - shift;
+      if (wave < kPiece / kShare) {
+        ShareOf<T> x, y;
+        x.load(p.x[0], x_at, p.vocab, shift, first, lane);
+        if (over) y.load(p.x[1], y_at, p.vocab, shift, first, lane);
+        if (!residual)
+          for (uint64_t m = refused; m; m &= m - 1) x.drop(__builtin_amdgcn_readlane(id, __builtin_ctzll(m)), first, lane);
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = weight(x.get(i), top, k);
+        if (over) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) w[i] = surplus(w[i], weight(y.get(i), y_top, k));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = 0.0;
+      }
+      const int in_piece = pick_number(w, c.before, draw * c.whole, lane, wave);
+      if (in_piece >= 0) token = in_piece + c.piece * kPiece - shift;
+    }
   }
-  if (lane == 0) p.out[(int64_t)row * p.max_new + v.count - 1] = token;
+  if (wave == 0) answer(p, row, taken, id, token, lane);
 }
 
 struct Layout {
-  int64_t pieces, verdicts, stats, left, bytes;  // of a row; where they lie in the workspace
+  int64_t pieces, stats, last, bytes;  // of a row; where they lie in the workspace
 };
 Layout layout_of(int64_t tokens, int32_t rows, int64_t vocab, int32_t drafts) {
   Layout l;
-  l.pieces = ceil_div(vocab, kPiece);
-  l.verdicts = BSG_KV_COUNTER_BYTES;
-  l.stats = l.verdicts + ceil_div((drafts ? rows : 0) * (int64_t)sizeof(Verdict), 256) * 256;
-  l.left = l.stats + tokens * (1 + drafts) * l.pieces * (int64_t)sizeof(Piece);
-  l.bytes = l.left + (drafts ? rows * l.pieces * 8 : 0);
+  l.pieces = ceil_div(vocab + 7, kPiece);  // with up to 7 numbers of the first granule before the row
+  l.stats = BSG_KV_COUNTER_BYTES;
+  l.last = l.stats + tokens * (1 + drafts) * l.pieces * (int64_t)sizeof(Piece);
+  l.bytes = l.last + rows * l.pieces * (int64_t)sizeof(Piece);
   return l;
 }
 
@@ -524,17 +659,20 @@ int check_sizes(int64_t tokens, int32_t rows, int64_t vocab, int32_t max_new, in
   if (tokens < 0 || rows < 0 || vocab < 1 || max_new < 0 || tokens > 0x7fffffff)
     return fail(BSG_ERR_ARG, "tokens=%lld rows=%d vocab=%lld max_new=%d", (long long)tokens, rows, (long long)vocab, max_new);
   if (max_new > BSG_TREE_NODES) return fail(BSG_ERR_UNSUPPORTED, "%d nodes in a tree (at most %d)", max_new, BSG_TREE_NODES);
-  if (vocab > (int64_t)kMostPieces * kPiece) return fail(BSG_ERR_UNSUPPORTED, "vocab=%lld (at most %d)", (long long)vocab, kMostPieces * kPiece);
+  if (vocab > kMostVocab) return fail(BSG_ERR_UNSUPPORTED, "vocab=%lld (at most %d)", (long long)vocab, kMostVocab);
   if (rows > BSG_KV_COUNTER_BYTES / 4) return fail(BSG_ERR_UNSUPPORTED, "%d sequences (at most %d)", rows, BSG_KV_COUNTER_BYTES / 4);
   return BSG_OK;
 }
 
 template <typename T>
 void launch(const VerifyParams& p, hipStream_t st) {
-  const dim3 grid((unsigned)(p.groups * (1 + p.drafts)), (unsigned)p.max_new, (unsigned)p.rows);
-  hipLaunchKernelGGL((bsg_verify_rows_kernel<T>), grid, dim3(64 * kWaves), 0, st, p);
-  if (p.drafts)
-    hipLaunchKernelGGL((bsg_verify_residual_kernel<T>), dim3((unsigned)p.groups, (unsigned)p.rows), dim3(64 * kWaves), 0, st, p);
+  if (p.max_new > 1) {  // else no node has children
+    // most of a large tree's nodes have no children, and their work-groups would only come and go
+    const int at_once = p.max_new <= 8 ? p.max_new - 1 : p.max_new / 2;
+    const dim3 grid((unsigned)(p.groups * (1 + p.drafts)), (unsigned)at_once, (unsigned)p.rows);
+    hipLaunchKernelGGL((bsg_verify_rows_kernel<T>), grid, dim3(64 * kWaves), 0, st, p);
+  }
+  hipLaunchKernelGGL((bsg_verify_walk_kernel<T>), dim3((unsigned)p.groups, (unsigned)p.rows), dim3(64 * kWaves), 0, st, p);
 }
 
 }  // namespace
@@ -579,9 +717,8 @@ extern "C" int bsg_verify_drafts(const void* logits, int64_t logits_stride, cons
   p.pieces = (int32_t)l.pieces, p.groups = (int32_t)ceil_div(l.pieces, kWaves);
   p.accepted = accepted, p.path = path, p.out = out_tokens;
   p.counters = (uint32_t*)ws;
-  p.verdicts = (Verdict*)((uint8_t*)ws + l.verdicts);
   p.stats = (Piece*)((uint8_t*)ws + l.stats);
-  p.left = (double*)((uint8_t*)ws + l.left);
+  p.last = (Piece*)((uint8_t*)ws + l.last);
   const hipStream_t st = (hipStream_t)stream;
   switch (dtype) {
     case BSG_F16: launch<_Float16>(p, st); break;
