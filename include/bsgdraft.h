@@ -99,10 +99,13 @@ int bsg_verify_drafts(const void* logits, int64_t logits_stride, const void* dra
  *   pool   : page_bytes = 2 n_heads page_size head_dim and page_scales = 2 n_heads, as bsg_kv_cache
  *   path   : int32 [rows][max_new]
  * Slots must be distinct and the pages of the new tokens a sequence's own; a slot out of range, or of fewer than n
- * tokens, is left as it is.  max_new <= BSG_TREE_NODES, rows <= BSG_PAGES_MAX_ROWS. */
+ * tokens, is left as it is.  max_new <= BSG_TREE_NODES, rows <= BSG_PAGES_MAX_ROWS.  Workspace:
+ * bsg_pages_keep_workspace_bytes(rows), no initialisation; as in bsg_pages_extend the first of two launches leaves the second
+ * its plan there, so threads that share a stream need one each. */
+int64_t bsg_pages_keep_workspace_bytes(int32_t rows);
 int bsg_pages_keep(const bsg_page_pool* pool, int32_t n_heads, int32_t head_dim, const int32_t* path,
                    const int32_t* accepted, const int32_t* cu, const int32_t* slots, int32_t rows, int32_t max_new,
-                   void* stream);
+                   void* ws, int64_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -27,7 +27,7 @@ UNITS = ("kv_rotate.hip", "kv_tree.hip", "verify.hip", "pages_keep.hip")
 def test_header_and_library_agree(tmp_path):
     text = re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
     names = set(re.findall(r"\b(bsg_[a-z0-9_]+)\s*\(", text))
-    assert len(names) == 6
+    assert len(names) == 7
     lib = bsa.load()
     for name in names:
         assert hasattr(lib, name) and name in _lib.SIGNATURES, name
@@ -152,8 +152,8 @@ def test_bad_verifications_are_refused():
 def test_bad_keeps_are_refused():
     lib = bsa.load()
 
-    def call(heads=2, d=64, path=FAKE, accepted=FAKE, slots=None, rows=4, max_new=8, **kw):
-        return lib.bsg_pages_keep(_pool(**kw), heads, d, path, accepted, None, slots, rows, max_new, None)
+    def call(heads=2, d=64, path=FAKE, accepted=FAKE, slots=None, rows=4, max_new=8, ws=FAKE, ws_bytes=1 << 30, **kw):
+        return lib.bsg_pages_keep(_pool(**kw), heads, d, path, accepted, None, slots, rows, max_new, ws, ws_bytes, None)
 
     # _pool is of 2 heads of 128
     ok = dict(d=128)
@@ -169,7 +169,12 @@ def test_bad_keeps_are_refused():
     assert call(**ok, max_new=65) == _lib.BSG_ERR_UNSUPPORTED
     over = dict(max_pages=(1 << 26) + 1, table_stride=(1 << 26) + 1)
     assert call(**ok, **over) == _lib.BSG_ERR_UNSUPPORTED
-    assert lib.bsg_pages_keep(None, 2, 128, FAKE, FAKE, None, None, 4, 8, None) == _lib.BSG_ERR_ARG
+    assert lib.bsg_pages_keep(None, 2, 128, FAKE, FAKE, None, None, 4, 8, FAKE, 1 << 30, None) == _lib.BSG_ERR_ARG
+    need = lib.bsg_pages_keep_workspace_bytes(4)
+    assert need > 0 and lib.bsg_pages_keep_workspace_bytes(1025) == -1
+    assert call(**ok, ws_bytes=need - 1) == _lib.BSG_ERR_WORKSPACE
+    assert call(**ok, ws=None) == _lib.BSG_ERR_WORKSPACE
+    assert call(**ok, ws=FAKE + 8) == _lib.BSG_ERR_ALIGN
 
 
 def test_python_layer_refuses_host_tensors():

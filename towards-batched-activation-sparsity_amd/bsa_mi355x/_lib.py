@@ -218,7 +218,8 @@ SIGNATURES = {
     "bsg_verify_drafts_workspace_bytes": (_i64, [_i64, _i32, _i64, _i32, _int, _i32]),
     "bsg_verify_drafts": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i32, _i32, _f32, _vp, _vp, _vp, _vp,
                                  _int, _vp, _i64, _vp]),
-    "bsg_pages_keep": (_int, [_ppool, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i32, _vp]),
+    "bsg_pages_keep_workspace_bytes": (_i64, [_i32]),
+    "bsg_pages_keep": (_int, [_ppool, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _i64, _vp]),
     # include/bsgemm_timeline.h
     "bsg_timeline_attach": (_int, [_vp, _i64, _i64]),
     "bsg_timeline_clock_khz": (_i64, []),

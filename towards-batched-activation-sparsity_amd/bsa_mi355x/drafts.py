@@ -25,8 +25,8 @@ import torch
 from . import _lib
 from ._lib import load
 from .runtime import _cu_count, _dtype_code, _require_cuda
-from .serving import (_CALLS, _LOGIT_DTYPES, _batch, _from_end, _i32, _launch, _layer, _mold, _ptr, _remember, _rows, _sigs, _storage,
-                      _table, _workspace)
+from .serving import (MAX_ROWS, _CALLS, _LOGIT_DTYPES, _batch, _from_end, _i32, _launch, _layer, _mold, _plan_workspace, _ptr, _remember,
+                      _rows, _sigs, _storage, _table, _workspace)
 
 MAX_NODES = 64  # BSG_TREE_NODES
 
@@ -274,7 +274,7 @@ def _verify_call(logits, tokens, uniforms, parents, draft_logits, temperatures, 
 
 def pages_keep(pages: torch.Tensor, scales: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
                refcounts: torch.Tensor, path: torch.Tensor, accepted: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None,
-               slots: Optional[torch.Tensor] = None) -> None:
+               slots: Optional[torch.Tensor] = None, workspace_prefix: Optional[str] = None) -> None:
     """What was accepted of a tree stays in the cache, in all layers of pages [layers, pages, heads, 2, page_size,
     head_dim]: of the newest tokens of row b (slot slots[b], or b), cu_seqlens[b + 1] - cu_seqlens[b] of them or as many
     as path has columns, those at the places path[b][:accepted[b]] (int32 [rows, places] and [rows], of verify_drafts) move
@@ -303,7 +303,11 @@ def pages_keep(pages: torch.Tensor, scales: torch.Tensor, page_table: torch.Tens
         _i32(cu_seqlens, dev, "cu_seqlens", rows + 1)
         _i32(slots, dev, "slots", rows)
         sizes = (layers, count, h * 2 * p * d, h * 2, p, n, each, page_table.stride(0) if n > 1 else each)
-        call = _remember(key, (dev.index, load().bsg_pages_keep, sizes, h, d, rows, most))
-    index, fn, sizes, h, d, rows, most = call
+        need = int(load().bsg_pages_keep_workspace_bytes(rows))
+        if need < 0:
+            raise ValueError(f"at most {MAX_ROWS} rows, got {rows}")
+        call = _remember(key, (dev.index, load().bsg_pages_keep, sizes, h, d, rows, most, need))
+    index, fn, sizes, h, d, rows, most, need = call
+    held, ws, room = _plan_workspace(index, need, workspace_prefix)  # held: till the launch
     pool = _lib.PagePool(pages.data_ptr(), scales.data_ptr(), *sizes, page_table.data_ptr(), lengths.data_ptr(), refcounts.data_ptr())
-    _launch(index, fn, pool, h, d, path.data_ptr(), accepted.data_ptr(), _ptr(cu_seqlens), _ptr(slots), rows, most)
+    _launch(index, fn, pool, h, d, path.data_ptr(), accepted.data_ptr(), _ptr(cu_seqlens), _ptr(slots), rows, most, ws, room)
