@@ -213,6 +213,22 @@ def test_rotated_edges(dev, case):
         assert (out.cpu()[torch.from_numpy(~mine)] == 7.0).all()  # nobody's rows
 
 
+@pytest.mark.parametrize("p,d", [(16, 64), (64, 128)])
+def test_rotated_magnitudes_past_every_scale(dev, p, d):
+    """bf16 numbers of 2^120 beside the largest scale, 2^80: the largest e4m3 number, with its sign, as kv_append."""
+    rng = np.random.default_rng(7)
+    lengths = [20, 5]
+    _, _, _, pages, scales, tab = _cache(rng, dev, lengths, 2, p, d)
+    pages2, scales2 = pages.view(torch.uint8).clone().view(F8), scales.clone()
+    q, k, v = (torch.randn(10, 2, d, device=dev).bfloat16() for _ in range(3))
+    k[2], v[3] = k[2] * 2.0 ** 120, v[3] * 2.0 ** 120
+    one, zero = torch.ones(30, d // 2, device=dev), torch.zeros(30, d // 2, device=dev)
+    bsa.kv_append_rotated(q, k, v, one, zero, pages, scales, tab, _i32(lengths, dev))
+    bsa.kv_append(k, v, pages2, scales2, tab, _i32(lengths, dev))
+    assert torch.equal(pages.view(torch.uint8), pages2.view(torch.uint8)) and torch.equal(scales, scales2)
+    assert float(scales.max()) == 2.0 ** 80 and not torch.isnan(pages.float()).any()
+
+
 def test_rotated_graph_and_streams(dev):
     """Captured and replayed with new inputs in the same tensors, and on another stream: the eager numbers."""
     rng = np.random.default_rng(5)

@@ -55,4 +55,43 @@ __device__ __forceinline__ float scale_for(float a) {
   return __builtin_bit_cast(float, (uint32_t)(c + 127) << 23);
 }
 
+// The largest finite magnitude in the wave.  Magnitudes of either 16-bit type order as their bits do; only where
+// infinities or NaN are among them are those taken out.
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+template <typename T>
+inline constexpr uint32_t kInfBits = 0x7c00u;
+template <>
+inline constexpr uint32_t kInfBits<__bf16> = 0x7f80u;
+
+template <int X>
+__device__ __forceinline__ u16x2 wave_max(u16x2 m) {
+  m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, lane_xor<X>(__builtin_bit_cast(uint32_t, m))));
+  if constexpr (X > 1) m = wave_max<X / 2>(m);
+  return m;
+}
+template <typename T, int C>
+__device__ __forceinline__ float largest_magnitude(const uint32_t x[C][8]) {
+  u16x2 m = {0, 0};
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, x[c][i] & 0x7fff7fffu));
+  m = wave_max<32>(m);
+  uint32_t top = m.x > m.y ? m.x : m.y;
+  if (top >= kInfBits<T>) {
+    m = u16x2{0, 0};
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t w = x[c][i] & 0x7fff7fffu;
+        const uint32_t lo = w & 0xffffu, hi = w >> 16;
+        m = __builtin_elementwise_max(m, u16x2{(unsigned short)(lo < kInfBits<T> ? lo : 0u), (unsigned short)(hi < kInfBits<T> ? hi : 0u)});
+      }
+    m = wave_max<32>(m);
+    top = m.x > m.y ? m.x : m.y;
+  }
+  return low_half<T>(top);
+}
+
 }  // namespace bsgk

@@ -5,11 +5,11 @@
 // pairs: (a, b) -> (a cos - b sin, a sin + b cos).  All of it is in 32 bits, of which the queries are rounded to their
 // type and the keys to e4m3 once.
 //
-// Two kinds of work-groups share a launch.  Those of the cache are kv_append.hip's: a wave a 16-token tile of a (page,
-// head, keys or values), lane 16 g + t with channels 64 c + 16 g .. +15 of token t, so that a pair's other half lies in the
+// Two kinds of work-groups share a launch.  Those of the cache are much like kv_append.hip's: a wave a 16-token tile of a (page,
+// head), keys and values, lane 16 g + t with channels 64 c + 16 g .. +15 of token t, so that a pair's other half lies in the
 // lane itself (R = 128: the other c; R = 16: 8 channels on; neighbours), or in lane ^ 32 or ^ 16 (R = 64, 32).  Those of
 // the queries take a row of D channels with D / 16 lanes, two runs of 8 channels each, chosen so that a pair's halves meet
-// in one lane: eight (D = 128) or sixteen rows a wave.
+// in one lane: eight (D = 128) or sixteen rows at a time, four times, with one load of a token's angles for its heads.
 
 #include "bsgdraft.h"
 #include "draft_tree.hpp"
@@ -69,15 +69,16 @@ __device__ __forceinline__ Sequence sequence(const RotateParams& p, int row, boo
   return s;
 }
 
+// Lane j: how deep node j of a sequence lies in its tree.  All lanes of the wave call it.
+__device__ __forceinline__ int depths(const RotateParams& p, const Sequence& s) {
+  const int lane = threadIdx.x & 63;
+  const int64_t n = s.to - s.from < kTreeNodes ? s.to - s.from : kTreeNodes;
+  return depth_of(load_parent(p.parents, s.from, s.fine ? (int)n : 0, lane), lane);
+}
 // By what position token i of a sequence turns.  All lanes of the wave call it.
-__device__ __forceinline__ int64_t turn_of(const RotateParams& p, const Sequence& s, int64_t i, bool on) {
+__device__ __forceinline__ int64_t turn_of(const RotateParams& p, const Sequence& s, int64_t i, bool on, int depth) {
   const int64_t start = s.len - (s.to - s.from);
-  if (p.parents) {
-    const int lane = threadIdx.x & 63;
-    const int64_t n = s.to - s.from < kTreeNodes ? s.to - s.from : kTreeNodes;
-    const int depth = depth_of(load_parent(p.parents, s.from, s.fine ? (int)n : 0, lane), lane);
-    return start + from_lane(depth, (int)i & 63);
-  }
+  if (p.parents) return start + from_lane(depth, (int)i & 63);
   if (p.turns) return on ? p.turns[s.from + i] : 0;
   return start + i;
 }
@@ -106,61 +107,60 @@ __device__ __forceinline__ uint32_t narrow<__bf16>(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
 }
 
-// cos and sin of N consecutive angles of a position; NaN where the table has no such position.
-template <int N>
-__device__ __forceinline__ void load_turn(const RotateParams& p, int64_t turn, int first, float* c, float* s) {
-  const bool there = turn >= 0 && turn < p.turn_count;
-  const float nan = __builtin_nanf("");
-  const int64_t at = (there ? turn : 0) * p.turn_stride + first;
+// cos and sin of eight angles of a position; NaN where the table has no such position.  Asked for in one place and looked
+// at in another, so that they are on their way beside what is turned.
+struct Angles {
+  f32x4 c[2], s[2];
+  bool there;
+  __device__ __forceinline__ void ask(const RotateParams& p, int64_t turn, int first) {
+    there = turn >= 0 && turn < p.turn_count;
+    const int64_t at = (there ? turn : 0) * p.turn_stride + first;
 #pragma unroll
-  for (int i = 0; i < N / 4; ++i) {
-    const f32x4 cv = *(const f32x4*)(p.cos + at + 4 * i), sv = *(const f32x4*)(p.sin + at + 4 * i);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c[4 * i + j] = there ? cv[j] : nan, s[4 * i + j] = there ? sv[j] : nan;
+    for (int i = 0; i < 2; ++i) c[i] = *(const f32x4*)(p.cos + at + 4 * i), s[i] = *(const f32x4*)(p.sin + at + 4 * i);
   }
-}
+  __device__ __forceinline__ float cos(int i) const { return there ? c[i / 4][i % 4] : __builtin_nanf(""); }
+  __device__ __forceinline__ float sin(int i) const { return there ? s[i / 4][i % 4] : __builtin_nanf(""); }
+};
 __device__ __forceinline__ void turn_pair(float& a, float& b, float c, float s) {
   const float x = a, y = b;
   a = x * c - y * s, b = x * s + y * c;
 }
 
-// A lane's channels 64 c + 16 g .. +15 of a key, turned.  All lanes of the wave call it.
-template <int C>
-__device__ __forceinline__ void turn_key(const RotateParams& p, int64_t turn, int g, float f[C][16]) {
+// A lane's channels 64 c + 16 g .. +15 of a key are turned by twice eight angles, the H-th of which key_angles names; they come
+// one after the other, for the registers (a wave more on each SIMD).  All lanes of the wave call it.
+__device__ __forceinline__ int key_angles(const RotateParams& p, int g, int H) {
+  const int R = p.dims, at = p.interleaved ? 8 * g + 32 * H : (R == 128 ? 16 * g : R == 64 ? 16 * (g & 1) : 0) + 8 * H;
+  return at < R / 2 ? at : 0;  // of channels that are not turned: any
+}
+template <int C, int H>
+__device__ __forceinline__ void turn_key(const RotateParams& p, const Angles& a, int g, float f[C][16]) {
   const int R = p.dims;
-  float c[16], s[16];
   if (p.interleaved) {
+    if (H < C && 64 * H + 16 * g < R) {
 #pragma unroll
-    for (int k = 0; k < C; ++k) {
-      if (64 * k + 16 * g >= R) continue;
-      load_turn<8>(p, turn, 32 * k + 8 * g, c, s);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) turn_pair(f[k][2 * i], f[k][2 * i + 1], c[i], s[i]);
+      for (int i = 0; i < 8; ++i) turn_pair(f[H < C ? H : 0][2 * i], f[H < C ? H : 0][2 * i + 1], a.cos(i), a.sin(i));
     }
-    return;
-  }
-  if (C == 2 && R == 128) {
-    load_turn<16>(p, turn, 16 * g, c, s);
+  } else if (C == 2 && R == 128) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) turn_pair(f[0][i], f[C - 1][i], c[i], s[i]);
+    for (int i = 0; i < 8; ++i) turn_pair(f[0][8 * H + i], f[C - 1][8 * H + i], a.cos(i), a.sin(i));
   } else if (R == 16) {
-    if (g != 0) return;
-    load_turn<8>(p, turn, 0, c, s);
+    if (H != 0 || g != 0) return;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) turn_pair(f[0][i], f[0][i + 8], c[i], s[i]);
+    for (int i = 0; i < 8; ++i) turn_pair(f[0][i], f[0][i + 8], a.cos(i), a.sin(i));
   } else {
     // the other half of a pair is lane ^ 32's (R = 64) or ^ 16's (R = 32) channel
     const bool second = R == 64 ? g >= 2 : g == 1, in = R == 64 || g < 2;
-    if (in) load_turn<16>(p, turn, R == 64 ? 16 * (g & 1) : 0, c, s);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float other = R == 64 ? lane_xor<32>(f[0][i]) : lane_xor<16>(f[0][i]);
-      if (in) f[0][i] = second ? other * s[i] + f[0][i] * c[i] : f[0][i] * c[i] - other * s[i];
+    for (int i = 0; i < 8; ++i) {
+      float& x = f[0][8 * H + i];
+      const float other = R == 64 ? lane_xor<32>(x) : lane_xor<16>(x);
+      if (in) x = second ? other * a.sin(i) + x * a.cos(i) : x * a.cos(i) - other * a.sin(i);
     }
   }
 }
 
-// The largest finite magnitude in the wave; only where an infinity is among them are those taken out.
+// The largest finite magnitude in the wave, and whether all of its numbers are finite.  Only where they are not are the
+// others looked at one by one.
 template <int X>
 __device__ __forceinline__ float wave_top(float m) {
   m = fmaxf(m, lane_xor<X>(m));
@@ -168,14 +168,15 @@ __device__ __forceinline__ float wave_top(float m) {
   return m;
 }
 template <int C>
-__device__ __forceinline__ float finite_top(const float f[C][16]) {
-  float m = 0.f;
+__device__ __forceinline__ float finite_top(const float f[C][16], bool* finite) {
+  float m = 0.f, none = 0.f;
 #pragma unroll
   for (int c = 0; c < C; ++c)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) m = fmaxf(m, __builtin_fabsf(f[c][i]));  // a NaN is no maximum
+    for (int i = 0; i < 16; ++i) m = fmaxf(m, __builtin_fabsf(f[c][i])), none = __builtin_fmaf(f[c][i], 0.f, none);
   m = wave_top<32>(m);
-  if (m == __builtin_inff()) {
+  *finite = !__any(none != 0.f);  // an infinity or NaN times 0 is NaN
+  if (!*finite) {
     m = 0.f;
 #pragma unroll
     for (int c = 0; c < C; ++c)
@@ -189,82 +190,124 @@ __device__ __forceinline__ float finite_top(const float f[C][16]) {
   return m;
 }
 
-// A wave's rows of queries.
+// A wave's rows of queries: kRows times as many as its lanes hold, since rows of one token, which follow each other, share
+// their angles and all share the norm.
+constexpr int kRows = 2;
 template <typename T, int D>
 __device__ __forceinline__ void turn_queries(const RotateParams& p, uint32_t unit) {
-  constexpr int L = D / 16, ROWS = 64 / L;  // lanes of a row, rows of a wave
+  constexpr int L = D / 16, ROWS = 64 / L;  // lanes of a row, rows of a wave at a time
   const int lane = threadIdx.x & 63, j = lane % L;
   const int row = unit / (uint32_t)p.per_row, nth = unit - row * p.per_row;
   const Sequence s = sequence(p, row, unit < (uint32_t)p.queries);
   const int64_t count = !s.fine ? 0 : s.to - s.from < p.max_new ? s.to - s.from : p.max_new;
-  const uint32_t r = nth * ROWS + lane / L, i = r / (uint32_t)p.q_heads;
-  const int head = r - i * p.q_heads;
-  const bool on = i < count;
-  if (!__any(on)) return;
-  const int64_t turn = turn_of(p, s, i, on);
-  if (!on) return;
+  const uint32_t first_row = nth * (kRows * ROWS);
+  if ((int64_t)first_row >= count * p.q_heads) return;
   const int R = p.dims;
   int lo, hi, first;
-  if (p.interleaved) lo = 16 * j, hi = lo + 8, first = 8 * j;
+  if (p.interleaved) lo = 16 * j, hi = lo + 8, first = 16 * j < R ? 8 * j : 0;
   else if (16 * j < R) lo = 8 * j, hi = lo + R / 2, first = lo;
   else lo = 16 * j, hi = lo + 8, first = 0;
-  const uint16_t* const src = p.q + (s.from + i) * p.q_st + (int64_t)head * p.q_sh;
-  float a[8], b[8];
-  widen8<T>(*(const u32x4*)(src + lo), a);
-  widen8<T>(*(const u32x4*)(src + hi), b);
-  float c[8], sn[8];
-  if (16 * j < R) load_turn<8>(p, turn, first, c, sn);
-  if (p.q_norm) {
-    float w[8], z[8];
-    widen8<T>(*(const u32x4*)(p.q_norm + lo), w);
-    widen8<T>(*(const u32x4*)(p.q_norm + hi), z);
-    float sum = 0.f;
+  uint32_t tok[kRows];
+  u32x4 v[kRows][2];
+  int64_t to[kRows];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) sum += a[k] * a[k] + b[k] * b[k];
-    sum += lane_xor<1>(sum);  // a row's lanes are on together
-    sum += lane_xor<2>(sum);
-    if constexpr (L == 8) sum += lane_xor<4>(sum);
-    const float by = __builtin_amdgcn_rsqf(sum * (1.f / D) + p.eps);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) a[k] = a[k] * by * w[k], b[k] = b[k] * by * z[k];
+  for (int i = 0; i < kRows; ++i) {
+    const uint32_t r = first_row + i * ROWS + lane / L;
+    tok[i] = r / (uint32_t)p.q_heads;
+    const int head = r - tok[i] * p.q_heads;
+    const int64_t t = s.from + (tok[i] < count ? tok[i] : 0);  // rows past the last one read the first
+    const uint16_t* const src = p.q + t * p.q_st + (int64_t)head * p.q_sh;
+    v[i][0] = *(const u32x4*)(src + lo), v[i][1] = *(const u32x4*)(src + hi);
+    to[i] = t * p.o_st + (int64_t)head * p.o_sh;
   }
-  if (16 * j < R) {
-    if (p.interleaved) {
+  u32x4 norm[2] = {{0u, 0u, 0u, 0u}, {0u, 0u, 0u, 0u}};
+  if (p.q_norm) norm[0] = *(const u32x4*)(p.q_norm + lo), norm[1] = *(const u32x4*)(p.q_norm + hi);
+  const int depth = p.parents ? depths(p, s) : 0;
+  Angles angles;
+  angles.ask(p, turn_of(p, s, tok[0], tok[0] < count, depth), first);
+  float w[16];
+  widen8<T>(norm[0], w);
+  widen8<T>(norm[1], w + 8);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        turn_pair(a[2 * k], a[2 * k + 1], c[k], sn[k]);
-        turn_pair(b[2 * k], b[2 * k + 1], c[k + 4], sn[k + 4]);
+  for (int i = 0; i < kRows; ++i) {
+    const bool on = tok[i] < count;
+    if (i > 0) {
+      const int64_t turn = turn_of(p, s, tok[i], on, depth);
+      if (tok[i] != tok[i - 1]) angles.ask(p, turn, first);
+    }
+    float a[8], b[8];
+    widen8<T>(v[i][0], a);
+    widen8<T>(v[i][1], b);
+    if (p.q_norm) {
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum += a[k] * a[k] + b[k] * b[k];
+      sum += lane_xor<1>(sum);
+      sum += lane_xor<2>(sum);
+      if constexpr (L == 8) sum += lane_xor<4>(sum);
+      const float by = __builtin_amdgcn_rsqf(sum * (1.f / D) + p.eps);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) a[k] = a[k] * by * w[k], b[k] = b[k] * by * w[k + 8];
+    }
+    if (16 * j < R) {
+      if (p.interleaved) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          turn_pair(a[2 * k], a[2 * k + 1], angles.cos(k), angles.sin(k));
+          turn_pair(b[2 * k], b[2 * k + 1], angles.cos(k + 4), angles.sin(k + 4));
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) turn_pair(a[k], b[k], angles.cos(k), angles.sin(k));
       }
-    } else {
+    }
+    u32x4 y, z;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) turn_pair(a[k], b[k], c[k], sn[k]);
+    for (int k = 0; k < 4; ++k) y[k] = narrow<T>(a[2 * k], a[2 * k + 1]), z[k] = narrow<T>(b[2 * k], b[2 * k + 1]);
+    if (on) {
+      *(u32x4*)(p.out + to[i] + lo) = y;
+      *(u32x4*)(p.out + to[i] + hi) = z;
     }
   }
-  uint16_t* const dst = p.out + (s.from + i) * p.o_st + (int64_t)head * p.o_sh;
-  u32x4 y, z;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) y[k] = narrow<T>(a[2 * k], a[2 * k + 1]), z[k] = narrow<T>(b[2 * k], b[2 * k + 1]);
-  *(u32x4*)(dst + lo) = y;
-  *(u32x4*)(dst + hi) = z;
+}
+
+// To e4m3, of numbers that are finite and within 448, or of any.
+__device__ __forceinline__ uint32_t quantise(float a, float b, float c, float d, bool plain) {
+  if (!plain) return to_e4m3(a, b, c, d);
+  const int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+}
+
+// A page's new scale for the largest magnitude of its new numbers, and its old one over that.
+struct Scale {
+  float now, ratio;
+};
+__device__ __forceinline__ Scale scale_of(float top, float old, bool holds) {
+  Scale s = {scale_for(top), 1.f};
+  if (holds) {
+    if (old >= s.now) s.now = old;
+    s.ratio = old / s.now;
+  }
+  return s;
 }
 
 template <typename T, int D, int P>
 __global__ __launch_bounds__(P <= 64 ? 256 : 512) void bsg_kv_append_rotated_kernel(RotateParams p) {
   constexpr int THREADS = P <= 64 ? 256 : 512;
   constexpr int W = P / 16;                   // waves of a page
-  constexpr int UNITS = P <= 64 ? 4 / W : 1;  // (page, head, K/V) units of a work-group
+  constexpr int UNITS = P <= 64 ? 4 / W : 1;  // (page, head) units of a work-group
   constexpr int C = D / 64;
-  __shared__ float s_max[UNITS][W];
+  __shared__ f32x2 s_max[UNITS][W];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if ((int)blockIdx.x >= p.kv_groups) {
     turn_queries<T, D>(p, p.first_query + (blockIdx.x - p.kv_groups) * (THREADS / 64) + wave);
     return;
   }
   const int unit = wave / W, tile = wave % W;
-  // units in the order head, K/V, page of the row, row: neighbours write neighbouring bytes
-  const uint32_t u = p.first_unit + blockIdx.x * UNITS + unit, per_page = 2 * p.heads;
-  const uint32_t rp = u / per_page, hk = u - rp * per_page;
-  const int head = hk >> 1, kv = hk & 1;
+  // units in the order head, page of the row, row: neighbours write neighbouring bytes
+  const uint32_t u = p.first_unit + blockIdx.x * UNITS + unit;
+  const uint32_t rp = u / (uint32_t)p.heads;
+  const int head = u - rp * p.heads;
   const int row = rp / p.pages_per_row, nth = rp - row * p.pages_per_row;
 
   const Sequence s = sequence(p, row, u < (uint32_t)p.units);
@@ -283,21 +326,63 @@ __global__ __launch_bounds__(P <= 64 ? 256 : 512) void bsg_kv_append_rotated_ker
   const int t = lane & 15, g = lane >> 4;
   const int tok = tile * 16 + t;
   const bool is_new = fine && tok >= lo && tok < hi;
-  const int64_t nth_new = j * P + tok - start;  // of the sequence's new tokens
-  float f[C][16];
+  const int64_t nth_new = is_new ? j * P + tok - start : 0;  // of the sequence's new tokens; lanes without one read the first
+  u32x4 raw[C][2];
+  uint32_t v[C][8];
+  Angles angles;
+  int64_t turn = 0;
 #pragma unroll
   for (int c = 0; c < C; ++c)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) f[c][i] = 0.f;
-  if (is_new) {
-    const uint16_t* src = p.x[kv] + (s.from + nth_new) * p.st[kv] + (int64_t)head * p.sh[kv] + 16 * g;
+    for (int i = 0; i < 8; ++i) v[c][i] = 0;
+  if (fine) {
+    const uint16_t* const k_src = p.x[0] + (s.from + nth_new) * p.st[0] + (int64_t)head * p.sh[0] + 16 * g;
+    const uint16_t* const v_src = p.x[1] + (s.from + nth_new) * p.st[1] + (int64_t)head * p.sh[1] + 16 * g;
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) widen8<T>(load8(src + 64 * c + 8 * i, p.wide), f[c] + 8 * i);
+      for (int i = 0; i < 2; ++i) raw[c][i] = load8(k_src + 64 * c + 8 * i, p.wide);
+    if (!p.parents) turn = turn_of(p, s, nth_new, is_new, 0), angles.ask(p, turn, key_angles(p, g, 0));
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const u32x4 x = load8(v_src + 64 * c + 8 * i, p.wide);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[c][4 * i + e] = is_new ? x[e] : 0u;
+      }
+    if (p.parents) turn = turn_of(p, s, nth_new, is_new, depths(p, s)), angles.ask(p, turn, key_angles(p, g, 0));
   }
-  if (kv == 0) {
-    const int64_t turn = turn_of(p, s, is_new ? nth_new : 0, is_new);
+  // The new numbers were asked for beside the page; what the page decides comes now, and is on its way while the new
+  // ones are turned and weighed.
+  fine = fine && page >= 0 && page < p.num_pages;
+  const int64_t block = ((int64_t)page * p.heads + head) * 2;
+  const f32x2 old = fine && lo > 0 ? *(const f32x2*)(p.scales + block) : f32x2{0.f, 0.f};
+  uint8_t* const k_dst = p.pages + block * (P * D) + (int64_t)tile * 16 * D;
+  uint8_t* const v_dst = k_dst + P * D;
+  // bytes of the values' dwords (tokens 4q .. 4q+3) that are new, and that hold earlier tokens
+  uint32_t fresh = 0, held = 0;
+  u32x4 was[C];
+  const int v_off = (t >> 2) * 256 + (4 * g + (t & 3)) * 16;
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    const int k = tile * 16 + (t & 12) + b;
+    if (k >= lo && k < hi) fresh |= 0xffu << (8 * b);
+    if (k < lo) held |= 0xffu << (8 * b);
+  }
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    was[c] = u32x4{0u, 0u, 0u, 0u};
+    if (fine && fresh != 0xffffffffu && (fresh | held) != 0) was[c] = *(const u32x4*)(v_dst + c * 1024 + v_off);
+  }
+
+  float f[C][16];
+  const bool any_new = __any(is_new);
+  if (any_new) {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) widen8<T>(raw[c][i], f[c] + 8 * i);
     if (p.k_norm) {
       float sum = 0.f;
 #pragma unroll
@@ -312,95 +397,74 @@ __global__ __launch_bounds__(P <= 64 ? 256 : 512) void bsg_kv_append_rotated_ker
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           float w[8];
-          widen8<T>(*(const u32x4*)(p.k_norm + 64 * c + 16 * g + 8 * i), w);
+          widen8<T>(*(const u32x4*)(p.k_norm + 64 * c + 16 * g + 8 * i), w);  // in every cache: not held till here
 #pragma unroll
           for (int k = 0; k < 8; ++k) f[c][8 * i + k] = f[c][8 * i + k] * by * w[k];
         }
     }
-    turn_key<C>(p, is_new ? turn : 0, g, f);
-    if (!is_new) {  // no token: 0 x inf may have made a NaN of it
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) f[c][i] = 0.f;
-    }
+    turn_key<C, 0>(p, angles, g, f);
+    angles.ask(p, turn, key_angles(p, g, 1));
+    turn_key<C, 1>(p, angles, g, f);
   }
-  // The new numbers were asked for beside the page; what the page decides comes now.
-  fine = fine && page >= 0 && page < p.num_pages;
-  float* const scale_at = p.scales + ((int64_t)page * p.heads + head) * 2 + kv;
-  const float old = fine && lo > 0 ? *scale_at : 0.f;
-  uint8_t* const dst = p.pages + (((int64_t)page * p.heads + head) * 2 + kv) * (P * D) + (int64_t)tile * 16 * D;
-  // Bytes of the values' dwords (tokens 4q .. 4q+3) that are new, and that hold earlier tokens; what
-  // is there is on its way while the new ones are weighed.
-  uint32_t fresh = 0, held = 0;
-  u32x4 was[C];
-  const int v_off = (t >> 2) * 256 + (4 * g + (t & 3)) * 16;
-#pragma unroll
-  for (int b = 0; b < 4; ++b) {
-    const int k = tile * 16 + (t & 12) + b;
-    if (k >= lo && k < hi) fresh |= 0xffu << (8 * b);
-    if (k < lo) held |= 0xffu << (8 * b);
-  }
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    was[c] = u32x4{0u, 0u, 0u, 0u};
-    if (kv == 1 && fine && fresh != 0xffffffffu && (fresh | held) != 0) was[c] = *(const u32x4*)(dst + c * 1024 + v_off);
-  }
-  float a = finite_top<C>(f);
-  if constexpr (W > 1) {  // also: every wave has the old scale before one writes the new
-    if (lane == 0) s_max[unit][tile] = a;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < W; ++i) a = fmaxf(a, s_max[unit][i]);
-  }
-  if (!fine) return;
-
-  float scale = scale_for(a), ratio = 1.f;
-  if (lo > 0) {
-    if (old >= scale) scale = old;
-    ratio = old / scale;
-  }
-  if (tile == 0 && lane == 0) *scale_at = scale;
-  // what this wave's tile does not have to write: no new token, and no earlier one to round again
-  if (tile * 16 >= hi || (tile * 16 + 16 <= lo && ratio == 1.f)) return;
-
-  const float inv = 1.f / scale;
-  uint32_t y[C][4];
 #pragma unroll
   for (int c = 0; c < C; ++c)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      y[c][i] = to_e4m3(f[c][4 * i] * inv, f[c][4 * i + 1] * inv, f[c][4 * i + 2] * inv, f[c][4 * i + 3] * inv);
-  if (kv == 0) {
+    for (int i = 0; i < 16; ++i) f[c][i] = is_new ? f[c][i] : 0.f;
+  bool finite;
+  f32x2 top = {finite_top<C>(f, &finite), largest_magnitude<T, C>(v)};
+  if constexpr (W > 1) {  // also: every wave has the old scales before one writes the new
+    if (lane == 0) s_max[unit][tile] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < W; ++i) top.x = fmaxf(top.x, s_max[unit][i].x), top.y = fmaxf(top.y, s_max[unit][i].y);
+  }
+  if (!fine) return;
+
+  const Scale ks = scale_of(top.x, old.x, lo > 0), vs = scale_of(top.y, old.y, lo > 0);
+  if (tile == 0 && lane == 0) *(f32x2*)(p.scales + block) = f32x2{ks.now, vs.now};
+  if (tile * 16 >= hi) return;  // none of this wave's tokens is there
+
+  // keys: no new one, and no earlier one to round again, leaves the tile as it is
+  if (tile * 16 + 16 > lo || ks.ratio != 1.f) {
+    const float inv = 1.f / ks.now;
+    const bool plain = finite && top.x * inv <= 448.f;  // which may fail where the scale is at its limit
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      u32x4* const at = (u32x4*)(dst + c * 1024 + lane * 16);
+      u32x4* const at = (u32x4*)(k_dst + c * 1024 + lane * 16);
       if (is_new) {
-        *at = u32x4{y[c][0], y[c][1], y[c][2], y[c][3]};
-      } else if (tok < lo && ratio != 1.f) {
-        const u32x4 v = *at;
-        *at = u32x4{rescale(v.x, ratio), rescale(v.y, ratio), rescale(v.z, ratio), rescale(v.w, ratio)};
+        u32x4 y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          y[i] = quantise(f[c][4 * i] * inv, f[c][4 * i + 1] * inv, f[c][4 * i + 2] * inv, f[c][4 * i + 3] * inv, plain);
+        *at = y;
+      } else if (tok < lo && ks.ratio != 1.f) {
+        const u32x4 x = *at;
+        *at = u32x4{rescale(x.x, ks.ratio), rescale(x.y, ks.ratio), rescale(x.z, ks.ratio), rescale(x.w, ks.ratio)};
       }
     }
-  } else {
+  }
+  if (tile * 16 + 16 > lo || vs.ratio != 1.f) {
+    const float inv = 1.f / vs.now, ratio = vs.ratio;
     const bool rounds = held != 0 && ratio != 1.f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       uint32_t w[4];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) w[n] = quad_transpose(y[c][n], t & 3);
+      for (int i = 0; i < 4; ++i)
+        w[i] = quad_transpose(to_e4m3(low_half<T>(v[c][2 * i]) * inv, high_half<T>(v[c][2 * i]) * inv, low_half<T>(v[c][2 * i + 1]) * inv,
+                                      high_half<T>(v[c][2 * i + 1]) * inv), t & 3);
       row_transpose(w);  // lane 16 g + 4 q + i: channels 16 n + 4 g + i of tokens 4 q .. 4 q + 3
-      u32x4* const at = (u32x4*)(dst + c * 1024 + v_off);
-      u32x4 v = {w[0], w[1], w[2], w[3]};
+      u32x4* const at = (u32x4*)(v_dst + c * 1024 + v_off);
+      u32x4 y = {w[0], w[1], w[2], w[3]};
       if (fresh != 0xffffffffu) {
         if (fresh == 0 && !rounds) continue;
         u32x4 kept = was[c];
         if (rounds)
           kept = (u32x4{rescale(kept.x, ratio), rescale(kept.y, ratio), rescale(kept.z, ratio), rescale(kept.w, ratio)} & held) |
                  (kept & ~held);
-        v = (v & fresh) | (kept & ~fresh);
+        y = (y & fresh) | (kept & ~fresh);
       }
-      *at = v;
+      *at = y;
     }
   }
 }
@@ -469,11 +533,11 @@ extern "C" int bsg_kv_append_rotated(const void* q, int64_t q_stride_t, int64_t 
   if (!is_aligned(k, 2) || !is_aligned(v, 2)) return fail(BSG_ERR_ALIGN, "k and v must be 2-byte aligned");
   const int P = cache->page_size;
   const int64_t per_row = ((int64_t)max_new + P - 2) / P + 1;  // pages that max_new tokens can touch
-  const int64_t units = per_row * rows * cache->n_heads * 2;
-  const int64_t q_row = ceil_div((int64_t)max_new * q_heads * (cache->head_dim / 16), 64), queries = q_row * rows;
+  const int64_t units = per_row * rows * cache->n_heads;
+  const int64_t q_row = ceil_div((int64_t)max_new * q_heads * (cache->head_dim / 16), 64 * kRows), queries = q_row * rows;
   if (units > 0x7fffffff - kLaunchUnits || queries > 0x7fffffff - kLaunchUnits)
     return fail(BSG_ERR_UNSUPPORTED, "%lld tiles of work", (long long)(units > queries ? units : queries));
-  if ((int64_t)max_new * q_heads > 0x7fffffff - 64) return fail(BSG_ERR_UNSUPPORTED, "%d tokens x %d heads", max_new, q_heads);
+  if ((int64_t)max_new * q_heads > 0x7fffffff - 64 * kRows) return fail(BSG_ERR_UNSUPPORTED, "%d tokens x %d heads", max_new, q_heads);
   RotateParams p;
   p.x[0] = (const uint16_t*)k, p.x[1] = (const uint16_t*)v;
   p.st[0] = k_stride_t, p.st[1] = v_stride_t, p.sh[0] = k_stride_h, p.sh[1] = v_stride_h;
