@@ -746,3 +746,127 @@ def test_keep_graph(dev):
         torch.cuda.synchronize()
         assert all(torch.equal(x, w) for x, w in zip(state, want))
     assert n.tolist() == [41, 20]
+
+
+# ---------------------------------------------------------------------------------------- a run of them together
+
+
+class _Toy:
+    """Two layers of the operators in turn, as a decoder that drafts calls them: a step takes a tree of each sequence's, whose first
+    node is its last token, and leaves the accepted nodes in the cache and the next last token."""
+
+    def __init__(self, dev, rng, prompts, dtype, slots, page=16, vocab=9, max_new=14):
+        self.dev, self.vocab, self.max_new, self.hq, self.heads, self.d = dev, vocab, max_new, 6, 2, 64
+        self.cache = bsa.KVCache(2, 64, self.heads, self.d, page, 6, 12, dev)
+        self.slots = _i32(slots, dev)
+
+        def weight(k, n):
+            return torch.from_numpy(rng.standard_normal((k, n)).astype(np.float32) * k ** -0.5).to(dev).to(dtype)
+
+        self.embed = weight(1, 64).expand(vocab, 64) * 0.3 + torch.from_numpy(rng.standard_normal((vocab, 64)).astype(np.float32)).to(dev).to(dtype)
+        self.qkv = [weight(64, (self.hq + 2 * self.heads) * self.d) for _ in range(2)]
+        self.o = [weight(self.hq * self.d, 64) for _ in range(2)]
+        self.head = weight(64, vocab)
+        self.norms = [torch.from_numpy((1 + 0.1 * rng.standard_normal(self.d)).astype(np.float32)).to(dev).to(dtype) for _ in range(2)]
+        self.angles = _angles(400, self.d)
+        self.cos, self.sin = (torch.from_numpy(x).to(dev) for x in self.angles)
+        flat = _i32([t for p in prompts for t in p], dev)
+        cu = _i32(_cu([len(p) for p in prompts]), dev)
+        assert bool(self.cache.extend(cu.diff().to(torch.int32), slots=self.slots).all())
+        self.forward(flat, cu, max(map(len, prompts)), None)
+        self.last = _i32([1] * len(prompts), dev)  # the prompts' continuation, not yet in the cache
+        self.seen = [list(p) + [1] for p in prompts]
+
+    def forward(self, tokens, cu, max_new, parents):
+        x = self.embed[tokens.long()]
+        batch = dict(cu_seqlens=cu, max_new=max_new, slots=self.slots)
+        for i in range(2):
+            qkv = (x @ self.qkv[i]).view(len(x), -1, self.d)
+            q, k, v = qkv.split([self.hq, self.heads, self.heads], 1)
+            q = self.cache.append_rotated(i, q, k, v, self.cos, self.sin, parents=parents, q_norm=self.norms[0], k_norm=self.norms[1], **batch)
+            out, _ = self.cache.attend(i, q, **batch) if parents is None else self.cache.attend_tree(i, q, parents, **batch)
+            x = x + out.view(len(x), -1) @ self.o[i]
+        return x @ self.head
+
+    def step(self, drafts, parents, cu, uniforms):
+        """drafts has the trees' tokens but for the first ones."""
+        first = cu[:-1].long()
+        tokens = drafts.index_copy(0, first, self.last)
+        self.cache.extend(cu.diff().to(torch.int32), slots=self.slots)
+        logits = self.forward(tokens, cu, self.max_new, parents)
+        got = bsa.verify_drafts(logits, tokens, uniforms, parents, temperature=0.7, cu_seqlens=cu, max_new=self.max_new)
+        self.cache.keep(got.path, got.accepted, cu_seqlens=cu, slots=self.slots)
+        self.last.copy_(got.tokens.gather(1, got.accepted.long()[:, None] - 1)[:, 0])
+        return tokens, logits, got
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_run_of_steps(dev, dtype, captured):
+    """Prompts, then steps of trees: each step's verdict is the oracle's of its logits, and at the end the first layer's cache
+    holds the accepted tokens' keys at their own positions, in order, and pages for no more.
+
+    Keys of the first layer depend on the token and its position alone: x W (computed here by the same call, one row's
+    product in other company: 64 terms in 32 bits and a rounding, 2 u of the largest sum of magnitudes), normed and turned
+    (34 x 2^-24), then e4m3 (2^-4 of it), then rounded again at most twice a step, which loses no more than half a step of
+    what is subnormal, 2^-10 of the scale each."""
+    rng = np.random.default_rng([5, captured])
+    prompts = [rng.integers(0, 9, n).tolist() for n in (21, 5, 48)]
+    toy = _Toy(dev, rng, prompts, DT[dtype], [4, 0, 2])
+    sizes = [14, 9, 1]
+    cu = _i32(_cu(sizes), dev)
+    drafts, uniforms = torch.zeros(24, dtype=torch.int32, device=dev), torch.zeros(24, device=dev)
+    parents = torch.zeros(24, dtype=torch.int32, device=dev)
+    steps, graph, accepted = 8, None, 0
+
+    def draw():
+        drafts.copy_(_i32(rng.integers(0, 9, 24), dev))
+        parents.copy_(_i32([x for n in sizes for x in _parents(rng, n)], dev))
+        uniforms.copy_(torch.from_numpy(rng.random(24, dtype=np.float32)).to(dev))
+
+    if captured:  # the capture itself runs nothing; allocations and first calls come before it, on a decoder of their own
+        draw()
+        _Toy(dev, np.random.default_rng(9), prompts, DT[dtype], [4, 0, 2]).step(drafts, parents, cu, uniforms)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = toy.step(drafts, parents, cu, uniforms)
+    for _ in range(steps):
+        draw()
+        if graph is None:
+            out = toy.step(drafts, parents, cu, uniforms)
+        else:
+            graph.replay()
+        torch.cuda.synchronize()
+        tokens, logits, got = out
+        assert torch.isfinite(logits).all()
+        _same_verdict(got, dft.verify(logits.double().cpu().numpy(), tokens.cpu().numpy(), uniforms.cpu().numpy(), parents.cpu().numpy(), None,
+                                      0.7, _cu(sizes)), 14)
+        for b, n in enumerate(got.accepted.tolist()):
+            accepted += n - 1
+            path = got.path[b, :n].tolist()
+            assert [tokens[sizes[0] * (b > 0) + sizes[1] * (b > 1) + i].item() for i in path[1:]] == got.tokens[b, : n - 1].tolist()
+            toy.seen[b] += got.tokens[b, :n].tolist()
+    assert accepted  # or the run has moved nothing
+    c = toy.cache
+    lengths, table, refs = c.lengths.tolist(), c.page_table.tolist(), c.refcounts.tolist()
+    assert [lengths[i] for i in (1, 3, 5)] == [0, 0, 0] and sum(refs) == sum(-(-n // 16) for n in lengths) and max(refs) == 1
+    norm = toy.norms[1].double().cpu().numpy()
+    for b, slot in enumerate((4, 0, 2)):
+        seen = toy.seen[b][:-1]
+        assert lengths[slot] == len(seen) and all(x < 0 for x in table[slot][-(-len(seen) // 16):])
+        x = toy.embed[torch.tensor(seen, device=dev)]
+        raw = (x @ toy.qkv[0]).view(len(seen), -1, 64)[:, 6:8]
+        slack = (x.abs().float() @ toy.qkv[0].abs().float()).view(len(seen), -1, 64)[:, 6:8].double().cpu().numpy()
+        cos, sin = toy.angles
+        pairs = [dft.turn(r, norm, 1e-6, cos, sin, i, False) for i, r in enumerate(raw.double().cpu().numpy())]
+        want = np.stack([w for w, _ in pairs]).transpose(1, 0, 2)
+        mag = np.stack([m for _, m in pairs]).transpose(1, 0, 2)
+        # an error e of each channel of x moves the normed x by at most 2 e |norm| / rms(x), and its turn by that of both channels
+        u = 2.0 ** -11 if dtype == "fp16" else 2.0 ** -8
+        rms = np.sqrt(np.square(raw.double().cpu().numpy()).mean(-1, keepdims=True))
+        off = (2 * 2 * u * slack.max(-1, keepdims=True) * 2 * np.abs(norm).max() / rms).transpose(1, 0, 2)
+        off = off + 34 * 2.0 ** -24 * mag
+        largest = 2.0 ** np.ceil(np.log2(np.abs(want).max() * 1.1 / 448))
+        got = c.read(0, slot)[0].double().cpu().numpy()
+        assert (np.abs(got - want) <= off + 2.0 ** -4 * (np.abs(want) + off) + (1 + 2 * steps) * 2.0 ** -10 * largest).all()
