@@ -493,6 +493,34 @@ def test_verify_hard_rows(dev, vocab, draft):
 
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("each", [False, True])
+def test_verify_temperatures_without_end(dev, dtype, draft, each):
+    """From the least to infinity, where every token that has a finite logit is as likely; among them -inf."""
+    rng = np.random.default_rng(12)
+    temps = np.array([1e-45, 1e-38, 1e-30, 1e-3, 1e3, 1e30, 3.4e38, np.inf], np.float32)
+    new = [4] * len(temps)
+    x, _, tokens, u = _drafts(rng, new, 700, False)
+    x[:, ::5] = -np.inf
+    for i, t in enumerate(tokens):  # some of which are likely
+        if i % 4:
+            x[i - 1, t] = np.nanmax(x[i - 1]) + 0.25 * (i % 2)
+    logits = torch.from_numpy(x).to(DT[dtype] if dtype != "fp32" else torch.float32).to(dev)
+    drafted = logits.roll(1, 1).contiguous() if draft else None
+    args = (logits.double().cpu().numpy(), tokens, u, None, None if drafted is None else drafted.double().cpu().numpy())
+    exact = np.where(np.isinf(temps), 1e300, np.maximum(temps.astype(np.float64), 2.0 ** -126))
+    with np.errstate(all="ignore"):
+        want = dft.verify(*args, exact, _cu(new))
+    ids, nums, cu = _i32(tokens, dev), torch.from_numpy(u).to(dev), _i32(_cu(new), dev)
+    if each:
+        _same_verdict(bsa.verify_drafts(logits, ids, nums, None, drafted, torch.from_numpy(temps).to(dev), cu, 4), want, 4)
+    else:
+        for b, t in enumerate(temps[:-1]):  # as a number infinity is refused
+            got = bsa.verify_drafts(logits, ids, nums, None, drafted, float(t), cu, 4)
+            _same_verdict([y[b:b + 1] for y in got], want[b:b + 1], 4)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
 def test_verify_ties_take_the_first(dev, dtype):
     rng = np.random.default_rng(1)
     x = rng.integers(0, 4, (24, 9000)).astype(np.float32)  # thousands of equal maxima

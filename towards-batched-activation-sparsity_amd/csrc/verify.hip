@@ -226,6 +226,8 @@ __device__ __forceinline__ Tree tree_of(const VerifyParams& p, int row, int lane
   int64_t to = t.from + p.max_new;
   if (p.cu) t.from = p.cu[row], to = p.cu[row + 1];
   t.temperature = p.temperatures ? p.temperatures[row] : p.temperature;
+  // whose inverse is a 32-bit number other than 0, and infinity: no product with it is NaN
+  if (t.temperature > 0.f) t.temperature = fminf(fmaxf(t.temperature, 0x1p-126f), 0x1.fffffep127f);
   const bool fine = t.from >= 0 && t.from < to && to <= p.tokens;
   t.count = !fine ? 0 : to - t.from < p.max_new ? (int)(to - t.from) : p.max_new;
   t.parent = load_parent(p.parents, t.from, t.count, lane);
