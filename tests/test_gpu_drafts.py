@@ -534,6 +534,40 @@ def test_verify_ties_take_the_first(dev, dtype):
     assert want[0][0] == 8 and want[1][0] == 2
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("vocab", [3, 2050, 40000])
+@pytest.mark.parametrize("each", [False, True])
+def test_verify_greedy_rows_without_probabilities(dev, dtype, vocab, each):
+    """By a number and by sequences: rows of nothing but -inf, with NaN, with +inf, at the root, within the path and at its end;
+    children of the first token, which a row of -inf has first."""
+    rng = np.random.default_rng(vocab)
+    new = [6, 6, 6, 6, 6, 1, 0, 20]
+    cu = _cu(new)
+    x = rng.standard_normal((cu[-1], vocab))
+    parents = [i - 1 for _ in range(5) for i in range(6)] + [-1] + _parents(rng, 20)
+    tokens = rng.integers(0, vocab, cu[-1])
+    for b in range(5):
+        for i in range(5):
+            tokens[cu[b] + i + 1] = int(np.argmax(x[cu[b] + i].astype(np.float16)))
+    for i in range(1, 20):
+        p = dft.tree_parent(parents[cu[7]:], i)
+        if p >= 0 and i % 3:
+            tokens[cu[7] + i] = int(np.argmax(x[cu[7] + p].astype(np.float16)))
+    x = x.astype(np.float16).astype(np.float64)
+    x[cu[0]], tokens[cu[0] + 1] = -np.inf, 0
+    x[cu[1] + 2], tokens[cu[1] + 3] = -np.inf, 0
+    x[cu[2] + 5] = -np.inf
+    x[cu[3] + 1, vocab // 2] = np.nan
+    x[cu[4] + 5, vocab - 1] = np.inf
+    logits = torch.from_numpy(x).to(DT[dtype] if dtype != "fp32" else torch.float32).to(dev)
+    u = rng.random(cu[-1]).astype(np.float32)
+    want = dft.verify(logits.double().cpu().numpy(), tokens, u, parents, None, 0.0, cu)
+    t = torch.zeros(len(new), device=dev) if each else 0.0
+    got = bsa.verify_drafts(logits, _i32(tokens, dev), torch.from_numpy(u).to(dev), _i32(parents, dev), None, t, _i32(cu, dev), 20)
+    _same_verdict(got, want, 20)
+    assert want[0][2] == [-1] and max(w[0] for w in want) >= (1 if dtype == "bf16" else 5)
+
+
 @pytest.mark.parametrize("offset,width,dtype", [(0, 5010, "fp16"), (3, 5007, "bf16"), (1, 2500, "fp32"), (5, 40, "fp16")])
 def test_verify_strided_logits(dev, offset, width, dtype):
     rng = np.random.default_rng(width)

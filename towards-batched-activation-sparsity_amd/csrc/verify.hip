@@ -541,7 +541,7 @@ __global__ __launch_bounds__(64 * kWaves) void bsg_verify_walk_kernel(VerifyPara
     const double u_j = read_lane(u, j), w_j = read_lane(mine, j);
     bool ok = (__ballot(known) >> j & 1) != 0 && !same;
     if (greedy) {
-      ok = ok && __builtin_amdgcn_readlane(id, j) == s_at[at] && total == total;
+      ok = ok && __builtin_amdgcn_readlane(id, j) == s_at[at] && total == total && s_top[0][at] > -__builtin_inff();
     } else if (drafts) {
       ok = ok && u_j * read_lane(theirs, j) < w_j;
     } else if (ok) {
