@@ -73,16 +73,19 @@ int bsg_kv_tree_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
  *                          max(p - q, 0), otherwise from p
  *   temperature <= 0       accepted if x is the likeliest token (the first of equal ones), which is also the new one
  * where nothing is left, from p.  Drawn: the first token whose running sum exceeds uniforms[node 0] times the whole.
- * Weights and sums are 64-bit, so that the answer is the definition's but for numbers within some 2^-40 of a border.
- *   logits, draft_logits : [tokens][vocab] fp16, bf16 or fp32 (the same), row strides in elements
+ * Decisions are those of 64-bit weights and sums (32-bit ones only decide what they cannot have wrong), so that the answer is
+ * the definition's but for numbers within some 2^-40 of a border.
+ *   logits, draft_logits : [tokens][vocab] fp16, bf16 or fp32 (the same), row strides in elements; the aligned 16 bytes in
+ *                          which a row begins and ends are read whole
  *   tokens, parents      : int32 [tokens]; a token outside the vocabulary is rejected
  *   uniforms             : fp32 [tokens] in [0, 1): a node's own number, node 0's draws the new token
- *   temperature          : of all rows, or temperatures fp32 [rows] where that is not NULL
+ *   temperature          : of all rows, finite and at least 0, or where it is not NULL temperatures fp32 [rows], any: 0 or
+ *                          less and NaN are greedy, infinity makes all tokens of finite logits alike
  *   accepted             : int32 [rows], accepted nodes, node 0 among them; 0 without nodes
  *   path, out_tokens     : int32 [rows][max_new]: the accepted nodes; the accepted nodes' tokens after the first's and the
  *                          new token, as many; then -1.  A row of logits with NaN, +inf, or nothing but -inf ends
  *                          the path with -1 as its new token.
- * max_new <= BSG_TREE_NODES.  Workspace as bsg_kv_attention. */
+ * max_new <= BSG_TREE_NODES, vocab <= 2^20, rows <= 16384.  Workspace as bsg_kv_attention. */
 int64_t bsg_verify_drafts_workspace_bytes(int64_t tokens, int32_t rows, int64_t vocab, int32_t max_new, int dtype,
                                           int32_t drafts);
 int bsg_verify_drafts(const void* logits, int64_t logits_stride, const void* draft_logits, int64_t draft_stride,

@@ -13,7 +13,8 @@ A tree is the newest tokens of a sequence, its nodes, at most 64 of them.  paren
 token its parent's place among its sequence's new tokens; what names no earlier node (-1) makes it a root.  One
 step: pages_extend gives every node a place, kv_append_rotated and kv_tree_attention run in each layer, verify_drafts
 reads the logits, and pages_keep leaves the accepted nodes behind the tokens that were there before.  Batches
-(cu_seqlens, max_new, slots) are described as in serving.py.
+(cu_seqlens, max_new, slots) are described as in serving.py.  A sequence that pages_extend had no room for takes no
+part: its slot is -1 in the calls that follow.
 """
 from __future__ import annotations
 
@@ -206,9 +207,10 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Te
         temperature 0          if x is the likeliest token (of equal ones the first), which is also the new one
 
     and drawn by the first token's number: the first token whose running sum exceeds it times the whole.  The tokens that
-    come out are then distributed as the target's own.  temperature is a number or fp32 [sequences], by which 0 or less
-    (or NaN) is greedy.  Weights and sums are 64-bit.  A row of logits with NaN, +inf, or nothing but -inf ends its path
-    with a new token of -1; a token outside the vocabulary is rejected.  At most 64 tokens a sequence."""
+    come out are then distributed as the target's own.  temperature is a finite number from 0 on, or fp32 [sequences], by which
+    0 or less (or NaN) is greedy and infinity makes all tokens of finite logits alike.  Decisions are those of 64-bit
+    weights and sums.  A row of logits with NaN, +inf, or nothing but -inf ends its path with a new token of -1; a token
+    outside the vocabulary is rejected.  At most 64 tokens a sequence, 2^20 in the vocabulary, 16384 sequences."""
     if max_new is not None:
         max_new = int(max_new)
     each = temperature if isinstance(temperature, torch.Tensor) else None

@@ -191,7 +191,8 @@ __device__ __forceinline__ float finite_top(const float f[C][16], bool* finite) 
 }
 
 // A wave's rows of queries: kRows times as many as its lanes hold, since rows of one token, which follow each other, share
-// their angles and all share the norm.
+// their angles and all share the norm.  1, 2, 4 times: 45, 41, 44 us for 6000 tokens x 32 heads (with their keys and values, each
+// of which had a wave of its own then).
 constexpr int kRows = 2;
 template <typename T, int D>
 __device__ __forceinline__ void turn_queries(const RotateParams& p, uint32_t unit) {
@@ -291,6 +292,10 @@ __device__ __forceinline__ Scale scale_of(float top, float old, bool holds) {
   return s;
 }
 
+// HBM bounds it: 6000 tokens of prompts, 32 heads on 8, norms (175 MB): 37 us, 4.7 TB/s.  What is on its way counts: keys and values in
+// one wave (in one each: 45), four waves a SIMD by halves of the angles (64 trees of up to 16 nodes, 32 heads: 15.3 us; all angles
+// at once 18).  One token is a chain of three loads, 6 us.  Keys in 64 bits, so that none is rounded to the neighbour of
+// what its exact value would be (of some 10^7 about 10 are): 47 and 23 us.
 template <typename T, int D, int P>
 __global__ __launch_bounds__(P <= 64 ? 256 : 512) void bsg_kv_append_rotated_kernel(RotateParams p) {
   constexpr int THREADS = P <= 64 ? 256 : 512;

@@ -2,7 +2,8 @@
 //
 // A row sees all tokens before the tree, and of the tree its own node and its ancestors, which each wave works out
 // once, one bit for each of 64 nodes.  Only the last steps hold nodes, so only they look at the bits.  Up to 32 rows of a
-// cached head go to kv_attention.hpp's kernel, more to the one below; the arithmetic is the same.
+// cached head go to kv_attention.hpp's kernel, more to the one below; the arithmetic is the same.  HBM bounds the first: 64
+// trees of up to 16 nodes, contexts to 1500 tokens, 32 heads (509 MB), 95 us, 5.3 TB/s (three waves a SIMD instead of two: 113).
 
 #include "bsgdraft.h"
 #include "kv_attention.hpp"
@@ -23,7 +24,12 @@ struct TreeParams {
 constexpr int kStep = 64;        // tokens
 constexpr int kLeastSteps = 4;   // of a work-group
 constexpr int kMostRows = 256;   // sequences that are dealt out
-constexpr int kDealUnits = 2;   // units of a compute unit from which on each has a work-group
+// When they are dealt out: fewer units than kDealUnits a compute unit, of more than kDealTokens tokens.  A work-group for
+// each unit / dealt out, us: 256 units of up to 2000 tokens 44 / 44, 512 of them 56 / 70, 1024 101 / 114; 8 sequences x 8 heads
+// x 100 rows of up to 3000 tokens 83 / 36, 16 x 8 x 240 rows of up to 6001 158 / 102; 32 units of up to 800 tokens 24 / 23, of 600
+// 21 / 23, 128 of them 23 / 27, of 300 16 / 26: parts and their launch cost as much as 8 steps.
+constexpr int kDealUnits = 2;
+constexpr int kDealTokens = 768;
 
 // A part: [16 rows][16 channels][lane] accumulators in the order the matrix unit leaves them, then base and sum of
 // each row.
@@ -63,6 +69,9 @@ __device__ __forceinline__ int tiles_of(const AttnParams& p, const Branch& b, in
 // A work-group of four waves has ROWS = 32 RG rows, each wave 32 of them, and takes the tokens they see 64 at a time,
 // brought once straight into LDS in the bytes they have in memory, two steps ahead.  With RG = 2 the other two waves
 // have the same rows and the second half of each step's tokens; the halves meet in LDS at the end.
+// What two waves a SIMD hide of the softmax between the products bounds it (the matrix unit is at work a fifth of the time, the
+// vector unit a third): 16 sequences of up to 6001 tokens, 8 heads x 240 rows, 43 GFLOP: 92 us and 10 of the join, some 1.3 us a
+// step of the two work-groups of a compute unit, and 20 for what begins and ends a unit or a part of one.  Memory is 7 of it.
 template <typename T, int D, int RG>
 __global__ __launch_bounds__(256, 2) void bsg_kv_tree_kernel(TreeParams tp) {
   const AttnParams& p = tp.a;
@@ -430,7 +439,8 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_tree_kernel(TreeParams tp) {
   }
 }
 
-// The parts of the units that several work-groups had, joined in order: a wave has 16 channels of 16 rows.
+// The parts of the units that several work-groups had, joined in order: a wave has 16 channels of 16 rows (all channels of them:
+// 81 us where the two launches now take 67, one tree of 60 nodes and 30000 tokens).
 template <typename T, int D, int RG>
 __global__ __launch_bounds__(256) void bsg_kv_tree_join_kernel(TreeParams tp) {
   const AttnParams& p = tp.a;
@@ -478,7 +488,9 @@ __global__ __launch_bounds__(256) void bsg_kv_tree_join_kernel(TreeParams tp) {
         nothing ? -__builtin_inff() : (top + __builtin_amdgcn_logf(sum)) * (1.f / kLog2e);
 }
 
-constexpr int kTileRows = 32;  // a cached head's rows past which the second kernel runs
+// A cached head's rows past which the second kernel runs.  First / second, us: 24 rows 22 / 28, 32 rows 67 / 73 and 41 / 44; 48
+// rows of 16 sequences 76 / 53, 64 of 64 160 / 114 (tiles of 128 rows: 65 and 147); 40 rows of one sequence 18 / 23.
+constexpr int kTileRows = 32;
 
 // How a call is cut.  shape: of the first kernel; for the second one rows are the tile's and `groups` work-groups share
 // the steps, or, 0, each unit has one.
@@ -492,6 +504,7 @@ Cut cut_of(int32_t rows, const bsg_kv_cache* cache, int32_t group, int32_t max_n
   Shape& s = c.shape;
   const int32_t kv_heads = cache->n_heads, d = cache->head_dim;
   const int64_t per_head = (int64_t)max_new * group;
+  // past 64 rows tiles of 128, of 64, us: 240 rows 102, 116; 100 rows of 64 sequences 82, 97, of 8 36, 35
   s.rows = per_head <= 16 ? 16 : per_head <= kTileRows ? 32 : per_head <= 64 ? 64 : 128;
   s.row_tiles = (int32_t)ceil_div(per_head, s.rows);
   const int64_t tiles = (int64_t)rows * kv_heads * s.row_tiles;
@@ -501,7 +514,7 @@ Cut cut_of(int32_t rows, const bsg_kv_cache* cache, int32_t group, int32_t max_n
   if (s.rows >= 64) {
     // all steps, of rows as long as a table's can be, are counted in 32 bits
     const int64_t most = ceil_div((int64_t)cache->max_pages * cache->page_size, kStep);
-    if (rows <= kMostRows && tiles < (int64_t)kDealUnits * cus && max_len > kStep * kLeastSteps && tiles * most < 0x7fffffff)
+    if (rows <= kMostRows && tiles < (int64_t)kDealUnits * cus && max_len > kDealTokens && tiles * most < 0x7fffffff)
       c.groups = 2 * cus;
     c.bytes = c.groups == 0 ? 0 : BSG_KV_COUNTER_BYTES + ceil_div(tiles * 8, 256) * 256 + (int64_t)c.groups * 2 * s.rows * (d + 2) * 4;
     return c;
