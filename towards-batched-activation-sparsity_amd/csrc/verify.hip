@@ -107,9 +107,15 @@ struct Numbers {
   static constexpr int PER = Logit<T>::PER, VECTORS = BYTES / 16, N = PER * VECTORS;
   u32x4 v[VECTORS];
   // f(number of the vector, vector) for one after the other, in a loop: a wave comes by here once or twice, and code
-  // that is not in the instruction cache yet costs more than the loop.
-  template <typename F>
+  // that is not in the instruction cache yet costs more than the loop.  OFTEN: a compute unit has many such waves, and
+  // the loop's moves cost more (64 chains, first launch: 17 against 18 us).
+  template <bool OFTEN = false, typename F>
   __device__ __forceinline__ void each(const F& f) {
+    if constexpr (OFTEN) {
+#pragma unroll
+      for (int k = 0; k < VECTORS; ++k) f(k, v[k]);
+      return;
+    }
 #pragma unroll 1
     for (int k = 0; k < VECTORS; ++k) {
       u32x4 first = v[0];
@@ -244,25 +250,25 @@ __device__ __forceinline__ uint64_t inner_of(const Tree& t) {
 
 // What a piece is to its row: its maximum, the sum of its weights against that, and greedy the place of the first
 // maximum.  first: the place of the piece's first number.
-template <typename T>
+template <bool OFTEN, typename T>
 __device__ __forceinline__ Piece piece_of(PieceOf<T>& x, bool greedy, bool exact, double k, int first, int lane) {
   constexpr int PER = PieceOf<T>::PER;
   bool bad = false;
   float top = -__builtin_inff();
-  x.each([&](int, u32x4& v) {
+  x.template each<OFTEN>([&](int, u32x4& v) {
 #pragma unroll
     for (int e = 0; e < PER; ++e) top = fmaxf(top, Logit<T>::of(v, e)), bad = bad || !(Logit<T>::of(v, e) < __builtin_inff());
   });
   Piece mine = {0.0, wave_max<32>(top), 0x7fffffff};
   if (greedy) {
-    x.each([&](int i, u32x4& v) {
+    x.template each<OFTEN>([&](int i, u32x4& v) {
 #pragma unroll
       for (int e = PER - 1; e >= 0; --e)
         if (Logit<T>::of(v, e) == mine.top && first + (64 * i + lane) * PER + e < mine.at) mine.at = first + (64 * i + lane) * PER + e;
     });
     mine.at = wave_min<32>(mine.at);
   } else if (exact) {
-    x.each([&](int, u32x4& v) {
+    x.template each<OFTEN>([&](int, u32x4& v) {
 #pragma unroll
       for (int e = 0; e < PER; ++e) mine.sum += weight(Logit<T>::of(v, e), mine.top, k);
     });
@@ -271,7 +277,7 @@ __device__ __forceinline__ Piece piece_of(PieceOf<T>& x, bool greedy, bool exact
     // a piece of nothing but -inf has no maximum to be weighed against
     const float by = (float)k, from = mine.top == -__builtin_inff() ? 0.f : mine.top;
     float sum = 0.f;
-    x.each([&](int, u32x4& v) {
+    x.template each<OFTEN>([&](int, u32x4& v) {
 #pragma unroll
       for (int e = 0; e < PER; ++e) sum += __builtin_amdgcn_exp2f((Logit<T>::of(v, e) - from) * by);
     });
@@ -282,7 +288,7 @@ __device__ __forceinline__ Piece piece_of(PieceOf<T>& x, bool greedy, bool exact
 }
 
 // The rows of the nodes that have children, by pieces: of a sequence's the blockIdx.y-th, and every gridDim.y-th from there.
-// 64 chains of up to 5 drawn drafts, 32000 fp16 logits of two models: 18 us, of which the 64-bit weights are some 12 (18
+// 64 chains of up to 5 drawn drafts, 32000 fp16 logits of two models: 17 us, of which the 64-bit weights are some 12 (18
 // instructions each, all at the rate of a fused multiply-add); 64 trees of up to 16 nodes: 13 us with 32-bit weights, 21 with
 // 64-bit ones.
 template <typename T>
@@ -302,7 +308,7 @@ __global__ __launch_bounds__(64 * kWaves) void bsg_verify_rows_kernel(VerifyPara
     const int shift = shift_of<T>(p.x[which], at);
     PieceOf<T> x;
     x.load(p.x[which], at, p.vocab, shift, piece, lane);
-    const Piece mine = piece_of<T>(x, greedy, p.drafts != 0, kLog2e / (double)t.temperature, piece * kPiece - shift, lane);
+    const Piece mine = piece_of<true, T>(x, greedy, p.drafts != 0, kLog2e / (double)t.temperature, piece * kPiece - shift, lane);
     if (lane == 0) p.stats[((t.from + node) * (1 + p.drafts) + which) * p.pieces + piece] = mine;
   }
 }
@@ -595,7 +601,7 @@ __global__ __launch_bounds__(64 * kWaves) void bsg_verify_walk_kernel(VerifyPara
       v.sum = wave_sum<32>(v.sum);
     } else {
       for (uint64_t m = refused; m; m &= m - 1) x.drop(__builtin_amdgcn_readlane(id, __builtin_ctzll(m)), shift, piece, lane);
-      v = piece_of<T>(x, greedy, true, k, piece * kPiece - shift, lane);
+      v = piece_of<false, T>(x, greedy, true, k, piece * kPiece - shift, lane);
     }
     if (lane == 0) store_piece(last + piece, v);
   }
