@@ -206,25 +206,26 @@ def test_no_spills_and_no_packed_floats(asm):
         assert not re.search(r"\bv_pk_(add|mul|fma)_f32", text), unit
 
 
-def test_tree_steps_issue_their_loads(asm):
-    """As for prompts: a step's keys and values are waited for by the count of loads, so between two barriers of the
-    pipeline each wave issues exactly that many, in one run of instructions."""
+def test_tree_steps_wait_for_their_loads(asm):
+    """A pair of steps' keys and values come straight into LDS: where waves meet before it, each has waited for all of its
+    own, and then asks for the next pair's."""
     found = 0
     for name, body in _functions(asm["kv_tree.hip"], r"_ZN12_GLOBAL__N_118bsg_kv_tree_kernel"):
-        loads = 2 * int(re.search(r"Li(\d+)E", name).group(1)) // 64
-        steps = 0
+        d, rows = (int(x) for x in re.findall(r"Li(\d+)E", name))
+        pairs = 0
         for i, line in enumerate(body):
             if not line.strip().startswith("s_barrier"):
                 continue
-            # what comes before the step's first product, or the next barrier
+            # what comes before the pair's first product, or the next barrier
             after = next((j for j in range(i + 1, len(body)) if "mfma" in body[j] or body[j].strip().startswith("s_barrier")), len(body))
-            lines = [j for j in range(i, after) if body[j].rstrip().endswith(" lds") or " lds" in body[j]]
+            lines = [j for j in range(i, after) if " lds" in body[j]]
             if after == len(body) or "mfma" not in body[after] or not lines:
                 continue
-            assert len(lines) == loads, name
-            assert not any(re.match(r"\s*(s_cbranch|\.LBB)", x) for x in body[lines[0]:lines[-1]]), name
-            steps += 1
-        assert steps == 3, (name, steps)
+            assert len(lines) == 2 * (2 * d // 64), name
+            waited = max(j for j in range(i) if "vmcnt(0)" in body[j])
+            assert not any(re.match(r"\s*(buffer|global|flat)_|\.LBB", x) for x in body[waited:i]), name
+            pairs += 1
+        assert pairs == 2 * rows // 64, (name, pairs)  # large tiles have small ones beside them
         found += 1
     assert found == 8  # two types x two head sizes x two tiles
 

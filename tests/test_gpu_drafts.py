@@ -310,6 +310,15 @@ def test_tree_split(dev, hq, heads, nodes, lengths, max_len):
     _attend(dev, rng, lengths, [nodes] * len(lengths), hq, heads, 64, 64, torch.bfloat16, max_len=max_len)
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("hq,heads,p,d", [(1, 1, 16, 128), (4, 2, 64, 64), (4, 1, 16, 128), (10, 2, 128, 64), (21, 7, 32, 128)])
+@pytest.mark.parametrize("lengths,new", [([3000, 900, 70, 1500, 5000], [64, 33, 17, 48, 21]), ([64, 1025, 2112], [64, 1, 50]),
+                                         ([40] * 40 + [2000], [34] * 40 + [43])])
+def test_tree_uneven_batches(dev, dtype, hq, heads, p, d, lengths, new):
+    """Work dealt out over sequences of very unequal lengths and tiles of unequal rows."""
+    _attend(dev, np.random.default_rng([hq, len(new)]), lengths, new, hq, heads, p, d, DT[dtype])
+
+
 @pytest.mark.parametrize("nodes,hq", [(9, 2), (30, 2), (40, 4)])
 def test_tree_odd_parents_and_slots(dev, nodes, hq):
     """Parents that are no earlier node make roots; slots out of range and trees of more nodes than the sequence has
