@@ -110,7 +110,8 @@ __device__ __forceinline__ float largest4(uint32_t w, float by) {  // of four ca
 template <int D, int KV>
 struct Movers {
   static constexpr int LANES = KV == 0 ? D / 16 : D / 4, EACH = 64 / LANES;  // lanes of a token, tokens of a load
-  static constexpr int LOADS = KV == 0 ? 1 : 4, TOKENS = LOADS * EACH;       // in flight
+  // in flight; few paths move more (64 paths below: 16.2 us, with four loads of the values 16.9, with two and eight 17.9)
+  static constexpr int LOADS = KV == 0 ? 1 : 2, TOKENS = LOADS * EACH;
   u32x4 v[LOADS];
   // Offset of a lane's 16 bytes of the token at place t of a page.
   static __device__ __forceinline__ int at(int t, int lane) {
@@ -122,15 +123,18 @@ struct Movers {
   __device__ __forceinline__ void load(const int4& move, int m, int end, int lane, const Bytes& bytes) {
 #pragma unroll
     for (int k = 0; k < LOADS; ++k) {
+      if (m + k * EACH >= end) break;
       const int i = m + k * EACH + lane / LANES, from = i < end ? i : m;
       const int page = from_lane(move.x, from), t = from_lane(move.z, from);
-      v[k] = *(const u32x4*)(bytes(page) + at(t, lane));
+      v[k] = u32x4{0u, 0u, 0u, 0u};
+      if (i < end) v[k] = *(const u32x4*)(bytes(page) + at(t, lane));
     }
   }
   template <typename Bytes>
   __device__ __forceinline__ void store(const int4& move, float ss, float ds, int m, int end, int lane, const Bytes& bytes) {
 #pragma unroll
     for (int k = 0; k < LOADS; ++k) {
+      if (m + k * EACH >= end) break;
       const int i = m + k * EACH + lane / LANES, from = i < end ? i : m;
       const int page = from_lane(move.y, from), t = from_lane(move.w, from), was = from_lane(move.z, from) & 3;
       const float a = from_lane(ss, from), b = from_lane(ds, from);
@@ -151,6 +155,7 @@ struct Movers {
     float r = 0.f;
 #pragma unroll
     for (int k = 0; k < LOADS; ++k) {
+      if (m + k * EACH >= end) break;
       const int i = m + k * EACH + lane / LANES, from = i < end ? i : m;
       const int was = from_lane(move.z, from) & 3;
       const float a = from_lane(ss, from);
@@ -213,7 +218,7 @@ __device__ __forceinline__ void keep(Movers<D, KV>& held, const int4& move, floa
 constexpr int kWaves = 4;
 
 // Latency and half-used sectors bound it: a token's keys are 16 bytes here and there, its values a byte of each dword, so that
-// 64 paths in trees of 16, 8 layers x 32 heads, 14 MB, read 33 and write 16: 18 us, after 4 of the plan.  (A work-group a
+// 64 paths in trees of 16, 8 layers x 32 heads, 14 MB, read 33 and write 16: 16 us, after 4 of the plan.  (A work-group a
 // sequence and layer, which works out the plan by itself and takes the page through LDS: 28 + 5.)
 template <int D>
 __global__ __launch_bounds__(64 * kWaves) void bsg_pages_keep_kernel(KeepParams p) {
