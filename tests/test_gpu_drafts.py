@@ -941,3 +941,68 @@ def test_a_run_of_steps(dev, dtype, captured):
         largest = 2.0 ** np.ceil(np.log2(np.abs(want).max() * 1.1 / 448))
         got = c.read(0, slot)[0].double().cpu().numpy()
         assert (np.abs(got - want) <= off + 2.0 ** -4 * (np.abs(want) + off) + (1 + 2 * steps) * 2.0 ** -10 * largest).all()
+
+
+def test_calls_without_anything_to_do(dev):
+    """No tokens, no sequences, no nodes: nothing is written, and what comes back has the shapes."""
+    cache = bsa.KVCache(2, 8, 2, 64, 16, 3, 2, dev)
+    before = [x.clone() for x in (cache.pages.view(torch.uint8), cache.scales, cache.page_table, cache.lengths, cache.refcounts)]
+    cos, sin = (torch.from_numpy(x).to(dev) for x in _angles(8, 64))
+    none = torch.zeros(0, dtype=torch.int32, device=dev)
+    for rows in (0, 3):
+        cu, slots = torch.zeros(rows + 1, dtype=torch.int32, device=dev), _i32(list(range(rows)), dev)
+        q, k = (torch.zeros(0, h, 64, dtype=torch.float16, device=dev) for h in (4, 2))
+        batch = dict(cu_seqlens=cu, max_new=5, slots=slots)
+        assert cache.append_rotated(1, q, k, k, cos, sin, parents=none, **batch).shape == (0, 4, 64)
+        out, lse = cache.attend_tree(1, q, none, **batch)
+        assert out.shape == (0, 4, 64) and lse.shape == (0, 4)
+        got = bsa.verify_drafts(torch.zeros(0, 50, device=dev), none, torch.zeros(0, device=dev), none, cu_seqlens=cu, max_new=5)
+        assert got.accepted.tolist() == [0] * rows and got.path.shape[0] == rows and (got.path == -1).all() and (got.tokens == -1).all()
+        cache.keep(torch.zeros(rows, 5, dtype=torch.int32, device=dev), torch.ones(rows, dtype=torch.int32, device=dev), cu_seqlens=cu, slots=slots)
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(before, (cache.pages.view(torch.uint8), cache.scales, cache.page_table, cache.lengths, cache.refcounts)))
+
+
+@pytest.mark.parametrize("nodes,hq", [(8, 2), (40, 4)])
+def test_tree_strided_q_and_out(dev, nodes, hq):
+    """q and out as slices of wider tensors; what lies between them is left as it is."""
+    rng = np.random.default_rng(nodes)
+    lengths, cu = [90, 300], [0, nodes, 2 * nodes]
+    raw, sc, table, pages, scales, tab = _cache(rng, dev, lengths, 2, 32, 128, poison=True)
+    parents = _parents(rng, nodes) + _parents(rng, nodes)
+    wide = torch.randn(2 * nodes, 2 * hq + 3, 128, device=dev).half()
+    out = torch.full((2 * nodes + 1, 4 * hq, 136), 7.0, dtype=torch.float16, device=dev)
+    q, y = wide[:, 2:2 + 2 * hq], out[1:, ::2, :128]
+    ref = dft.tree_attention(q.double().cpu().numpy(), parents, orc.Layer(raw, sc), table, np.array(lengths), cu)
+    got, lse = bsa.kv_tree_attention(q, _i32(parents, dev), pages, scales, tab, _i32(lengths, dev), max_new=nodes, out=y)
+    assert got is y
+    _check_attention(y, lse, ref, torch.float16, 128)
+    y.fill_(7.0)
+    assert (out == 7.0).all()
+
+
+@pytest.mark.parametrize("nodes,hq", [(12, 8), (50, 16)])
+def test_pages_past_four_gigabytes(dev, nodes, hq):
+    """The last pages of a pool of 4.4 GB give what its first ones do."""
+    heads, p, d, count = 8, 128, 128, 17000
+    rng = np.random.default_rng(nodes)
+    pages = torch.empty(1, count, heads, 2, p, d, dtype=torch.uint8, device=dev)
+    scales = torch.ones(1, count, heads, 2, device=dev)
+    first = torch.from_numpy(rng.integers(0, 120, (3, heads, 2, p, d)).astype(np.uint8)).to(dev)
+    length = 2 * p + 20
+    q, k, v = (torch.from_numpy(rng.standard_normal((nodes, h, d)).astype(np.float32)).half().to(dev) for h in (hq, heads, heads))
+    cos, sin = (torch.from_numpy(x).to(dev) for x in _angles(400, d))
+    parents = _i32(_parents(rng, nodes), dev)
+    path = _i32([sorted(rng.choice(nodes, 6, replace=False).tolist()) + [-1] * (nodes - 6)], dev)
+    results = []
+    for at in (0, count - 3):
+        pages[0, at:at + 3], scales[0, at:at + 3] = first, 2.0 ** -8
+        tab, n, refs = _i32([[at, at + 1, at + 2]], dev), _i32([length], dev), torch.ones(count, dtype=torch.int32, device=dev)
+        args = (pages[0].view(F8), scales[0], tab, n)
+        y = bsa.kv_append_rotated(q, k, v, cos, sin, *args, parents=parents)
+        out, lse = bsa.kv_tree_attention(y, parents, *args)
+        bsa.pages_keep(pages.view(F8), scales, tab, n, refs, path, _i32([6], dev))
+        torch.cuda.synchronize()
+        results.append([x.clone() for x in (y, out, lse, pages[0, at:at + 3], scales[0, at:at + 3], n)] + [refs[at:at + 3].tolist()])
+    assert all(torch.equal(a, b) for a, b in zip(results[0][:-1], results[1][:-1])) and results[0][-1] == results[1][-1]
+    assert results[0][5].tolist() == [length - nodes + 6] and not torch.equal(results[0][3], first)
