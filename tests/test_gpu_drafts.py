@@ -319,6 +319,26 @@ def test_tree_uneven_batches(dev, dtype, hq, heads, p, d, lengths, new):
     _attend(dev, np.random.default_rng([hq, len(new)]), lengths, new, hq, heads, p, d, DT[dtype])
 
 
+@pytest.mark.parametrize("rows", [65, 130])
+def test_tree_of_many_sequences(dev, rows):
+    """More work-groups than begin at once: the longest sequences' first, of each 64; equal ones, empty ones, slots out of range."""
+    rng = np.random.default_rng(rows)
+    lengths = rng.choice([34, 40, 41, 90, 130], rows + 3).tolist()
+    lengths[3] = lengths[70 % rows] = 0
+    slots = rng.permutation(rows + 3)[:rows].tolist()
+    slots[5], slots[rows - 1] = -1, rows + 3
+    raw, sc, table, pages, scales, tab = _cache(rng, dev, lengths, 10, 16, 64, poison=True)
+    new = rng.choice([33, 34], rows).tolist()
+    cu = _cu(new)
+    parents = [x for n in new for x in _parents(rng, n)]
+    q = torch.randn(cu[-1], 10, 64, device=dev).half()
+    with np.errstate(invalid="ignore"):
+        ref = dft.tree_attention(q.double().cpu().numpy(), parents, orc.Layer(raw, sc), table, np.array(lengths), cu, slots)
+    got, lse = bsa.kv_tree_attention(q, _i32(parents, dev), pages, scales, tab, _i32(lengths, dev), cu_seqlens=_i32(cu, dev),
+                                     max_new=34, slots=_i32(slots, dev))
+    _check_attention(got, lse, ref, torch.float16, 64)
+
+
 @pytest.mark.parametrize("nodes,hq", [(9, 2), (30, 2), (40, 4)])
 def test_tree_odd_parents_and_slots(dev, nodes, hq):
     """Parents that are no earlier node make roots; slots out of range and trees of more nodes than the sequence has

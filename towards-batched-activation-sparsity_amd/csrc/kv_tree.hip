@@ -18,6 +18,7 @@ namespace {
 struct TreeParams {
   AttnParams a;
   int32_t tiles, groups, rows;  // of a cached head, at most; work-groups (0: one for each unit, and no parts); sequences
+  int32_t sorted;               // without a deal: long sequences first
   uint2* units;   // [sequence][head][tile]: the first work-group that has a part, how many have
   float* parts;   // [work-group][2]: of the unit that it finishes, of the one that it begins
 };
@@ -35,6 +36,10 @@ constexpr uint32_t kWeight = 8, kSmallWeight = 5, kBegin = 24;
 // 600 21 / 19, 128 of them 22 / 25, of 300 17 / 22.
 constexpr int kDealUnits = 2;
 constexpr int kDealTokens = 768;
+// Work-groups for each unit begin with the longest sequences where not all have room at once (two a compute unit have) and there
+// are fewer than kSortUnits a compute unit, so that the last ones to begin matter.  As they come / sorted, us: 1024 units of up to
+// 2000 tokens 99 / 82; 2048 of up to 1000 113 / 115; 512, which begin at once, 51 / 54 and 80 / 78.
+constexpr int kSortUnits = 6;
 // Two waves share a SIMD, and the older one goes first, so that it ends early and the other one has nobody beside it for the
 // rest (at 60 and 100 us in the case below).  Every 2^kTurn cycles the other one has priority: 97 us in all, 102 without.
 constexpr int kTurn = 14;
@@ -81,6 +86,24 @@ constexpr uint32_t kTileWeight = ROWS == kSmallRows ? kSmallWeight : kWeight;
 template <int ROWS>
 __device__ __forceinline__ uint32_t weight_of(const AttnParams& p, const Branch& b) {  // of a step of all tiles of a head
   return b.count == 0 ? 0 : tiles_of<ROWS>(p, b) * kTileWeight<ROWS> - (ends_small<ROWS>(p, b) ? kTileWeight<ROWS> - kSmallWeight : 0);
+}
+
+// The sequence of work-group z where those of long sequences come first, of each 64.
+__device__ __forceinline__ int longest_first(const AttnParams& p, int rows) {
+  const int lane = threadIdx.x & 63, of = blockIdx.z & ~63, row = of + lane;
+  int len = -1;
+  if (row < rows) {
+    const int slot = p.slots ? p.slots[row] : row;
+    len = slot >= 0 && slot < p.num_slots ? p.lengths[slot] : 0;
+    if (len < 0) len = 0;
+  }
+  int before = 0;
+#pragma unroll 8
+  for (int i = 0; i < 64; ++i) {
+    const int other = __builtin_amdgcn_readlane(len, i);
+    before += other > len || (other == len && i < lane);
+  }
+  return of + __builtin_ctzll(__ballot(before == (int)(blockIdx.z & 63)));
 }
 
 // A work-group of four waves has a tile of rows, each wave 32 of them, and takes the tokens they see 64 at a time,
@@ -167,7 +190,7 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_tree_kernel(TreeParams tp) {
       pos = step1 == steps ? unit_at + steps * weight : stop;
       if (step0 >= step1) continue;
     } else {
-      row = blockIdx.z, head = blockIdx.x / tp.tiles;
+      row = tp.sorted ? longest_first(p, tp.rows) : blockIdx.z, head = blockIdx.x / tp.tiles;
       b = branch_of(p, row);
       rt = blockIdx.x - head * tp.tiles;
       step1 = steps = steps_of(b);
@@ -545,7 +568,7 @@ constexpr int kTileRows = 32;
 // the steps, or, 0, each unit has one.
 struct Cut {
   Shape shape;
-  int32_t groups;
+  int32_t groups, sorted;
   int64_t units, bytes;  // of the second kernel: units at most; of the workspace
 };
 Cut cut_of(int32_t rows, const bsg_kv_cache* cache, int32_t group, int32_t max_new, int64_t max_len, int32_t cus) {
@@ -559,6 +582,7 @@ Cut cut_of(int32_t rows, const bsg_kv_cache* cache, int32_t group, int32_t max_n
   s.row_tiles = (int32_t)ceil_div(per_head, s.rows);
   const int64_t tiles = (int64_t)rows * kv_heads * s.row_tiles;
   c.groups = 0, c.units = tiles;
+  c.sorted = rows > 1 && tiles > (int64_t)kDealUnits * cus && tiles < (int64_t)kSortUnits * cus;
   if (max_len < 1) max_len = 1;
   s.chunk = (int32_t)(ceil_div(max_len, 128) * 128), s.splits = 1;
   if (s.rows >= kSmallRows) {
@@ -602,7 +626,7 @@ void launch(const AttnParams& p, const Cut& c, int32_t rows, hipStream_t st) {
   }
   TreeParams t;
   t.a = p;
-  t.tiles = s.row_tiles, t.groups = c.groups, t.rows = rows;
+  t.tiles = s.row_tiles, t.groups = c.groups, t.rows = rows, t.sorted = c.sorted;
   t.units = (uint2*)((uint8_t*)p.counters + BSG_KV_COUNTER_BYTES);
   t.parts = (float*)((uint8_t*)t.units + ceil_div(c.units * 8, 256) * 256);
   if (s.rows == kSmallRows) launch_tiles<T, D, kSmallRows>(t, c, st);
