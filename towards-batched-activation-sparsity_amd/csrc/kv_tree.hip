@@ -163,6 +163,7 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_tree_kernel(TreeParams tp) {
     pos = (uint32_t)begin;
     stop = total - pos > per ? pos + per : total;
   }
+  const int own_row = __builtin_amdgcn_readfirstlane(tp.sorted ? longest_first(p, tp.rows) : (int)blockIdx.z);
   while (pos < stop) {
     int row, head, rt, step0 = 0, step1, steps;
     uint32_t unit_at = 0, weight = 1;  // where the unit's weights begin, the weight of its steps
@@ -190,7 +191,7 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_tree_kernel(TreeParams tp) {
       pos = step1 == steps ? unit_at + steps * weight : stop;
       if (step0 >= step1) continue;
     } else {
-      row = tp.sorted ? longest_first(p, tp.rows) : blockIdx.z, head = blockIdx.x / tp.tiles;
+      row = own_row, head = blockIdx.x / tp.tiles;
       b = branch_of(p, row);
       rt = blockIdx.x - head * tp.tiles;
       step1 = steps = steps_of(b);
