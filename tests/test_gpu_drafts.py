@@ -976,6 +976,8 @@ def test_calls_without_anything_to_do(dev):
         assert cache.append_rotated(1, q, k, k, cos, sin, parents=none, **batch).shape == (0, 4, 64)
         out, lse = cache.attend_tree(1, q, none, **batch)
         assert out.shape == (0, 4, 64) and lse.shape == (0, 4)
+        used = [torch.full((n,), 9, dtype=torch.int32, device=dev) for n in (3, 3, 3, 15, 15)]
+        del used  # memory that the answers are given holds something
         got = bsa.verify_drafts(torch.zeros(0, 50, device=dev), none, torch.zeros(0, device=dev), none, cu_seqlens=cu, max_new=5)
         assert got.accepted.tolist() == [0] * rows and got.path.shape[0] == rows and (got.path == -1).all() and (got.tokens == -1).all()
         cache.keep(torch.zeros(rows, 5, dtype=torch.int32, device=dev), torch.ones(rows, dtype=torch.int32, device=dev), cu_seqlens=cu, slots=slots)

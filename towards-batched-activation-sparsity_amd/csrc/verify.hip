@@ -706,8 +706,8 @@ extern "C" int bsg_verify_drafts(const void* logits, int64_t logits_stride, cons
   if (draft_logits && parents) return fail(BSG_ERR_UNSUPPORTED, "draft_logits go with chains: parents must be NULL");
   if (!temperatures && !(temperature >= 0.f && temperature < __builtin_inff()))
     return fail(BSG_ERR_ARG, "temperature=%g", temperature);
-  if (rows == 0 || max_new == 0) return BSG_OK;
-  if (!accepted || !path || !out_tokens)
+  if (rows == 0) return BSG_OK;
+  if (!accepted || (max_new > 0 && (!path || !out_tokens)))
     return fail(BSG_ERR_ARG, "null pointer (accepted=%p path=%p out_tokens=%p)", (void*)accepted, (void*)path, (void*)out_tokens);
   if (tokens > 0 && (!logits || !token_ids || !uniforms))
     return fail(BSG_ERR_ARG, "null pointer (logits=%p token_ids=%p uniforms=%p)", logits, (const void*)token_ids, (const void*)uniforms);
