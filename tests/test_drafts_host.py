@@ -149,6 +149,26 @@ def test_bad_verifications_are_refused():
     assert lib.bsg_verify_drafts_workspace_bytes(8, 2, 0, 4, 0, 0) == -1
 
 
+def test_a_verification_of_slots_is_one_of_the_others():
+    """bsgdraft_slots.h declares what ctypes calls, and its checks are bsg_verify_drafts's, whatever slots are."""
+    text = re.sub(r"/\*.*?\*/", "", open(os.path.join(ROOT, "include", "bsgdraft_slots.h")).read(), flags=re.S)
+    assert re.findall(r"\b(bsg_[a-z0-9_]+)\s*\(", text) == ["bsg_verify_drafts_slots"]
+    declared = re.search(r"bsg_verify_drafts_slots\s*\((.*?)\);", text, re.S).group(1)
+    types = _lib.SIGNATURES["bsg_verify_drafts_slots"][1]
+    assert len(declared.split(",")) == len(types)
+    plain = _lib.SIGNATURES["bsg_verify_drafts"][1]
+    assert types[:10] + types[11:] == plain and declared.split(",")[10].split() == ["const", "int32_t*", "slots"]
+    args = [FAKE, 1000, None, 1000, 8, 1000, FAKE, FAKE, None, None, FAKE, 2, 4, 1.0, None, FAKE, FAKE, FAKE, 0, FAKE, 1 << 30, None]
+    lib = bsa.load()
+    for i, bad, code in ((0, None, _lib.BSG_ERR_ARG), (4, 7, _lib.BSG_ERR_ARG), (15, None, _lib.BSG_ERR_ARG), (18, 3, _lib.BSG_ERR_DTYPE),
+                         (12, 65, _lib.BSG_ERR_ARG), (19, None, _lib.BSG_ERR_WORKSPACE), (20, 64, _lib.BSG_ERR_WORKSPACE)):
+        for slots in (FAKE, None):
+            call = args[:i] + [bad] + args[i + 1:]
+            call[10] = slots
+            assert lib.bsg_verify_drafts_slots(*call) == (_lib.BSG_ERR_UNSUPPORTED if bad == 65 else code), (i, slots)
+    assert lib.bsg_verify_drafts_slots(*args[:4], 0, *args[5:11], 0, *args[12:]) == 0  # no sequences
+
+
 def test_bad_keeps_are_refused():
     lib = bsa.load()
 

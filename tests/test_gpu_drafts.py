@@ -682,6 +682,64 @@ def test_verify_leaves_the_targets_distribution(dev, kind):
     assert ((share - want).abs() <= 5 * (want * (1 - want) / rows).sqrt()).all()
 
 
+@pytest.mark.parametrize("kind", ["trees", "drawn", "greedy"])
+@pytest.mark.parametrize("vocab", [300, 32000])
+def test_verify_leaves_sequences_out(dev, kind, vocab):
+    """A slot below 0: nothing accepted, no path, no tokens, whatever the sequence's rows hold; the others as without it.
+    Eager, of equal sequences without offsets, all left out, and captured with other slots at each replay."""
+    rng = np.random.default_rng([vocab, len(kind)])
+    new = [5, 3, 1, 0, 8, 5]
+    x, parents, tokens, u = _drafts(rng, [n for n in new if n], vocab, kind == "trees")
+    temperature = 0.0 if kind == "greedy" else 0.8
+    logits = torch.from_numpy(x).half().to(dev)
+    draft = (logits.float() + 0.5 * torch.randn(logits.shape, device=dev)).half() if kind == "drawn" else None
+    par = _i32(parents, dev) if kind == "trees" else None
+    ids, nums, cu = _i32(tokens, dev), torch.from_numpy(u).to(dev), _i32(_cu(new), dev)
+    host = (logits.double().cpu().numpy(), tokens, u, parents if par is not None else None, None if draft is None else draft.double().cpu().numpy(),
+            temperature)
+    want = dft.verify(*host, _cu(new))
+    left_out = (0, [], [])
+
+    def expected(slots):
+        return [w if s >= 0 else left_out for w, s in zip(want, slots)]
+
+    def call(slots):
+        return bsa.verify_drafts(logits, ids, nums, par, draft, temperature, cu, 8, slots=slots)
+
+    first, last = [4, -1, -9, 0, 70000, -(2 ** 31)], [-1, 3, 2, -1, -1, 2 ** 31 - 1]
+    kept = logits.clone()
+    logits[5:9], logits[17:] = float("nan"), float("inf")  # of the ones that are left out at first
+    for _ in range(2):
+        _same_verdict(call(_i32(first, dev)), expected(first), 8)
+    logits.copy_(kept)
+    for slots in (last, [-1] * 6, [0] * 6):
+        _same_verdict(call(_i32(slots, dev)), expected(slots), 8)
+    _same_verdict(call(None), want, 8)
+    # sequences of equally many tokens, the last one and the first one of which are left out
+    each = torch.cat([torch.arange(5), torch.arange(9, 14), torch.arange(17, 22)]).to(dev)
+    even = (logits[each], ids[each], nums[each], None if par is None else par[each], None if draft is None else draft[each], temperature)
+    verdict = [want[0], None, want[5]]
+    for slots in ([3, -1, -1], [-1, -1, 5]):
+        got = bsa.verify_drafts(*even, max_new=5, slots=_i32(slots, dev))
+        _same_verdict(got, [w if s >= 0 else left_out for w, s in zip(verdict, slots)], 5)
+    held = _i32(first, dev)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(held)
+    for slots in (first, last, [-1] * 6, [1] * 6, first):
+        held.copy_(_i32(slots, dev))
+        [t.fill_(99) for t in out]
+        graph.replay()
+        eager = call(held)
+        torch.cuda.synchronize()
+        _same_verdict(out, expected(slots), 8)
+        _same_verdict(eager, expected(slots), 8)
+    for bad, error in ((held.long(), TypeError), (held[:5], ValueError), (held.cpu(), ValueError), (_i32([0] * 12, dev)[::2], ValueError)):
+        with pytest.raises(error):
+            call(bad)
+
+
 def test_verify_graph_threads_and_prefix(dev):
     rng = np.random.default_rng(8)
     new = [5, 3, 8, 1]

@@ -165,7 +165,7 @@ _pkv = ctypes.POINTER(KvCache)
 _ppool = ctypes.POINTER(PagePool)
 _protary = ctypes.POINTER(Rotary)
 
-# name -> (restype, argtypes); every function declared in include/bsgemm.h, bsgserve.h and bsgdraft.h
+# name -> (restype, argtypes); every function declared in include/bsgemm.h, bsgserve.h, bsgdraft.h and bsgdraft_slots.h
 SIGNATURES = {
     "bsg_version": (ctypes.c_char_p, []),
     "bsg_last_error": (ctypes.c_char_p, []),
@@ -209,7 +209,7 @@ SIGNATURES = {
     "bsg_pages_compact": (_int, [_ppool, _vp, _vp, _i64, _vp]),
     "bsg_token_logprobs_workspace_bytes": (_i64, [_i64, _i64, _i32, _int, _i32]),
     "bsg_token_logprobs": (_int, [_vp, _i64, _i64, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _int, _vp, _i64, _i32, _vp]),
-    # include/bsgdraft.h
+    # include/bsgdraft.h, bsgdraft_slots.h
     "bsg_kv_append_rotated": (_int, [_vp, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _protary,
                                      _pkv, _vp, _i32, _vp, _i32, _int, _vp]),
     "bsg_kv_tree_attention_workspace_bytes": (_i64, [_pkv, _i32, _i32, _i32, _i64, _i32]),
@@ -218,6 +218,8 @@ SIGNATURES = {
     "bsg_verify_drafts_workspace_bytes": (_i64, [_i64, _i32, _i64, _i32, _int, _i32]),
     "bsg_verify_drafts": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i32, _i32, _f32, _vp, _vp, _vp, _vp,
                                  _int, _vp, _i64, _vp]),
+    "bsg_verify_drafts_slots": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _f32, _vp, _vp, _vp,
+                                       _vp, _int, _vp, _i64, _vp]),
     "bsg_pages_keep_workspace_bytes": (_i64, [_i32]),
     "bsg_pages_keep": (_int, [_ppool, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _i64, _vp]),
     # include/bsgemm_timeline.h

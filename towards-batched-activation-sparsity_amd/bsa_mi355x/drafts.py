@@ -6,7 +6,7 @@
     pages_keep         the accepted tokens stay in the cache, the others leave it
 
 All of it runs on the device with no host round trip (csrc/kv_rotate.hip, kv_tree.hip, verify.hip, pages_keep.hip
-through include/bsgdraft.h), on torch's current stream, and can be captured.  The reference decodes one token at a
+through include/bsgdraft.h and bsgdraft_slots.h), on torch's current stream, and can be captured.  The reference decodes one token at a
 time, so these have no counterpart there.
 
 A tree is the newest tokens of a sequence, its nodes, at most 64 of them.  parents int32 [tokens] holds for each
@@ -14,7 +14,7 @@ token its parent's place among its sequence's new tokens; what names no earlier 
 step: pages_extend gives every node a place, kv_append_rotated and kv_tree_attention run in each layer, verify_drafts
 reads the logits, and pages_keep leaves the accepted nodes behind the tokens that were there before.  Batches
 (cu_seqlens, max_new, slots) are described as in serving.py.  A sequence that pages_extend had no room for takes no
-part: its slot is -1 in the calls that follow.
+part: its slot is -1 in the calls that follow, verify_drafts among them.
 """
 from __future__ import annotations
 
@@ -191,7 +191,7 @@ class Verified(NamedTuple):
 def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Tensor, parents: Optional[torch.Tensor] = None,
                   draft_logits: Optional[torch.Tensor] = None, temperature: Union[float, torch.Tensor] = 1.0,
                   cu_seqlens: Optional[torch.Tensor] = None, max_new: Optional[int] = None,
-                  workspace_prefix: Optional[str] = None) -> Verified:
+                  workspace_prefix: Optional[str] = None, slots: Optional[torch.Tensor] = None) -> Verified:
     """Which drafted tokens the target model accepts, and the token that follows them, from given random numbers.
 
     Row t of logits [tokens, vocab] (fp16, bf16 or fp32, any row stride) is the target's after token t; tokens int32,
@@ -210,24 +210,25 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Te
     come out are then distributed as the target's own.  temperature is a finite number from 0 on, or fp32 [sequences], by which
     0 or less (or NaN) is greedy and infinity makes all tokens of finite logits alike.  Decisions are those of 64-bit
     weights and sums.  A row of logits with NaN, +inf, or nothing but -inf ends its path with a new token of -1; a token
-    outside the vocabulary is rejected.  At most 64 tokens a sequence, 2^20 in the vocabulary, 16384 sequences."""
+    outside the vocabulary is rejected.  slots (int32 [sequences]) are the batch's: one below 0 leaves its sequence out, which
+    then has nothing accepted, no path and no tokens, whatever its logits hold.  At most 64 tokens a sequence, 2^20 in the vocabulary, 16384 sequences."""
     if max_new is not None:
         max_new = int(max_new)
     each = temperature if isinstance(temperature, torch.Tensor) else None
-    key = ("verify", _sigs(logits, tokens, uniforms, parents, draft_logits, each, cu_seqlens), max_new)
+    key = ("verify", _sigs(logits, tokens, uniforms, parents, draft_logits, each, cu_seqlens, slots), max_new)
     call = _CALLS.get(key)
     if call is None:
-        call = _remember(key, _verify_call(logits, tokens, uniforms, parents, draft_logits, each, cu_seqlens, max_new))
+        call = _remember(key, _verify_call(logits, tokens, uniforms, parents, draft_logits, each, cu_seqlens, max_new, slots))
     index, fn, rows, most, vocab, count, stride, draft_stride, code, need, molds = call
     out = Verified(*map(torch.empty_like, molds))
     held = _workspace(index, need, workspace_prefix)
     _launch(index, fn, logits.data_ptr(), stride, _ptr(draft_logits), draft_stride, count, vocab, tokens.data_ptr(),
-            uniforms.data_ptr(), _ptr(parents), _ptr(cu_seqlens), rows, most, 0.0 if each is not None else temperature, _ptr(each),
+            uniforms.data_ptr(), _ptr(parents), _ptr(cu_seqlens), _ptr(slots), rows, most, 0.0 if each is not None else temperature, _ptr(each),
             out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), code, held.data_ptr(), held.numel())
     return out
 
 
-def _verify_call(logits, tokens, uniforms, parents, draft_logits, temperatures, cu_seqlens, max_new) -> tuple:
+def _verify_call(logits, tokens, uniforms, parents, draft_logits, temperatures, cu_seqlens, max_new, slots) -> tuple:
     """The checks of verify_drafts and what follows from its arguments' shapes."""
     dev = _require_cuda(logits)
     if logits.dtype not in _LOGIT_DTYPES:
@@ -260,6 +261,7 @@ def _verify_call(logits, tokens, uniforms, parents, draft_logits, temperatures, 
         if rows < 0:
             raise ValueError("cu_seqlens has no entries")
     _nodes(most)
+    _i32(slots, dev, "slots", rows)
     if temperatures is not None and (temperatures.dtype is not torch.float32 or temperatures.device != dev
                                      or temperatures.shape != (rows,) or not temperatures.is_contiguous()):
         raise ValueError(f"temperature must be a number or contiguous float32 [{rows}] on {dev}, got {tuple(temperatures.shape)} "
@@ -270,7 +272,7 @@ def _verify_call(logits, tokens, uniforms, parents, draft_logits, temperatures, 
     if need < 0:
         raise _lib.BsgUnsupported(_lib.BSG_ERR_UNSUPPORTED, _lib.last_error())
     molds = [_mold(s, torch.int32, dev) for s in ((rows,), (rows, most), (rows, most))]
-    return (dev.index, lib.bsg_verify_drafts, rows, most, vocab, count, logits.stride(0),
+    return (dev.index, lib.bsg_verify_drafts_slots, rows, most, vocab, count, logits.stride(0),
             0 if draft_logits is None else draft_logits.stride(0), code, need, molds)
 
 

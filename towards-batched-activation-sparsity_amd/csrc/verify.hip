@@ -1,4 +1,5 @@
-// verify.hip — which drafted tokens a target model accepts, and the token that follows them (include/bsgdraft.h).
+// verify.hip — which drafted tokens a target model accepts, and the token that follows them (include/bsgdraft.h,
+// bsgdraft_slots.h).
 //
 // Answers are whole numbers next to borders: a number u against a ratio of probabilities, and the first running sum past
 // u of the whole.  So weights w = 2^((x - m) k), k = log2(e) / temperature, and their sums are 64-bit.  2^t is
@@ -15,7 +16,7 @@
 // weights in 32 bits, kNear off at most; where a number is as near as that to its border the wave adds the row again in
 // 64.  Against draft_logits the last row's sums are wanted exactly, and both are 64-bit from the start.
 
-#include "bsgdraft.h"
+#include "bsgdraft_slots.h"
 #include "draft_tree.hpp"
 
 using namespace bsgk;
@@ -45,6 +46,7 @@ struct VerifyParams {
   const float* uniforms;
   const int32_t* parents;
   const int32_t* cu;
+  const int32_t* slots;  // below 0: the sequence takes no part
   const float* temperatures;
   float temperature;
   int32_t rows, max_new, pieces, groups, drafts;  // pieces of a row, work-groups of a row
@@ -235,7 +237,7 @@ __device__ __forceinline__ Tree tree_of(const VerifyParams& p, int row, int lane
   t.temperature = p.temperatures ? p.temperatures[row] : p.temperature;
   // whose inverse is a 32-bit number other than 0, and infinity: no product with it is NaN
   if (t.temperature > 0.f) t.temperature = fminf(fmaxf(t.temperature, 0x1p-126f), 0x1.fffffep127f);
-  const bool fine = t.from >= 0 && t.from < to && to <= p.tokens;
+  const bool fine = t.from >= 0 && t.from < to && to <= p.tokens && !(p.slots && p.slots[row] < 0);
   t.count = !fine ? 0 : to - t.from < p.max_new ? (int)(to - t.from) : p.max_new;
   t.parent = load_parent(p.parents, t.from, t.count, lane);
   return t;
@@ -700,6 +702,17 @@ extern "C" int bsg_verify_drafts(const void* logits, int64_t logits_stride, cons
                                  const int32_t* parents, const int32_t* cu, int32_t rows, int32_t max_new,
                                  float temperature, const float* temperatures, int32_t* accepted, int32_t* path,
                                  int32_t* out_tokens, int dtype, void* ws, int64_t ws_bytes, void* stream) {
+  return bsg_verify_drafts_slots(logits, logits_stride, draft_logits, draft_stride, tokens, vocab, token_ids, uniforms, parents,
+                                 cu, nullptr, rows, max_new, temperature, temperatures, accepted, path, out_tokens, dtype, ws,
+                                 ws_bytes, stream);
+}
+
+extern "C" int bsg_verify_drafts_slots(const void* logits, int64_t logits_stride, const void* draft_logits,
+                                       int64_t draft_stride, int64_t tokens, int64_t vocab, const int32_t* token_ids,
+                                       const float* uniforms, const int32_t* parents, const int32_t* cu,
+                                       const int32_t* slots, int32_t rows, int32_t max_new, float temperature,
+                                       const float* temperatures, int32_t* accepted, int32_t* path, int32_t* out_tokens,
+                                       int dtype, void* ws, int64_t ws_bytes, void* stream) {
   if (const int rc = check_sizes(tokens, rows, vocab, max_new, dtype)) return rc;
   if (!cu && tokens != (int64_t)rows * max_new)
     return fail(BSG_ERR_ARG, "without cu, tokens=%lld must be rows x max_new = %lld", (long long)tokens, (long long)rows * max_new);
@@ -723,7 +736,7 @@ extern "C" int bsg_verify_drafts(const void* logits, int64_t logits_stride, cons
   p.x[0] = logits, p.x[1] = draft_logits;
   p.stride[0] = logits_stride, p.stride[1] = draft_stride;
   p.vocab = vocab, p.tokens = tokens;
-  p.ids = token_ids, p.uniforms = uniforms, p.parents = parents, p.cu = cu;
+  p.ids = token_ids, p.uniforms = uniforms, p.parents = parents, p.cu = cu, p.slots = slots;
   p.temperatures = temperatures, p.temperature = temperature;
   p.rows = rows, p.max_new = max_new, p.drafts = drafts;
   p.pieces = (int32_t)l.pieces, p.groups = (int32_t)ceil_div(l.pieces, kWaves);
