@@ -169,6 +169,17 @@ def test_a_verification_of_slots_is_one_of_the_others():
     assert lib.bsg_verify_drafts_slots(*args[:4], 0, *args[5:11], 0, *args[12:]) == 0  # no sequences
 
 
+def test_documented_last_tokens():
+    """INTEGRATION.md's line for what the next tree begins with, run as it stands: the new token, or, where nothing was accepted,
+    what it was before."""
+    line = next(x for x in open(os.path.join(ROOT, "INTEGRATION.md")).read().splitlines() if x.startswith("last = "))
+    got = drafts.Verified(torch.tensor([0, 1, 3, 0, 2], dtype=torch.int32), None,
+                          torch.tensor([[-1, -1, -1], [7, -1, -1], [4, 5, 6], [-1, -1, -1], [8, -1, -1]], dtype=torch.int32))
+    names = {"torch": torch, "got": got, "last": torch.tensor([11, 12, 13, 14, 15], dtype=torch.int32)}
+    exec(line, names)
+    assert names["last"].dtype is torch.int32 and names["last"].tolist() == [11, 7, 6, 14, -1]
+
+
 def test_bad_keeps_are_refused():
     lib = bsa.load()
 

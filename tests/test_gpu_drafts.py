@@ -1021,6 +1021,78 @@ def test_a_run_of_steps(dev, dtype, captured):
         assert (np.abs(got - want) <= off + 2.0 ** -4 * (np.abs(want) + off) + (1 + 2 * steps) * 2.0 ** -10 * largest).all()
 
 
+class _GappyToy(_Toy):
+    """Sequences that found no room, or have no nodes, take no part in a step; a sequence's last token is then what it was."""
+
+    def step(self, drafts, parents, cu, uniforms):
+        first = cu[:-1].long().clamp(max=len(drafts) - 1)
+        tokens = drafts.scatter(0, torch.where(cu.diff() > 0, first, len(drafts) - 1), self.last)
+        served = self.cache.extend(cu.diff().to(torch.int32), slots=self.slots)
+        own = self.slots
+        self.slots = torch.where(served > 0, own, -1)
+        logits = self.forward(tokens, cu, self.max_new, parents)
+        got = bsa.verify_drafts(logits, tokens, uniforms, parents, temperature=0.7, cu_seqlens=cu, max_new=self.max_new, slots=self.slots)
+        self.cache.keep(got.path, got.accepted, cu_seqlens=cu, slots=self.slots)
+        self.slots = own
+        new = got.tokens.gather(1, (got.accepted.long() - 1).clamp(min=0)[:, None])[:, 0]
+        self.last.copy_(torch.where(got.accepted > 0, new, self.last))
+        return tokens, logits, got, served
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_run_of_steps_some_take_no_part_in(dev, captured):
+    """Every other step the pool is full, so that who needs a page is refused; one sequence has no nodes.  Who takes no part keeps
+    its last token, its length and its bytes; the others' verdicts are the oracle's."""
+    rng = np.random.default_rng(21)
+    prompts = [rng.integers(0, 9, n).tolist() for n in (21, 5, 48, 30)]
+    slots = [4, 0, 2, 5]
+    toy = _GappyToy(dev, rng, prompts, torch.float16, slots)
+    sizes = [14, 9, 0, 1]
+    cu = _i32(_cu(sizes), dev)
+    # one row more than the sequences have: where a sequence without nodes puts its last token
+    drafts, uniforms, parents = _i32([0] * 25, dev), torch.zeros(25, device=dev), _i32([-1] * 25, dev)
+
+    def draw():
+        drafts.copy_(_i32(rng.integers(0, 9, 25), dev))
+        parents.copy_(_i32([x for n in sizes if n for x in _parents(rng, n)] + [-1], dev))
+        uniforms.copy_(torch.from_numpy(rng.random(25, dtype=np.float32)).to(dev))
+
+    if captured:
+        draw()
+        _GappyToy(dev, np.random.default_rng(9), prompts, torch.float16, slots).step(drafts, parents, cu, uniforms)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = toy.step(drafts, parents, cu, uniforms)
+    c, refused = toy.cache, 0
+    for step in range(8):
+        draw()
+        held = (c.refcounts == 0).int() * (step % 2)  # a full pool
+        c.refcounts.add_(held)
+        before, last = [c.read(1, s) for s in slots], toy.last.tolist()
+        if captured:
+            graph.replay()
+        else:
+            out = toy.step(drafts, parents, cu, uniforms)
+        torch.cuda.synchronize()
+        c.refcounts.sub_(held)
+        tokens, logits, got, served = out
+        want = dft.verify(logits.double().cpu().numpy(), tokens.cpu().numpy(), uniforms.cpu().numpy(), parents.cpu().numpy(), None, 0.7, _cu(sizes))
+        served = served.tolist()
+        refused += served.count(0)
+        _same_verdict(got, [w if ok else (0, [], []) for w, ok in zip(want, served)], 14)
+        for b, (slot, n) in enumerate(zip(slots, got.accepted.tolist())):
+            assert (n > 0) == (served[b] > 0 and sizes[b] > 0)
+            toy.seen[b] += got.tokens[b, :n].tolist()
+            assert toy.last[b].item() == (toy.seen[b][-1] if n else last[b]) and c.lengths[slot].item() == len(toy.seen[b]) - 1
+            if n == 0:
+                assert all(torch.equal(x, y) for x, y in zip(before[b], c.read(1, slot)))
+    assert refused
+    refs, table = c.refcounts.tolist(), c.page_table.tolist()
+    assert sum(refs) == sum(-(-n // 16) for n in c.lengths.tolist()) and max(refs) == 1
+    assert all(x < 0 for b, slot in enumerate(slots) for x in table[slot][-(-(len(toy.seen[b]) - 1) // 16):])
+
+
 def test_calls_without_anything_to_do(dev):
     """No tokens, no sequences, no nodes: nothing is written, and what comes back has the shapes."""
     cache = bsa.KVCache(2, 8, 2, 64, 16, 3, 2, dev)

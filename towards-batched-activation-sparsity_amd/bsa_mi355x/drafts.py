@@ -209,7 +209,8 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Te
     and drawn by the first token's number: the first token whose running sum exceeds it times the whole.  The tokens that
     come out are then distributed as the target's own.  temperature is a finite number from 0 on, or fp32 [sequences], by which
     0 or less (or NaN) is greedy and infinity makes all tokens of finite logits alike.  Decisions are those of 64-bit
-    weights and sums.  A row of logits with NaN, +inf, or nothing but -inf ends its path with a new token of -1; a token
+    weights and sums.  A row of logits with NaN, +inf, or nothing but -inf ends its path with a new token of -1, which is no
+    token for a next step: the sequence has failed; a token
     outside the vocabulary is rejected.  slots (int32 [sequences]) are the batch's: one below 0 leaves its sequence out, which
     then has nothing accepted, no path and no tokens, whatever its logits hold.  At most 64 tokens a sequence, 2^20 in the vocabulary, 16384 sequences."""
     if max_new is not None:
