@@ -1115,6 +1115,24 @@ def test_calls_without_anything_to_do(dev):
     assert all(torch.equal(x, y) for x, y in zip(before, (cache.pages.view(torch.uint8), cache.scales, cache.page_table, cache.lengths, cache.refcounts)))
 
 
+def test_batches_without_tokens_have_any_strides(dev):
+    """An empty array's tensor has strides of 0, and is contiguous all the same."""
+    cache = bsa.KVCache(1, 8, 2, 64, 16, 3, 2, dev)
+    cos, sin = (torch.from_numpy(x).to(dev) for x in _angles(8, 64))
+    none = torch.zeros(0, dtype=torch.int32, device=dev)
+    q, k = (torch.from_numpy(np.zeros((0, h, 64), np.float16)).to(dev) for h in (4, 2))
+    q, k, logits = (torch.as_strided(x, x.shape, (0,) * x.dim()) for x in (q, k, torch.zeros(0, 50, device=dev)))
+    assert q.stride(2) == k.stride(2) == logits.stride(1) == 0 and q.is_contiguous()
+    batch = dict(cu_seqlens=_i32([0, 0, 0], dev), max_new=5, slots=_i32([2, 0], dev))
+    cache.append(0, k, k, **batch)
+    assert cache.append_rotated(0, q, k, k, cos, sin, parents=none, **batch).shape == (0, 4, 64)
+    for out, lse in (cache.attend(0, q, **batch), cache.attend_tree(0, q, none, **batch)):
+        assert out.shape == (0, 4, 64) and lse.shape == (0, 4)
+    for draft in (None, logits):
+        got = bsa.verify_drafts(logits, none, torch.zeros(0, device=dev), None, draft, **batch)
+        assert got.accepted.tolist() == [0, 0] and (got.path == -1).all() and (got.tokens == -1).all()
+
+
 @pytest.mark.parametrize("nodes,hq", [(8, 2), (40, 4)])
 def test_tree_strided_q_and_out(dev, nodes, hq):
     """q and out as slices of wider tensors; what lies between them is left as it is."""

@@ -244,7 +244,7 @@ def _verify_call(logits, tokens, uniforms, parents, draft_logits, temperatures, 
         if parents is not None:
             raise ValueError("draft_logits go with chains: parents must be None")
     for what, t in (("logits", logits), ("draft_logits", draft_logits)):
-        if t is not None and t.stride(1) != 1 and vocab > 1:
+        if t is not None and t.stride(1) != 1 and vocab > 1 and count > 0:
             raise ValueError(f"{what} rows must be contiguous, strides {t.stride()}")
     _i32(tokens, dev, "tokens", count)
     _i32(parents, dev, "parents", count)

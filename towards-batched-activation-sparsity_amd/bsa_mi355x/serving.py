@@ -184,7 +184,7 @@ def _batch(x: torch.Tensor, what: str, heads: int, d: int, dev: torch.device, ro
         raise ValueError(f"{what} must be [tokens, {heads or 'heads'}, {d}], got {tuple(x.shape)}")
     if x.device != dev:
         raise ValueError(f"{what} must be on {dev}, got {x.device}")
-    if x.stride(2) != 1:
+    if x.stride(2) != 1 and x.shape[0] > 0:  # without tokens any strides are contiguous
         raise ValueError(f"{what} must have contiguous channels, strides {x.stride()}")
     if cu is None:
         if rows and x.shape[0] % rows:
