@@ -657,6 +657,26 @@ def test_verify_max_new_bounds_the_nodes(dev):
     _same_verdict(got, want, 4)
 
 
+@pytest.mark.parametrize("new", [[5], [2, 0, 4], [0, 0, 0]])
+@pytest.mark.parametrize("max_new,width", [(16, 16), (64, 64), (1000, 64), (5, 5), (3, 3), (1, 1), (0, 0)])
+def test_verify_answers_are_as_wide_as_max_new(dev, new, max_new, width):
+    """[sequences, max_new], also where a batch has fewer tokens than that, and at most 64 columns; without max_new a column a token."""
+    rng = np.random.default_rng(max_new)
+    total, cu = sum(new), _cu(new)
+    x, parents, tokens, u = _drafts(rng, [n for n in new if n], 300, True) if total else (np.zeros((0, 300)), [], [], np.zeros(0, np.float32))
+    logits = torch.from_numpy(x).float().to(dev)
+    args = (logits, _i32(tokens, dev), torch.from_numpy(u).to(dev), _i32(parents, dev))
+    used = [torch.full((len(new) * 64,), 9, dtype=torch.int32, device=dev) for _ in range(3)]
+    del used  # memory that the answers are given holds something
+    host = (logits.double().cpu().numpy(), tokens, u, parents, None, 1.0, cu)
+    got = bsa.verify_drafts(*args, cu_seqlens=_i32(cu, dev), max_new=max_new)
+    assert got.accepted.shape == (len(new),) and got.path.shape == got.tokens.shape == (len(new), width)
+    _same_verdict(got, dft.verify(*host, max_new=max_new), width)
+    got = bsa.verify_drafts(*args, cu_seqlens=_i32(cu, dev))
+    assert got.path.shape == got.tokens.shape == (len(new), total)
+    _same_verdict(got, dft.verify(*host), total)
+
+
 @pytest.mark.parametrize("kind", ["drawn", "likeliest"])
 def test_verify_leaves_the_targets_distribution(dev, kind):
     """The first token that comes out is distributed as the target's first row says, whatever was drafted: of 16000

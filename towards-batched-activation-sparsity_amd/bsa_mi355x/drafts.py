@@ -184,7 +184,7 @@ def _tree_call(q, parents, pages, scales, page_table, lengths, cu_seqlens, max_n
 
 class Verified(NamedTuple):
     accepted: torch.Tensor  # int32 [sequences]: accepted nodes, the first one among them
-    path: torch.Tensor      # int32 [sequences, max_new]: the accepted nodes, then -1
+    path: torch.Tensor      # int32 [sequences, max_new]: the accepted nodes, then -1 (max_new: at most 64; where not given, the tokens)
     tokens: torch.Tensor    # int32 [sequences, max_new]: the accepted drafts and the new token, then -1
 
 
@@ -258,10 +258,12 @@ def _verify_call(logits, tokens, uniforms, parents, draft_logits, temperatures, 
         rows, most = count // max_new, max_new
     else:
         _i32(cu_seqlens, dev, "cu_seqlens")
-        rows, most = cu_seqlens.numel() - 1, count if max_new is None else max(0, min(max_new, count))
+        # the answers' width is max_new whatever the batch's tokens are; only these are a tree's nodes
+        rows, most = cu_seqlens.numel() - 1, count if max_new is None else max(0, max_new)
         if rows < 0:
             raise ValueError("cu_seqlens has no entries")
-    _nodes(most)
+    _nodes(min(most, count))
+    most = min(most, MAX_NODES)
     _i32(slots, dev, "slots", rows)
     if temperatures is not None and (temperatures.dtype is not torch.float32 or temperatures.device != dev
                                      or temperatures.shape != (rows,) or not temperatures.is_contiguous()):
