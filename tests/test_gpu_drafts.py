@@ -647,6 +647,27 @@ def test_verify_numbers_next_to_their_border(dev, dtype, vocab):
     assert [w[0] for w in want] == [1, 1, 1, 2, 2, 2] * 2
 
 
+@pytest.mark.parametrize("vocab,places", [(40, (4, 5, 6)), (40, (36, 37, 2)), (5004, (8, 9, 4801)), (5004, (4104, 4105, 30)), (70000, (12, 13, 69999))])
+def test_verify_where_nothing_is_left(dev, vocab, places):
+    """A row of three tokens of weights 1, 2^-23 and 2^-46, all of them drafted and asked with 1 - 2^-24.  The last one's border is 1,
+    from which its number is 2^-70 of the row away: it may be accepted.  Where it is refused nothing is left of the row, and
+    the new token is drawn from all of it."""
+    numbers = [0.0, 0.5, 1 - 2.0 ** -22, 1 - 2.0 ** -24]
+    x = np.full((4 * len(numbers), vocab), -np.inf, np.float32)
+    x[:, list(places)] = [0.0, -15.942384719848633, -31.8847713470459]
+    u = np.full(len(x), 1 - 2.0 ** -24, np.float32)
+    u[::4] = numbers
+    got = bsa.verify_drafts(torch.from_numpy(x).to(dev), _i32([0, *places] * len(numbers), dev), torch.from_numpy(u).to(dev),
+                            _i32([-1, 0, 0, 0] * len(numbers), dev), max_new=4)
+    sums = np.cumsum(np.exp(x[0].astype(np.float64)))
+    for b, number in enumerate(numbers):
+        drawn = int(np.argmax(sums > number * sums[-1]))
+        if got.accepted[b] == 1:
+            assert got.path[b].tolist() == [0, -1, -1, -1] and got.tokens[b].tolist() == [drawn, -1, -1, -1], (b, got)
+        else:
+            assert got.path[b].tolist() == [0, 3, -1, -1] and got.tokens[b].tolist() == [places[2], drawn, -1, -1], (b, got)
+
+
 def test_verify_max_new_bounds_the_nodes(dev):
     rng = np.random.default_rng(4)
     new = [9, 2, 7]

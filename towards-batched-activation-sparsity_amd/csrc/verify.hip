@@ -585,40 +585,43 @@ __global__ __launch_bounds__(64 * kWaves) void bsg_verify_walk_kernel(VerifyPara
   const float y_top = residual ? s_top[1][at] : 0.f;
   const auto surplus = [&](double x, double y) { return __builtin_fmax(x * by[0] - y * by[1], 0.0); };
   Piece* const last = p.last + (int64_t)row * p.pieces;
-  const int piece = group * kWaves + wave;
-  if (piece < p.pieces) {
-    PieceOf<T> x;
-    x.load(p.x[0], x_at, p.vocab, shift, piece, lane);
-    Piece v = {0.0, 0.f, 0};
-    if (residual) {
-      PieceOf<T> y;
-      y.load(p.x[1], y_at, p.vocab, shift, piece, lane);
-      x.each([&](int, u32x4& a) {
-        const u32x4 b = y.v[0];
-#pragma unroll
-        for (int e = 0; e < PER; ++e) v.sum += surplus(weight(Logit<T>::of(a, e), top, k), weight(Logit<T>::of(b, e), y_top, k));
-#pragma unroll
-        for (int i = 0; i + 1 < PieceOf<T>::VECTORS; ++i) y.v[i] = y.v[i + 1];
-      });
-      v.sum = wave_sum<32>(v.sum);
-    } else {
-      for (uint64_t m = refused; m; m &= m - 1) x.drop(__builtin_amdgcn_readlane(id, __builtin_ctzll(m)), shift, piece, lane);
-      v = piece_of<false, T>(x, greedy, true, k, piece * kPiece - shift, lane);
-    }
-    if (lane == 0) store_piece(last + piece, v);
-  }
-  hand_publish();
-  __syncthreads();
-  if (threadIdx.x == 0) s_last = hand_arrive(p.counters + row) == (uint32_t)(p.groups - 1);
-  __syncthreads();
-  if (!s_last) return;
-  if (threadIdx.x == 0) hand_reset(p.counters + row);
-
   int token = -1;
-  if (greedy) {
-    const Row r = row_of(p.pieces, k, 64, lane, [&](int c) { return load_piece(last + c); });
-    if (r.total == r.total && r.top > -__builtin_inff()) token = r.at;
-  } else {
+  for (bool again = false;; again = true) {
+    // its own piece; again: all of them
+    for (int piece = again ? wave : group * kWaves + wave; piece < p.pieces; piece += again ? kWaves : p.pieces) {
+      PieceOf<T> x;
+      x.load(p.x[0], x_at, p.vocab, shift, piece, lane);
+      Piece v = {0.0, 0.f, 0};
+      if (residual) {
+        PieceOf<T> y;
+        y.load(p.x[1], y_at, p.vocab, shift, piece, lane);
+        x.each([&](int, u32x4& a) {
+          const u32x4 b = y.v[0];
+#pragma unroll
+          for (int e = 0; e < PER; ++e) v.sum += surplus(weight(Logit<T>::of(a, e), top, k), weight(Logit<T>::of(b, e), y_top, k));
+#pragma unroll
+          for (int i = 0; i + 1 < PieceOf<T>::VECTORS; ++i) y.v[i] = y.v[i + 1];
+        });
+        v.sum = wave_sum<32>(v.sum);
+      } else {
+        for (uint64_t m = refused; m; m &= m - 1) x.drop(__builtin_amdgcn_readlane(id, __builtin_ctzll(m)), shift, piece, lane);
+        v = piece_of<false, T>(x, greedy, true, k, piece * kPiece - shift, lane);
+      }
+      if (lane == 0) store_piece(last + piece, v);
+    }
+    hand_publish();
+    __syncthreads();
+    if (!again) {
+      if (threadIdx.x == 0) s_last = hand_arrive(p.counters + row) == (uint32_t)(p.groups - 1);
+      __syncthreads();
+      if (!s_last) return;
+      if (threadIdx.x == 0) hand_reset(p.counters + row);
+    }
+    if (greedy) {
+      const Row r = row_of(p.pieces, k, 64, lane, [&](int c) { return load_piece(last + c); });
+      if (r.total == r.total && r.top > -__builtin_inff()) token = r.at;
+      break;
+    }
     const double draw = read_lane(u, 0);
     bool over = residual;  // something is left of the row over its drafts; else from the row
     Picked c;
@@ -628,6 +631,13 @@ __global__ __launch_bounds__(64 * kWaves) void bsg_verify_walk_kernel(VerifyPara
       const Piece* const own = stats(at, 0);
       c = pick_piece<false>(p.pieces, draw, k, lane, [&](int i) { return residual ? own[i] : load_piece(last + i); });
       top = c.top;
+    }
+    if (!(c.whole > 0.0) && refused != 0 && !residual) {
+      // the rejected tokens had all of the row's weight: the new token is drawn from all of it, of which only this work-group is
+      // still here
+      refused = 0;
+      __syncthreads();  // every wave has read the sums, which are alike for all
+      continue;
     }
     if (c.whole > 0.0) {
       double w[N];
@@ -651,6 +661,7 @@ __global__ __launch_bounds__(64 * kWaves) void bsg_verify_walk_kernel(VerifyPara
       const int in_piece = pick_number(w, c.before, draw * c.whole, lane, wave);
       if (in_piece >= 0) token = in_piece + c.piece * kPiece - shift;
     }
+    break;
   }
   if (wave == 0) answer(p, row, taken, id, token, lane);
 }
