@@ -418,6 +418,139 @@ def test_tree_graph_streams_and_threads(dev):
         assert len(got) == 3 and all(torch.equal(o, want) and torch.equal(l, want_l) for o, l in got)
 
 
+# ---- hard scores, at 16 and 32 rows of a cached head (one kernel), and at 50 (small tiles), 120 (a large one) and 192 (a large
+# and a small one) of the other: by max_len in parts, which are joined, and a work-group for each
+
+HARD_TREES = [(8, 4), (16, 4), (50, 2), (60, 4), (64, 6)]  # nodes, query heads over two cached ones
+CUTS = (None, 500)
+
+
+def _hard(dev, rng, raw, sc, table, lengths, nodes, hq, dtype, d, q=None, **kw):
+    """Both cuts against the oracle, whose answer for q is returned with theirs."""
+    cu = [i * nodes for i in range(len(lengths) + 1)]
+    parents = [x for _ in lengths for x in _parents(rng, nodes)]
+    if q is None:
+        q = torch.from_numpy(rng.standard_normal((cu[-1], hq, d)).astype(np.float32)).to(DT[dtype]).to(dev)
+    with np.errstate(over="ignore"):
+        ref = dft.tree_attention(q.double().cpu().numpy(), parents, orc.Layer(raw, sc), table, np.array(lengths), cu, **kw)
+    for max_len in CUTS:
+        yield ref, bsa.kv_tree_attention(q, _i32(parents, dev), torch.from_numpy(raw).to(dev).view(F8), torch.from_numpy(sc).to(dev),
+                                         _i32(table, dev), _i32(lengths, dev), max_len=max_len, **kw)
+
+
+@pytest.mark.parametrize("nodes,hq", HARD_TREES)
+@pytest.mark.parametrize("kind", ["keys_grow", "keys_shrink", "sink", "value_scales", "values_grow", "values_shrink", "uneven"])
+def test_tree_maximum_moves(dev, kind, nodes, hq):
+    """Scores and value scales that outgrow, late and by many octaves, what was the maximum at first, or never come near it
+    again: within a part, between the halves of a small tile's steps, and from part to part."""
+    rng = np.random.default_rng([len(kind), nodes])
+    p, d, lengths = 16, 64, [2200, 700]
+    raw, sc, table, *_ = _cache(rng, dev, lengths, 2, p, d)
+    for row, n in enumerate(lengths):
+        ids, at = table[row, : -(-n // p)], np.arange(-(-n // p))[:, None]
+        if kind == "keys_grow":
+            sc[ids, :, 0] = 2.0 ** (at * 8 // len(at) - 8)
+        elif kind == "keys_shrink":
+            sc[ids, :, 0] = 2.0 ** (-1 - at * 8 // len(at))
+        elif kind == "sink":
+            sc[ids[:1], :, 0] = 1.0
+        elif kind in ("value_scales", "uneven"):
+            sc[ids, :, 1] = 2.0 ** rng.integers(-38, 20, (len(ids), 2))
+            if kind == "uneven":
+                sc[ids, :, 0] = 2.0 ** rng.integers(-12, -4, (len(ids), 2))
+        else:
+            steps = at * 40 // len(at) - 20
+            sc[ids, :, 1] = 2.0 ** (steps if kind == "values_grow" else -steps)
+    for dtype in ("fp16", "bf16"):
+        for ref, (out, lse) in _hard(dev, rng, raw, sc, table, lengths, nodes, hq, dtype, d):
+            if dtype == "fp16":
+                # Outputs past its range are infinite, and what lies within its error of that, from either side, may be: an output's
+                # is _check_attention's, the weights' 2^-11 of the magnitudes that it is the sum of, which are up to 2^8 times the
+                # output's (1.7e7 for one of 64358: an error of up to 12336), and half a step of its own.
+                o, _, mag, dots, vmax, count = ref
+                eps = (d + 8) * 2.0 ** -24 * dots + 2.0 ** -20
+                off = 2.0 ** -11 * np.abs(o) + (2.0 ** -11 + 2 * eps[..., None]) * mag + (count * vmax * 2.0 ** -38)[..., None] + 2.0 ** -24
+                past, sure = np.abs(o) + off >= 65520, np.abs(o) - off >= 65520
+                assert (out.double().cpu().numpy()[sure] == np.copysign(np.inf, ref[0][sure])).all()
+                out = torch.where(torch.from_numpy(past).to(dev), 0, out)
+                ref = (np.where(past, 0.0, ref[0]), *ref[1:])
+            _check_attention(out, lse, ref, DT[dtype], d)
+
+
+@pytest.mark.parametrize("nodes,hq", HARD_TREES)
+@pytest.mark.parametrize("sm_scale", [-0.125, -1.0, 0.0, -0.0, 1e-30, -1e-30, 2.0])
+def test_tree_scales_of_any_sign(dev, sm_scale, nodes, hq):
+    rng = np.random.default_rng(nodes)
+    lengths = [1500, 70]
+    raw, sc, table, *_ = _cache(rng, dev, lengths, 2, 32, 64, poison=True)
+    for dtype in ("fp16", "bf16"):
+        for ref, (out, lse) in _hard(dev, rng, raw, sc, table, lengths, nodes, hq, dtype, 64, sm_scale=sm_scale):
+            _check_attention(out, lse, ref, DT[dtype], 64)
+
+
+@pytest.mark.parametrize("nodes,hq", HARD_TREES)
+@pytest.mark.parametrize("octaves", [10, 20, 24, 26, 27, 28, 30, 40, 70])
+def test_tree_far_scores(dev, octaves, nodes, hq):
+    """Scores of up to 2^octaves that differ by as much, as test_attention_far_scores: the values of the largest are averaged, the
+    products of small integers are exact, and outputs and lse carry a few roundings."""
+    rng = np.random.default_rng([octaves, nodes])
+    p, d, lengths = 16, 64, [1300, 70]
+    raw, sc, table, *_ = _cache(rng, dev, lengths, 2, p, d)
+    raw[:, :, 0] = torch.from_numpy(rng.integers(-1, 2, raw[:, :, 0].shape).astype(np.float32)).to(F8).view(torch.uint8).numpy()
+    sc[..., 0], sc[..., 1] = 2.0 ** octaves, 0.125
+    for dtype in ("fp16", "bf16"):
+        q = torch.from_numpy(rng.integers(-2, 3, (2 * nodes, hq, d)).astype(np.float32)).to(DT[dtype]).to(dev)
+        u = 2.0 ** -10 if dtype == "fp16" else 2.0 ** -7
+        for (o, l, *_), (out, lse) in _hard(dev, rng, raw, sc, table, lengths, nodes, hq, dtype, d, q, sm_scale=0.25):
+            assert (np.abs(out.double().cpu().numpy() - o) <= u * np.abs(o) + 2.0 ** -10).all()
+            assert (np.abs(lse.double().cpu().numpy() - l) <= 2.0 ** -21 * np.abs(l)).all()
+
+
+@pytest.mark.parametrize("nodes,hq", HARD_TREES)
+@pytest.mark.parametrize("octaves", [4, 8, 10, 12, 14, 16, 17, 18])
+def test_tree_equal_scores_weigh_the_same(dev, octaves, nodes, hq):
+    """Every token has the same key, so that a row's scores, however far from 0, are one number, and its output is the mean of what it
+    sees: weights that are off by their rounding to fp16, 2^-11, and by at most 2^-13 of each other before."""
+    rng = np.random.default_rng([octaves, nodes])
+    p, d, lengths = 16, 64, [2200, 700]
+    raw, sc, table, *_ = _cache(rng, dev, lengths, 2, p, d)
+    key = torch.from_numpy(rng.integers(-2, 3, d).astype(np.float32)).to(F8).view(torch.uint8).numpy()
+    one = np.zeros(p * d, np.uint8)
+    for t in range(p):
+        one[[orc.key_offset(t, x, d) for x in range(d)]] = key
+    raw[:, :, 0] = one.reshape(p, d)
+    sc[..., 0], sc[..., 1] = 2.0 ** octaves, 0.125
+    for dtype in ("fp16", "bf16"):
+        q = torch.from_numpy(rng.integers(-2, 3, (2 * nodes, hq, d)).astype(np.float32)).to(DT[dtype]).to(dev)
+        u = 2.0 ** -11 if dtype == "fp16" else 2.0 ** -8
+        for (o, l, mag, *_), (out, lse) in _hard(dev, rng, raw, sc, table, lengths, nodes, hq, dtype, d, q, sm_scale=0.25):
+            bound = u * np.abs(o) + (2.0 ** -11 + 2.0 ** -13) * mag + 2.0 ** -20
+            assert (np.abs(out.double().cpu().numpy() - o) <= bound).all()
+            assert (np.abs(lse.double().cpu().numpy() - l) <= 2.0 ** -21 * np.abs(l) + 2.0 ** -10).all()
+
+
+@pytest.mark.parametrize("nodes,hq", HARD_TREES)
+def test_tree_scores_of_minus_infinity_first(dev, nodes, hq):
+    """The first 600 tokens' scores pass the end of 32 bits, whole parts of them: the later ones are seen as if alone."""
+    rng = np.random.default_rng(nodes)
+    p, d, length, first = 16, 64, 1100, 600
+    raw, sc, table, *_ = _cache(rng, dev, [length], 2, p, d)
+    sc[:] = 1.0
+    minus = torch.tensor([-448.0, -8.0]).to(F8).view(torch.uint8).numpy()
+    for t in range(length):
+        for h in range(2):
+            tile = raw[table[0, t // p], h, 0].reshape(-1)
+            for x in range(d):
+                tile[orc.key_offset(t % p, x, d)] = 0
+            tile[orc.key_offset(t % p, 0, d)] = minus[0] if t < first else 0
+            tile[orc.key_offset(t % p, 1, d)] = minus[1]
+    q = torch.zeros(nodes, hq, d)
+    q[..., 0], q[..., 1] = 1e38, 128
+    for ref, (out, lse) in _hard(dev, rng, raw, sc, table, [length], nodes, hq, "bf16", d, q.bfloat16().to(dev)):
+        assert (ref[1] >= np.log(length - first - nodes + 1) - 128 - 1e-9).all() and (ref[1] <= np.log(length - first) - 128 + 1e-9).all()
+        _check_attention(out, lse, (*ref[:3], np.full_like(ref[3], 128.0), *ref[4:]), torch.bfloat16, d)
+
+
 # ---------------------------------------------------------------------------------------- verification
 
 

@@ -392,6 +392,29 @@ def test_attention_far_scores(dev, dtype, new, hq, octaves):
     assert (np.abs(lse.double().cpu().numpy() - l) <= 2.0 ** -21 * np.abs(l)).all()
 
 
+@pytest.mark.parametrize("octaves", [4, 8, 10, 12, 14, 16, 17, 18])
+def test_prompt_equal_scores_weigh_the_same(dev, octaves):
+    """Every token has the same key, so that a row's scores, however far from 0, are one number, and its output is the mean of what it
+    sees: weights that are off by their rounding to fp16, 2^-11, and by at most 2^-13 of each other before."""
+    rng = np.random.default_rng(octaves)
+    p, d, lengths, new = 16, 64, [2200, 700], 50
+    raw, sc, table, *_ = _cache(rng, dev, lengths, 2, p, d)
+    key = torch.from_numpy(rng.integers(-2, 3, d).astype(np.float32)).to(F8).view(torch.uint8).numpy()
+    one = np.zeros(p * d, np.uint8)
+    for t in range(p):
+        one[[orc.key_offset(t, x, d) for x in range(d)]] = key
+    raw[:, :, 0] = one.reshape(p, d)
+    sc[..., 0], sc[..., 1] = 2.0 ** octaves, 0.125
+    args = (torch.from_numpy(raw).to(dev).view(F8), torch.from_numpy(sc).to(dev), _i32(table, dev), _i32(lengths, dev))
+    for dtype, u in (("fp16", 2.0 ** -11), ("bf16", 2.0 ** -8)):
+        q = torch.from_numpy(rng.integers(-2, 3, (2 * new, 4, d)).astype(np.float32)).to(DT[dtype]).to(dev)
+        o, l, mag, *_ = orc.attention(q.double().cpu().numpy(), orc.Layer(raw, sc), table, np.array(lengths), [0, new, 2 * new], sm_scale=0.25)
+        for max_len in (None, 500):
+            out, lse = bsa.kv_attention(q, *args, sm_scale=0.25, max_len=max_len)
+            assert (np.abs(out.double().cpu().numpy() - o) <= u * np.abs(o) + (2.0 ** -11 + 2.0 ** -13) * mag + 2.0 ** -20).all()
+            assert (np.abs(lse.double().cpu().numpy() - l) <= 2.0 ** -21 * np.abs(l) + 2.0 ** -10).all()
+
+
 def test_prompt_scores_of_minus_infinity_first(dev):
     """A prompt whose first tokens' scores pass the end of 32 bits: the later ones are seen as if alone."""
     rng = np.random.default_rng(17)

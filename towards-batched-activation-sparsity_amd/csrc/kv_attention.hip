@@ -167,7 +167,7 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
     for (int d = 0; d < DT; ++d) acc[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  bool started = false;  // every row has a base, and one that is not far
+  bool started = false;  // every row has a base, and one that is near 0
   const auto take = [&](auto stage, int t0) {
     const u32x4* const kv = prefill_stage<D, decltype(stage)::value>() + lane;
     const int first_tile = (t0 - t_begin) / 16 & 63;
@@ -207,9 +207,9 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
       }
     }
     // Weights against the base so far; only where four of them together outgrow fp16 (or a row has no
-    // base yet, or a far one) is a new one looked for.  The sums are wanted anyway: asking each weight took 590 us
-    // instead of 566 for a prompt of 8192.  Against a new base the score is rounded first, so that the maximum's
-    // weight is 2^13 or 1 however far it is; otherwise both come in one step.
+    // base yet, or none near 0) is a new one looked for.  The sums are wanted anyway: asking each weight took 590 us
+    // instead of 566 for a prompt of 8192.  Against a new base, and one that is not near 0, the score is rounded first, so that
+    // the maximum's weight is 2^13 or 1 however far it is, and equal scores weigh the same; otherwise both come in one step.
     f16x8 pf[RT][2];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
@@ -256,7 +256,7 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_prefill_kernel(AttnParams p) {
       pf[i][1] = __builtin_bit_cast(f16x8, u32x4{w[4], w[5], w[6], w[7]});
     }
     if (!started)
-      started = !partial && !__any(!(__builtin_fabsf(base[0]) < kFarScore) || !(__builtin_fabsf(base[1]) < kFarScore));
+      started = !partial && !__any(!(__builtin_fabsf(base[0]) < kNearScore) || !(__builtin_fabsf(base[1]) < kNearScore));
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
 #pragma unroll

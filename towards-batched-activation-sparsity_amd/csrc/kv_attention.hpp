@@ -34,6 +34,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxSplits = 32;    // parts of one row
 constexpr float kShift = 13.f;  // weights go up to 2^(kShift + kSlack), within fp16
 constexpr float kFarScore = 0x1p22f;  // octaves from which on a score's last bit is half an octave or more
+// Octaves within which score and base may come in one step, rounded once: against a base that was made from rounded scores a weight is
+// then off by up to half a score's last bit, 2^-13 octaves here, a quarter of what its rounding to fp16 takes (at 2^21 it would be 9%).
+constexpr float kNearScore = 0x1p11f;
 constexpr float kSlack = 1.5f;  // octaves by which, in the first kernel, a score may exceed the running maximum before that moves
 constexpr float kMostWeight = 65504.f;  // of fp16; four weights at the maximum make half of it
 

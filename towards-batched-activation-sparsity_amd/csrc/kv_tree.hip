@@ -306,7 +306,7 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_tree_kernel(TreeParams tp) {
         for (int d = 0; d < DT; ++d) acc[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
 
-      bool started = false;  // every row has a base, and one that is not far
+      bool started = false;  // every row has a base, and one that is near 0
       const auto take = [&](auto stage, int step_at) {
         const u32x4* const kv = prefill_stage<D, decltype(stage)::value>() + lane + tg * NT * TILE;
         const int first_tile = ((step_at - t_begin) / 16 & 63) + tg * NT;
@@ -347,8 +347,9 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_tree_kernel(TreeParams tp) {
             }
         }
         // Weights against the base so far; only where four of them together outgrow fp16 (or a row has no
-        // base yet, or a far one) is a new one looked for.  Against a new base the score is rounded first, so that the
-        // maximum's weight is 2^13 or 1 however far it is; otherwise both come in one step.
+        // base yet, or none near 0) is a new one looked for.  Against a new base, and one that is not near 0, the score is rounded
+        // first, so that the maximum's weight is 2^13 or 1 however far it is, and equal scores weigh the same; otherwise both
+        // come in one step.
         f16x8 pf[RT][NT / 2];
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
@@ -396,7 +397,7 @@ __global__ __launch_bounds__(256, 2) void bsg_kv_tree_kernel(TreeParams tp) {
             pf[i][n] = __builtin_bit_cast(f16x8, u32x4{w[4 * n], w[4 * n + 1], w[4 * n + 2], w[4 * n + 3]});
         }
         if (!started)
-          started = !partial && !__any(!(__builtin_fabsf(base[0]) < kFarScore) || !(__builtin_fabsf(base[1]) < kFarScore));
+          started = !partial && !__any(!(__builtin_fabsf(base[0]) < kNearScore) || !(__builtin_fabsf(base[1]) < kNearScore));
 #pragma unroll
         for (int n = 0; n < NT / 2; ++n) {
 #pragma unroll
