@@ -780,6 +780,32 @@ def test_verify_numbers_next_to_their_border(dev, dtype, vocab):
     assert [w[0] for w in want] == [1, 1, 1, 2, 2, 2] * 2
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("vocab", [40, 5003, 65529])
+@pytest.mark.parametrize("offset,constant", [(0, 0), (1, 0), (0, 8), (3, -16)])
+def test_verify_drafts_as_likely_leave_nothing(dev, dtype, vocab, offset, constant):
+    """A draft whose probabilities are the target's own, of the same logits or of ones that differ by a constant, cut at other addresses:
+    what a rejected token (which does not exist) leaves is nothing, and the new one is drawn from the target's row."""
+    rng = np.random.default_rng([vocab, offset])
+    new = [2, 3, 2, 4, 2, 2]
+    cu = _cu(new)
+    x = rng.integers(-40, 41, (cu[-1], vocab)) / 4.0  # exact, and so with the constant, in each type
+    x[np.arange(cu[-1]), rng.integers(0, vocab, cu[-1])] = 14.0
+    tokens, u = rng.integers(0, vocab, cu[-1]), rng.random(cu[-1]).astype(np.float32)
+    for b, bad in enumerate([-1, vocab, -7, vocab + 1, 2 ** 31 - 1, -1]):
+        tokens[cu[b] + 1 + (b % 2) * (new[b] > 2)] = bad
+    logits = torch.from_numpy(x.astype(np.float32)).to(DT[dtype]).to(dev)
+    draft = torch.zeros(cu[-1], vocab + 5, dtype=DT[dtype], device=dev)[:, offset:offset + vocab]
+    draft.copy_(logits + constant)
+    assert torch.equal(draft.double() - constant, logits.double())
+    args = (logits, _i32(tokens, dev), torch.from_numpy(u).to(dev))
+    temps = np.array([1, 0.5, 2, 1, 0.25, 1], np.float32)
+    want = dft.verify(logits.double().cpu().numpy(), tokens, u, None, logits.double().cpu().numpy(), temps, cu)
+    got = bsa.verify_drafts(*args, draft_logits=draft, temperature=torch.from_numpy(temps).to(dev), cu_seqlens=_i32(cu, dev), max_new=4)
+    _same_verdict(got, want, 4)
+    assert [w[0] for w in want] == [1, 2, 1, 2, 1, 1]
+
+
 @pytest.mark.parametrize("vocab,places", [(40, (4, 5, 6)), (40, (36, 37, 2)), (5004, (8, 9, 4801)), (5004, (4104, 4105, 30)), (70000, (12, 13, 69999))])
 def test_verify_where_nothing_is_left(dev, vocab, places):
     """A row of three tokens of weights 1, 2^-23 and 2^-46, all of them drafted and asked with 1 - 2^-24.  The last one's border is 1,
