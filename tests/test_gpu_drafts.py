@@ -213,6 +213,47 @@ def test_rotated_edges(dev, case):
         assert (out.cpu()[torch.from_numpy(~mine)] == 7.0).all()  # nobody's rows
 
 
+@pytest.mark.parametrize("p,d", [(16, 64), (128, 128)])
+def test_rotated_batches_of_many_sequences_without_a_bound(dev, p, d):
+    """300 sequences of 1 to 2000 new tokens with no max_new: more tiles and more rows of queries than one launch takes.  The numbers of
+    the call that is told of the longest, and some sequences' against the oracle."""
+    rng = np.random.default_rng([19, p])
+    hq, heads, n = 6, 24, 300
+    new = rng.integers(1, 600, n)
+    new[::60] = 2000
+    lengths = new + rng.integers(0, 40, n)
+    per = -(-lengths // p)
+    table = np.full((n, per.max()), -1)
+    ids = rng.permutation(int(per.sum()))
+    for b, at in enumerate(np.cumsum(per) - per):
+        table[b, : per[b]] = ids[at: at + per[b]]
+    cu = np.asarray(_cu(new))
+    g = torch.Generator(device=dev).manual_seed(1)
+    q, k, v = (torch.randn(int(cu[-1]), h, d, generator=g, device=dev, dtype=torch.float16) for h in (hq, heads, heads))
+    cos, sin = _angles(2100, d)
+    got = []
+    for most in (2000, None):
+        pages = torch.zeros(len(ids), heads, 2, p, d, dtype=torch.uint8, device=dev).view(F8)
+        scales = torch.ones(len(ids), heads, 2, device=dev)
+        out = bsa.kv_append_rotated(q, k, v, torch.from_numpy(cos).to(dev), torch.from_numpy(sin).to(dev), pages, scales, _i32(table, dev),
+                                    _i32(lengths, dev), cu_seqlens=_i32(cu, dev), max_new=most)
+        got.append((pages.view(torch.uint8), scales, out))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    some = [0, 1, 137, n - 1]
+    index = torch.from_numpy(np.concatenate([table[b, : per[b]] for b in some])).to(dev)
+    own, at = np.full((len(some), per.max()), -1), 0
+    for i, b in enumerate(some):
+        own[i, : per[b]] = np.arange(at, at + per[b])
+        at += per[b]
+    own_cu = _cu(new[some])
+    rows = torch.cat([torch.arange(cu[b], cu[b + 1]) for b in some]).to(dev)
+    host = [t[rows].double().cpu().numpy() for t in (q, k, v)]
+    (rq, mq), (rk, mk) = (dft.turned(t, None, 1e-6, cos, sin, False, lengths[some], own_cu) for t in host[:2])
+    layer = orc.Layer(np.zeros((at, heads, 2, p, d), np.uint8), np.ones((at, heads, 2), np.float32))
+    _check_rotated(got[1][2][rows], got[1][0][index].view(F8), got[1][1][index], layer, rq, mq, rk, mk, host[2], own, lengths[some], own_cu,
+                   torch.float16, False)
+
+
 @pytest.mark.parametrize("p,d", [(16, 64), (64, 128)])
 def test_rotated_magnitudes_past_every_scale(dev, p, d):
     """bf16 numbers of 2^120 beside the largest scale, 2^80: the largest e4m3 number, with its sign, as kv_append."""
@@ -804,6 +845,83 @@ def test_verify_drafts_as_likely_leave_nothing(dev, dtype, vocab, offset, consta
     got = bsa.verify_drafts(*args, draft_logits=draft, temperature=torch.from_numpy(temps).to(dev), cu_seqlens=_i32(cu, dev), max_new=4)
     _same_verdict(got, want, 4)
     assert [w[0] for w in want] == [1, 2, 1, 2, 1, 1]
+
+
+# ---- rows of more pieces (1024 logits each) than a wave has lanes: 64 up to 65529 logits, 65 from there on
+
+LARGE = [65529, 65530, 131073, 2 ** 20]
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("vocab", LARGE)
+@pytest.mark.parametrize("kind", ["trees", "drawn", "same"])
+def test_verify_large_vocabularies(dev, dtype, vocab, kind):
+    """Trees, chains of drawn drafts, and chains whose drafts have the target's own logits, of which nothing is left where a token is
+    rejected because it does not exist.  New tokens from all over the rows: of the first and the last piece, of rows whose
+    only weights lie at one end, of rows of few weights far apart."""
+    rng = np.random.default_rng([vocab, len(kind)])
+    new = [1, 5, 4, 3, 2, 2, 3]
+    cu = _cu(new)
+    x, parents, tokens, u = _drafts(rng, new, vocab, kind == "trees")
+    u[cu[1]], u[cu[2]] = 1 - 2.0 ** -24, 2.0 ** -24
+    x[cu[3]:cu[4], : vocab - 70] = -np.inf
+    x[cu[4]:cu[5], 70:] = -np.inf
+    x[cu[5]:cu[6]] = np.where(np.arange(vocab) % (vocab // 7) == 3, x[cu[5]:cu[6]], -np.inf)
+    tokens[cu[5] + 1] = 3 + 4 * (vocab // 7)
+    if kind != "drawn":
+        tokens[cu[2] + 2], tokens[cu[6] + 1] = vocab, -1
+    logits = torch.from_numpy(x.astype(np.float32)).to(DT[dtype]).to(dev)
+    draft = None
+    if kind != "trees":
+        noise = torch.from_numpy(rng.standard_normal(x.shape).astype(np.float32)).to(dev)
+        draft = logits.clone() if kind == "same" else (logits.float() + noise).to(DT[dtype])
+    temps = np.array([1, 0.7, 1, 0.8, 1, 2, 0.9], np.float32)
+    host = (logits.double().cpu().numpy(), tokens, u, parents if kind == "trees" else None, None if draft is None else draft.double().cpu().numpy())
+    with np.errstate(invalid="ignore"):
+        want = dft.verify(*host, temps, cu)
+    got = bsa.verify_drafts(logits, _i32(tokens, dev), torch.from_numpy(u).to(dev), _i32(parents, dev) if kind == "trees" else None, draft,
+                            torch.from_numpy(temps).to(dev), _i32(cu, dev), 5)
+    _same_verdict(got, want, 5)
+    assert all(w[2][-1] >= vocab - 70 for w in want[3:4]) and 0 <= want[4][2][-1] < 70
+    if kind == "same":  # accepted but for what does not exist, or has no weight in its row (the fourth and fifth)
+        assert [w[0] for w in want[:3] + want[5:]] == [1, 5, 2, 2, 1]
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("vocab", [65529, 65530, 131073])
+def test_verify_large_vocabularies_next_to_their_border(dev, dtype, vocab):
+    """What 32-bit sums do not decide is added again over all of a row's pieces."""
+    test_verify_numbers_next_to_their_border(dev, dtype, vocab)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("vocab", [300, 5003, 65530])
+def test_verify_drawn_numbers_next_to_their_border(dev, dtype, vocab):
+    """Against a draft: the 32-bit number below p(x) / q(x) accepts the token, the one above does not; and numbers of the new token next
+    to a running sum of what p has over q."""
+    rng = np.random.default_rng(vocab)
+    x, _, _, u = _drafts(rng, [2] * 12, vocab, False)
+    logits = torch.from_numpy(x.astype(np.float32)).to(DT[dtype]).to(dev)
+    draft = (logits.float() + torch.from_numpy(rng.standard_normal(x.shape).astype(np.float32)).to(dev)).to(DT[dtype])
+    hosts = [t.double().cpu().numpy() for t in (logits, draft)]
+    tokens = np.zeros(24, np.int64)
+    for b in range(12):
+        p, q = (np.exp(h[2 * b] - h[2 * b].max()) for h in hosts)
+        p, q = p / p.sum(), q / q.sum()
+        shy = np.flatnonzero((p < 0.9 * q) & (p > 1e-3 * q))  # what the draft likes more
+        tokens[2 * b + 1] = shy[np.argsort(-q[shy])[b % 3]]
+        border, above = (p / q)[tokens[2 * b + 1]], b % 2 == 0
+        near = np.float32(border)
+        near = near if (float(near) >= border) == above else np.nextafter(near, np.float32(2 if above else 0))
+        u[2 * b + 1] = near
+        assert (float(near) >= border) == above and abs(float(near) / border - 1) < 2.0 ** -22
+        left = np.maximum(p - q, 0) if above else np.exp(hosts[0][2 * b + 1] - hosts[0][2 * b + 1].max())
+        u[2 * b] = np.float32((np.cumsum(left) / left.sum())[(7919 * b) % vocab])
+        u[2 * b] = min(u[2 * b], np.float32(1 - 2.0 ** -24))
+    want = dft.verify(hosts[0], tokens, u, None, hosts[1], 1.0, _cu([2] * 12))
+    got = bsa.verify_drafts(logits, _i32(tokens, dev), torch.from_numpy(u).to(dev), draft_logits=draft, max_new=2)
+    _same_verdict(got, want, 2)
+    assert [w[0] for w in want] == [1, 2] * 6
 
 
 @pytest.mark.parametrize("vocab,places", [(40, (4, 5, 6)), (40, (36, 37, 2)), (5004, (8, 9, 4801)), (5004, (4104, 4105, 30)), (70000, (12, 13, 69999))])
