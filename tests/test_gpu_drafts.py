@@ -592,6 +592,47 @@ def test_tree_scores_of_minus_infinity_first(dev, nodes, hq):
         _check_attention(out, lse, (*ref[:3], np.full_like(ref[3], 128.0), *ref[4:]), torch.bfloat16, d)
 
 
+@pytest.mark.parametrize("nodes,hq", HARD_TREES)
+def test_tree_queries_that_are_not_numbers(dev, nodes, hq):
+    """A NaN or an infinity in a query makes its own row NaN and leaves the others what they are."""
+    rng = np.random.default_rng(nodes)
+    p, d, lengths = 16, 64, [1500, 90]
+    raw, sc, table, *_ = _cache(rng, dev, lengths, 2, p, d, poison=True)
+    q = torch.from_numpy(rng.standard_normal((2 * nodes, hq, d)).astype(np.float32)).half().to(dev)
+    bad = torch.zeros(q.shape[:2], dtype=torch.bool, device=dev)
+    for t, h, x in ((0, 0, float("nan")), (nodes // 2, hq - 1, float("inf")), (nodes, 1, float("-inf")), (2 * nodes - 1, hq // 2, float("nan"))):
+        q[t, h, 7 + t % 5], bad[t, h] = x, True
+    plain = torch.where(bad[..., None], torch.zeros_like(q), q)
+    parents = [x for _ in lengths for x in _parents(rng, nodes)]
+    ref = dft.tree_attention(plain.double().cpu().numpy(), parents, orc.Layer(raw, sc), table, np.array(lengths), [0, nodes, 2 * nodes])
+    for max_len in CUTS:
+        out, lse = bsa.kv_tree_attention(q, _i32(parents, dev), torch.from_numpy(raw).to(dev).view(F8), torch.from_numpy(sc).to(dev),
+                                         _i32(table, dev), _i32(lengths, dev), max_len=max_len)
+        assert torch.isnan(out[bad]).all() and torch.isnan(lse[bad]).all()
+        zero = bad.cpu().numpy()  # whose reference is that of a row of zeros
+        masked = [np.where(zero.reshape(zero.shape + (1,) * (x.ndim - 2)), 0.0, x) for x in ref]
+        _check_attention(out.masked_fill(bad[..., None], 0.0), lse.masked_fill(bad, 0.0), masked, torch.float16, d)
+
+
+@pytest.mark.parametrize("hq", [2, 4, 16])
+def test_tree_max_new_bounds_the_rows(dev, hq):
+    """The nodes past max_new are not computed; the others see what they do in the whole tree."""
+    rng = np.random.default_rng(hq)
+    new, lengths, most = [20, 9, 12], [150, 900, 12], 11
+    raw, sc, table, pages, scales, tab = _cache(rng, dev, lengths, 2, 16, 64, poison=True)
+    cu, parents = _cu(new), [x for n in new for x in _parents(rng, n)]
+    q = torch.from_numpy(rng.standard_normal((cu[-1], hq, 64)).astype(np.float32)).half().to(dev)
+    ref = dft.tree_attention(q.double().cpu().numpy(), parents, orc.Layer(raw, sc), table, np.array(lengths), cu)
+    rows = np.concatenate([np.arange(a, min(b, a + most)) for a, b in zip(cu, cu[1:])])
+    rest = np.setdiff1d(np.arange(cu[-1]), rows)
+    for max_len in CUTS:
+        out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device=dev)
+        bsa.kv_tree_attention(q, _i32(parents, dev), pages, scales, tab, _i32(lengths, dev), cu_seqlens=_i32(cu, dev), max_new=most,
+                              max_len=max_len, out=out, lse=lse)
+        assert (out[rest] == 7.0).all() and (lse[rest] == 7.0).all() and len(rest) == 10
+        _check_attention(out[rows], lse[rows], [x[rows] for x in ref], torch.float16, 64)
+
+
 # ---------------------------------------------------------------------------------------- verification
 
 
@@ -892,6 +933,28 @@ def test_verify_large_vocabularies(dev, dtype, vocab, kind):
 def test_verify_large_vocabularies_next_to_their_border(dev, dtype, vocab):
     """What 32-bit sums do not decide is added again over all of a row's pieces."""
     test_verify_numbers_next_to_their_border(dev, dtype, vocab)
+
+
+@pytest.mark.parametrize("draft", [False, True])
+def test_verify_rows_past_four_gigabytes(dev, draft):
+    """The last rows of 4.6 GB of logits, and sequences that begin there: what the same rows give by themselves."""
+    count, vocab, new = 1100, 2 ** 20, [3, 5]
+    g = torch.Generator(device=dev).manual_seed(5)
+    big = [torch.empty(count, vocab, device=dev) for _ in range(1 + draft)]
+    last = [torch.randn(8, vocab, generator=g, device=dev) for _ in big]
+    for x, rows in zip(big, last):
+        rows[torch.arange(8), torch.arange(8) * 100000 + 77] += 14.0
+        x[-8:] = rows
+    tokens, u = torch.zeros(count, dtype=torch.int32, device=dev), torch.rand(count, generator=g, device=dev)
+    tokens[-7:] = torch.arange(7, device=dev, dtype=torch.int32) * 100000 + 77
+    first = count - 8
+    want = bsa.verify_drafts(last[0], tokens[-8:].contiguous(), u[-8:].contiguous(), draft_logits=last[1] if draft else None, cu_seqlens=_i32([0, 3, 8], dev),
+                             max_new=5)
+    got = bsa.verify_drafts(big[0], tokens, u, draft_logits=big[1] if draft else None, cu_seqlens=_i32([first, first + 3, count], dev), max_new=5)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and int(want.accepted.max()) > 1 and (want.tokens.gather(1, want.accepted.long()[:, None] - 1) >= 0).all()
+    if not draft:
+        host = dft.verify(last[0].double().cpu().numpy(), tokens[-8:].cpu().numpy(), u[-8:].cpu().numpy(), None, None, 1.0, [0, 3, 8])
+        _same_verdict(got, host, 5)
 
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
@@ -1449,6 +1512,66 @@ def test_batches_without_tokens_have_any_strides(dev):
     for draft in (None, logits):
         got = bsa.verify_drafts(logits, none, torch.zeros(0, device=dev), None, draft, **batch)
         assert got.accepted.tolist() == [0, 0] and (got.path == -1).all() and (got.tokens == -1).all()
+
+
+def test_refusals(dev):
+    """Types, shapes, strides and devices that cannot be right, of each call; and the right ones, unharmed."""
+    cache = bsa.KVCache(1, 8, 2, 64, 16, 3, 2, dev)
+    q, k, n = torch.zeros(3, 4, 64, dtype=torch.float16, device=dev), torch.zeros(3, 2, 64, dtype=torch.float16, device=dev), _i32([-1, -1, -1], dev)
+    cos, sin = (torch.from_numpy(x).to(dev) for x in _angles(8, 64))
+    norm = torch.ones(64, dtype=torch.float16, device=dev)
+    odd = torch.zeros(3 * 4 * 64 + 1, dtype=torch.float16, device=dev)[1:].view(3, 4, 64)
+    turned = torch.zeros(3, 64, 4, dtype=torch.float16, device=dev).transpose(1, 2)
+
+    def append(q=q, k=k, v=k, cos=cos, sin=sin, **kw):
+        return cache.append_rotated(0, q, k, v, cos, sin, **kw)
+
+    def attend(q=q, parents=n, **kw):
+        return cache.attend_tree(0, q, parents, **kw)
+
+    def verify(logits=torch.zeros(3, 30, device=dev), tokens=n, uniforms=torch.zeros(3, device=dev), max_new=3, **kw):
+        return bsa.verify_drafts(logits, tokens, uniforms, max_new=max_new, **kw)
+
+    def keep(path=_i32([[0], [0], [0]], dev), accepted=_i32([1, 1, 1], dev), **kw):
+        return cache.keep(path, accepted, **kw)
+
+    for call in (append, attend, verify, keep):
+        call()
+    many = torch.zeros(195, 4, 64, dtype=torch.float16, device=dev)
+    for call, error, bads in (
+            (append, TypeError, (dict(q=q.float(), k=k.float(), v=k.float()), dict(cos=cos.double()), dict(sin=sin.cpu()), dict(parents=n.long()),
+                                 dict(positions=n.float()))),
+            (append, ValueError, (dict(q=q[:2]), dict(q=q.bfloat16()), dict(v=k.bfloat16()), dict(k=k[:, :1], v=k[:, :1]), dict(q=q.cpu()), dict(q=turned),
+                                  dict(sin=sin[:7]), dict(cos=cos.repeat(1, 2)[:, ::2]), dict(q_norm=norm[:32]), dict(k_norm=norm.float()),
+                                  dict(q_norm=norm.cpu()), dict(parents=n[:2]), dict(positions=n.repeat(2)), dict(out=q[:2]), dict(out=q.float()),
+                                  dict(out=turned), dict(max_new=2), dict(slots=n[:2]), dict(eps=-1.0), dict(positions=n, parents=n),
+                                  dict(cos=cos[:0], sin=sin[:0]), dict(q=odd))),
+            (append, NotImplementedError, (dict(cos=cos[:, :24].contiguous(), sin=sin[:, :24].contiguous()),)),
+            (attend, TypeError, (dict(q=q.float()), dict(parents=n.long()))),
+            (attend, ValueError, (dict(q=q[:, :3]), dict(q=q.cpu()), dict(q=turned), dict(q=odd), dict(parents=n[:2]), dict(parents=n.cpu()), dict(out=q[:2]),
+                                  dict(out=turned), dict(lse=cos), dict(max_new=2), dict(sm_scale=float("inf")),
+                                  dict(q=many, parents=n.repeat(65)))),
+            (verify, TypeError, (dict(logits=torch.zeros(3, 30, device=dev).double()), dict(tokens=n.long()), dict(uniforms=torch.zeros(3, device=dev).half()),
+                                 dict(parents=n.long()), dict(slots=torch.zeros(1, device=dev)))),
+            (verify, ValueError, (dict(logits=torch.zeros(3, 30)), dict(logits=torch.zeros(30, device=dev)), dict(logits=torch.zeros(3, 0, device=dev)),
+                                  dict(logits=torch.zeros(30, 3, device=dev).t()), dict(tokens=n[:2]), dict(uniforms=torch.zeros(2, device=dev)),
+                                  dict(uniforms=torch.zeros(3)), dict(max_new=2), dict(max_new=None), dict(max_new=0),
+                                  dict(draft_logits=torch.zeros(3, 30, device=dev), parents=n), dict(draft_logits=torch.zeros(3, 29, device=dev)),
+                                  dict(draft_logits=torch.zeros(3, 30, device=dev).half()), dict(temperature=torch.ones(2, device=dev)),
+                                  dict(temperature=torch.ones(1, device=dev).double()), dict(temperature=-1.0), dict(temperature=float("inf")),
+                                  dict(temperature=float("nan")), dict(slots=n), dict(cu_seqlens=n[:0]),
+                                  dict(logits=torch.zeros(65, 30, device=dev), tokens=n.new_zeros(65), uniforms=torch.zeros(65, device=dev), max_new=65))),
+            (keep, TypeError, (dict(path=_i32([[0], [0], [0]], dev).long()), dict(accepted=torch.ones(3, device=dev)))),
+            (keep, ValueError, (dict(path=n), dict(accepted=n[:2]), dict(slots=n[:2]), dict(cu_seqlens=n), dict(path=n.new_zeros(3, 65)),
+                                dict(path=n.new_zeros(1025, 1), accepted=n.new_zeros(1025), slots=n.new_full((1025,), -1))))):
+        for bad in bads:
+            with pytest.raises(error):
+                call(**bad)
+    with pytest.raises((ValueError, NotImplementedError)):
+        verify(logits=torch.zeros(3, 2 ** 20 + 1, device=dev))
+    for call in (append, attend, verify, keep):
+        call()
+    torch.cuda.synchronize()
 
 
 @pytest.mark.parametrize("nodes,hq", [(8, 2), (40, 4)])
