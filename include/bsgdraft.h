@@ -72,7 +72,8 @@ int bsg_kv_tree_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
  *                          accepted if u q(x) < p(x); after a rejection the new token is drawn from
  *                          max(p - q, 0), otherwise from p
  *   temperature <= 0       accepted if x is the likeliest token (the first of equal ones), which is also the new one
- * where nothing is left, from p.  Drawn: the first token whose running sum exceeds uniforms[node 0] times the whole.
+ * where nothing is left (a p within 2^-43 of its q leaves nothing), from p.  Drawn: the first token whose running sum
+ * exceeds uniforms[node 0] times the whole.
  * Decisions are those of 64-bit weights and sums (32-bit ones only decide what they cannot have wrong), so that the answer is
  * the definition's but for numbers within some 2^-40 of a border.
  *   logits, draft_logits : [tokens][vocab] fp16, bf16 or fp32 (the same), row strides in elements; the aligned 16 bytes in
@@ -84,8 +85,9 @@ int bsg_kv_tree_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
  *   accepted             : int32 [rows], accepted nodes, node 0 among them; 0 without nodes
  *   path, out_tokens     : int32 [rows][max_new]: the accepted nodes; the accepted nodes' tokens after the first's and the
  *                          new token, as many; then -1.  A row of logits with NaN, +inf, or nothing but -inf ends
- *                          the path with -1 as its new token.
- * max_new <= BSG_TREE_NODES, vocab <= 2^20, rows <= 16384.  Workspace as bsg_kv_attention. */
+ *                          the path with -1 as its new token: the sequence has failed, and -1 is no token to go on with.
+ * max_new <= BSG_TREE_NODES, vocab <= 2^20, rows <= 16384.  Workspace as bsg_kv_attention.  It has no slots: in a batch some of
+ * whose sequences take no part, bsg_verify_drafts_slots (bsgdraft_slots.h) leaves those out. */
 int64_t bsg_verify_drafts_workspace_bytes(int64_t tokens, int32_t rows, int64_t vocab, int32_t max_new, int dtype,
                                           int32_t drafts);
 int bsg_verify_drafts(const void* logits, int64_t logits_stride, const void* draft_logits, int64_t draft_stride,
@@ -98,7 +100,9 @@ int bsg_verify_drafts(const void* logits, int64_t logits_stride, const void* dra
  * slot slots[b] (NULL: slot b), n = cu[b+1] - cu[b] (max_new where cu is NULL), those at the places path[b][0 ..
  * accepted[b]) move, in order, to the place of the first; the length shrinks to hold them, the pages past it are released.
  * Of a path only what ascends, from 0 .. n-1, counts.  A token that changes its page is rounded again under that page's
- * scale, which grows as bsg_kv_append's does, the page's other tokens with it; within a page, bytes move.
+ * scale, which grows as bsg_kv_append's does, the page's other tokens with it; within a page, bytes move.  A page's scale
+ * never shrinks: where a rejected token had raised it, the page's other tokens were rounded again under it when that one was
+ * appended, the smallest to steps of 2^-9 of the larger scale, and stay so.
  *   pool   : page_bytes = 2 n_heads page_size head_dim and page_scales = 2 n_heads, as bsg_kv_cache
  *   path   : int32 [rows][max_new]
  * Slots must be distinct and the pages of the new tokens a sequence's own; a slot out of range, or of fewer than n

@@ -288,7 +288,8 @@ def pages_keep(pages: torch.Tensor, scales: torch.Tensor, page_table: torch.Tens
     together, in order, behind the tokens that were there before; the length shrinks to hold them and the pages past
     it are released.
 
-    A token that changes its page is rounded again under that page's scale, which grows as kv_append's does.  Of a
+    A token that changes its page is rounded again under that page's scale, which grows as kv_append's does.  No scale
+    shrinks: what a louder token that is rejected now cost its page's other tokens when it was appended stays lost.  Of a
     path only what ascends and exists counts.  A slot out of range, or of fewer tokens than its new ones, is left as it
     is.  Slots must be distinct, and the new tokens' pages a sequence's own (pages_extend sees to that); at most 64
     places and 1024 rows."""

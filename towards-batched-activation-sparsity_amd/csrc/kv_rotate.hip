@@ -9,7 +9,7 @@
 // head), keys and values, lane 16 g + t with channels 64 c + 16 g .. +15 of token t, so that a pair's other half lies in the
 // lane itself (R = 128: the other c; R = 16: 8 channels on; neighbours), or in lane ^ 32 or ^ 16 (R = 64, 32).  Those of
 // the queries take a row of D channels with D / 16 lanes, two runs of 8 channels each, chosen so that a pair's halves meet
-// in one lane: eight (D = 128) or sixteen rows at a time, four times, with one load of a token's angles for its heads.
+// in one lane: eight (D = 128) or sixteen rows at a time, kRows times, with one load of a token's angles for the rows that share it.
 
 #include "bsgdraft.h"
 #include "draft_tree.hpp"

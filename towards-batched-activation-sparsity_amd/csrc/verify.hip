@@ -4,7 +4,7 @@
 // Answers are whole numbers next to borders: a number u against a ratio of probabilities, and the first running sum past
 // u of the whole.  So weights w = 2^((x - m) k), k = log2(e) / temperature, and their sums are 64-bit.  2^t is
 // 2^n times a polynomial of the 9th degree in f, t = n + f, |f| <= 1/2, which interpolates 2^f in the Chebyshev points of
-// that interval (relative error 2^-46).
+// that interval (relative error 2^-45.6).
 //
 // First launch: of the rows of nodes that have children a wave has kPiece logits in registers and leaves their maximum
 // and the sum of their weights against it (or, greedy, where the first maximum is).  Second launch: the work-groups
@@ -29,7 +29,7 @@ constexpr int kWaves = 4;     // of a work-group
 constexpr int kMostVocab = 1 << 20;
 constexpr double kLog2e = 1.4426950408889634;
 // The 32-bit sum of a row: a weight of t octaves is off by 0.7 x 3 |t| 2^-24 (the difference, k, their product) and 2^-22 of
-// itself; |t|, averaged by the weights, is at most the logarithm of the vocabulary, 20.  Sums of 32 numbers add 2^-19.
+// itself; |t|, averaged by the weights, is at most the logarithm of the vocabulary, 20.  A lane's sum of 16 numbers adds 2^-20.
 constexpr double kNear = 0x1p-17;
 // What the sums of a target's and a draft's rows of the same probabilities may differ by.  Where the rows lie at other addresses they are
 // cut into other pieces: a weight in a sum is the product of two polynomials, each off by 2^-45.6, and chains of at most 50
@@ -295,8 +295,8 @@ __device__ __forceinline__ Piece piece_of(PieceOf<T>& x, bool greedy, bool exact
 
 // The rows of the nodes that have children, by pieces: of a sequence's the blockIdx.y-th, and every gridDim.y-th from there.
 // 64 chains of up to 5 drawn drafts, 32000 fp16 logits of two models: 17 us, of which the 64-bit weights are some 12 (18
-// instructions each, all at the rate of a fused multiply-add); 64 trees of up to 16 nodes: 13 us with 32-bit weights, 21 with
-// 64-bit ones.
+// instructions each, the sum's among them, all at the rate of a fused multiply-add); 64 trees of up to 16 nodes: 13 us with
+// 32-bit weights, 21 with 64-bit ones.
 template <typename T>
 __global__ __launch_bounds__(64 * kWaves) void bsg_verify_rows_kernel(VerifyParams p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -470,7 +470,7 @@ __device__ __forceinline__ Row row_of(int pieces, double k, int seg, int lane, c
 }
 
 // A chain of waits bounds it, of which none is long: the tree, the rows' pieces, the walk, a piece of the last row, the meeting
-// of the work-groups, the piece and the number that are drawn.  64 chains 14 us, 64 trees 15, of 32000 logits; greedy 9.
+// of the work-groups, the piece and the number that are drawn.  64 chains 15 us, 64 trees 16, of 32000 logits; greedy 9.
 template <typename T>
 __global__ __launch_bounds__(64 * kWaves) void bsg_verify_walk_kernel(VerifyParams p) {
   constexpr int PER = PieceOf<T>::PER, N = ShareOf<T>::N;
