@@ -254,6 +254,33 @@ def test_rotated_batches_of_many_sequences_without_a_bound(dev, p, d):
                    torch.float16, False)
 
 
+@pytest.mark.parametrize("dims,interleaved", [(16, False), (64, True), (128, False)])
+def test_rotated_by_slices_of_a_table(dev, dims, interleaved):
+    """cos and sin beside each other in one table, from a later position on, and a table of one position."""
+    rng = np.random.default_rng(dims)
+    lengths, new = [30, 17], [9, 17]
+    _, _, _, pages, scales, tab = _cache(rng, dev, lengths, 2, 16, 128)
+    n, cu = _i32(lengths, dev), _i32(_cu(new), dev)
+    q, k, v = (torch.randn(26, h, 128, device=dev).half() for h in (4, 2, 2))
+    cos, sin = (torch.from_numpy(x).to(dev) for x in _angles(50, dims))
+    both = torch.cat([cos, sin], 1)
+    was = pages.view(torch.uint8).clone(), scales.clone()
+
+    def call(cos, sin, positions):
+        pages.view(torch.uint8).copy_(was[0])
+        scales.copy_(was[1])
+        out = bsa.kv_append_rotated(q, k, v, cos, sin, pages, scales, tab, n, cu_seqlens=cu, max_new=17, interleaved=interleaved,
+                                    positions=_i32(positions, dev))
+        return out, pages.view(torch.uint8).clone(), scales.clone()
+
+    at = rng.integers(7, 50, 26)
+    want = call(cos, sin, at)
+    for c, s, moved in ((both[:, :dims // 2], both[:, dims // 2:], 0), (both[7:, :dims // 2], both[7:, dims // 2:], 7), (cos[7:], sin[7:], 7)):
+        assert all(torch.equal(x, y) for x, y in zip(call(c, s, at - moved), want))
+    want = call(cos, sin, [11] * 26)
+    assert all(torch.equal(x, y) for x, y in zip(call(both[11:12, :dims // 2], both[11:12, dims // 2:], [0] * 26), want))
+
+
 @pytest.mark.parametrize("p,d", [(16, 64), (64, 128)])
 def test_rotated_magnitudes_past_every_scale(dev, p, d):
     """bf16 numbers of 2^120 beside the largest scale, 2^80: the largest e4m3 number, with its sign, as kv_append."""
@@ -590,6 +617,24 @@ def test_tree_scores_of_minus_infinity_first(dev, nodes, hq):
     for ref, (out, lse) in _hard(dev, rng, raw, sc, table, [length], nodes, hq, "bf16", d, q.bfloat16().to(dev)):
         assert (ref[1] >= np.log(length - first - nodes + 1) - 128 - 1e-9).all() and (ref[1] <= np.log(length - first) - 128 + 1e-9).all()
         _check_attention(out, lse, (*ref[:3], np.full_like(ref[3], 128.0), *ref[4:]), torch.bfloat16, d)
+
+
+@pytest.mark.parametrize("hq,p,d", [(2, 16, 64), (8, 64, 128), (10, 16, 64)])
+def test_tree_parts_of_sequences_that_take_no_part(dev, hq, p, d):
+    """Work dealt out in parts over slots in any order, some of them out of range, sequences without tokens, shorter than their
+    trees or empty, before, between and after long ones."""
+    rng = np.random.default_rng(hq)
+    lengths = [1500, 0, 2500, 30, 700, 64, 1100]
+    slots, new = [9, 2, 1, -1, 6, 3, 0, 5, 4, 7], [50, 40, 33, 64, 0, 45, 37, 64, 0, 48]
+    raw, sc, table, pages, scales, tab = _cache(rng, dev, lengths, 2, p, d, poison=True)
+    cu, parents = _cu(new), [x for n in new if n for x in _parents(rng, n)]
+    q = torch.from_numpy(rng.standard_normal((cu[-1], hq, d)).astype(np.float32)).bfloat16().to(dev)
+    with np.errstate(invalid="ignore"):
+        ref = dft.tree_attention(q.double().cpu().numpy(), parents, orc.Layer(raw, sc), table, np.array(lengths), cu, slots)
+    for max_len in CUTS:
+        out, lse = bsa.kv_tree_attention(q, _i32(parents, dev), pages, scales, tab, _i32(lengths, dev), cu_seqlens=_i32(cu, dev), max_new=64,
+                                         slots=_i32(slots, dev), max_len=max_len)
+        _check_attention(out, lse, ref, torch.bfloat16, d)
 
 
 @pytest.mark.parametrize("nodes,hq", HARD_TREES)
