@@ -170,8 +170,8 @@ def test_a_verification_of_slots_is_one_of_the_others():
 
 
 def test_documented_last_tokens():
-    """INTEGRATION.md's line for what the next tree begins with, run as it stands: the new token, or, where nothing was accepted,
-    what it was before."""
+    """The documented line for what the next trees begin with, run as it stands: the new token, or, where nothing was accepted, what
+    it was before."""
     line = next(x for x in open(os.path.join(ROOT, "INTEGRATION.md")).read().splitlines() if x.startswith("last = "))
     got = drafts.Verified(torch.tensor([0, 1, 3, 0, 2], dtype=torch.int32), None,
                           torch.tensor([[-1, -1, -1], [7, -1, -1], [4, 5, 6], [-1, -1, -1], [8, -1, -1]], dtype=torch.int32))
