@@ -72,8 +72,7 @@ int bsg_kv_tree_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
  *                          accepted if u q(x) < p(x); after a rejection the new token is drawn from
  *                          max(p - q, 0), otherwise from p
  *   temperature <= 0       accepted if x is the likeliest token (the first of equal ones), which is also the new one
- * where nothing is left (a p within 2^-43 of its q leaves nothing), from p.  Drawn: the first token whose running sum
- * exceeds uniforms[node 0] times the whole.
+ * where nothing is left, from p.  Drawn: the first token whose running sum exceeds uniforms[node 0] times the whole.
  * Decisions are those of 64-bit weights and sums (32-bit ones only decide what they cannot have wrong), so that the answer is
  * the definition's but for numbers within some 2^-40 of a border.
  *   logits, draft_logits : [tokens][vocab] fp16, bf16 or fp32 (the same), row strides in elements; the aligned 16 bytes in

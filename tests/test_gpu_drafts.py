@@ -1032,6 +1032,31 @@ def test_verify_drawn_numbers_next_to_their_border(dev, dtype, vocab):
     assert [w[0] for w in want] == [1, 2] * 6
 
 
+@pytest.mark.parametrize("vocab,gap", [(50, 24.0), (50, 27.0), (50, 30.0), (3001, 12.0), (3001, 17.0), (3001, 20.0)])
+def test_verify_drafts_almost_as_likely(dev, vocab, gap):
+    """Two rows with all but e^-gap or so of their weight on the same token, and rejected drafts (which do not exist): little is
+    left, 1e-5 to 1e-14 of the row, and the new token is drawn from just that.  A p or q near 1 is off by a sum's, an inverse's and a
+    product's rounding, 3 x 2^-53 each, here and in the oracle: what is left, and each of its running sums, by 12 x 2^-53 of
+    the row.  The others' polynomials are off by 2^-45.6 of what is not on that token, which is some three times what is left: 2^-43
+    of that.  Numbers as near as twice that to a border are drawn again."""
+    rng = np.random.default_rng([vocab, int(gap)])
+    rows = 64
+    x = (-gap - np.log(vocab) + rng.standard_normal((2, 2 * rows, vocab))).astype(np.float32)
+    x[:, np.arange(2 * rows), rng.integers(0, vocab, rows).repeat(2)] = 0.0
+    tokens, u = np.full(2 * rows, -1), rng.random(2 * rows).astype(np.float32)
+    for b in range(rows):
+        p, q = (np.exp(r.astype(np.float64)) / np.exp(r.astype(np.float64)).sum() for r in x[:, 2 * b])
+        sums = np.cumsum(np.maximum(p - q, 0))
+        assert 1e-14 < sums[-1] < 1e-5
+        while np.abs(sums / sums[-1] - u[2 * b]).min() < 2 * (12 * 2.0 ** -53 / sums[-1] + 2.0 ** -43):
+            u[2 * b] = rng.random(dtype=np.float32)
+    logits, draft = (torch.from_numpy(r).to(dev) for r in x)
+    want = dft.verify(x[0].astype(np.float64), tokens, u, None, x[1].astype(np.float64), 1.0, _cu([2] * rows))
+    got = bsa.verify_drafts(logits, _i32(tokens, dev), torch.from_numpy(u).to(dev), draft_logits=draft, max_new=2)
+    _same_verdict(got, want, 2)
+    assert all(w[0] == 1 for w in want)
+
+
 @pytest.mark.parametrize("vocab,places", [(40, (4, 5, 6)), (40, (36, 37, 2)), (5004, (8, 9, 4801)), (5004, (4104, 4105, 30)), (70000, (12, 13, 69999))])
 def test_verify_where_nothing_is_left(dev, vocab, places):
     """A row of three tokens of weights 1, 2^-23 and 2^-46, all of them drafted and asked with 1 - 2^-24.  The last one's border is 1,

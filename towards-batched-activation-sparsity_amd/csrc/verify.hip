@@ -31,10 +31,6 @@ constexpr double kLog2e = 1.4426950408889634;
 // The 32-bit sum of a row: a weight of t octaves is off by 0.7 x 3 |t| 2^-24 (the difference, k, their product) and 2^-22 of
 // itself; |t|, averaged by the weights, is at most the logarithm of the vocabulary, 20.  A lane's sum of 16 numbers adds 2^-20.
 constexpr double kNear = 0x1p-17;
-// What the sums of a target's and a draft's rows of the same probabilities may differ by.  Where the rows lie at other addresses they are
-// cut into other pieces: a weight in a sum is the product of two polynomials, each off by 2^-45.6, and chains of at most 50
-// roundings, of 2^-53, add them up; twice that is 2^-43.4.
-constexpr double kAlike = 0x1p-43;
 
 struct Piece {  // of a row
   double sum;   // of its weights; NaN: a logit is NaN or +inf
@@ -311,7 +307,8 @@ __global__ __launch_bounds__(64 * kWaves) void bsg_verify_rows_kernel(VerifyPara
     const int node = __builtin_amdgcn_readfirstlane(__builtin_ctzll(left));
     left &= left - 1;
     const int64_t at = (t.from + node) * p.stride[which];
-    const int shift = shift_of<T>(p.x[which], at);
+    // a draft's row is cut as the target's beside it is, so that of equal rows the sums are equal to the last bit
+    const int shift = shift_of<T>(p.x[0], (t.from + node) * p.stride[0]);
     PieceOf<T> x;
     x.load(p.x[which], at, p.vocab, shift, piece, lane);
     const Piece mine = piece_of<true, T>(x, greedy, p.drafts != 0, kLog2e / (double)t.temperature, piece * kPiece - shift, lane);
@@ -585,10 +582,12 @@ __global__ __launch_bounds__(64 * kWaves) void bsg_verify_walk_kernel(VerifyPara
   // what is left of the last row: the row without the rejected tokens, or what it has over its drafts
   const int64_t x_at = (t.from + at) * p.stride[0], y_at = (t.from + at) * p.stride[1];
   const int shift = shift_of<T>(p.x[0], x_at);
-  // p is taken as less by kAlike, so that a draft's q that is p has all of it, and not what their roundings leave
-  const double by[2] = {(1.0 - kAlike) / total, residual ? 1.0 / s_total[1][at] : 0.0};
+  const double by[2] = {1.0 / total, residual ? 1.0 / s_total[1][at] : 0.0};
   const float y_top = residual ? s_top[1][at] : 0.f;
-  const auto surplus = [&](double x, double y) { return __builtin_fmax(x * by[0] - y * by[1], 0.0); };
+  const auto surplus = [&](double x, double y) {
+#pragma clang fp contract(off)  // each product rounded: a q that is p leaves nothing of it
+    return __builtin_fmax(x * by[0] - y * by[1], 0.0);
+  };
   Piece* const last = p.last + (int64_t)row * p.pieces;
   int token = -1;
   for (bool again = false;; again = true) {
